@@ -690,6 +690,77 @@ int noalloc_scratch(void** out) {
     return KLP_OK;
 }
 
+// Rows of the norms and of the 8-bit matrices: `ld` elements apart.
+int check_matrix(const void* p, int64_t ld, int64_t cols, size_t align, const char* name) {
+    if (p == nullptr) return fail(KLP_EINVAL, "%s must be non-null", name);
+    if (!aligned(p, align))
+        return fail(KLP_EINVAL, "%s is not %zu-byte aligned", name, align);
+    if (ld < 0) return fail(KLP_EINVAL, "%s: row stride must be non-negative", name);
+    if (cols < 1) return fail(KLP_EINVAL, "%s must have at least one column", name);
+    return KLP_OK;
+}
+
+int check_dtype3(int dtype, const char* name) {
+    if (dtype == KLP_BF16 || dtype == KLP_FP16 || dtype == KLP_FP32) return KLP_OK;
+    return fail(KLP_EDTYPE, "%s dtype must be bf16, fp16, or fp32", name);
+}
+
+int check_norm(const void* x, int dtype, int64_t rows, int64_t dim, const void* weight,
+               int weight_dtype) {
+    int rc = check_dtype3(dtype, "x");
+    if (rc != KLP_OK) return rc;
+    if (weight_dtype != dtype && weight_dtype != KLP_FP32)
+        return fail(KLP_EDTYPE, "weight must be float32 or of x's dtype");
+    if (rows < 0) return fail(KLP_EINVAL, "rows must be >= 0");
+    if (dim < 1 || dim > klp::kNormMaxDim)
+        return fail(KLP_EINVAL, "dim must be in [1, %lld], got %lld",
+                    static_cast<long long>(klp::kNormMaxDim), static_cast<long long>(dim));
+    if (rows > INT32_MAX) return fail(KLP_EINVAL, "rows above 2^31-1 are not supported");
+    if (rows == 0) return KLP_OK;
+    if (x == nullptr || !aligned(x, elem_bytes(dtype)))
+        return fail(KLP_EINVAL, "x must be non-null and aligned to its elements");
+    if (weight == nullptr || !aligned(weight, elem_bytes(weight_dtype)))
+        return fail(KLP_EINVAL, "weight must be non-null and aligned to its elements");
+    return KLP_OK;
+}
+
+// The forward's operands into p, but for its outputs.
+int norm_setup(const void* x, int dtype, int64_t ld_x, const void* residual, int64_t ld_residual,
+               const void* weight, int weight_dtype, int64_t rows, int64_t dim, float eps, void* h,
+               klp::NormParams* p) {
+    int rc = check_norm(x, dtype, rows, dim, weight, weight_dtype);
+    if (rc != KLP_OK) return rc;
+    if (!(eps >= 0.0f) || isinf(eps)) return fail(KLP_EINVAL, "eps must be finite and >= 0");
+    if (rows == 0) return KLP_OK;
+    if (ld_x < 0 || ld_residual < 0)
+        return fail(KLP_EINVAL, "row strides must be non-negative");
+    if (residual != nullptr) {
+        if (!aligned(residual, elem_bytes(dtype)))
+            return fail(KLP_EINVAL, "residual is not aligned to its elements");
+        if (h == nullptr || !aligned(h, elem_bytes(dtype)))
+            return fail(KLP_EINVAL,
+                        "h must be non-null with a residual, and aligned to its elements");
+    }
+    *p = klp::NormParams{};
+    p->x = x;
+    p->ld_x = ld_x;
+    p->residual = residual;
+    p->ld_r = ld_residual;
+    p->weight = weight;
+    p->weight_f32 = weight_dtype == KLP_FP32;
+    p->rows = rows;
+    p->dim = dim;
+    p->eps = eps;
+    p->h = h;
+    p->n_blocks = ceil_div(dim, klp::kScaleBlock);
+    return KLP_OK;
+}
+
+size_t norm_bwd_workspace(int64_t rows, int64_t dim) {
+    if (rows <= 0 || dim < 1 || dim > klp::kNormMaxDim) return 0;
+    return static_cast<size_t>(klp::norm_bwd_groups(rows, dim) * dim) * sizeof(float);
+}
+
 }  // namespace
 
 extern "C" {
@@ -1511,6 +1582,205 @@ int klp_fwd_noalloc(const void* logits, int dtype, int64_t n_rows, int64_t vocab
     return fwd_impl(logits, dtype, n_rows, vocab, rows_inner, stride_outer, stride_inner, targets,
                     logprob, entropy, lse, ws, ws ? size_t{KLP_FWD_NOALLOC_SCRATCH_BYTES} : 0, cfg,
                     1.0f, stream);
+}
+
+int klp_rms_norm(const void* x, int dtype, int64_t ld_x, const void* residual,
+                 int64_t ld_residual, const void* weight, int weight_dtype, int64_t rows,
+                 int64_t dim, float eps, void* y, void* h, float* rstd, void* stream) {
+    klp::NormParams p;
+    const int rc = norm_setup(x, dtype, ld_x, residual, ld_residual, weight, weight_dtype, rows,
+                              dim, eps, h, &p);
+    if (rc != KLP_OK) return rc;
+    if (rows == 0) return ok();
+    if (y == nullptr || !aligned(y, elem_bytes(dtype)))
+        return fail(KLP_EINVAL, "y must be non-null and aligned to its elements");
+    if (rstd != nullptr && !aligned(rstd, 4))
+        return fail(KLP_EINVAL, "rstd is not 4-byte aligned");
+    p.y = y;
+    p.rstd = rstd;
+    if (injected_failure("rms norm")) return KLP_ELAUNCH;
+    return after_launch(klp::launch_norm(dtype, p, static_cast<hipStream_t>(stream)), "rms norm");
+}
+
+int klp_rms_norm_fp8(const void* x, int dtype, int64_t ld_x, const void* residual,
+                     int64_t ld_residual, const void* weight, int weight_dtype, int64_t rows,
+                     int64_t dim, float eps, uint8_t* q, float* scales, void* h, void* stream) {
+    klp::NormParams p;
+    int rc = norm_setup(x, dtype, ld_x, residual, ld_residual, weight, weight_dtype, rows, dim,
+                        eps, h, &p);
+    if (rc != KLP_OK) return rc;
+    if (rows == 0) return ok();
+    if (q == nullptr) return fail(KLP_EINVAL, "q must be non-null");
+    if ((rc = check_f32(scales, "scales")) != KLP_OK) return rc;
+    p.q = q;
+    p.scales = scales;
+    if (injected_failure("rms norm")) return KLP_ELAUNCH;
+    return after_launch(klp::launch_norm(dtype, p, static_cast<hipStream_t>(stream)), "rms norm");
+}
+
+size_t klp_rms_norm_bwd_workspace_bytes(int64_t rows, int64_t dim) {
+    return norm_bwd_workspace(rows, dim);
+}
+
+int klp_rms_norm_bwd(const void* h, int dtype, int64_t ld_h, const void* weight, int weight_dtype,
+                     const float* rstd, const void* g_y, const void* g_h, int64_t rows,
+                     int64_t dim, void* d_x, void* d_weight, void* workspace,
+                     size_t workspace_bytes, void* stream) {
+    int rc = check_norm(h, dtype, rows, dim, weight, weight_dtype);
+    if (rc != KLP_OK) return rc;
+    if (rows == 0) return fail(KLP_EINVAL, "rows must be >= 1");
+    if (ld_h < 0) return fail(KLP_EINVAL, "row strides must be non-negative");
+    if ((rc = check_f32(rstd, "rstd")) != KLP_OK) return rc;
+    const size_t e = elem_bytes(dtype);
+    if (g_y == nullptr || !aligned(g_y, e) || !aligned(g_h, e) || d_x == nullptr ||
+        !aligned(d_x, e))
+        return fail(KLP_EINVAL, "g_y and d_x must be non-null, and gradients aligned to their "
+                                "elements");
+    klp::NormBwdParams p{};
+    if (d_weight != nullptr) {
+        if (!aligned(d_weight, elem_bytes(weight_dtype)))
+            return fail(KLP_EINVAL, "d_weight is not aligned to its elements");
+        const size_t need = norm_bwd_workspace(rows, dim);
+        if (workspace == nullptr || workspace_bytes < need || !aligned(workspace, 16))
+            return fail(KLP_EWORKSPACE,
+                        "workspace missing, too small or not 16-byte aligned: have %zu bytes, "
+                        "need %zu",
+                        workspace_bytes, need);
+        p.partials = static_cast<float*>(workspace);
+    }
+    p.h = h;
+    p.ld_h = ld_h;
+    p.weight = weight;
+    p.weight_f32 = weight_dtype == KLP_FP32;
+    p.rstd = rstd;
+    p.g_y = g_y;
+    p.g_h = g_h;
+    p.rows = rows;
+    p.dim = dim;
+    p.groups = klp::norm_bwd_groups(rows, dim);
+    p.d_x = d_x;
+    p.d_weight = d_weight;
+    if (injected_failure("rms norm backward")) return KLP_ELAUNCH;
+    rc = after_launch(klp::launch_norm_bwd(dtype, p, static_cast<hipStream_t>(stream)),
+                      "rms norm backward");
+    if (rc != KLP_OK || d_weight == nullptr) return rc;
+    return after_launch(klp::launch_norm_dw(weight_dtype, p, static_cast<hipStream_t>(stream)),
+                        "rms norm d_weight");
+}
+
+int klp_quantize_fp8(const void* x, int dtype, int64_t ld_x, int64_t rows, int64_t dim,
+                     int block_rows, uint8_t* q, float* scales, void* stream) {
+    int rc = check_dtype3(dtype, "x");
+    if (rc != KLP_OK) return rc;
+    if (block_rows != 1 && block_rows != klp::kScaleBlock)
+        return fail(KLP_EINVAL, "block_rows must be 1 or 128, got %d", block_rows);
+    if (rows < 0 || dim < 1) return fail(KLP_EINVAL, "rows must be >= 0 and dim >= 1");
+    if (rows == 0) return ok();
+    if ((rc = check_matrix(x, ld_x, dim, elem_bytes(dtype), "x")) != KLP_OK) return rc;
+    if (q == nullptr) return fail(KLP_EINVAL, "q must be non-null");
+    if ((rc = check_f32(scales, "scales")) != KLP_OK) return rc;
+    const int64_t n_blocks = ceil_div(dim, klp::kScaleBlock);
+    // The grid: one 16-lane group per block of a row, or a workgroup per
+    // block with at most 65535 along the rows.
+    if (n_blocks > INT32_MAX / rows ||
+        (block_rows != 1 && ceil_div(rows, klp::kScaleBlock) > 65535))
+        return fail(KLP_EINVAL, "too many scale blocks: %lld rows of %lld",
+                    static_cast<long long>(rows), static_cast<long long>(n_blocks));
+    klp::QuantizeParams p{};
+    p.x = x;
+    p.ld_x = ld_x;
+    p.rows = rows;
+    p.dim = dim;
+    p.n_blocks = n_blocks;
+    p.block_rows = block_rows;
+    p.q = q;
+    p.scales = scales;
+    if (injected_failure("quantize")) return KLP_ELAUNCH;
+    return after_launch(klp::launch_quantize(dtype, p, static_cast<hipStream_t>(stream)),
+                        "quantize");
+}
+
+int klp_fp8_linear(const uint8_t* x, int64_t ld_x, const float* x_scales, const uint8_t* w,
+                   int64_t ld_w, const float* w_scales, int64_t m, int64_t n, int64_t k,
+                   int out_dtype, void* out, int64_t ld_out, void* stream) {
+    int rc = check_dtype3(out_dtype, "out");
+    if (rc != KLP_OK) return rc;
+    if (m < 0 || n < 1) return fail(KLP_EINVAL, "m must be >= 0 and n >= 1");
+    if (k < 16 || k % 16 != 0)
+        return fail(KLP_EINVAL, "k must be a positive multiple of 16, got %lld",
+                    static_cast<long long>(k));
+    if (m == 0) return ok();
+    if ((rc = check_matrix(x, ld_x, k, 16, "x")) != KLP_OK) return rc;
+    if ((rc = check_matrix(w, ld_w, k, 16, "w")) != KLP_OK) return rc;
+    if (ld_x % 16 != 0 || ld_w % 16 != 0)
+        return fail(KLP_EINVAL, "row strides of x and w must be multiples of 16");
+    if ((rc = check_f32(x_scales, "x_scales")) != KLP_OK) return rc;
+    if ((rc = check_f32(w_scales, "w_scales")) != KLP_OK) return rc;
+    if (out == nullptr || !aligned(out, elem_bytes(out_dtype)) || ld_out < n)
+        return fail(KLP_EINVAL,
+                    "out must be non-null and aligned to its elements, with a row stride >= n");
+    if (m > (1 << 20) || n > (int64_t{1} << 31) || k > (1 << 24))
+        return fail(KLP_EINVAL, "m, n and k must not exceed 2^20, 2^31 and 2^24");
+    klp::Fp8LinearParams p{};
+    p.x = x;
+    p.ld_x = ld_x;
+    p.xs = x_scales;
+    p.w = w;
+    p.ld_w = ld_w;
+    p.ws = w_scales;
+    p.m = m;
+    p.n = n;
+    p.k = k;
+    p.n_blocks = ceil_div(k, klp::kScaleBlock);
+    p.out = out;
+    p.ld_out = ld_out;
+    if (injected_failure("fp8 linear")) return KLP_ELAUNCH;
+    return after_launch(klp::launch_fp8_linear(out_dtype, p, static_cast<hipStream_t>(stream)),
+                        "fp8 linear");
+}
+
+int klp_sample(const void* logits, int dtype, int64_t n_rows, int64_t vocab, int64_t rows_inner,
+               int64_t stride_outer, int64_t stride_inner, const float* uniform,
+               float temperature, const float* temperatures, int32_t top_k, const int32_t* top_ks,
+               float top_p, const float* top_ps, float min_p, const float* min_ps,
+               int64_t* tokens, float* logp, float* sample_logp, void* stream) {
+    static const int64_t no_targets = 0;  // not read
+    int rc = check_rows(logits, dtype, n_rows, vocab, rows_inner, stride_outer, stride_inner,
+                        &no_targets);
+    if (rc != KLP_OK) return rc;
+    if (n_rows == 0) return ok();
+    if (tokens == nullptr || !aligned(tokens, 8))
+        return fail(KLP_EINVAL, "tokens must be non-null and 8-byte aligned");
+    if (vocab > klp::kSampleMaxVocab)
+        return fail(KLP_EINVAL, "vocab above 2^26 is not supported");
+    if ((rc = check_f32(uniform, "uniform")) != KLP_OK) return rc;
+    if ((rc = check_f32(logp, "logp")) != KLP_OK) return rc;
+    if ((rc = check_f32(sample_logp, "sample_logp")) != KLP_OK) return rc;
+    if (temperatures == nullptr && !(temperature >= 0.0f && !isinf(temperature)))
+        return fail(KLP_EINVAL, "temperature must be finite and >= 0, got %g",
+                    static_cast<double>(temperature));
+    if (!aligned(temperatures, 4) || !aligned(top_ks, 4) || !aligned(top_ps, 4) ||
+        !aligned(min_ps, 4))
+        return fail(KLP_EINVAL, "per-row parameters must be 4-byte aligned");
+    klp::SampleParams p{};
+    p.logits = logits;
+    p.rm = klp::RowMap{rows_inner, stride_outer, stride_inner};
+    p.n_rows = n_rows;
+    p.vocab = vocab;
+    p.uniform = uniform;
+    p.temperature = temperature;
+    p.top_p = top_p;
+    p.min_p = min_p;
+    p.top_k = top_k;
+    p.temperatures = temperatures;
+    p.top_ps = top_ps;
+    p.min_ps = min_ps;
+    p.top_ks = top_ks;
+    p.tokens = tokens;
+    p.logp = logp;
+    p.sample_logp = sample_logp;
+    if (injected_failure("sample")) return KLP_ELAUNCH;
+    return after_launch(klp::launch_sample(dtype, p, static_cast<hipStream_t>(stream)), "sample");
 }
 
 }  // extern "C"

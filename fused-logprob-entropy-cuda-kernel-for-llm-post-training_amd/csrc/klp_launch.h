@@ -5,6 +5,8 @@
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
+#include <type_traits>
+
 #include "../../include/kernel_opt_hip.h"
 #include "klp_device.h"
 
@@ -283,6 +285,100 @@ constexpr int64_t kHeadGemmCus = 256;
 constexpr int64_t kHeadGemmGroup = 6;
 hipError_t launch_head_gemm(int dtype, const HeadGemmParams& p, hipStream_t stream);
 hipError_t launch_head_sum(int dtype, const HeadSumParams& p, hipStream_t stream);
+
+// Root-mean-square norm (klp_norm.hip).  Rows of x, residual at row strides;
+// every other array dense.
+constexpr int kScaleBlock = 128;        // elements along a row that share an e4m3 scale
+constexpr int64_t kNormMaxDim = 65536;  // a row is held by one workgroup
+struct NormParams {
+    const void* x;         // [rows, ld_x]
+    int64_t ld_x;
+    const void* residual;  // [rows, ld_r], nullable
+    int64_t ld_r;
+    const void* weight;    // [dim], float32 with weight_f32, else of the rows' dtype
+    int weight_f32;
+    int64_t rows;
+    int64_t dim;
+    float eps;
+    void* h;               // [rows, dim]: written with a residual
+    void* y;               // [rows, dim]
+    float* rstd;           // [rows], nullable
+    uint8_t* q;            // [rows, dim] e4m3 codes, instead of y; nullable
+    float* scales;         // [rows, n_blocks]
+    int64_t n_blocks;      // ceil(dim / kScaleBlock)
+};
+struct NormBwdParams {
+    const void* h;         // [rows, ld_h]
+    int64_t ld_h;
+    const void* weight;
+    int weight_f32;
+    const float* rstd;     // [rows]
+    const void* g_y;       // [rows, dim]
+    const void* g_h;       // [rows, dim], nullable
+    int64_t rows;
+    int64_t dim;
+    int64_t groups;        // norm_bwd_groups(rows, dim)
+    void* d_x;             // [rows, dim]
+    float* partials;       // [groups, dim], nullable: no d_weight
+    void* d_weight;        // [dim]
+};
+// Threads of the backward's grid: 1024 a CU.
+constexpr int64_t kNormBwdThreads = 256 * 1024;
+int64_t norm_bwd_groups(int64_t rows, int64_t dim);
+hipError_t launch_norm(int dtype, const NormParams& p, hipStream_t stream);
+hipError_t launch_norm_bwd(int dtype, const NormBwdParams& p, hipStream_t stream);
+hipError_t launch_norm_dw(int weight_dtype, const NormBwdParams& p, hipStream_t stream);
+
+// e4m3 codes and scales (klp_fp8.hip): 128 elements of a row share a scale,
+// or 128 x 128 elements do.
+struct QuantizeParams {
+    const void* x;      // [rows, ld_x]
+    int64_t ld_x;
+    int64_t rows;
+    int64_t dim;
+    int64_t n_blocks;   // ceil(dim / kScaleBlock)
+    int block_rows;     // 1 or 128
+    uint8_t* q;         // [rows, dim]
+    float* scales;      // [ceil(rows / block_rows), n_blocks]
+};
+hipError_t launch_quantize(int dtype, const QuantizeParams& p, hipStream_t stream);
+
+// Product of e4m3 matrices with a scale for each 128 of K (klp_fp8.hip):
+// out[m, n] = sum_b xs[m, b] ws[n / 128, b] sum_{k in b} x[m, k] w[n, k].
+struct Fp8LinearParams {
+    const uint8_t* x;   // [m, ld_x]
+    int64_t ld_x;
+    const float* xs;    // [m, n_blocks]
+    const uint8_t* w;   // [n, ld_w]
+    int64_t ld_w;
+    const float* ws;    // [ceil(n / 128), n_blocks]
+    int64_t m, n, k;
+    int64_t n_blocks;   // ceil(k / 128)
+    void* out;          // [m, ld_out]
+    int64_t ld_out;
+};
+hipError_t launch_fp8_linear(int out_dtype, const Fp8LinearParams& p, hipStream_t stream);
+
+// Sampling (klp_sample.hip).
+constexpr int64_t kSampleMaxVocab = int64_t{1} << 26;
+struct SampleParams {
+    const void* logits;
+    RowMap rm;
+    int64_t n_rows;
+    int64_t vocab;
+    const float* uniform;       // [n_rows]
+    // A parameter of every row, or an array of one per row where non-null.
+    float temperature, top_p, min_p;
+    int top_k;
+    const float* temperatures;
+    const float* top_ps;
+    const float* min_ps;
+    const int32_t* top_ks;
+    int64_t* tokens;            // [n_rows]
+    float* logp;                // [n_rows]
+    float* sample_logp;         // [n_rows]
+};
+hipError_t launch_sample(int dtype, const SampleParams& p, hipStream_t stream);
 
 // Calibration kernels (klp_ceiling.hip): rows of `row_bytes` (a multiple of
 // 16) at `src` (and `dst`), 16-byte aligned and contiguous; `splits`

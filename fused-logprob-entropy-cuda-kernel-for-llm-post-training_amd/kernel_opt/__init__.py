@@ -19,6 +19,14 @@ from .lmhead import (  # noqa: F401
     vocab_chunk,
     vocab_chunks,
 )
+from .norm import (  # noqa: F401
+    fused_add_rms_norm,
+    fused_add_rms_norm_fp8,
+    fused_rms_norm,
+    fused_rms_norm_fp8,
+)
+from .fp8 import fp8_linear, quantize_fp8  # noqa: F401
+from .sample import fused_sample  # noqa: F401
 
 
 # Lazy import so users without trl can still use the kernels.

@@ -91,6 +91,18 @@ SIGNATURES = {
                                       _vp]),
     "klp_grpo_step": (_i32, _ROWS + [_vp, ctypes.c_float] + [_vp] * 4 + [_i64]
                       + [ctypes.c_float] * 3 + [_i32, ctypes.c_float] + [_vp] * 7),
+    "klp_rms_norm": (_i32, [_vp, _i32, _i64, _vp, _i64, _vp, _i32, _i64, _i64, ctypes.c_float]
+                     + [_vp] * 4),
+    "klp_rms_norm_fp8": (_i32, [_vp, _i32, _i64, _vp, _i64, _vp, _i32, _i64, _i64,
+                                ctypes.c_float] + [_vp] * 4),
+    "klp_rms_norm_bwd_workspace_bytes": (_sz, [_i64, _i64]),
+    "klp_rms_norm_bwd": (_i32, [_vp, _i32, _i64, _vp, _i32, _vp, _vp, _vp, _i64, _i64, _vp, _vp,
+                                _vp, _sz, _vp]),
+    "klp_quantize_fp8": (_i32, [_vp, _i32, _i64, _i64, _i64, _i32, _vp, _vp, _vp]),
+    "klp_fp8_linear": (_i32, [_vp, _i64, _vp, _vp, _i64, _vp, _i64, _i64, _i64, _i32, _vp, _i64,
+                              _vp]),
+    "klp_sample": (_i32, _ROWS + [_vp, ctypes.c_float, _vp, ctypes.c_int32, _vp, ctypes.c_float,
+                                  _vp, ctypes.c_float, _vp, _vp, _vp, _vp, _vp]),
     # include/kernel_opt_hip_tuning.h
     "klp_grpo_step_persistent_min_rows": (_i64, [_i32, _i64, _i32]),
     "klp_fwd_workspace_bytes_ex": (_sz, [_i64, _i32]),

@@ -536,6 +536,95 @@ int klp_head_dhidden(int dtype, const void* d_logits, int64_t ld_d, int64_t n_to
                      size_t workspace_bytes, void* stream);
 
 /*
+ * Root-mean-square norm with the residual's addition:
+ *   h = round(x + residual)   (h = x with `residual` NULL; `h` is then unused)
+ *   rstd = (mean(h^2) + eps)^-1/2,   y = round(h * rstd * weight)
+ * x [rows, ld_x] and residual [rows, ld_residual] are of `dtype` with unit
+ * stride along dim (row strides in elements, any value >= 0); weight [dim] is
+ * of `dtype` or KLP_FP32 (`weight_dtype`); y, h [rows, dim] are dense.  rstd
+ * (nullable, float32 [rows]) is what the backward needs.  Sums are float32;
+ * the statistics are those of the rounded h.  dim is at most 65536.
+ */
+int klp_rms_norm(const void* x, int dtype, int64_t ld_x, const void* residual,
+                 int64_t ld_residual, const void* weight, int weight_dtype, int64_t rows,
+                 int64_t dim, float eps, void* y, void* h, float* rstd, void* stream);
+
+/*
+ * The same norm with its output in e4m3: per row and 128 columns (the last
+ * block may hold fewer) with a = max |h * rstd * weight|,
+ *   scale = a / 448 (1 where a is 0),  q = e4m3(h * rstd * weight * (448 / a)),
+ * from the unrounded products.  q [rows, dim] and scales [rows,
+ * ceil(dim / 128)] are dense.  a below 2^-100 counts as 2^-100.  A block with
+ * a NaN or an infinity has a scale that is none either: all of it stands for NaN.
+ */
+int klp_rms_norm_fp8(const void* x, int dtype, int64_t ld_x, const void* residual,
+                     int64_t ld_residual, const void* weight, int weight_dtype, int64_t rows,
+                     int64_t dim, float eps, uint8_t* q, float* scales, void* h, void* stream);
+
+/*
+ * Backward of klp_rms_norm: from h ([rows, ld_h]; x where there was no
+ * residual), rstd and the gradients of y (g_y) and of h as an output (g_h,
+ * nullable: 0), both dense [rows, dim] of `dtype`:
+ *   d_x = round(g_h + rstd (g_y w - h rstd^2 mean(g_y w h)))
+ * the gradient of x and of the residual alike, and, with d_weight non-null,
+ *   d_weight = round(sum over rows of g_y h rstd)   (of weight_dtype).
+ * d_weight needs a workspace of klp_rms_norm_bwd_workspace_bytes bytes
+ * (16-byte aligned, any contents), shared only by calls ordered on one
+ * stream.  Its sums have a fixed order for given sizes.
+ */
+size_t klp_rms_norm_bwd_workspace_bytes(int64_t rows, int64_t dim);
+int klp_rms_norm_bwd(const void* h, int dtype, int64_t ld_h, const void* weight, int weight_dtype,
+                     const float* rstd, const void* g_y, const void* g_h, int64_t rows,
+                     int64_t dim, void* d_x, void* d_weight, void* workspace,
+                     size_t workspace_bytes, void* stream);
+
+/*
+ * e4m3 codes and float32 scales of x [rows, ld_x], with the formula of
+ * klp_rms_norm_fp8, over blocks of 128 elements of a row (block_rows = 1:
+ * scales [rows, ceil(dim / 128)]) or of 128 x 128 elements (block_rows = 128:
+ * scales [ceil(rows / 128), ceil(dim / 128)]); q [rows, dim], all dense.
+ */
+int klp_quantize_fp8(const void* x, int dtype, int64_t ld_x, int64_t rows, int64_t dim,
+                     int block_rows, uint8_t* q, float* scales, void* stream);
+
+/*
+ * Product of e4m3 matrices, a scale for each 128 of k:
+ *   out[i, j] = round(sum_b x_scales[i, b] w_scales[j / 128, b]
+ *                           sum_{l in block b} x[i, l] w[j, l])
+ * x [m, ld_x], w [n, ld_w] (16-byte aligned, row strides multiples of 16; k a
+ * positive multiple of 16), x_scales [m, ceil(k / 128)], w_scales
+ * [ceil(n / 128), ceil(k / 128)] dense, out [m, ld_out] of out_dtype.
+ * Products and sums are float32.  m <= 2^20, n <= 2^31, k <= 2^24.
+ */
+int klp_fp8_linear(const uint8_t* x, int64_t ld_x, const float* x_scales, const uint8_t* w,
+                   int64_t ld_w, const float* w_scales, int64_t m, int64_t n, int64_t k,
+                   int out_dtype, void* out, int64_t ld_out, void* stream);
+
+/*
+ * One token a row, drawn from logits (row addressing as above) by inverse
+ * transform of uniform[row] in [0, 1).  With y = (x - max x) / T, w = exp(y)
+ * and the row ordered by falling x (equal ones by index): K are its first
+ * top_k, P those of K before which less than top_p * mass(K) lies, M those of
+ * P with w >= min_p; the first always stays.  tokens[row] is the lowest index
+ * whose running sum (in index order) of M's weights exceeds uniform * mass(M),
+ *   logp = y - ln sum w,   sample_logp = y - ln mass(M)
+ * of that token, the sums in float64.
+ * Each parameter is one value, or with its array non-null one per row
+ * (float32, top_k int32; [n_rows]).  top_k <= 0 or >= vocab, top_p >= 1 and
+ * min_p <= 0 (or NaN) are off.  T = 0 takes the largest logit (lowest index),
+ * logp at T = 1 and sample_logp 0.  uniform below 0 (or NaN) counts as 0, and
+ * from 1 on takes M's last token with a weight above 0.
+ * A row without a distribution has token -1: with every logit -inf its
+ * log-probabilities are -inf, with a NaN or +inf logit, or a temperature in
+ * the array that is negative or not finite, NaN.  vocab <= 2^26.
+ */
+int klp_sample(const void* logits, int dtype, int64_t n_rows, int64_t vocab, int64_t rows_inner,
+               int64_t stride_outer, int64_t stride_inner, const float* uniform,
+               float temperature, const float* temperatures, int32_t top_k, const int32_t* top_ks,
+               float top_p, const float* top_ps, float min_p, const float* min_ps,
+               int64_t* tokens, float* logp, float* sample_logp, void* stream);
+
+/*
  * Test hook with no counterpart in the reference: the next `count` compute
  * calls on the calling thread return KLP_ELAUNCH without launching anything,
  * as if hipGetLastError() had reported a failure.  Lets the error path be
