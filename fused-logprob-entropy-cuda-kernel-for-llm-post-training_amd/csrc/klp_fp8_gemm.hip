@@ -388,7 +388,10 @@ __global__ __launch_bounds__(kTileThreads, 2) void klp_fp8_tile_kernel(Fp8Linear
     };
     int64_t wrow = v0 + wv * (16 * VB);
     if (wrow >= p.n) wrow = 0;  // a wave past the weight: its outputs are not stored
-    const float* ws = p.ws + wrow / kScaleBlock * p.n_blocks;
+    // Constant memory: a scalar load.  A vector load's wait would also wait for
+    // the copies before it.
+    typedef __attribute__((address_space(4))) const float const_float;
+    const const_float* ws = (const const_float*)(uintptr_t)(p.ws + wrow / kScaleBlock * p.n_blocks);
 
     f32x4 acc[VB][MB];
 #pragma unroll
@@ -415,7 +418,11 @@ __global__ __launch_bounds__(kTileThreads, 2) void klp_fp8_tile_kernel(Fp8Linear
         f[j] = read_s(0, j);
     }
     float g = ws[0];
-    f32x4 c[2];
+    // The sums of a matrix instruction are scaled and added kLag instructions
+    // later: 2 (4 + 1) + 1 instructions lie between, the 11 wait states of an
+    // 8-pass instruction's result.
+    constexpr int kLag = 3;
+    f32x4 c[kLag + 1];
     int slot = 0;
     for (int b = 0; b < nb; ++b) {
         const float g_next = ws[b + 1 < nb ? b + 1 : b];
@@ -426,13 +433,14 @@ __global__ __launch_bounds__(kTileThreads, 2) void klp_fp8_tile_kernel(Fp8Linear
         auto fold = [&](int q) {
             const int i = q / MB, j = q % MB;
 #pragma unroll
-            for (int r = 0; r < 4; ++r) acc[i][j][r] = fmaf(c[q & 1][r], f[j], acc[i][j][r]);
+            for (int r = 0; r < 4; ++r)
+                acc[i][j][r] = fmaf(c[q % (kLag + 1)][r], f[j], acc[i][j][r]);
         };
+        constexpr int kMeet = (VB - 1) * MB;  // matrix instructions before the barrier
 #pragma unroll
         for (int q = 0; q < VB * MB; ++q) {
             const int i = q / MB, j = q % MB;
-            if (j == 0 && i + 1 < VB) av[(i + 1) & 1] = read_v(slot, i + 1);
-            if (q == (VB - 1) * MB) {
+            if (q == kMeet) {
                 // The stage is read (the last operands are waited for here);
                 // the next one has landed.
                 pin();
@@ -440,21 +448,24 @@ __global__ __launch_bounds__(kTileThreads, 2) void klp_fp8_tile_kernel(Fp8Linear
                 __builtin_amdgcn_s_barrier();
                 pin();
                 slot ^= 1;
-                av[(i + 1) & 1] = read_v(slot, 0);
-#pragma unroll
-                for (int z = 0; z < MB; ++z) f_next[z] = read_s(slot, z);
             }
-            c[q & 1] = mul_block(av[i & 1], bv[j]);
-            if (q > 0) fold(q - 1);
-            if (i == VB - 1) bv[j] = read_m(slot, j);
+            c[q % (kLag + 1)] = mul_block(av[i & 1], bv[j]);
+            pin();
+            if (j == 0) av[(i + 1) & 1] = read_v(slot, (i + 1) % VB);
+            if (i == VB - 1) {
+                bv[j] = read_m(slot, j);
+                f_next[j] = read_s(slot, j);
+#pragma unroll
+                for (int z = 0; z < Shape::kCopies; ++z)
+                    if (z * MB / Shape::kCopies == j) copy(z);
+            }
+            if (q >= kLag) fold(q - kLag);
             pin();
         }
-        fold(VB * MB - 1);
+#pragma unroll
+        for (int z = VB * MB - kLag; z < VB * MB; ++z) fold(z);
 #pragma unroll
         for (int j = 0; j < MB; ++j) f[j] = f_next[j];
-#pragma unroll
-        for (int j = 0; j < Shape::kCopies; ++j) copy(j);
-        pin();
     }
     // The last copies write zeros to LDS: before the workgroup gives it up.
     __builtin_amdgcn_s_waitcnt(waitcnt(0, 15));
