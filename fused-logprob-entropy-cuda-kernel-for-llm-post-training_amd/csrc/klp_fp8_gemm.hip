@@ -258,11 +258,14 @@ __global__ __launch_bounds__(256, 2) void klp_fp8_stream_kernel(Fp8LinearParams 
 // the tokens' scales of the block behind them.  A wave reads 16 VB weight rows
 // and 16 MB token rows a stage.
 //
-// A stage's last reads are done two rows of blocks before its last matrix
-// instructions.  There the workgroup meets: every wave has read the stage, and
-// its copies of the next one have landed.  Behind that barrier the copies of
-// the stage after the next start, into the slots just read, and the next
-// stage's first operands are read under the remaining matrix instructions.
+// A stage's token rows are held in registers, its weight rows read as they are
+// needed.  Twice a stage the workgroup meets, each time before the last row of
+// blocks of a half: every wave has then read that half's weight rows (and, at
+// the first meeting, the token rows, long since).  Behind the first meeting
+// go the copies of the first half's weight rows and the token rows of the
+// stage after the next, into the slots just read; behind the second those of
+// the second half's weight rows.  The meetings wait for the copies that the
+// next half reads, which were started one and a half stages before.
 template <int VB_, int MB_, int kTokenWaves_>
 struct TileShape {
     static constexpr int VB = VB_, MB = MB_, kTokenWaves = kTokenWaves_;
@@ -273,9 +276,10 @@ struct TileShape {
     static constexpr int kSlotM = kRowsM * kK;
     static constexpr int kSlotS = kRowsM * 4;
     static constexpr int kLds = 2 * (kSlotV + kSlotM + kSlotS);
-    static constexpr int kCopiesV = kRowsV / 64;  // of 1 KB, a wave
+    static constexpr int kHalfV = kRowsV / 128;  // copies of 1 KB, a wave
     static constexpr int kCopiesM = kRowsM / 64;
-    static constexpr int kCopies = kCopiesV + kCopiesM + 1;
+    static constexpr int kFirst = kHalfV + kCopiesM + 1;
+    static constexpr int kSecond = kHalfV;
 };
 constexpr int kTileThreads = 512;
 
@@ -318,17 +322,18 @@ __global__ __launch_bounds__(kTileThreads, 2) void klp_fp8_tile_kernel(Fp8Linear
     const int rows_m = static_cast<int>(p.m - t0 < Shape::kRowsM ? p.m - t0 : Shape::kRowsM);
     const int nb = static_cast<int>(p.n_blocks);
 
-    // Copy j of wave w fills slot rows 64 j + 8 w .. + 7: lane l chunk l % 8
-    // of row l / 8, which holds the row's chunk (l % 8) ^ swz(row).
+    // A copy fills 8 slot rows: lane l chunk l % 8 of row l / 8, which holds
+    // the row's chunk (l % 8) ^ swz(row).  Token rows: copy j of wave w rows
+    // 64 j + 8 w.  Weight rows: a half is 8 VB rows of each of the 16 VB that
+    // a vocabulary wave reads, copy j of wave w takes rows 128 j + wrow of it.
     constexpr uint32_t kNowhere = 0x80000000u;  // past every descriptor
     const int crow = wave * 8 + (lane >> 3);
     const int cchunk = (lane & 7) ^ swz(crow);
+    const int wrow = wave / VB * (16 * VB) + wave % VB * 8;
+    static_assert(VB == 4 || VB == 8, "8 waves fill 128 rows' half");
     const uint32_t ld_v = static_cast<uint32_t>(p.ld_w), ld_m = static_cast<uint32_t>(p.ld_x);
-    const uint32_t off_v = crow * ld_v + cchunk * 16;
-    const uint32_t off_m = crow * ld_m + cchunk * 16;
     constexpr int kScaleWaves = Shape::kRowsM / 64;  // the others copy the same again
     const uint32_t stok = static_cast<uint32_t>((wave % kScaleWaves) * 64 + lane);
-    const uint32_t off_s = stok * static_cast<uint32_t>(nb) * 4;
     const uint32_t lds0 = static_cast<uint32_t>(reinterpret_cast<uintptr_t>((lds_void*)lds));
 
     // Copies of block b into slot b % 2.  Chunks past K, and all of a block
@@ -337,33 +342,34 @@ __global__ __launch_bounds__(kTileThreads, 2) void klp_fp8_tile_kernel(Fp8Linear
     const u32x4 rs_v = bytes_rsrc(p.w + v0 * p.ld_w, (rows_v - 1) * ld_v + static_cast<uint32_t>(p.k));
     const u32x4 rs_m = bytes_rsrc(p.x + t0 * p.ld_x, (rows_m - 1) * ld_m + static_cast<uint32_t>(p.k));
     const u32x4 rs_s = bytes_rsrc(p.xs + t0 * p.n_blocks, static_cast<uint32_t>(rows_m) * nb * 4);
-    int c_block = 0, c_slot = 0;
-    uint32_t cv = off_v, cm = off_m, cs = off_s;  // of block c_block
-    auto close = [&]() {  // K's end
-        const int64_t at = static_cast<int64_t>(c_block) * kK + cchunk * 16;
-        if (at >= p.k) cv = cm = kNowhere;
-        if (c_block >= nb) cs = kNowhere;
+    const uint32_t lane_v = static_cast<uint32_t>(wrow + (lane >> 3)) * ld_v + cchunk * 16;
+    const uint32_t lane_m = static_cast<uint32_t>(crow) * ld_m + cchunk * 16;
+    const uint32_t lane_s = stok * static_cast<uint32_t>(nb) * 4;
+    const int chunks = static_cast<int>((p.k - cchunk * 16 + kK - 1) / kK);  // blocks with this chunk
+    int block[2] = {0, 0};  // the first and second copies' next
+    auto copy_v = [&](int half, int j) {
+        const int b = block[half];
+        copy_to_lds(rs_v, lds0 + (b & 1) * Shape::kSlotV + (wrow + 128 * j + 8 * VB * half) * kK,
+                    b < chunks ? lane_v + (128 * j + 8 * VB * half) * ld_v + b * kK : kNowhere, 0);
     };
-    close();
-    auto copy = [&](int j) {
-        if (j < Shape::kCopiesV) {
-            copy_to_lds(rs_v, lds0 + c_slot * Shape::kSlotV + (wave + 8 * j) * 1024,
-                        cv + j * 64 * ld_v, 0);
-        } else if (j < Shape::kCopiesV + Shape::kCopiesM) {
-            const int i = j - Shape::kCopiesV;
-            copy_to_lds(rs_m, lds0 + kAt_m + c_slot * Shape::kSlotM + (wave + 8 * i) * 1024,
-                        cm + i * 64 * ld_m, 0);
+    auto copy_first = [&](int z) {
+        const int b = block[0];
+        if (z < Shape::kHalfV) {
+            copy_v(0, z);
+        } else if (z < Shape::kHalfV + Shape::kCopiesM) {
+            const int j = z - Shape::kHalfV;
+            copy_to_lds(rs_m, lds0 + kAt_m + (b & 1) * Shape::kSlotM + (wave + 8 * j) * 1024,
+                        b < chunks ? lane_m + j * 64 * ld_m + b * kK : kNowhere, 0);
         } else {
-            copy_dwords_to_lds(rs_s, lds0 + kAt_s + c_slot * Shape::kSlotS +
+            copy_dwords_to_lds(rs_s, lds0 + kAt_s + (b & 1) * Shape::kSlotS +
                                          (wave % kScaleWaves) * 256,
-                               cs);
-            ++c_block;
-            c_slot ^= 1;
-            cv += kK;
-            cm += kK;
-            cs += 4;
-            close();
+                               b < nb ? lane_s + b * 4 : kNowhere);
+            ++block[0];
         }
+    };
+    auto copy_second = [&](int z) {
+        copy_v(1, z);
+        if (z == Shape::kSecond - 1) ++block[1];
     };
 
     // Operands: lane l holds row l % 16 of a block, chunks l / 16 and 4 + l / 16.
@@ -386,12 +392,12 @@ __global__ __launch_bounds__(kTileThreads, 2) void klp_fp8_tile_kernel(Fp8Linear
         return *reinterpret_cast<const float*>(lds + kAt_s + slot * Shape::kSlotS +
                                                (wm * 16 * MB + 16 * j + lrow) * 4);
     };
-    int64_t wrow = v0 + wv * (16 * VB);
-    if (wrow >= p.n) wrow = 0;  // a wave past the weight: its outputs are not stored
+    int64_t first_row = v0 + wv * (16 * VB);
+    if (first_row >= p.n) first_row = 0;  // a wave past the weight: its outputs are not stored
     // Constant memory: a scalar load.  A vector load's wait would also wait for
     // the copies before it.
     typedef __attribute__((address_space(4))) const float const_float;
-    const const_float* ws = (const const_float*)(uintptr_t)(p.ws + wrow / kScaleBlock * p.n_blocks);
+    const const_float* ws = (const const_float*)(uintptr_t)(p.ws + first_row / kScaleBlock * p.n_blocks);
 
     f32x4 acc[VB][MB];
 #pragma unroll
@@ -400,13 +406,20 @@ __global__ __launch_bounds__(kTileThreads, 2) void klp_fp8_tile_kernel(Fp8Linear
         for (int j = 0; j < MB; ++j) acc[i][j] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
 
 #pragma unroll
-    for (int j = 0; j < Shape::kCopies; ++j) copy(j);
+    for (int b = 0; b < 2; ++b) {
 #pragma unroll
-    for (int j = 0; j < Shape::kCopies; ++j) copy(j);
-    pin();
-    __builtin_amdgcn_s_waitcnt(waitcnt(Shape::kCopies, 15));
-    __builtin_amdgcn_s_barrier();
-    pin();
+        for (int z = 0; z < Shape::kFirst; ++z) copy_first(z);
+#pragma unroll
+        for (int z = 0; z < Shape::kSecond; ++z) copy_second(z);
+    }
+    constexpr int kStage = Shape::kFirst + Shape::kSecond;
+    auto meet = [&](auto in_flight) {
+        pin();
+        __builtin_amdgcn_s_waitcnt(waitcnt(decltype(in_flight)::value, 0));
+        __builtin_amdgcn_s_barrier();
+        pin();
+    };
+    meet(std::integral_constant<int, kStage + Shape::kSecond>{});
 
     typedef Operand<DT == kFP32> Op;
     Op av[2], bv[MB];
@@ -422,6 +435,8 @@ __global__ __launch_bounds__(kTileThreads, 2) void klp_fp8_tile_kernel(Fp8Linear
     // later: 2 (4 + 1) + 1 instructions lie between, the 11 wait states of an
     // 8-pass instruction's result.
     constexpr int kLag = 3;
+    constexpr int kSteps = VB * MB, kMeet = kSteps - MB, kMid = kSteps / 2 - MB;
+    static_assert(kMid + Shape::kFirst <= kMeet && Shape::kSecond <= MB, "before the next meeting");
     f32x4 c[kLag + 1];
     int slot = 0;
     for (int b = 0; b < nb; ++b) {
@@ -436,34 +451,25 @@ __global__ __launch_bounds__(kTileThreads, 2) void klp_fp8_tile_kernel(Fp8Linear
             for (int r = 0; r < 4; ++r)
                 acc[i][j][r] = fmaf(c[q % (kLag + 1)][r], f[j], acc[i][j][r]);
         };
-        constexpr int kMeet = (VB - 1) * MB;  // matrix instructions before the barrier
 #pragma unroll
-        for (int q = 0; q < VB * MB; ++q) {
+        for (int q = 0; q < kSteps; ++q) {
             const int i = q / MB, j = q % MB;
-            if (q == kMeet) {
-                // The stage is read (the last operands are waited for here);
-                // the next one has landed.
-                pin();
-                __builtin_amdgcn_s_waitcnt(waitcnt(0, 0));
-                __builtin_amdgcn_s_barrier();
-                pin();
-                slot ^= 1;
-            }
+            if (q == kMid || q == kMeet) meet(std::integral_constant<int, kStage>{});
+            if (q == kMeet) slot ^= 1;
             c[q % (kLag + 1)] = mul_block(av[i & 1], bv[j]);
             pin();
             if (j == 0) av[(i + 1) & 1] = read_v(slot, (i + 1) % VB);
             if (i == VB - 1) {
                 bv[j] = read_m(slot, j);
                 f_next[j] = read_s(slot, j);
-#pragma unroll
-                for (int z = 0; z < Shape::kCopies; ++z)
-                    if (z * MB / Shape::kCopies == j) copy(z);
             }
+            if (q >= kMid && q - kMid < Shape::kFirst) copy_first(q - kMid);
+            if (q >= kMeet && q - kMeet < Shape::kSecond) copy_second(q - kMeet);
             if (q >= kLag) fold(q - kLag);
             pin();
         }
 #pragma unroll
-        for (int z = VB * MB - kLag; z < VB * MB; ++z) fold(z);
+        for (int z = kSteps - kLag; z < kSteps; ++z) fold(z);
 #pragma unroll
         for (int j = 0; j < MB; ++j) f[j] = f_next[j];
     }
