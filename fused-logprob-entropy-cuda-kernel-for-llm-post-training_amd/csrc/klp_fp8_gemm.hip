@@ -110,31 +110,24 @@ __device__ __forceinline__ void store4(typename Traits<DT>::elem* p, int64_t lef
     }
 }
 
-// Few tokens: a wave streams 16 VB rows of the weight against 16 MB tokens,
-// both straight from memory to registers (the tokens' rows stay in the
-// caches).  kSplit waves of a workgroup share those rows' K; their sums meet
-// in LDS and are added in order.
-template <int DT, int MB, int VB, int kSplit, bool kExact>
-__global__ __launch_bounds__(256, 2) void klp_fp8_stream_kernel(Fp8LinearParams p) {
-    __shared__ f32x4 part[kSplit > 1 ? (kSplit - 1) * MB * VB * 64 : 1];
+// Small products: a workgroup's waves share the K of 16 weight rows and 16 MB
+// tokens, both straight from memory to registers (the tokens' rows stay in the
+// caches); their sums meet in LDS and are added in order.
+constexpr int kSplit = 4;
+template <int DT, int MB, bool kExact>
+__global__ __launch_bounds__(64 * kSplit) void klp_fp8_stream_kernel(Fp8LinearParams p) {
+    __shared__ f32x4 part[(kSplit - 1) * MB * 64];
     const int lane = threadIdx.x & 63;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int64_t tile = kSplit > 1 ? static_cast<int64_t>(blockIdx.x)
-                                    : static_cast<int64_t>(blockIdx.x) * 4 + wave;
-    const int64_t v0 = tile * 16 * VB;
+    const int64_t v0 = static_cast<int64_t>(blockIdx.x) * 16;
     const int64_t t0 = static_cast<int64_t>(blockIdx.y) * 16 * MB;
-    if (v0 >= p.n) return;  // a whole wave; with kSplit > 1 a whole workgroup
     const int lrow = lane & 15, lq = lane >> 4;
 
     // Rows past the end repeat the last one; their outputs are not stored.
-    const uint8_t* w[VB];
+    const int64_t wrow = v0 + lrow < p.n ? v0 + lrow : p.n - 1;
+    const uint8_t* w = p.w + wrow * p.ld_w + 16 * lq;
     const uint8_t* x[MB];
     const float* xs[MB];
-#pragma unroll
-    for (int i = 0; i < VB; ++i) {
-        const int64_t r = v0 + 16 * i + lrow;
-        w[i] = p.w + (r < p.n ? r : p.n - 1) * p.ld_w + 16 * lq;
-    }
 #pragma unroll
     for (int j = 0; j < MB; ++j) {
         const int64_t r = t0 + 16 * j + lrow;
@@ -145,34 +138,25 @@ __global__ __launch_bounds__(256, 2) void klp_fp8_stream_kernel(Fp8LinearParams 
     const float* ws = p.ws + v0 / kScaleBlock * p.n_blocks;
 
     const int nb = static_cast<int>(p.n_blocks);
-    const int first = kSplit > 1 ? nb * wave / kSplit : 0;
-    const int end = kSplit > 1 ? nb * (wave + 1) / kSplit : nb;
-    f32x4 acc[VB][MB];
+    const int first = static_cast<int>(static_cast<int64_t>(nb) * wave / kSplit);
+    const int end = static_cast<int>(static_cast<int64_t>(nb) * (wave + 1) / kSplit);
+    f32x4 acc[MB];
 #pragma unroll
-    for (int i = 0; i < VB; ++i)
-#pragma unroll
-        for (int j = 0; j < MB; ++j) acc[i][j] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+    for (int j = 0; j < MB; ++j) acc[j] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
 
-    auto fold = [&](const i32x8 (&a)[VB], const i32x8 (&b)[MB], const float (&s)[MB], float g) {
-        Operand<kExact> row[VB];
-#pragma unroll
-        for (int i = 0; i < VB; ++i) row[i] = Operand<kExact>::from(a[i]);
+    auto fold = [&](i32x8 a, const i32x8 (&b)[MB], const float (&s)[MB], float g) {
+        const Operand<kExact> row = Operand<kExact>::from(a);
 #pragma unroll
         for (int j = 0; j < MB; ++j) {
+            const f32x4 c = mul_block(row, Operand<kExact>::from(b[j]));
             const float f = s[j] * g;
-            const Operand<kExact> token = Operand<kExact>::from(b[j]);
 #pragma unroll
-            for (int i = 0; i < VB; ++i) {
-                const f32x4 c = mul_block(row[i], token);
-#pragma unroll
-                for (int r = 0; r < 4; ++r) acc[i][j][r] = fmaf(c[r], f, acc[i][j][r]);
-            }
+            for (int r = 0; r < 4; ++r) acc[j][r] = fmaf(c[r], f, acc[j][r]);
         }
     };
-    auto load = [&](int b, i32x8 (&a)[VB], i32x8 (&c)[MB], float (&s)[MB], float& g) {
+    auto load = [&](int b, i32x8& a, i32x8 (&c)[MB], float (&s)[MB], float& g) {
         const int64_t k0 = static_cast<int64_t>(b) * kK;
-#pragma unroll
-        for (int i = 0; i < VB; ++i) a[i] = load_operand(w[i], k0);
+        a = load_operand(w, k0);
 #pragma unroll
         for (int j = 0; j < MB; ++j) {
             c[j] = load_operand(x[j], k0);
@@ -184,7 +168,7 @@ __global__ __launch_bounds__(256, 2) void klp_fp8_stream_kernel(Fp8LinearParams 
     // Whole blocks, the next one's loads in flight; then K's last part.
     const int whole = static_cast<int>(p.k / kK);
     const int stop = end < whole ? end : whole;
-    i32x8 a[2][VB], c[2][MB];
+    i32x8 a[2], c[2][MB];
     float s[2][MB], g[2];
     int b = first;
     if (b < stop) {
@@ -206,8 +190,7 @@ __global__ __launch_bounds__(256, 2) void klp_fp8_stream_kernel(Fp8LinearParams 
     if (end > whole) {
         const int64_t k0 = static_cast<int64_t>(whole) * kK;
         const int64_t left = p.k - 16 * lq;  // the rows' pointers start at 16 lq
-#pragma unroll
-        for (int i = 0; i < VB; ++i) a[0][i] = load_operand_tail(w[i], k0, left);
+        a[0] = load_operand_tail(w, k0, left);
 #pragma unroll
         for (int j = 0; j < MB; ++j) {
             c[0][j] = load_operand_tail(x[j], k0, left);
@@ -216,39 +199,23 @@ __global__ __launch_bounds__(256, 2) void klp_fp8_stream_kernel(Fp8LinearParams 
         fold(a[0], c[0], s[0], ws[whole]);
     }
 
-    if constexpr (kSplit > 1) {
-        if (wave > 0) {
+    if (wave > 0) {
 #pragma unroll
-            for (int i = 0; i < VB; ++i)
-#pragma unroll
-                for (int j = 0; j < MB; ++j)
-                    part[((wave - 1) * VB * MB + i * MB + j) * 64 + lane] = acc[i][j];
-        }
-        __syncthreads();
-        if (wave > 0) return;
-#pragma unroll
-        for (int z = 0; z < kSplit - 1; ++z)
-#pragma unroll
-            for (int i = 0; i < VB; ++i)
-#pragma unroll
-                for (int j = 0; j < MB; ++j) {
-                    const f32x4 o = part[(z * VB * MB + i * MB + j) * 64 + lane];
-#pragma unroll
-                    for (int r = 0; r < 4; ++r) acc[i][j][r] += o[r];
-                }
+        for (int j = 0; j < MB; ++j) part[((wave - 1) * MB + j) * 64 + lane] = acc[j];
     }
+    __syncthreads();
+    if (wave > 0) return;
+#pragma unroll
+    for (int z = 0; z < kSplit - 1; ++z)
+#pragma unroll
+        for (int j = 0; j < MB; ++j) acc[j] += part[(z * MB + j) * 64 + lane];
 
     typedef typename Traits<DT>::elem elem;
 #pragma unroll
     for (int j = 0; j < MB; ++j) {
         const int64_t m = t0 + 16 * j + lrow;
-        if (m >= p.m) continue;
-        elem* out = static_cast<elem*>(p.out) + m * p.ld_out;
-#pragma unroll
-        for (int i = 0; i < VB; ++i) {
-            const int64_t n = v0 + 16 * i + 4 * lq;
-            store4<DT>(out + n, p.n - n, acc[i][j]);
-        }
+        const int64_t n = v0 + 4 * lq;
+        if (m < p.m) store4<DT>(static_cast<elem*>(p.out) + m * p.ld_out + n, p.n - n, acc[j]);
     }
 }
 
@@ -276,6 +243,8 @@ struct TileShape {
     static constexpr int kSlotM = kRowsM * kK;
     static constexpr int kSlotS = kRowsM * 4;
     static constexpr int kLds = 2 * (kSlotV + kSlotM + kSlotS);
+    // Registers for two workgroups a CU (float32 outputs' operands need more).
+    static constexpr bool kSmall = VB * MB <= 8;
     static constexpr int kHalfV = kRowsV / 128;  // copies of 1 KB, a wave
     static constexpr int kCopiesM = kRowsM / 64;
     static constexpr int kFirst = kHalfV + kCopiesM + 1;
@@ -292,7 +261,7 @@ __device__ __forceinline__ void copy_dwords_to_lds(u32x4 rsrc, uint32_t lds, uin
 }
 
 template <int DT, typename Shape>
-__global__ __launch_bounds__(kTileThreads, 2) void klp_fp8_tile_kernel(Fp8LinearParams p) {
+__global__ __launch_bounds__(kTileThreads, Shape::kSmall && DT != kFP32 ? 4 : 2) void klp_fp8_tile_kernel(Fp8LinearParams p) {
     using namespace mfma;
     constexpr int VB = Shape::VB, MB = Shape::MB;
     __shared__ __attribute__((aligned(1024))) unsigned char lds[Shape::kLds];
@@ -436,7 +405,8 @@ __global__ __launch_bounds__(kTileThreads, 2) void klp_fp8_tile_kernel(Fp8Linear
     // 8-pass instruction's result.
     constexpr int kLag = 3;
     constexpr int kSteps = VB * MB, kMeet = kSteps - MB, kMid = kSteps / 2 - MB;
-    static_assert(kMid + Shape::kFirst <= kMeet && Shape::kSecond <= MB, "before the next meeting");
+    static_assert(Shape::kSecond <= MB, "before the next meeting");
+    constexpr bool kFits = kMid + Shape::kFirst <= kMeet;  // a copy an instruction
     f32x4 c[kLag + 1];
     int slot = 0;
     for (int b = 0; b < nb; ++b) {
@@ -463,7 +433,9 @@ __global__ __launch_bounds__(kTileThreads, 2) void klp_fp8_tile_kernel(Fp8Linear
                 bv[j] = read_m(slot, j);
                 f_next[j] = read_s(slot, j);
             }
-            if (q >= kMid && q - kMid < Shape::kFirst) copy_first(q - kMid);
+#pragma unroll
+            for (int z = 0; z < Shape::kFirst; ++z)
+                if (q == kMid + (kFits ? z : z * (kMeet - kMid) / Shape::kFirst)) copy_first(z);
             if (q >= kMeet && q - kMeet < Shape::kSecond) copy_second(q - kMeet);
             if (q >= kLag) fold(q - kLag);
             pin();
@@ -498,39 +470,68 @@ hipError_t launch_tile(const Fp8LinearParams& p, hipStream_t stream) {
     return launch_kernel(klp_fp8_tile_kernel<DT, Shape>, grid, dim3(kTileThreads), stream, p);
 }
 
-#ifndef KLP_EX
-#define KLP_EX false
-#endif
-template <int DT> constexpr bool kStreamExact = DT == kFP32 || KLP_EX;
-
-template <int DT, int MB, int VB, int kSplit>
+template <int DT, int MB>
 hipError_t launch_stream(const Fp8LinearParams& p, hipStream_t stream) {
-    const int64_t tiles = (p.n + 16 * VB - 1) / (16 * VB);
-    const dim3 grid(static_cast<unsigned>(kSplit > 1 ? tiles : (tiles + 3) / 4),
+    const dim3 grid(static_cast<unsigned>((p.n + 15) / 16),
                     static_cast<unsigned>((p.m + 16 * MB - 1) / (16 * MB)));
-    return launch_kernel(klp_fp8_stream_kernel<DT, MB, VB, kSplit, kStreamExact<DT>>, grid,
-                         dim3(256), stream, p);
+    return launch_kernel(klp_fp8_stream_kernel<DT, MB, DT == kFP32>, grid, dim3(256), stream, p);
 }
 
-template <int DT, int VB, int kSplit>
-hipError_t launch_stream_tokens(const Fp8LinearParams& p, hipStream_t stream) {
-    if (p.m <= 16) return launch_stream<DT, 1, VB, kSplit>(p, stream);
-    if (p.m <= 32) return launch_stream<DT, 2, VB, kSplit>(p, stream);
-    return launch_stream<DT, 4, VB == 1 ? 1 : 2, kSplit>(p, stream);
+template <typename Shape>
+int64_t tiles_of(const Fp8LinearParams& p) {
+    return ((p.n + Shape::kRowsV - 1) / Shape::kRowsV) * ((p.m + Shape::kRowsM - 1) / Shape::kRowsM);
+}
+// Rounds of one tile a CU, times a round's time.
+template <typename Shape>
+int64_t cost_of(const Fp8LinearParams& p, int round) {
+    return (tiles_of<Shape>(p) + kHeadGemmCus - 1) / kHeadGemmCus * round;
 }
 
+// Tiles of 256 x 256, 256 x 128, 128 x 128 and 128 x 64 (weight rows x
+// tokens) take 64, 39, 25 and 18 us a round at k = 4096: the wider a tile, the
+// fewer bytes it moves through LDS for its products, the narrower, the more
+// CUs a small product fills.  (us, bf16 out:)
+//   m     n       k       256x256  256x128  128x128  128x64  split
+//   16    152064  3584    128      108      104      100     137
+//   64    152064  3584    143      124      124      122     322
+//   128   152064  3584    171      148      164      193     633
+//   256   152064  3584    197      218      260              1250
+//   512   152064  3584    319      403      452              2493
+//   64    32000   4096    44       28       23       23      90
+//   256   32000   4096    56       40       51       68      351
+//   1024  32000   4096    133      149      192              1362
+//   512   4096    4096    50       33       25       21      90
+//   1024  4096    4096    51       33       27       35      177
+//   2048  4096    4096    52       40       49       67      351
+//   64    4096    4096    42       27       20       18      14.6
+//   16    8192    8192             47       34       32      19
+//   512   512     4096    47       29       20       18      14
+// With at most 4 blocks of 16 x 16 outputs a CU, splitting their K over a
+// workgroup's waves is faster than any tile.
 template <int DT>
 hipError_t launch_fp8_linear_dt(const Fp8LinearParams& p, hipStream_t stream) {
     // 32-bit offsets within a tile's rows.
     const bool near = p.ld_x <= kFp8TileMaxStride && p.ld_w <= kFp8TileMaxStride;
-    if (near && p.m > 128) {
-        // Registers: the exact operands are twice as large.
-        if constexpr (DT != kFP32) return launch_tile<DT, TileShape<8, 4, 4>>(p, stream);
+    if (!near || ((p.n + 15) / 16) * ((p.m + 15) / 16) <= 4 * kHeadGemmCus) {
+        if (p.m <= 16) return launch_stream<DT, 1>(p, stream);
+        if (p.m <= 32) return launch_stream<DT, 2>(p, stream);
+        return launch_stream<DT, 4>(p, stream);
     }
-    if (near && p.m > 64) return launch_tile<DT, TileShape<4, 4, 2>>(p, stream);
-    // Too few waves of 64 rows to fill the chip: 16 rows, K split four ways.
-    if (p.n < 64 * 1024) return launch_stream_tokens<DT, 1, 4>(p, stream);
-    return launch_stream_tokens<DT, 4, 1>(p, stream);
+    typedef TileShape<8, 4, 4> Wide;
+    typedef TileShape<4, 4, 2> Half;
+    typedef TileShape<4, 2, 4> Square;
+    typedef TileShape<4, 1, 4> Narrow;
+    const int64_t half = cost_of<Half>(p, 39), square = cost_of<Square>(p, 25),
+                  narrow = cost_of<Narrow>(p, 18);
+    // The exact operands of a 256 x 256 tile do not fit the registers.
+    if constexpr (DT != kFP32) {
+        const int64_t wide = cost_of<Wide>(p, 64);
+        if (wide <= half && wide <= square && wide <= narrow)
+            return launch_tile<DT, Wide>(p, stream);
+    }
+    if (half <= square && half <= narrow) return launch_tile<DT, Half>(p, stream);
+    if (square <= narrow) return launch_tile<DT, Square>(p, stream);
+    return launch_tile<DT, Narrow>(p, stream);
 }
 
 }  // namespace

@@ -101,8 +101,7 @@ def _bound(ref, size, dropped, k, dtype):
     off by at most a rounding an addition (2^-23, half a step or a truncation),
     the scales' product and the multiply-add to the accumulator round once a
     block each: (128 + 2 blocks) 2^-23 of the terms' magnitudes.  16-bit
-    outputs of more than 64 tokens come from the e4m3 instruction, which drops
-    from each of 8 neighbouring products what lies below 2^-13 of 2^E, E the
+    outputs come from the e4m3 instruction, which drops from each of 8 neighbouring products what lies below 2^-13 of 2^E, E the
     largest exponent sum of the 8: that product itself, 6 bits behind its
     leading one, loses nothing, the other 7 less than 2^-13 2^E <= 2^-13 of it
     each (`dropped`: the sum of the groups' largest products).  The output
@@ -119,8 +118,6 @@ def _bound(ref, size, dropped, k, dtype):
 def _check_linear(out, xq, xs, wq, ws):
     ref, size, dropped = fp8_oracle.linear(fp8_oracle.decode(_codes(xq)), xs.cpu().numpy(),
                                            fp8_oracle.decode(_codes(wq)), ws.cpu().numpy())
-    if out.size(0) <= 64:
-        dropped = 0.0
     got = out.double().cpu().numpy()
     bound = _bound(ref, size, dropped, xq.size(1), out.dtype)
     over = np.abs(got - ref) > bound
@@ -128,14 +125,21 @@ def _check_linear(out, xq, xs, wq, ws):
         int(over.sum()), np.argwhere(over)[:3].tolist(), float(np.abs(got - ref).max()))
 
 
-# Both kernels: up to 64 tokens (stream, 16 / 32 / 64 at a time, with and
-# without a split K), up to 128 and above (tiles); token, row and K counts
-# around the tiles' sides.
+# Every kernel: small products split over K (16, 32 or 64 tokens at a time) and
+# the four tiles (tokens x weight rows 64 x 128, 128 x 128, 128 x 256, and, but
+# for float32 outputs, 256 x 256); token, row and K counts around their sides.
 @pytest.mark.parametrize("m,n,k", [
+    # split
     (1, 1, 16), (1, 512, 128), (3, 129, 144), (16, 1000, 272), (17, 257, 1024), (33, 640, 3584),
-    (64, 65, 48), (1, 65536, 256), (20, 65600, 144), (64, 65537, 400),
-    (65, 300, 128), (127, 513, 656), (128, 1024, 3584), (129, 255, 16), (200, 2050, 272),
-    (256, 256, 1040), (300, 1537, 512), (515, 4100, 400),
+    (64, 65, 48), (129, 255, 16), (256, 256, 1040),
+    # 64 x 128
+    (1, 65536, 256), (20, 65600, 144), (64, 65537, 400), (65, 3001, 128), (300, 1537, 512),
+    # 128 x 128
+    (128, 20000, 272), (127, 17025, 656),
+    # 128 x 256
+    (130, 25000, 144), (255, 25090, 16),
+    # 256 x 256
+    (500, 30001, 144), (257, 40000, 400),
 ])
 @pytest.mark.parametrize("dtype", DTYPES, ids=IDS)
 def test_linear(m, n, k, dtype):
@@ -146,11 +150,11 @@ def test_linear(m, n, k, dtype):
     _check_linear(out, xq, xs, wq, ws)
 
 
-@pytest.mark.parametrize("m", [5, 100, 300])
-def test_linear_layouts(m):
+@pytest.mark.parametrize("m,n", [(5, 300), (100, 8300), (300, 8300), (500, 30001)])
+def test_linear_layouts(m, n):
     """Row strides above K on both sides, leading dims, scales in another
     order in memory; what lies behind the rows' K (NaN codes) never enters."""
-    n, k = 300, 208
+    k = 208
     xq, xs, wq, ws = _matrices(m, n, k, 11)
     want = _ko().fp8_linear(xq, xs, wq, ws)
     xb = torch.full((m, k + 48), 0x7F, dtype=torch.uint8, device=DEV)
@@ -166,11 +170,11 @@ def test_linear_layouts(m):
         assert got.shape == (4, m // 4, n) and torch.equal(got.view(m, n), want)
 
 
-@pytest.mark.parametrize("m", [1, 64, 96, 260])
-def test_linear_nan_and_zero_scales(m):
+@pytest.mark.parametrize("m,n", [(1, 384), (64, 384), (96, 8320), (260, 8320)])
+def test_linear_nan_and_zero_scales(m, n):
     """A NaN code or scale enters its outputs and no others; a scale of zero
     takes its block away."""
-    n, k = 384, 400
+    k = 400
     xq, xs, wq, ws = _matrices(m, n, k, 5)
     xs, ws = xs.clone(), ws.clone()
     xs[0, 1] = 0.0
@@ -194,8 +198,8 @@ def test_linear_writes_its_rows_only():
     """Through the C entry: an output with a row stride above n keeps what lies
     behind each row and behind the last one."""
     from kernel_opt._library import check_status, lib, ptr, stream_handle
-    for m in (3, 70, 150):
-        n, k = 261, 144
+    k = 144
+    for m, n in ((3, 261), (70, 8197), (150, 8197), (150, 25001), (500, 30001)):
         xq, xs, wq, ws = _matrices(m, n, k, 9)
         want = _ko().fp8_linear(xq, xs, wq, ws)
         buf = torch.full((m + 2, n + 5), -7.0, dtype=torch.bfloat16, device=DEV)
