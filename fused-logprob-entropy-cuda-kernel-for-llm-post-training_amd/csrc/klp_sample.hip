@@ -17,12 +17,22 @@
 // as 64-bit integers of 2^-44, whose sums do not depend on the order of the
 // atomics.
 //
-// No row is sorted.  The kept set is {key > tau} and the first r of
-// {key == tau}, key the logit's bits in order; tau is found with a histogram
-// of counts and masses over 2048 buckets, linear in y, and then inside the
-// bucket that holds the border by histograms over the key's bits, 11 at a
-// time, of the bucket's elements: from a list in LDS, or of the whole row
-// where the list overflows (a row of equal logits).
+// A row is read by one workgroup, a contiguous part of it by each wave.
+//   No filter: one pass sums the weights, relative to one of the row's first
+// logits; the part whose running sum crosses the target is read again.
+//   Filters: one pass for the maximum, then one that collects, in LDS, every
+// logit that could be kept, and is followed by work on that list alone: sorted
+// by value it gives the kept set, sorted by index the token.  What could be
+// kept is bounded beforehand by a bucket of a scale that is linear in y: for
+// top-k the bucket of the k-th largest of the threads' maxima (k of the logits
+// are at least that large), for min-p that of its border, for top-p without a
+// top-k that in which a histogram of the masses, one more pass, reaches top_p.
+//   Where the list overflows (more than 4096 logits above the bound: a row of
+// equal logits, a wide nucleus) the kept set is {key > tau} and the first r of
+// {key == tau}, key the logit's bits in order; tau is found with histograms of
+// counts and masses, first over the linear buckets, then inside the bucket
+// that holds the border over the key's bits, 11 at a time, and the kept
+// weights are summed and searched as those of an unfiltered row.
 #include "klp_launch.h"
 #include "klp_rows.h"
 
@@ -36,18 +46,27 @@ constexpr int kBucketBits = 11;
 constexpr int kBuckets = 1 << kBucketBits;
 constexpr int kPerThread = kBuckets / kThreads;
 constexpr int kList = 4096;
+constexpr int kListPerThread = kList / kThreads;
+constexpr int kBatch = 4;  // chunks of a lane in flight
 // Range of the first histogram, in units of log2 of the weight; lighter
 // elements share the last bucket.
 constexpr float kRangeBits = 44.0f;
 constexpr double kLog2eD = 1.44269504088896340736;
 constexpr double kLn2D = 0.69314718055994530942;
 
-// 2^y for y <= 0: 2^f with f = y - rint(y) as 1 + f q(f), q interpolating
-// (2^f - 1) / f at the Chebyshev points of [-1/2, 1/2].
+// Weights below this one are none: exp2_d's smallest is 2^-1000, for a logit
+// of -inf too, and a row of 2^26 of those sums to less than this.
+constexpr double kNothing = 0x1p-960;
+
+// 2^y for y < 1000: 2^f with f = y - rint(y) as 1 + f q(f), q interpolating
+// (2^f - 1) / f at the Chebyshev points of [-1/2, 1/2].  Adding 1.5 2^52
+// rounds to an integer and leaves it in the sum's low bits, from where it goes
+// into the result's exponent.
 __device__ __forceinline__ double exp2_d(double y) {
-    y = fmax(y, -1100.0);  // 0 from there on, -inf included
-    const double n = rint(y);
-    const double f = y - n;
+    constexpr double kRound = 0x1.8p52;
+    y = fmax(y, -1000.0);
+    const double z = y + kRound;
+    const double f = y - (z - kRound);
     double q = 0x1.63b2dp-20;
     q = fma(q, f, 0x1.00c0e454p-16);
     q = fma(q, f, 0x1.4308c71ep-13);
@@ -56,7 +75,8 @@ __device__ __forceinline__ double exp2_d(double y) {
     q = fma(q, f, 0x1.c6b08da70c1c8p-5);
     q = fma(q, f, 0x1.ebfbdff82a73dp-3);
     q = fma(q, f, 0x1.62e42fef9cc6cp-1);
-    return ldexp(fma(q, f, 1.0), static_cast<int>(n));
+    const double r = fma(q, f, 1.0);
+    return __hiloint2double(__double2hiint(r) + (__double2loint(z) << 20), __double2loint(r));
 }
 
 // Bits in the order of the values; -0 becomes +0, which it equals.
@@ -71,10 +91,11 @@ __device__ __forceinline__ float value_of(uint32_t key) {
 struct Shared {
     uint32_t count[kBuckets];
     unsigned long long mass[kBuckets];
-    uint32_t list[kList];
+    uint2 list[kList];  // x before y in the order of a sort
     unsigned long long wave_mass[kWaves];
     double wave_sum[kWaves];
     double wave_all[kWaves];
+    float wave_top[kWaves];
     uint32_t wave_count[kWaves];
     uint32_t n_list, key_min, key_max;
     // find()'s answer
@@ -95,6 +116,48 @@ __device__ __forceinline__ uint32_t wave_sum_u(uint32_t v) {
     return v;
 }
 
+// What the threads before this one have of v; `total`: what all have.
+__device__ __forceinline__ double block_before(Shared& s, double v, double& total) {
+    const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
+    double run = v;
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+        const double x = __shfl_up(run, o, 64);
+        if (lane >= o) run += x;
+    }
+    __syncthreads();  // the last call's readers
+    if (lane == 63) s.wave_sum[wave] = run;
+    __syncthreads();
+    double before = run - v;
+    total = 0.0;
+#pragma unroll
+    for (int i = 0; i < kWaves; ++i) {
+        if (i == wave) before += total;
+        total += s.wave_sum[i];
+    }
+    return before;
+}
+__device__ __forceinline__ uint32_t block_before(Shared& s, uint32_t v, uint32_t& total) {
+    const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
+    uint32_t run = v;
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+        const uint32_t x = __shfl_up(run, o, 64);
+        if (lane >= o) run += x;
+    }
+    __syncthreads();
+    if (lane == 63) s.wave_count[wave] = run;
+    __syncthreads();
+    uint32_t before = run - v;
+    total = 0;
+#pragma unroll
+    for (int i = 0; i < kWaves; ++i) {
+        if (i == wave) before += total;
+        total += s.wave_count[i];
+    }
+    return before;
+}
+
 template <int DT>
 struct Row {
     typedef typename Traits<DT>::elem elem;
@@ -105,15 +168,35 @@ struct Row {
     __device__ __forceinline__ void load(int at, float (&v)[kChunk]) const {
         load_chunk<DT>(x + at, vocab - at, -INFINITY, v);
     }
-    // f(first element, 8 values) for each chunk of this wave's part.  Values
-    // behind the row's end are -inf.
+    // f(first element, 8 values) for each chunk of this wave's part, kBatch of
+    // them loaded at a time.  Values behind the row's end are -inf.
     template <typename F>
     __device__ __forceinline__ void each(F f) const {
         const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
-        const int begin = wave * span;
-        int end = begin + span;
+        constexpr int kStep = 64 * kChunk;
+        const int begin = wave * span + lane * kChunk;
+        int end = (wave + 1) * span;
         if (end > vocab) end = vocab;
-        for (int at = begin + lane * kChunk; at < end; at += 64 * kChunk) {
+        typedef Unaligned16<elem> Vec;
+        constexpr int kVecs = DT == kFP32 ? 2 : 1;
+        int at = begin;
+        // Whole batches: the last chunk of the last lane included.
+        for (; at - lane * kChunk + kBatch * kStep <= end; at += kBatch * kStep) {
+            u32x4 raw[kBatch][kVecs];
+#pragma unroll
+            for (int i = 0; i < kBatch; ++i)
+#pragma unroll
+                for (int k = 0; k < kVecs; ++k)
+                    raw[i][k] = reinterpret_cast<const Vec*>(x + at + i * kStep)[k].v;
+#pragma unroll
+            for (int i = 0; i < kBatch; ++i) {
+                float v[kChunk];
+                unpack<DT>(raw[i][0], v);
+                if constexpr (DT == kFP32) unpack<DT>(raw[i][1], v + 4);
+                f(at + i * kStep, v);
+            }
+        }
+        for (; at < end; at += kStep) {
             float v[kChunk];
             load(at, v);
             f(at, v);
@@ -124,7 +207,7 @@ struct Row {
 // The first bucket, in order, at which the running count reaches `count` (or,
 // with by_mass, the running mass reaches `mass`); the last one with anything
 // in it when none does.  Into s.at, with what lies before it.
-__device__ __forceinline__ void find(Shared& s, bool by_mass, uint32_t count, double mass) {
+__device__ void find(Shared& s, bool by_mass, uint32_t count, double mass) {
     const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
     const int first = threadIdx.x * kPerThread;
     uint32_t c[kPerThread], c_sum = 0;
@@ -167,6 +250,7 @@ __device__ __forceinline__ void find(Shared& s, bool by_mass, uint32_t count, do
     }
     // A target that rounding left above the total is the total.
     const double want = fmin(mass, static_cast<double>(m_all));
+    count = min(count, c_all);
 #pragma unroll
     for (int i = 0; i < kPerThread; ++i) {
         const bool before = by_mass ? static_cast<double>(m_run) < want : c_run < count;
@@ -184,6 +268,31 @@ __device__ __forceinline__ void find(Shared& s, bool by_mass, uint32_t count, do
     __syncthreads();
 }
 
+// The first `n` entries of the list in order (n <= 1 << bits <= kList, what
+// lies between filled here): a bitonic sort.
+__device__ void sort_list(Shared& s, uint32_t n) {
+    uint32_t size = 2;
+    while (size < n) size <<= 1;
+    for (uint32_t i = n + threadIdx.x; i < size; i += kThreads)
+        s.list[i] = make_uint2(0xFFFFFFFFu, 0xFFFFFFFFu);
+    for (uint32_t width = 2; width <= size; width <<= 1) {
+        for (uint32_t step = width >> 1; step > 0; step >>= 1) {
+            __syncthreads();
+            for (uint32_t t = threadIdx.x; t < size / 2; t += kThreads) {
+                const uint32_t i = 2 * t - (t & (step - 1));
+                const uint2 a = s.list[i], b = s.list[i + step];
+                const bool up = (i & width) == 0;
+                const bool less = b.x < a.x || (b.x == a.x && b.y < a.y);
+                if (less == up) {
+                    s.list[i] = b;
+                    s.list[i + step] = a;
+                }
+            }
+        }
+    }
+    __syncthreads();
+}
+
 struct Border {
     uint32_t tau;        // key
     uint32_t ties;       // elements of that key
@@ -196,21 +305,27 @@ template <int DT>
 struct Sampler {
     Row<DT> row;
     Shared& s;
-    float top;           // max x
+    float top;           // weights are relative to this logit
     double c;            // log2(e) / T
-    float bucket_scale;
+    float c32;
     double fixed_one;    // added to a weight, it leaves its fixed-point value in the low bits
 
+    __device__ __forceinline__ double log2_weight(float x) const {
+        return (static_cast<double>(x) - static_cast<double>(top)) * c;
+    }
     __device__ __forceinline__ double weight(float x) const {
-        return exp2_d((static_cast<double>(x) - static_cast<double>(top)) * c);
+        return exp2_d(log2_weight(x));
     }
     __device__ __forceinline__ unsigned long long fixed(double w) const {
         return static_cast<unsigned long long>(__double_as_longlong(w + fixed_one)) &
                ((1ull << 52) - 1);
     }
-    // Monotone in x: equal logits share a bucket.
+    // -log2 of the weight in float32, and in buckets: monotone in x, so that
+    // equal logits share a bucket.
+    __device__ __forceinline__ float depth(float x) const { return (top - x) * c32; }
     __device__ __forceinline__ uint32_t bucket(float x) const {
-        return static_cast<uint32_t>(fminf((top - x) * bucket_scale, kBuckets - 1.0f));
+        return static_cast<uint32_t>(
+            fminf(depth(x) * ((kBuckets - 1) / kRangeBits), kBuckets - 1.0f));
     }
     __device__ __forceinline__ void clear() {
 #pragma unroll
@@ -218,6 +333,7 @@ struct Sampler {
             s.count[threadIdx.x + i * kThreads] = 0;
             s.mass[threadIdx.x + i * kThreads] = 0;
         }
+        __syncthreads();
     }
 
     // The border inside first-histogram bucket b, among keys >= floor, with
@@ -225,23 +341,24 @@ struct Sampler {
     __device__ Border resolve(uint32_t b, uint32_t floor, uint32_t above,
                               unsigned long long above_mass, bool by_mass, uint32_t count,
                               double mass) {
+        __syncthreads();
         if (threadIdx.x == 0) {
             s.n_list = 0;
             s.key_min = 0xFFFFFFFFu;
             s.key_max = 0;
         }
         __syncthreads();
-        row.each([&](int at, const float (&v)[kChunk]) {
+        row.each([&](int, const float (&v)[kChunk]) {
             uint32_t lo = 0xFFFFFFFFu, hi = 0;
 #pragma unroll
             for (int j = 0; j < kChunk; ++j) {
-                if (bucket(v[j]) != b || at + j >= row.vocab) continue;
+                if (bucket(v[j]) != b) continue;
                 const uint32_t k = key_of(v[j]);
                 if (k < floor) continue;
                 lo = min(lo, k);
                 hi = max(hi, k);
                 const uint32_t i = atomicAdd(&s.n_list, 1u);
-                if (i < kList) s.list[i] = k;
+                if (i < kList) s.list[i].x = k;
             }
             if (hi >= lo) {
                 atomicMin(&s.key_min, lo);
@@ -257,20 +374,18 @@ struct Sampler {
             const int shift = bits > kBucketBits ? bits - kBucketBits : 0;
             __syncthreads();
             clear();
-            __syncthreads();
             auto add = [&](uint32_t k) {
                 if (k < lo || k > hi) return;
                 const uint32_t i = (hi - k) >> shift;
                 atomicAdd(&s.count[i], 1u);
-                atomicAdd(&s.mass[i], fixed(weight(value_of(k))));
+                if (by_mass) atomicAdd(&s.mass[i], fixed(weight(value_of(k))));
             };
             if (n <= kList) {
-                for (uint32_t i = threadIdx.x; i < n; i += kThreads) add(s.list[i]);
+                for (uint32_t i = threadIdx.x; i < n; i += kThreads) add(s.list[i].x);
             } else {
-                row.each([&](int at, const float (&v)[kChunk]) {
+                row.each([&](int, const float (&v)[kChunk]) {
 #pragma unroll
-                    for (int j = 0; j < kChunk; ++j)
-                        if (at + j < row.vocab) add(key_of(v[j]));
+                    for (int j = 0; j < kChunk; ++j) add(key_of(v[j]));
                 });
             }
             __syncthreads();
@@ -286,9 +401,108 @@ struct Sampler {
         __syncthreads();
         return Border{lo, ties, above, above_mass};
     }
+
+    // The token of {key > tau, or one of the first keep_ties of {key == tau},
+    // with a weight of at least min_w}: each wave has its part's sum of the
+    // weights above tau in `kept` and its count of ties.
+    __device__ int search(float u, uint32_t tau, uint32_t keep_ties, double min_w, double kept,
+                          uint32_t ties, double& mass) {
+        const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
+        double tau_w = keep_ties > 0 ? weight(value_of(tau)) : 0.0;
+        if (tau_w < min_w) tau_w = 0.0;
+        kept = wave_sum_d(kept);
+        ties = wave_sum_u(ties);
+        __syncthreads();
+        if (lane == 0) {
+            s.wave_sum[wave] = kept;
+            s.wave_count[wave] = ties;
+        }
+        if (threadIdx.x == 0) {
+            s.token = 0x7FFFFFFF;
+            s.last = -1;
+        }
+        __syncthreads();
+        uint32_t ties_before = 0;
+        auto part_mass = [&](int i) {  // in order, from 0
+            const uint32_t n = s.wave_count[i];
+            const uint32_t left = keep_ties - min(keep_ties, ties_before);
+            ties_before += n;
+            return s.wave_sum[i] + min(n, left) * tau_w;
+        };
+        mass = 0.0;
+        for (int i = 0; i < kWaves; ++i) mass += part_mass(i);
+        const double target = static_cast<double>(u) * mass;
+        // The part in which the running sum crosses the target: the last one
+        // that holds anything if rounding (or u = 1) lets none.
+        int part = 0;
+        double base = 0.0, run = 0.0;
+        uint32_t base_ties = 0;
+        ties_before = 0;
+        for (int i = 0; i < kWaves; ++i) {
+            const uint32_t before = ties_before;
+            const double m = part_mass(i);
+            if (m > kNothing) {
+                part = i;
+                base = run;
+                base_ties = before;
+                if (run + m > target) break;
+            }
+            run += m;
+        }
+
+        // That part again, 8 consecutive elements a thread.
+        const int begin = part * row.span;
+        int end = begin + row.span;
+        if (end > row.vocab) end = row.vocab;
+        for (int first = begin; first < end; first += kThreads * kChunk) {
+            const int at = first + threadIdx.x * kChunk;
+            float v[kChunk];
+            double w[kChunk];
+            uint32_t tie = 0;  // a bit an element
+            row.load(at < end ? at : row.vocab, v);
+#pragma unroll
+            for (int j = 0; j < kChunk; ++j) {
+                const uint32_t k = key_of(v[j]);
+                const bool in = at + j < end;
+                w[j] = in && k > tau ? weight(v[j]) : 0.0;
+                if (w[j] < min_w) w[j] = 0.0;
+                if (in && k == tau) tie |= 1u << j;
+            }
+            uint32_t all_ties = 0;
+            if (keep_ties > 0) {
+                uint32_t rank = base_ties + block_before(s, __popc(tie), all_ties);
+#pragma unroll
+                for (int j = 0; j < kChunk; ++j) {
+                    if (!(tie >> j & 1)) continue;
+                    if (rank < keep_ties) w[j] = tau_w;
+                    ++rank;
+                }
+                base_ties += all_ties;
+            }
+            double sum = 0.0, all = 0.0;
+#pragma unroll
+            for (int j = 0; j < kChunk; ++j) sum += w[j];
+            double pos = base + block_before(s, sum, all);
+            base += all;
+            int mine = 0x7FFFFFFF, last = -1;
+#pragma unroll
+            for (int j = 0; j < kChunk; ++j) {
+                pos += w[j];
+                if (w[j] > kNothing) {
+                    last = at + j;
+                    if (pos > target && mine == 0x7FFFFFFF) mine = at + j;
+                }
+            }
+            if (mine != 0x7FFFFFFF) atomicMin(&s.token, mine);
+            if (last >= 0) atomicMax(&s.last, last);
+        }
+        __syncthreads();
+        return s.token != 0x7FFFFFFF ? s.token : s.last;
+    }
 };
 
-template <int DT>
+// kFilters: rows may have filters, or a temperature of 0.
+template <int DT, bool kFilters>
 __global__ __launch_bounds__(kThreads) void klp_sample_kernel(SampleParams p) {
     __shared__ Shared s;
     const int64_t r = blockIdx.x;
@@ -299,289 +513,301 @@ __global__ __launch_bounds__(kThreads) void klp_sample_kernel(SampleParams p) {
     row.vocab = vocab;
     row.span = (vocab + kWaves * 64 * kChunk - 1) / (kWaves * 64 * kChunk) * 64 * kChunk;
 
-    // The largest logit; NaN where there is one.
-    float top = -INFINITY;
-    row.each([&](int, const float (&v)[kChunk]) {
-#pragma unroll
-        for (int j = 0; j < kChunk; ++j) top = fmax_nan(top, v[j]);
-    });
-    top = xrow_max(row_max16(top));
-    float* tops = reinterpret_cast<float*>(s.count);
-    if (lane == 0) tops[wave] = top;
-    __syncthreads();
-#pragma unroll
-    for (int i = 0; i < kWaves; ++i) top = fmax_nan(top, tops[i]);
-    __syncthreads();
-    top += 0.0f;
-
     float t = p.temperatures != nullptr ? p.temperatures[r] : p.temperature;
     const float top_p = p.top_ps != nullptr ? p.top_ps[r] : p.top_p;
-    const float min_p_raw = p.min_ps != nullptr ? p.min_ps[r] : p.min_p;
+    const float min_p = p.min_ps != nullptr ? p.min_ps[r] : p.min_p;
     int top_k = p.top_ks != nullptr ? p.top_ks[r] : p.top_k;
-    const bool greedy = t == 0.0f;
-    if (greedy) {
+    float u = p.uniform[r];
+    u = u > 0.0f ? fminf(u, 1.0f) : 0.0f;
+    if (t == 0.0f) {
         t = 1.0f;
         top_k = 1;
     }
-    if (!(fabsf(top) < INFINITY) || !(t > 0.0f && t < INFINITY)) {
+    const bool bad_t = !(t > 0.0f && t < INFINITY);
+    if (bad_t) t = 1.0f;
+    const bool by_k = top_k > 0 && top_k < vocab;
+    const bool by_p = top_p < 1.0f;  // a NaN is no filter
+    const bool by_m = min_p > 0.0f;
+    const double min_w = by_m ? fmin(static_cast<double>(min_p), 1.0) : 0.0;
+
+    // Fixed point: sums of `vocab` weights of at most 1 stay below 2^63.
+    int frac = 62 - (32 - __clz(vocab));
+    if (frac > 44) frac = 44;
+    const double c = kLog2eD / static_cast<double>(t);
+    Sampler<DT> sm{row, s, 0.0f, c, fminf(static_cast<float>(c), 1e30f),
+                   ldexp(1.0, 52 - frac)};
+
+    float top = -INFINITY;  // the largest logit; NaN where there is one
+    auto over_row = [&]() {
+        top = xrow_max(row_max16(top));
+        __syncthreads();
+        if (lane == 0) s.wave_top[wave] = top;
+        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < kWaves; ++i) top = fmax_nan(top, s.wave_top[i]);
+        if (fabsf(top) < INFINITY && !bad_t) return true;
         if (threadIdx.x == 0) {
-            const float none = top == -INFINITY ? -INFINITY : NAN;
+            const float none = top == -INFINITY && !bad_t ? -INFINITY : NAN;
             p.tokens[r] = -1;
             p.logp[r] = none;
             p.sample_logp[r] = none;
         }
-        return;
-    }
-    const double c = kLog2eD / static_cast<double>(t);
-    const float bucket_scale =
-        fminf(static_cast<float>(c) * ((kBuckets - 1) / kRangeBits), 1e30f);
-    // Fixed point: sums of `vocab` weights of at most 1 stay below 2^63.
-    int frac = 62 - (32 - __clz(vocab));
-    if (frac > 44) frac = 44;
-    const double fixed_one = ldexp(1.0, 52 - frac);
-    Sampler<DT> sm{row, s, top, c, bucket_scale, fixed_one};
-
-    const bool by_k = top_k > 0 && top_k < vocab;
-    const bool by_p = top_p < 1.0f;  // a NaN is no filter
-    const bool by_m = min_p_raw > 0.0f;
-    const double min_w = by_m ? fmin(static_cast<double>(min_p_raw), 1.0) : 0.0;
-
-    // Weights of the whole row: their sum, and their histogram where a border
-    // is to be found.
-    double all = 0.0, kept = 0.0;
-    if (by_k || by_p) {
-        sm.clear();
+        return false;
+    };
+    auto over_waves = [&](double v) {
+        v = wave_sum_d(v);
         __syncthreads();
-    }
-    row.each([&](int at, const float (&v)[kChunk]) {
+        if (lane == 0) s.wave_all[wave] = v;
+        __syncthreads();
+        v = 0.0;
 #pragma unroll
-        for (int j = 0; j < kChunk; ++j) {
-            const double w = sm.weight(v[j]);
-            all += w;
-            if (by_k || by_p) {
-                if (at + j < vocab) {
-                    const uint32_t b = sm.bucket(v[j]);
-                    atomicAdd(&s.count[b], 1u);
-                    atomicAdd(&s.mass[b], sm.fixed(w));
-                }
-            } else if (w >= min_w) {
-                kept += w;
-            }
-        }
-    });
+        for (int i = 0; i < kWaves; ++i) v += s.wave_all[i];
+        return v;
+    };
+    int token;
+    double all = 0.0, mass;
 
-    uint32_t tau = 0, keep_ties = 0xFFFFFFFFu;
-    double tau_w = 0.0;
-    if (by_k || by_p) {
-        __syncthreads();
-        uint32_t floor = 0, floor_bucket = kBuckets, k_ties = 0xFFFFFFFFu;
+    if (!kFilters || (!by_k && !by_p && !by_m)) {
+        // Weights relative to the largest of the first 64 logits; again, to the
+        // row's largest, if that overflows (2^900 of them).
+        float first = lane < vocab ? to_f32<DT>(row.x[lane]) : -INFINITY;
+        first = xrow_max(row_max16(first));
+        sm.top = fabsf(first) < INFINITY ? first : 0.0f;
+        double sum;
+        auto add_up = [&]() {
+            sum = 0.0;
+            row.each([&](int, const float (&v)[kChunk]) {
+#pragma unroll
+                for (int j = 0; j < kChunk; ++j) {
+                    top = fmax_nan(top, v[j]);
+                    sum += sm.weight(v[j]);
+                }
+            });
+        };
+        add_up();
+        if (!over_row()) return;
+        if (sm.log2_weight(top) > 900.0) {
+            sm.top = top;
+            add_up();
+        }
+        token = sm.search(u, 0, 0, 0.0, sum, 0, mass);
+        all = mass;
+    } else {
+        row.each([&](int, const float (&v)[kChunk]) {
+#pragma unroll
+            for (int j = 0; j < kChunk; ++j) top = fmax_nan(top, v[j]);
+        });
+        const float thread_top = top;
+        if (!over_row()) return;
+        sm.top = top + 0.0f;
+        // What could be kept lies in buckets up to `bound`.
+        uint32_t bound = kBuckets - 1;
         double share = 0.0;
-        unsigned long long total = 0;
-        if (by_p) {  // the whole row's mass, for want of a top-k
-            find(s, true, 0, 1e30);
-            total = s.above_mass + s.mass[s.at];
-            __syncthreads();
-        }
-        uint32_t p_at = 0, p_above = 0;
-        unsigned long long p_above_mass = 0;
-        bool p_early = false;
+        unsigned long long p_above = 0;
         if (by_k) {
+            sm.clear();
+            if (top_k <= kThreads) {
+                if (thread_top != -INFINITY) atomicAdd(&s.count[sm.bucket(thread_top)], 1u);
+            } else {
+                row.each([&](int, const float (&v)[kChunk]) {
+#pragma unroll
+                    for (int j = 0; j < kChunk; ++j) atomicAdd(&s.count[sm.bucket(v[j])], 1u);
+                });
+            }
+            __syncthreads();
             find(s, false, static_cast<uint32_t>(top_k), 0.0);
-            floor_bucket = s.at;
-            const uint32_t above = s.above_count;
-            const unsigned long long above_mass = s.above_mass;
-            // The first histogram is needed again for top-p: its border is
-            // looked for in it once the mass of K is known.
-            uint32_t hold_c[kPerThread];
-            unsigned long long hold_m[kPerThread];
+            // Fewer threads than top_k have a logit: no bound from them.
+            if (s.above_count + s.at_count >= static_cast<uint32_t>(top_k)) bound = s.at;
+        } else if (by_p) {
+            sm.clear();
+            row.each([&](int, const float (&v)[kChunk]) {
 #pragma unroll
-            for (int i = 0; i < kPerThread; ++i) {
-                hold_c[i] = s.count[threadIdx.x + i * kThreads];
-                hold_m[i] = s.mass[threadIdx.x + i * kThreads];
-            }
-            __syncthreads();
-            const Border k = sm.resolve(floor_bucket, 0, above, above_mass, false,
-                                        static_cast<uint32_t>(top_k), 0.0);
-            floor = tau = k.tau;
-            k_ties = keep_ties = static_cast<uint32_t>(top_k) - k.above;
-            tau_w = sm.weight(value_of(tau));
-            if (by_p) {
-                total = k.above_mass + k_ties * sm.fixed(tau_w);
-#pragma unroll
-                for (int i = 0; i < kPerThread; ++i) {
-                    s.count[threadIdx.x + i * kThreads] = hold_c[i];
-                    s.mass[threadIdx.x + i * kThreads] = hold_m[i];
+                for (int j = 0; j < kChunk; ++j) {
+                    const double w = sm.weight(v[j]);
+                    all += w;
+                    atomicAdd(&s.mass[sm.bucket(v[j])], sm.fixed(w));
                 }
-                __syncthreads();
-            }
-        }
-        if (by_p) {
-            share = static_cast<double>(fmaxf(top_p, 0.0f)) * static_cast<double>(total);
-            // The first element is always kept.
-            share = fmax(share, 1.0);
+            });
+            all = over_waves(all);
+            // In fixed point; the first element is always kept.
+            share = fmax(static_cast<double>(fmaxf(top_p, 0.0f)) * all * ldexp(1.0, frac), 1.0);
             find(s, true, 0, share);
-            p_at = s.at;
-            p_above = s.above_count;
-            p_above_mass = s.above_mass;
-            __syncthreads();
-            p_early = p_at < floor_bucket;
-            const Border b = sm.resolve(p_at, p_early ? 0 : floor, p_above, p_above_mass, true, 0,
-                                        share);
-            uint32_t limit = b.ties;
-            if (b.tau == floor && by_k) limit = min(limit, k_ties);
-            tau = b.tau;
-            tau_w = sm.weight(value_of(tau));
-            const double one = static_cast<double>(sm.fixed(tau_w));
-            const double left = share - static_cast<double>(b.above_mass);
-            const double need = one > 0.0 ? ceil(left / one) : 1.0;
-            keep_ties = need < 1.0 ? 1u : need < limit ? static_cast<uint32_t>(need) : limit;
+            bound = s.at;
+            p_above = s.above_mass;
         }
-        // Sums of what is kept, a wave's part each; equal keys at the border
-        // are counted and shared out in index order below.
-        uint32_t ties = 0;
+        if (by_m && !(by_k && by_p)) {
+            // One bucket on for the rounding of its border's logarithm.
+            const double b = -log2(min_w) * ((kBuckets - 1) / kRangeBits) + 1.0;
+            if (b < bound) bound = static_cast<uint32_t>(b);
+        }
+        __syncthreads();
+        if (threadIdx.x == 0) s.n_list = 0;
+        __syncthreads();
+        const float deep = bound < kBuckets - 1 ? static_cast<float>(bound + 1) : INFINITY;
+        const bool summed = !by_k && by_p;
         row.each([&](int at, const float (&v)[kChunk]) {
+            float w[kChunk];
+            uint32_t in = 0;
 #pragma unroll
             for (int j = 0; j < kChunk; ++j) {
-                const uint32_t k = key_of(v[j]);
-                if (k < tau || at + j >= vocab) continue;
-                if (k == tau) {
-                    ++ties;
-                } else {
-                    const double w = sm.weight(v[j]);
-                    if (w >= min_w) kept += w;
+                const float d = sm.depth(v[j]);
+                w[j] = exp2_hw(-d);
+                if (d * ((kBuckets - 1) / kRangeBits) < deep && at + j < vocab) in |= 1u << j;
+            }
+            if (!summed)
+                all += static_cast<double>(((w[0] + w[1]) + (w[2] + w[3])) +
+                                           ((w[4] + w[5]) + (w[6] + w[7])));
+            if (in != 0) {
+                uint32_t i = atomicAdd(&s.n_list, static_cast<uint32_t>(__popc(in)));
+#pragma unroll
+                for (int j = 0; j < kChunk; ++j) {
+                    if (!(in >> j & 1)) continue;
+                    if (i < kList) s.list[i] = make_uint2(~key_of(v[j]), at + j);
+                    ++i;
                 }
             }
         });
-        ties = wave_sum_u(ties);
-        if (lane == 0) s.wave_count[wave] = ties;
-    } else if (lane == 0) {
-        s.wave_count[wave] = 0;
-    }
-    if (tau_w < min_w) tau_w = 0.0;
-
-    all = wave_sum_d(all);
-    kept = wave_sum_d(kept);
-    if (lane == 0) {
-        s.wave_all[wave] = all;
-        s.wave_sum[wave] = kept;
+        if (!summed) all = over_waves(all);
+        else __syncthreads();
+        const uint32_t n = s.n_list;
+        if (n <= kList) {
+            // By falling value, then index: the kept ones are the first.
+            sort_list(s, n);
+            const uint32_t at = threadIdx.x * kListPerThread;
+            double w[kListPerThread], sum = 0.0, total;
+            uint2 e[kListPerThread];
+#pragma unroll
+            for (int j = 0; j < kListPerThread; ++j) {
+                const uint32_t i = at + j;
+                const bool in = i < n && (!by_k || i < static_cast<uint32_t>(top_k));
+                e[j] = in ? s.list[i] : make_uint2(0xFFFFFFFFu, 0xFFFFFFFFu);
+                w[j] = in ? sm.weight(value_of(~e[j].x)) : 0.0;
+                sum += w[j];
+            }
+            double before = block_before(s, sum, total);
+            const double most = static_cast<double>(fmaxf(top_p, 0.0f)) * (by_k ? total : all);
+            uint32_t kept = 0;
+            double left = 0.0;
+#pragma unroll
+            for (int j = 0; j < kListPerThread; ++j) {
+                const uint32_t i = at + j;
+                const bool in = i < n && (!by_k || i < static_cast<uint32_t>(top_k)) &&
+                                (i == 0 || ((!by_p || before < most) && w[j] >= min_w));
+                before += w[j];
+                if (!in) w[j] = 0.0;
+                else ++kept;
+                left += w[j];
+            }
+            uint32_t n_kept;
+            block_before(s, kept, n_kept);
+            block_before(s, left, mass);
+            // By index: block_before's barriers lie behind the reads above.
+#pragma unroll
+            for (int j = 0; j < kListPerThread; ++j)
+                if (at + j < n_kept) s.list[at + j] = make_uint2(e[j].y, e[j].x);
+            __syncthreads();
+            sort_list(s, n_kept);
+            if (threadIdx.x == 0) {
+                s.token = 0x7FFFFFFF;
+                s.last = -1;
+            }
+            sum = 0.0;
+#pragma unroll
+            for (int j = 0; j < kListPerThread; ++j) {
+                const bool in = at + j < n_kept;
+                e[j] = in ? s.list[at + j] : make_uint2(0, 0);
+                w[j] = in ? sm.weight(value_of(~e[j].y)) : 0.0;
+                sum += w[j];
+            }
+            double pos = block_before(s, sum, total);
+            const double target = static_cast<double>(u) * total;
+#pragma unroll
+            for (int j = 0; j < kListPerThread; ++j) {
+                pos += w[j];
+                if (w[j] <= kNothing) continue;
+                if (pos > target) atomicMin(&s.token, static_cast<int>(e[j].x));
+                atomicMax(&s.last, static_cast<int>(e[j].x));
+            }
+            __syncthreads();
+            token = s.token != 0x7FFFFFFF ? s.token : s.last;
+        } else {
+            uint32_t tau = 0, keep_ties = 0;
+            if (by_k) {
+                sm.clear();
+                row.each([&](int at, const float (&v)[kChunk]) {
+#pragma unroll
+                    for (int j = 0; j < kChunk; ++j)
+                        if (at + j < vocab) atomicAdd(&s.count[sm.bucket(v[j])], 1u);
+                });
+                __syncthreads();
+                find(s, false, static_cast<uint32_t>(top_k), 0.0);
+                const uint32_t b = s.at, above = s.above_count;
+                const Border k = sm.resolve(b, 0, above, 0, false, static_cast<uint32_t>(top_k),
+                                            0.0);
+                tau = k.tau;
+                keep_ties = static_cast<uint32_t>(top_k) - k.above;
+            }
+            if (by_p) {
+                uint32_t b = bound;
+                const uint32_t floor = tau, most_ties = keep_ties;
+                if (by_k) {
+                    // The masses of K.
+                    sm.clear();
+                    double part = 0.0, total;
+                    row.each([&](int, const float (&v)[kChunk]) {
+#pragma unroll
+                        for (int j = 0; j < kChunk; ++j) {
+                            if (key_of(v[j]) <= tau) continue;
+                            const double w = sm.weight(v[j]);
+                            part += w;
+                            atomicAdd(&s.mass[sm.bucket(v[j])], sm.fixed(w));
+                        }
+                    });
+                    const double tau_w = sm.weight(value_of(tau));
+                    if (threadIdx.x == 0) {
+                        part += keep_ties * tau_w;
+                        atomicAdd(&s.mass[sm.bucket(value_of(tau))], keep_ties * sm.fixed(tau_w));
+                    }
+                    total = over_waves(part);
+                    share = fmax(static_cast<double>(fmaxf(top_p, 0.0f)) * total *
+                                     ldexp(1.0, frac), 1.0);
+                    find(s, true, 0, share);
+                    b = s.at;
+                    p_above = s.above_mass;
+                } else {
+                    // `bound` may be min-p's by now.
+                    find(s, true, 0, share);
+                    b = s.at;
+                }
+                const Border q = sm.resolve(b, floor, 0, p_above, true, 0, share);
+                tau = q.tau;
+                const double one = static_cast<double>(sm.fixed(sm.weight(value_of(tau))));
+                const double left = share - static_cast<double>(q.above_mass);
+                const double need = one > 0.0 ? ceil(left / one) : 1.0;
+                uint32_t limit = q.ties;
+                if (by_k && tau == floor) limit = min(limit, most_ties);
+                keep_ties = need < 1.0 ? 1u : need < limit ? static_cast<uint32_t>(need) : limit;
+            }
+            double kept = 0.0;
+            uint32_t ties = 0;
+            row.each([&](int, const float (&v)[kChunk]) {
+#pragma unroll
+                for (int j = 0; j < kChunk; ++j) {
+                    const uint32_t k = key_of(v[j]);
+                    if (k < tau) continue;
+                    if (k == tau) {
+                        ++ties;
+                    } else {
+                        const double w = sm.weight(v[j]);
+                        if (w >= min_w) kept += w;
+                    }
+                }
+            });
+            token = sm.search(u, tau, keep_ties, min_w, kept, ties, mass);
+        }
     }
     if (threadIdx.x == 0) {
-        s.token = 0x7FFFFFFF;
-        s.last = -1;
-    }
-    __syncthreads();
-    all = 0.0;
-    double mass = 0.0;
-    uint32_t ties_before = 0;
-#pragma unroll
-    for (int i = 0; i < kWaves; ++i) {
-        const uint32_t n = s.wave_count[i];
-        const uint32_t left = keep_ties - min(keep_ties, ties_before);
-        all += s.wave_all[i];
-        mass += s.wave_sum[i] + min(n, left) * tau_w;
-        ties_before += n;
-    }
-    float u = p.uniform[r];
-    u = u > 0.0f ? fminf(u, 1.0f) : 0.0f;
-    const double target = static_cast<double>(u) * mass;
-    // The part of the row in which the running sum crosses the target: the
-    // last one that holds anything if rounding (or u = 1) lets none.
-    int part = 0;
-    double before = 0.0, run = 0.0;
-    uint32_t part_ties = 0;
-    ties_before = 0;
-    bool found = false;
-#pragma unroll
-    for (int i = 0; i < kWaves; ++i) {
-        const uint32_t n = s.wave_count[i];
-        const uint32_t left = keep_ties - min(keep_ties, ties_before);
-        const double m = s.wave_sum[i] + min(n, left) * tau_w;
-        if (!found && m > 0.0) {
-            part = i;
-            before = run;
-            part_ties = ties_before;
-            found = run + m > target;
-        }
-        run += m;
-        ties_before += n;
-    }
-
-    // That part again, 8 consecutive elements a thread.
-    double base = before;
-    uint32_t base_ties = part_ties;
-    int begin = part * row.span, end = begin + row.span;
-    if (end > vocab) end = vocab;
-    for (int first = begin; first < end; first += kThreads * kChunk) {
-        const int at = first + threadIdx.x * kChunk;
-        float v[kChunk];
-        double w[kChunk];
-        uint32_t n_ties = 0;
-        row.load(at < end ? at : vocab, v);
-#pragma unroll
-        for (int j = 0; j < kChunk; ++j) {
-            const uint32_t k = key_of(v[j]);
-            const bool in = at + j < end;
-            w[j] = in && k > tau ? sm.weight(v[j]) : 0.0;
-            if (w[j] < min_w) w[j] = 0.0;
-            if (in && k == tau && tau != 0) ++n_ties;
-        }
-        // Ties before this thread's elements.
-        uint32_t t_run = n_ties;
-#pragma unroll
-        for (int o = 1; o < 64; o <<= 1) {
-            const uint32_t x = __shfl_up(t_run, o, 64);
-            if (lane >= o) t_run += x;
-        }
-        __syncthreads();
-        if (lane == 63) s.wave_count[wave] = t_run;
-        __syncthreads();
-        uint32_t rank = base_ties + t_run - n_ties;
-#pragma unroll
-        for (int i = 0; i < kWaves; ++i) {
-            if (i < wave) rank += s.wave_count[i];
-            base_ties += s.wave_count[i];
-        }
-        double sum = 0.0;
-#pragma unroll
-        for (int j = 0; j < kChunk; ++j) {
-            if (at + j < end && key_of(v[j]) == tau && tau != 0) {
-                if (rank < keep_ties) w[j] = tau_w;
-                ++rank;
-            }
-            sum += w[j];
-        }
-        double s_run = sum;
-#pragma unroll
-        for (int o = 1; o < 64; o <<= 1) {
-            const double x = __shfl_up(s_run, o, 64);
-            if (lane >= o) s_run += x;
-        }
-        __syncthreads();
-        if (lane == 63) s.wave_sum[wave] = s_run;
-        __syncthreads();
-        double pos = base + (s_run - sum);
-#pragma unroll
-        for (int i = 0; i < kWaves; ++i) {
-            if (i < wave) pos += s.wave_sum[i];
-            base += s.wave_sum[i];
-        }
-        int mine = 0x7FFFFFFF, last = -1;
-#pragma unroll
-        for (int j = 0; j < kChunk; ++j) {
-            pos += w[j];
-            if (w[j] > 0.0) {
-                last = at + j;
-                if (pos > target && mine == 0x7FFFFFFF) mine = at + j;
-            }
-        }
-        if (mine != 0x7FFFFFFF) atomicMin(&s.token, mine);
-        if (last >= 0) atomicMax(&s.last, last);
-    }
-    __syncthreads();
-    if (threadIdx.x == 0) {
-        const int token = s.token != 0x7FFFFFFF ? s.token : s.last;
-        const float x = to_f32<DT>(row.x[token]);
-        const double y = (static_cast<double>(x) - static_cast<double>(top)) * c * kLn2D;
+        const double y = sm.log2_weight(to_f32<DT>(row.x[token])) * kLn2D;
         p.tokens[r] = token;
         p.logp[r] = static_cast<float>(y - log(all));
         p.sample_logp[r] = static_cast<float>(y - log(mass));
@@ -590,12 +816,27 @@ __global__ __launch_bounds__(kThreads) void klp_sample_kernel(SampleParams p) {
 
 }  // namespace
 
-hipError_t launch_sample(int dtype, const SampleParams& p, hipStream_t stream) {
+namespace {
+
+template <int DT>
+hipError_t launch_sample_dt(const SampleParams& p, hipStream_t stream) {
     const dim3 grid(static_cast<unsigned>(p.n_rows));
+    const bool plain = p.temperatures == nullptr && p.top_ks == nullptr && p.top_ps == nullptr &&
+                       p.min_ps == nullptr && p.temperature != 0.0f &&
+                       !(p.top_k > 0 && p.top_k < p.vocab) && !(p.top_p < 1.0f) &&
+                       !(p.min_p > 0.0f);
+    if (plain)
+        return launch_kernel(klp_sample_kernel<DT, false>, grid, dim3(kThreads), stream, p);
+    return launch_kernel(klp_sample_kernel<DT, true>, grid, dim3(kThreads), stream, p);
+}
+
+}  // namespace
+
+hipError_t launch_sample(int dtype, const SampleParams& p, hipStream_t stream) {
     switch (dtype) {
-        case kBF16: return launch_kernel(klp_sample_kernel<kBF16>, grid, dim3(kThreads), stream, p);
-        case kFP16: return launch_kernel(klp_sample_kernel<kFP16>, grid, dim3(kThreads), stream, p);
-        case kFP32: return launch_kernel(klp_sample_kernel<kFP32>, grid, dim3(kThreads), stream, p);
+        case kBF16: return launch_sample_dt<kBF16>(p, stream);
+        case kFP16: return launch_sample_dt<kFP16>(p, stream);
+        case kFP32: return launch_sample_dt<kFP32>(p, stream);
         default: return hipErrorInvalidValue;
     }
 }
