@@ -40,14 +40,16 @@ namespace klp {
 
 namespace {
 
-constexpr int kThreads = 1024;
-constexpr int kWaves = kThreads / 64;
+constexpr int kMaxWaves = 16;
 constexpr int kBucketBits = 11;
 constexpr int kBuckets = 1 << kBucketBits;
-constexpr int kPerThread = kBuckets / kThreads;
 constexpr int kList = 4096;
-constexpr int kListPerThread = kList / kThreads;
+// What one wave sorts, a few entries a lane; longer lists go through histograms.
+constexpr int kSorted = 512;
+constexpr int kPerLane = kSorted / 64;
 constexpr int kBatch = 4;  // chunks of a lane in flight
+// The histogram for top-p counts one of so many chunks, to foresee the list's length.
+constexpr int kCountEvery = 8;
 // Range of the first histogram, in units of log2 of the weight; lighter
 // elements share the last bucket.
 constexpr float kRangeBits = 44.0f;
@@ -92,12 +94,12 @@ struct Shared {
     uint32_t count[kBuckets];
     unsigned long long mass[kBuckets];
     uint2 list[kList];  // x before y in the order of a sort
-    unsigned long long wave_mass[kWaves];
-    double wave_sum[kWaves];
-    double wave_all[kWaves];
-    float wave_top[kWaves];
-    uint32_t wave_count[kWaves];
-    uint32_t n_list, key_min, key_max;
+    unsigned long long wave_mass[kMaxWaves];
+    double wave_sum[kMaxWaves];
+    double wave_all[kMaxWaves];
+    float wave_top[kMaxWaves];
+    uint32_t wave_count[kMaxWaves];
+    uint32_t n_list, key_min, key_max, key_count;
     // find()'s answer
     uint32_t at, at_count, above_count;
     unsigned long long above_mass;
@@ -117,7 +119,9 @@ __device__ __forceinline__ uint32_t wave_sum_u(uint32_t v) {
 }
 
 // What the threads before this one have of v; `total`: what all have.
+template <int T>
 __device__ __forceinline__ double block_before(Shared& s, double v, double& total) {
+    constexpr int kWaves = T / 64;
     const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
     double run = v;
 #pragma unroll
@@ -137,7 +141,9 @@ __device__ __forceinline__ double block_before(Shared& s, double v, double& tota
     }
     return before;
 }
+template <int T>
 __device__ __forceinline__ uint32_t block_before(Shared& s, uint32_t v, uint32_t& total) {
+    constexpr int kWaves = T / 64;
     const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
     uint32_t run = v;
 #pragma unroll
@@ -207,7 +213,9 @@ struct Row {
 // The first bucket, in order, at which the running count reaches `count` (or,
 // with by_mass, the running mass reaches `mass`); the last one with anything
 // in it when none does.  Into s.at, with what lies before it.
+template <int T>
 __device__ void find(Shared& s, bool by_mass, uint32_t count, double mass) {
+    constexpr int kWaves = T / 64, kPerThread = kBuckets / T;
     const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
     const int first = threadIdx.x * kPerThread;
     uint32_t c[kPerThread], c_sum = 0;
@@ -268,17 +276,33 @@ __device__ void find(Shared& s, bool by_mass, uint32_t count, double mass) {
     __syncthreads();
 }
 
-// The first `n` entries of the list in order (n <= 1 << bits <= kList, what
-// lies between filled here): a bitonic sort.
+// What the lanes before this one have of v; `total`: what the wave has.
+template <typename V>
+__device__ __forceinline__ V wave_before(V v, V& total) {
+    const int lane = threadIdx.x & 63;
+    V run = v;
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+        const V x = __shfl_up(run, o, 64);
+        if (lane >= o) run += x;
+    }
+    total = __shfl(run, 63, 64);
+    return run - v;
+}
+
+// The first `n` <= kSorted entries of the list in order: a bitonic sort by one
+// wave, whose LDS accesses take effect in program order.
 __device__ void sort_list(Shared& s, uint32_t n) {
+    const uint32_t lane = threadIdx.x & 63;
     uint32_t size = 2;
     while (size < n) size <<= 1;
-    for (uint32_t i = n + threadIdx.x; i < size; i += kThreads)
+    for (uint32_t i = n + lane; i < size; i += 64)
         s.list[i] = make_uint2(0xFFFFFFFFu, 0xFFFFFFFFu);
     for (uint32_t width = 2; width <= size; width <<= 1) {
         for (uint32_t step = width >> 1; step > 0; step >>= 1) {
-            __syncthreads();
-            for (uint32_t t = threadIdx.x; t < size / 2; t += kThreads) {
+            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+            __builtin_amdgcn_wave_barrier();
+            for (uint32_t t = lane; t < size / 2; t += 64) {
                 const uint32_t i = 2 * t - (t & (step - 1));
                 const uint2 a = s.list[i], b = s.list[i + step];
                 const bool up = (i & width) == 0;
@@ -290,7 +314,8 @@ __device__ void sort_list(Shared& s, uint32_t n) {
             }
         }
     }
-    __syncthreads();
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
 }
 
 struct Border {
@@ -301,8 +326,9 @@ struct Border {
 };
 
 // What a row's passes share.
-template <int DT>
+template <int DT, int T>
 struct Sampler {
+    static constexpr int kWaves = T / 64, kPerThread = kBuckets / T;
     Row<DT> row;
     Shared& s;
     float top;           // weights are relative to this logit
@@ -330,67 +356,68 @@ struct Sampler {
     __device__ __forceinline__ void clear() {
 #pragma unroll
         for (int i = 0; i < kPerThread; ++i) {
-            s.count[threadIdx.x + i * kThreads] = 0;
-            s.mass[threadIdx.x + i * kThreads] = 0;
+            s.count[threadIdx.x + i * T] = 0;
+            s.mass[threadIdx.x + i * T] = 0;
         }
         __syncthreads();
     }
 
+    // f(key) for every element of the list, or of the row.
+    template <typename F>
+    __device__ __forceinline__ void candidates(bool listed, F f) {
+        if (listed) {
+            const uint32_t n = s.n_list;
+            for (uint32_t i = threadIdx.x; i < n; i += T) f(~s.list[i].x);
+        } else {
+            row.each([&](int, const float (&v)[kChunk]) {
+#pragma unroll
+                for (int j = 0; j < kChunk; ++j) f(key_of(v[j]));
+            });
+        }
+    }
+
     // The border inside first-histogram bucket b, among keys >= floor, with
     // `above` elements and above_mass before the bucket.
-    __device__ Border resolve(uint32_t b, uint32_t floor, uint32_t above,
+    __device__ Border resolve(bool listed, uint32_t b, uint32_t floor, uint32_t above,
                               unsigned long long above_mass, bool by_mass, uint32_t count,
                               double mass) {
         __syncthreads();
         if (threadIdx.x == 0) {
-            s.n_list = 0;
+            s.key_count = 0;
             s.key_min = 0xFFFFFFFFu;
             s.key_max = 0;
         }
         __syncthreads();
-        row.each([&](int, const float (&v)[kChunk]) {
-            uint32_t lo = 0xFFFFFFFFu, hi = 0;
-#pragma unroll
-            for (int j = 0; j < kChunk; ++j) {
-                if (bucket(v[j]) != b) continue;
-                const uint32_t k = key_of(v[j]);
-                if (k < floor) continue;
-                lo = min(lo, k);
-                hi = max(hi, k);
-                const uint32_t i = atomicAdd(&s.n_list, 1u);
-                if (i < kList) s.list[i].x = k;
-            }
-            if (hi >= lo) {
-                atomicMin(&s.key_min, lo);
-                atomicMax(&s.key_max, hi);
-            }
+        uint32_t lo = 0xFFFFFFFFu, hi = 0, n = 0;
+        candidates(listed, [&](uint32_t k) {
+            if (k < floor || bucket(value_of(k)) != b) return;
+            lo = min(lo, k);
+            hi = max(hi, k);
+            ++n;
         });
+        if (n > 0) {
+            atomicMin(&s.key_min, lo);
+            atomicMax(&s.key_max, hi);
+            atomicAdd(&s.key_count, n);
+        }
         __syncthreads();
-        const uint32_t n = s.n_list;
-        uint32_t lo = s.key_min, hi = s.key_max;
-        uint32_t ties = n;
+        lo = s.key_min;
+        hi = s.key_max;
+        uint32_t ties = s.key_count;
         while (lo != hi) {  // at most 3 times: 32 bits, 11 at a time
             const int bits = 32 - __clz(hi - lo);
             const int shift = bits > kBucketBits ? bits - kBucketBits : 0;
             __syncthreads();
             clear();
-            auto add = [&](uint32_t k) {
+            candidates(listed, [&](uint32_t k) {
                 if (k < lo || k > hi) return;
                 const uint32_t i = (hi - k) >> shift;
                 atomicAdd(&s.count[i], 1u);
                 if (by_mass) atomicAdd(&s.mass[i], fixed(weight(value_of(k))));
-            };
-            if (n <= kList) {
-                for (uint32_t i = threadIdx.x; i < n; i += kThreads) add(s.list[i].x);
-            } else {
-                row.each([&](int, const float (&v)[kChunk]) {
-#pragma unroll
-                    for (int j = 0; j < kChunk; ++j) add(key_of(v[j]));
-                });
-            }
+            });
             __syncthreads();
-            find(s, by_mass, by_mass ? 0 : count - above,
-                 by_mass ? mass - static_cast<double>(above_mass) : 0.0);
+            find<T>(s, by_mass, by_mass ? 0 : count - above,
+                    by_mass ? mass - static_cast<double>(above_mass) : 0.0);
             above += s.above_count;
             above_mass += s.above_mass;
             ties = s.at_count;
@@ -402,21 +429,23 @@ struct Sampler {
         return Border{lo, ties, above, above_mass};
     }
 
-    // The token of {key > tau, or one of the first keep_ties of {key == tau},
-    // with a weight of at least min_w}: each wave has its part's sum of the
-    // weights above tau in `kept` and its count of ties.
-    __device__ int search(float u, uint32_t tau, uint32_t keep_ties, double min_w, double kept,
-                          uint32_t ties, double& mass) {
-        const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
-        double tau_w = keep_ties > 0 ? weight(value_of(tau)) : 0.0;
-        if (tau_w < min_w) tau_w = 0.0;
+    // Each wave's part of the row: its sum of kept weights above the border,
+    // and its count of ties.
+    __device__ __forceinline__ void set_parts(double kept, uint32_t ties) {
         kept = wave_sum_d(kept);
         ties = wave_sum_u(ties);
         __syncthreads();
-        if (lane == 0) {
-            s.wave_sum[wave] = kept;
-            s.wave_count[wave] = ties;
+        if ((threadIdx.x & 63) == 0) {
+            s.wave_sum[threadIdx.x >> 6] = kept;
+            s.wave_count[threadIdx.x >> 6] = ties;
         }
+    }
+
+    // The token of {key > tau, or one of the first keep_ties of {key == tau},
+    // with a weight of at least min_w}, by the parts set before.
+    __device__ int search(float u, uint32_t tau, uint32_t keep_ties, double min_w, double& mass) {
+        double tau_w = keep_ties > 0 ? weight(value_of(tau)) : 0.0;
+        if (tau_w < min_w) tau_w = 0.0;
         if (threadIdx.x == 0) {
             s.token = 0x7FFFFFFF;
             s.last = -1;
@@ -454,7 +483,7 @@ struct Sampler {
         const int begin = part * row.span;
         int end = begin + row.span;
         if (end > row.vocab) end = row.vocab;
-        for (int first = begin; first < end; first += kThreads * kChunk) {
+        for (int first = begin; first < end; first += T * kChunk) {
             const int at = first + threadIdx.x * kChunk;
             float v[kChunk];
             double w[kChunk];
@@ -470,7 +499,7 @@ struct Sampler {
             }
             uint32_t all_ties = 0;
             if (keep_ties > 0) {
-                uint32_t rank = base_ties + block_before(s, __popc(tie), all_ties);
+                uint32_t rank = base_ties + block_before<T>(s, static_cast<uint32_t>(__popc(tie)), all_ties);
 #pragma unroll
                 for (int j = 0; j < kChunk; ++j) {
                     if (!(tie >> j & 1)) continue;
@@ -482,7 +511,7 @@ struct Sampler {
             double sum = 0.0, all = 0.0;
 #pragma unroll
             for (int j = 0; j < kChunk; ++j) sum += w[j];
-            double pos = base + block_before(s, sum, all);
+            double pos = base + block_before<T>(s, sum, all);
             base += all;
             int mine = 0x7FFFFFFF, last = -1;
 #pragma unroll
@@ -502,8 +531,9 @@ struct Sampler {
 };
 
 // kFilters: rows may have filters, or a temperature of 0.
-template <int DT, bool kFilters>
-__global__ __launch_bounds__(kThreads) void klp_sample_kernel(SampleParams p) {
+template <int DT, int T, bool kFilters>
+__global__ __launch_bounds__(T, 4) void klp_sample_kernel(SampleParams p) {
+    constexpr int kWaves = T / 64;
     __shared__ Shared s;
     const int64_t r = blockIdx.x;
     const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
@@ -528,14 +558,16 @@ __global__ __launch_bounds__(kThreads) void klp_sample_kernel(SampleParams p) {
     const bool by_k = top_k > 0 && top_k < vocab;
     const bool by_p = top_p < 1.0f;  // a NaN is no filter
     const bool by_m = min_p > 0.0f;
+    const uint32_t k_left = by_k ? static_cast<uint32_t>(top_k) : 0xFFFFFFFFu;
+    const double p_left = static_cast<double>(fmaxf(top_p, 0.0f));
     const double min_w = by_m ? fmin(static_cast<double>(min_p), 1.0) : 0.0;
 
     // Fixed point: sums of `vocab` weights of at most 1 stay below 2^63.
     int frac = 62 - (32 - __clz(vocab));
     if (frac > 44) frac = 44;
     const double c = kLog2eD / static_cast<double>(t);
-    Sampler<DT> sm{row, s, 0.0f, c, fminf(static_cast<float>(c), 1e30f),
-                   ldexp(1.0, 52 - frac)};
+    Sampler<DT, T> sm{row, s, 0.0f, c, fminf(static_cast<float>(c), 1e30f),
+                      ldexp(1.0, 52 - frac)};
 
     float top = -INFINITY;  // the largest logit; NaN where there is one
     auto over_row = [&]() {
@@ -564,8 +596,12 @@ __global__ __launch_bounds__(kThreads) void klp_sample_kernel(SampleParams p) {
         for (int i = 0; i < kWaves; ++i) v += s.wave_all[i];
         return v;
     };
-    int token;
-    double all = 0.0, mass;
+    auto finish = [&](int token, double all, double mass) {  // by one thread
+        const double y = sm.log2_weight(to_f32<DT>(row.x[token])) * kLn2D;
+        p.tokens[r] = token;
+        p.logp[r] = static_cast<float>(y - log(all));
+        p.sample_logp[r] = static_cast<float>(y - log(mass));
+    };
 
     if (!kFilters || (!by_k && !by_p && !by_m)) {
         // Weights relative to the largest of the first 64 logits; again, to the
@@ -590,9 +626,13 @@ __global__ __launch_bounds__(kThreads) void klp_sample_kernel(SampleParams p) {
             sm.top = top;
             add_up();
         }
-        token = sm.search(u, 0, 0, 0.0, sum, 0, mass);
-        all = mass;
-    } else {
+        sm.set_parts(sum, 0);
+        double mass;
+        const int token = sm.search(u, 0, 0, 0.0, mass);
+        if (threadIdx.x == 0) finish(token, mass, mass);
+        return;
+    }
+    if constexpr (kFilters) {
         row.each([&](int, const float (&v)[kChunk]) {
 #pragma unroll
             for (int j = 0; j < kChunk; ++j) top = fmax_nan(top, v[j]);
@@ -601,12 +641,14 @@ __global__ __launch_bounds__(kThreads) void klp_sample_kernel(SampleParams p) {
         if (!over_row()) return;
         sm.top = top + 0.0f;
         // What could be kept lies in buckets up to `bound`.
-        uint32_t bound = kBuckets - 1;
-        double share = 0.0;
+        constexpr float kPerBit = (kBuckets - 1) / kRangeBits;
+        uint32_t bound = kBuckets - 1, p_at = kBuckets;
+        double all = 0.0, share = 0.0;
         unsigned long long p_above = 0;
+        bool wide = false;  // top-p alone, with more than the list takes
         if (by_k) {
             sm.clear();
-            if (top_k <= kThreads) {
+            if (top_k <= T) {
                 if (thread_top != -INFINITY) atomicAdd(&s.count[sm.bucket(thread_top)], 1u);
             } else {
                 row.each([&](int, const float (&v)[kChunk]) {
@@ -615,181 +657,218 @@ __global__ __launch_bounds__(kThreads) void klp_sample_kernel(SampleParams p) {
                 });
             }
             __syncthreads();
-            find(s, false, static_cast<uint32_t>(top_k), 0.0);
+            find<T>(s, false, k_left, 0.0);
             // Fewer threads than top_k have a logit: no bound from them.
-            if (s.above_count + s.at_count >= static_cast<uint32_t>(top_k)) bound = s.at;
+            if (s.above_count + s.at_count >= k_left) bound = s.at;
         } else if (by_p) {
             sm.clear();
-            row.each([&](int, const float (&v)[kChunk]) {
+            row.each([&](int at, const float (&v)[kChunk]) {
+                const bool counted = (at / (64 * kChunk)) % kCountEvery == 0;
 #pragma unroll
                 for (int j = 0; j < kChunk; ++j) {
                     const double w = sm.weight(v[j]);
+                    const uint32_t b = sm.bucket(v[j]);
                     all += w;
-                    atomicAdd(&s.mass[sm.bucket(v[j])], sm.fixed(w));
+                    atomicAdd(&s.mass[b], sm.fixed(w));
+                    if (counted) atomicAdd(&s.count[b], 1u);
                 }
             });
             all = over_waves(all);
             // In fixed point; the first element is always kept.
-            share = fmax(static_cast<double>(fmaxf(top_p, 0.0f)) * all * ldexp(1.0, frac), 1.0);
-            find(s, true, 0, share);
-            bound = s.at;
+            share = fmax(p_left * all * ldexp(1.0, frac), 1.0);
+            find<T>(s, true, 0, share);
+            bound = p_at = s.at;
             p_above = s.above_mass;
+            wide = (s.above_count + s.at_count) * kCountEvery > kList * 3 / 4;
         }
         if (by_m && !(by_k && by_p)) {
             // One bucket on for the rounding of its border's logarithm.
-            const double b = -log2(min_w) * ((kBuckets - 1) / kRangeBits) + 1.0;
-            if (b < bound) bound = static_cast<uint32_t>(b);
+            const double b = -log2(min_w) * kPerBit + 1.0;
+            if (b < bound) {
+                bound = static_cast<uint32_t>(b);
+                wide = false;
+            }
         }
         __syncthreads();
         if (threadIdx.x == 0) s.n_list = 0;
         __syncthreads();
-        const float deep = bound < kBuckets - 1 ? static_cast<float>(bound + 1) : INFINITY;
-        const bool summed = !by_k && by_p;
-        row.each([&](int at, const float (&v)[kChunk]) {
-            float w[kChunk];
-            uint32_t in = 0;
+        auto append = [&](uint32_t in, int at, const float (&v)[kChunk]) {
+            // Past kList only the count matters, and not how far.
+            if (in == 0 || *static_cast<volatile uint32_t*>(&s.n_list) > kList) return;
+            uint32_t i = atomicAdd(&s.n_list, static_cast<uint32_t>(__popc(in)));
 #pragma unroll
             for (int j = 0; j < kChunk; ++j) {
-                const float d = sm.depth(v[j]);
-                w[j] = exp2_hw(-d);
-                if (d * ((kBuckets - 1) / kRangeBits) < deep && at + j < vocab) in |= 1u << j;
+                if (!(in >> j & 1)) continue;
+                if (i < kList) s.list[i] = make_uint2(~key_of(v[j]), at + j);
+                ++i;
             }
-            if (!summed)
-                all += static_cast<double>(((w[0] + w[1]) + (w[2] + w[3])) +
-                                           ((w[4] + w[5]) + (w[6] + w[7])));
-            if (in != 0) {
-                uint32_t i = atomicAdd(&s.n_list, static_cast<uint32_t>(__popc(in)));
+        };
+        double kept = 0.0;
+        if (wide) {
+            // What lies before the border's bucket is kept; the bucket's
+            // elements are listed.
+            row.each([&](int at, const float (&v)[kChunk]) {
+                uint32_t in = 0;
 #pragma unroll
                 for (int j = 0; j < kChunk; ++j) {
-                    if (!(in >> j & 1)) continue;
-                    if (i < kList) s.list[i] = make_uint2(~key_of(v[j]), at + j);
-                    ++i;
+                    const uint32_t b = sm.bucket(v[j]);
+                    if (b < bound) {
+                        const double w = sm.weight(v[j]);
+                        if (w >= min_w) kept += w;
+                    }
+                    if (b == bound && at + j < vocab) in |= 1u << j;
                 }
-            }
-        });
-        if (!summed) all = over_waves(all);
-        else __syncthreads();
+                append(in, at, v);
+            });
+            __syncthreads();
+        } else {
+            const float deep = bound < kBuckets - 1 ? static_cast<float>(bound + 1) : INFINITY;
+            const bool summed = !by_k && by_p;
+            row.each([&](int at, const float (&v)[kChunk]) {
+                float w[kChunk];
+                uint32_t in = 0;
+#pragma unroll
+                for (int j = 0; j < kChunk; ++j) {
+                    const float d = sm.depth(v[j]);
+                    w[j] = exp2_hw(-d);
+                    if (d * kPerBit < deep && at + j < vocab) in |= 1u << j;
+                }
+                if (!summed)
+                    all += static_cast<double>(((w[0] + w[1]) + (w[2] + w[3])) +
+                                               ((w[4] + w[5]) + (w[6] + w[7])));
+                append(in, at, v);
+            });
+            if (!summed) all = over_waves(all);
+            else __syncthreads();
+        }
         const uint32_t n = s.n_list;
-        if (n <= kList) {
+        if (!wide && n <= kSorted) {
+            if (wave != 0) return;
             // By falling value, then index: the kept ones are the first.
             sort_list(s, n);
-            const uint32_t at = threadIdx.x * kListPerThread;
-            double w[kListPerThread], sum = 0.0, total;
-            uint2 e[kListPerThread];
+            const uint32_t at = lane * kPerLane;
+            double w[kPerLane], sum = 0.0, total, mass;
+            uint2 e[kPerLane];
 #pragma unroll
-            for (int j = 0; j < kListPerThread; ++j) {
-                const uint32_t i = at + j;
-                const bool in = i < n && (!by_k || i < static_cast<uint32_t>(top_k));
-                e[j] = in ? s.list[i] : make_uint2(0xFFFFFFFFu, 0xFFFFFFFFu);
+            for (int j = 0; j < kPerLane; ++j) {
+                const bool in = at + j < n && at + j < k_left;
+                e[j] = in ? s.list[at + j] : make_uint2(0xFFFFFFFFu, 0xFFFFFFFFu);
                 w[j] = in ? sm.weight(value_of(~e[j].x)) : 0.0;
                 sum += w[j];
             }
-            double before = block_before(s, sum, total);
-            const double most = static_cast<double>(fmaxf(top_p, 0.0f)) * (by_k ? total : all);
-            uint32_t kept = 0;
-            double left = 0.0;
+            double before = wave_before(sum, total);
+            const double most = p_left * (by_k ? total : all);
+            uint32_t count = 0, n_kept;
 #pragma unroll
-            for (int j = 0; j < kListPerThread; ++j) {
+            for (int j = 0; j < kPerLane; ++j) {
                 const uint32_t i = at + j;
-                const bool in = i < n && (!by_k || i < static_cast<uint32_t>(top_k)) &&
-                                (i == 0 || ((!by_p || before < most) && w[j] >= min_w));
+                if (i < n && i < k_left &&
+                    (i == 0 || ((!by_p || before < most) && w[j] >= min_w)))
+                    ++count;
                 before += w[j];
-                if (!in) w[j] = 0.0;
-                else ++kept;
-                left += w[j];
             }
-            uint32_t n_kept;
-            block_before(s, kept, n_kept);
-            block_before(s, left, mass);
-            // By index: block_before's barriers lie behind the reads above.
+            wave_before(count, n_kept);
+            // By index.
 #pragma unroll
-            for (int j = 0; j < kListPerThread; ++j)
+            for (int j = 0; j < kPerLane; ++j)
                 if (at + j < n_kept) s.list[at + j] = make_uint2(e[j].y, e[j].x);
-            __syncthreads();
             sort_list(s, n_kept);
-            if (threadIdx.x == 0) {
-                s.token = 0x7FFFFFFF;
-                s.last = -1;
-            }
             sum = 0.0;
 #pragma unroll
-            for (int j = 0; j < kListPerThread; ++j) {
+            for (int j = 0; j < kPerLane; ++j) {
                 const bool in = at + j < n_kept;
                 e[j] = in ? s.list[at + j] : make_uint2(0, 0);
                 w[j] = in ? sm.weight(value_of(~e[j].y)) : 0.0;
                 sum += w[j];
             }
-            double pos = block_before(s, sum, total);
-            const double target = static_cast<double>(u) * total;
+            double pos = wave_before(sum, mass);
+            const double target = static_cast<double>(u) * mass;
+            int token = 0x7FFFFFFF, last = -1;
 #pragma unroll
-            for (int j = 0; j < kListPerThread; ++j) {
+            for (int j = 0; j < kPerLane; ++j) {
                 pos += w[j];
                 if (w[j] <= kNothing) continue;
-                if (pos > target) atomicMin(&s.token, static_cast<int>(e[j].x));
-                atomicMax(&s.last, static_cast<int>(e[j].x));
+                last = static_cast<int>(e[j].x);
+                if (pos > target) token = min(token, last);
+            }
+#pragma unroll
+            for (int o = 32; o > 0; o >>= 1) {
+                token = min(token, __shfl_xor(token, o, 64));
+                last = max(last, __shfl_xor(last, o, 64));
+            }
+            if (lane == 0) finish(token != 0x7FFFFFFF ? token : last, all, mass);
+            return;
+        }
+        const bool listed = n <= kList;
+        uint32_t tau = 0, keep_ties = 0;
+        if (by_k) {
+            sm.clear();
+            sm.candidates(listed, [&](uint32_t k) {
+                atomicAdd(&s.count[sm.bucket(value_of(k))], 1u);
+            });
+            __syncthreads();
+            find<T>(s, false, k_left, 0.0);
+            const uint32_t b = s.at, above = s.above_count;
+            const Border k = sm.resolve(listed, b, 0, above, 0, false, k_left, 0.0);
+            tau = k.tau;
+            // A list may end before top_k: what is not in it has no weight.
+            keep_ties = min(k_left - k.above, k.ties);
+        }
+        // Where min-p's bound lies before top-p's border, that keeps all.
+        if (by_p && (by_k || bound == p_at)) {
+            const uint32_t floor = tau, most_ties = keep_ties;
+            if (by_k) {
+                // The masses of K.
+                sm.clear();
+                double part = 0.0;
+                sm.candidates(listed, [&](uint32_t k) {
+                    if (k <= tau) return;
+                    const double w = sm.weight(value_of(k));
+                    part += w;
+                    atomicAdd(&s.mass[sm.bucket(value_of(k))], sm.fixed(w));
+                });
+                if (threadIdx.x == 0) {
+                    const double w = sm.weight(value_of(tau));
+                    part += keep_ties * w;
+                    atomicAdd(&s.mass[sm.bucket(value_of(tau))], keep_ties * sm.fixed(w));
+                }
+                share = fmax(p_left * over_waves(part) * ldexp(1.0, frac), 1.0);
+                find<T>(s, true, 0, share);
+                p_at = s.at;
+                p_above = s.above_mass;
+            }
+            const Border q = sm.resolve(listed, p_at, floor, 0, p_above, true, 0, share);
+            tau = q.tau;
+            const double one = static_cast<double>(sm.fixed(sm.weight(value_of(tau))));
+            const double left = share - static_cast<double>(q.above_mass);
+            const double need = one > 0.0 ? ceil(left / one) : 1.0;
+            uint32_t limit = q.ties;
+            if (by_k && tau == floor) limit = min(limit, most_ties);
+            keep_ties = need < 1.0 ? 1u : need < limit ? static_cast<uint32_t>(need) : limit;
+        }
+        uint32_t ties = 0;
+        if (listed) {
+            // The list's kept weights by part of the row, in fixed point.
+            __syncthreads();
+            sm.clear();
+            for (uint32_t i = threadIdx.x; i < n; i += T) {
+                const uint32_t k = ~s.list[i].x;
+                if (k < tau) continue;
+                const int part = static_cast<int>(s.list[i].y) / row.span;
+                if (k == tau) {
+                    atomicAdd(&s.count[part], 1u);
+                } else {
+                    const double w = sm.weight(value_of(k));
+                    if (w >= min_w) atomicAdd(&s.mass[part], sm.fixed(w));
+                }
             }
             __syncthreads();
-            token = s.token != 0x7FFFFFFF ? s.token : s.last;
+            if (lane == 0) {
+                kept += static_cast<double>(s.mass[wave]) * ldexp(1.0, -frac);
+                ties = s.count[wave];
+            }
         } else {
-            uint32_t tau = 0, keep_ties = 0;
-            if (by_k) {
-                sm.clear();
-                row.each([&](int at, const float (&v)[kChunk]) {
-#pragma unroll
-                    for (int j = 0; j < kChunk; ++j)
-                        if (at + j < vocab) atomicAdd(&s.count[sm.bucket(v[j])], 1u);
-                });
-                __syncthreads();
-                find(s, false, static_cast<uint32_t>(top_k), 0.0);
-                const uint32_t b = s.at, above = s.above_count;
-                const Border k = sm.resolve(b, 0, above, 0, false, static_cast<uint32_t>(top_k),
-                                            0.0);
-                tau = k.tau;
-                keep_ties = static_cast<uint32_t>(top_k) - k.above;
-            }
-            if (by_p) {
-                uint32_t b = bound;
-                const uint32_t floor = tau, most_ties = keep_ties;
-                if (by_k) {
-                    // The masses of K.
-                    sm.clear();
-                    double part = 0.0, total;
-                    row.each([&](int, const float (&v)[kChunk]) {
-#pragma unroll
-                        for (int j = 0; j < kChunk; ++j) {
-                            if (key_of(v[j]) <= tau) continue;
-                            const double w = sm.weight(v[j]);
-                            part += w;
-                            atomicAdd(&s.mass[sm.bucket(v[j])], sm.fixed(w));
-                        }
-                    });
-                    const double tau_w = sm.weight(value_of(tau));
-                    if (threadIdx.x == 0) {
-                        part += keep_ties * tau_w;
-                        atomicAdd(&s.mass[sm.bucket(value_of(tau))], keep_ties * sm.fixed(tau_w));
-                    }
-                    total = over_waves(part);
-                    share = fmax(static_cast<double>(fmaxf(top_p, 0.0f)) * total *
-                                     ldexp(1.0, frac), 1.0);
-                    find(s, true, 0, share);
-                    b = s.at;
-                    p_above = s.above_mass;
-                } else {
-                    // `bound` may be min-p's by now.
-                    find(s, true, 0, share);
-                    b = s.at;
-                }
-                const Border q = sm.resolve(b, floor, 0, p_above, true, 0, share);
-                tau = q.tau;
-                const double one = static_cast<double>(sm.fixed(sm.weight(value_of(tau))));
-                const double left = share - static_cast<double>(q.above_mass);
-                const double need = one > 0.0 ? ceil(left / one) : 1.0;
-                uint32_t limit = q.ties;
-                if (by_k && tau == floor) limit = min(limit, most_ties);
-                keep_ties = need < 1.0 ? 1u : need < limit ? static_cast<uint32_t>(need) : limit;
-            }
-            double kept = 0.0;
-            uint32_t ties = 0;
+            kept = 0.0;
             row.each([&](int, const float (&v)[kChunk]) {
 #pragma unroll
                 for (int j = 0; j < kChunk; ++j) {
@@ -803,14 +882,11 @@ __global__ __launch_bounds__(kThreads) void klp_sample_kernel(SampleParams p) {
                     }
                 }
             });
-            token = sm.search(u, tau, keep_ties, min_w, kept, ties, mass);
         }
-    }
-    if (threadIdx.x == 0) {
-        const double y = sm.log2_weight(to_f32<DT>(row.x[token])) * kLn2D;
-        p.tokens[r] = token;
-        p.logp[r] = static_cast<float>(y - log(all));
-        p.sample_logp[r] = static_cast<float>(y - log(mass));
+        sm.set_parts(kept, ties);
+        double mass;
+        const int token = sm.search(u, tau, keep_ties, min_w, mass);
+        if (threadIdx.x == 0) finish(token, all, mass);
     }
 }
 
@@ -818,16 +894,25 @@ __global__ __launch_bounds__(kThreads) void klp_sample_kernel(SampleParams p) {
 
 namespace {
 
+template <int DT, int T>
+hipError_t launch_sample_threads(bool plain, const SampleParams& p, hipStream_t stream) {
+    const dim3 grid(static_cast<unsigned>(p.n_rows));
+    if (plain)
+        return launch_kernel(klp_sample_kernel<DT, T, false>, grid, dim3(T), stream, p);
+    return launch_kernel(klp_sample_kernel<DT, T, true>, grid, dim3(T), stream, p);
+}
+
 template <int DT>
 hipError_t launch_sample_dt(const SampleParams& p, hipStream_t stream) {
-    const dim3 grid(static_cast<unsigned>(p.n_rows));
     const bool plain = p.temperatures == nullptr && p.top_ks == nullptr && p.top_ps == nullptr &&
                        p.min_ps == nullptr && p.temperature != 0.0f &&
                        !(p.top_k > 0 && p.top_k < p.vocab) && !(p.top_p < 1.0f) &&
                        !(p.min_p > 0.0f);
-    if (plain)
-        return launch_kernel(klp_sample_kernel<DT, false>, grid, dim3(kThreads), stream, p);
-    return launch_kernel(klp_sample_kernel<DT, true>, grid, dim3(kThreads), stream, p);
+#ifdef KLP_ST
+    return launch_sample_threads<DT, KLP_ST>(plain, p, stream);
+#endif
+    if (p.n_rows > kHeadGemmCus) return launch_sample_threads<DT, 512>(plain, p, stream);
+    return launch_sample_threads<DT, 1024>(plain, p, stream);
 }
 
 }  // namespace
