@@ -13,7 +13,8 @@
 // the whole row crosses a border, and a row of 10^5 comparable weights has
 // 10^5 such borders: sums off by 10^-7 (float32) pick another token in one of
 // 100 rows.  So weights are computed in float64 (2^f by a polynomial of
-// degree 8, off by 2 10^-12 at most) and added in float64, or, in histograms,
+// degree 7, off by 10^-10 at most and, its error changing sign over f, far less
+// in a sum) and added in float64, or, in histograms,
 // as 64-bit integers of 2^-44, whose sums do not depend on the order of the
 // atomics.
 //
@@ -25,7 +26,8 @@
 // by value it gives the kept set, sorted by index the token.  What could be
 // kept is bounded beforehand by a bucket of a scale that is linear in y: for
 // top-k the bucket of the k-th largest of the threads' maxima (k of the logits
-// are at least that large), for min-p that of its border, for top-p without a
+// are at least that large; for a k above a quarter of the threads a histogram
+// of the counts, since the k-th of few maxima is low), for min-p that of its border, for top-p without a
 // top-k that in which a histogram of the masses, one more pass, reaches top_p.
 //   Where the list overflows (more than 4096 logits above the bound: a row of
 // equal logits, a wide nucleus) the kept set is {key > tau} and the first r of
@@ -40,6 +42,9 @@ namespace klp {
 
 namespace {
 
+#ifndef KLP_OCC
+#define KLP_OCC 6
+#endif
 constexpr int kMaxWaves = 16;
 constexpr int kBucketBits = 11;
 constexpr int kBuckets = 1 << kBucketBits;
@@ -69,16 +74,22 @@ __device__ __forceinline__ double exp2_d(double y) {
     y = fmax(y, -1000.0);
     const double z = y + kRound;
     const double f = y - (z - kRound);
-    double q = 0x1.63b2dp-20;
-    q = fma(q, f, 0x1.00c0e454p-16);
-    q = fma(q, f, 0x1.4308c71ep-13);
-    q = fma(q, f, 0x1.5d87759912p-10);
-    q = fma(q, f, 0x1.3b2ab70adp-7);
-    q = fma(q, f, 0x1.c6b08da70c1c8p-5);
-    q = fma(q, f, 0x1.ebfbdff82a73dp-3);
-    q = fma(q, f, 0x1.62e42fef9cc6cp-1);
+    double q = 0x1.00a581cp-16;
+    q = fma(q, f, 0x1.443fffc96db6ep-13);
+    q = fma(q, f, 0x1.5d879eac8p-10);
+    q = fma(q, f, 0x1.3b2a1b71525b6p-7);
+    q = fma(q, f, 0x1.c6b08d883e1b7p-5);
+    q = fma(q, f, 0x1.ebfbe045f4d3ep-3);
+    q = fma(q, f, 0x1.62e42fefa39efp-1);
     const double r = fma(q, f, 1.0);
     return __hiloint2double(__double2hiint(r) + (__double2loint(z) << 20), __double2loint(r));
+}
+
+// The largest, a NaN where there is one: three operands an instruction.
+__device__ __forceinline__ float chunk_max(const float (&v)[kChunk]) {
+    const float a = fmax_nan(fmax_nan(v[0], v[1]), v[2]);
+    const float b = fmax_nan(fmax_nan(v[3], v[4]), v[5]);
+    return fmax_nan(fmax_nan(a, b), fmax_nan(v[6], v[7]));
 }
 
 // Bits in the order of the values; -0 becomes +0, which it equals.
@@ -90,10 +101,13 @@ __device__ __forceinline__ float value_of(uint32_t key) {
     return __uint_as_float(key & 0x80000000u ? key ^ 0x80000000u : ~key);
 }
 
+// kFilters: with the histograms and the list, which leave room for two
+// workgroups of 512 threads a CU; without them registers set their number.
+template <bool kFilters>
 struct Shared {
-    uint32_t count[kBuckets];
-    unsigned long long mass[kBuckets];
-    uint2 list[kList];  // x before y in the order of a sort
+    uint32_t count[kFilters ? kBuckets : 1];
+    unsigned long long mass[kFilters ? kBuckets : 1];
+    uint2 list[kFilters ? kList : 1];  // x before y in the order of a sort
     unsigned long long wave_mass[kMaxWaves];
     double wave_sum[kMaxWaves];
     double wave_all[kMaxWaves];
@@ -119,8 +133,8 @@ __device__ __forceinline__ uint32_t wave_sum_u(uint32_t v) {
 }
 
 // What the threads before this one have of v; `total`: what all have.
-template <int T>
-__device__ __forceinline__ double block_before(Shared& s, double v, double& total) {
+template <int T, typename S>
+__device__ __forceinline__ double block_before(S& s, double v, double& total) {
     constexpr int kWaves = T / 64;
     const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
     double run = v;
@@ -141,8 +155,8 @@ __device__ __forceinline__ double block_before(Shared& s, double v, double& tota
     }
     return before;
 }
-template <int T>
-__device__ __forceinline__ uint32_t block_before(Shared& s, uint32_t v, uint32_t& total) {
+template <int T, typename S>
+__device__ __forceinline__ uint32_t block_before(S& s, uint32_t v, uint32_t& total) {
     constexpr int kWaves = T / 64;
     const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
     uint32_t run = v;
@@ -174,32 +188,40 @@ struct Row {
     __device__ __forceinline__ void load(int at, float (&v)[kChunk]) const {
         load_chunk<DT>(x + at, vocab - at, -INFINITY, v);
     }
-    // f(first element, 8 values) for each chunk of this wave's part, kBatch of
-    // them loaded at a time.  Values behind the row's end are -inf.
+    // f(first element, 8 values) for each chunk of this wave's part, the next
+    // kBatch of them being loaded.  Values behind the row's end are -inf.
     template <typename F>
     __device__ __forceinline__ void each(F f) const {
         const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
         constexpr int kStep = 64 * kChunk;
-        const int begin = wave * span + lane * kChunk;
-        int end = (wave + 1) * span;
+        const int begin = wave * span;
+        int end = begin + span;
         if (end > vocab) end = vocab;
         typedef Unaligned16<elem> Vec;
         constexpr int kVecs = DT == kFP32 ? 2 : 1;
-        int at = begin;
-        // Whole batches: the last chunk of the last lane included.
-        for (; at - lane * kChunk + kBatch * kStep <= end; at += kBatch * kStep) {
+        const int batches = end > begin ? (end - begin) / (kBatch * kStep) : 0;
+        int at = begin + lane * kChunk;
+        if (batches > 0) {
             u32x4 raw[kBatch][kVecs];
-#pragma unroll
-            for (int i = 0; i < kBatch; ++i)
+            auto fetch = [&](int i, int from) {
 #pragma unroll
                 for (int k = 0; k < kVecs; ++k)
-                    raw[i][k] = reinterpret_cast<const Vec*>(x + at + i * kStep)[k].v;
+                    raw[i][k] = reinterpret_cast<const Vec*>(x + from + i * kStep)[k].v;
+            };
 #pragma unroll
-            for (int i = 0; i < kBatch; ++i) {
-                float v[kChunk];
-                unpack<DT>(raw[i][0], v);
-                if constexpr (DT == kFP32) unpack<DT>(raw[i][1], v + 4);
-                f(at + i * kStep, v);
+            for (int i = 0; i < kBatch; ++i) fetch(i, at);
+            for (int b = 1; b <= batches; ++b) {
+                const int next = b < batches ? at + kBatch * kStep : at;  // or the last again
+#pragma unroll
+                for (int i = 0; i < kBatch; ++i) {
+                    float v[kChunk];
+                    unpack<DT>(raw[i][0], v);
+                    if constexpr (DT == kFP32) unpack<DT>(raw[i][1], v + 4);
+                    fetch(i, next);
+                    f(at + i * kStep, v);
+                    __builtin_amdgcn_sched_barrier(0);
+                }
+                at += kBatch * kStep;
             }
         }
         for (; at < end; at += kStep) {
@@ -214,7 +236,7 @@ struct Row {
 // with by_mass, the running mass reaches `mass`); the last one with anything
 // in it when none does.  Into s.at, with what lies before it.
 template <int T>
-__device__ void find(Shared& s, bool by_mass, uint32_t count, double mass) {
+__device__ void find(Shared<true>& s, bool by_mass, uint32_t count, double mass) {
     constexpr int kWaves = T / 64, kPerThread = kBuckets / T;
     const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
     const int first = threadIdx.x * kPerThread;
@@ -292,7 +314,7 @@ __device__ __forceinline__ V wave_before(V v, V& total) {
 
 // The first `n` <= kSorted entries of the list in order: a bitonic sort by one
 // wave, whose LDS accesses take effect in program order.
-__device__ void sort_list(Shared& s, uint32_t n) {
+__device__ void sort_list(Shared<true>& s, uint32_t n) {
     const uint32_t lane = threadIdx.x & 63;
     uint32_t size = 2;
     while (size < n) size <<= 1;
@@ -326,18 +348,21 @@ struct Border {
 };
 
 // What a row's passes share.
-template <int DT, int T>
+template <int DT, int T, bool kFilters>
 struct Sampler {
     static constexpr int kWaves = T / 64, kPerThread = kBuckets / T;
     Row<DT> row;
-    Shared& s;
+    Shared<kFilters>& s;
     float top;           // weights are relative to this logit
     double c;            // log2(e) / T
     float c32;
     double fixed_one;    // added to a weight, it leaves its fixed-point value in the low bits
 
+    // Exactly 0 for x = top, whose weight is exactly 1.  16-bit logits have 11
+    // bits at most and their c 42: both products are exact.
     __device__ __forceinline__ double log2_weight(float x) const {
-        return (static_cast<double>(x) - static_cast<double>(top)) * c;
+        if constexpr (DT == kFP32) return (static_cast<double>(x) - static_cast<double>(top)) * c;
+        return fma(static_cast<double>(x), c, -static_cast<double>(top) * c);
     }
     __device__ __forceinline__ double weight(float x) const {
         return exp2_d(log2_weight(x));
@@ -532,9 +557,9 @@ struct Sampler {
 
 // kFilters: rows may have filters, or a temperature of 0.
 template <int DT, int T, bool kFilters>
-__global__ __launch_bounds__(T, 4) void klp_sample_kernel(SampleParams p) {
+__global__ __launch_bounds__(T, kFilters ? 4 : KLP_OCC) void klp_sample_kernel(SampleParams p) {
     constexpr int kWaves = T / 64;
-    __shared__ Shared s;
+    __shared__ Shared<kFilters> s;
     const int64_t r = blockIdx.x;
     const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
     const int vocab = static_cast<int>(p.vocab);
@@ -565,8 +590,10 @@ __global__ __launch_bounds__(T, 4) void klp_sample_kernel(SampleParams p) {
     // Fixed point: sums of `vocab` weights of at most 1 stay below 2^63.
     int frac = 62 - (32 - __clz(vocab));
     if (frac > 44) frac = 44;
-    const double c = kLog2eD / static_cast<double>(t);
-    Sampler<DT, T> sm{row, s, 0.0f, c, fminf(static_cast<float>(c), 1e30f),
+    double c = kLog2eD / static_cast<double>(t);
+    if constexpr (DT != kFP32)  // 42 bits, 2^-42 of it off at most
+        c = __longlong_as_double(__double_as_longlong(c) & ~0x7FFll);
+    Sampler<DT, T, kFilters> sm{row, s, 0.0f, c, fminf(static_cast<float>(c), 1e30f),
                       ldexp(1.0, 52 - frac)};
 
     float top = -INFINITY;  // the largest logit; NaN where there is one
@@ -613,11 +640,9 @@ __global__ __launch_bounds__(T, 4) void klp_sample_kernel(SampleParams p) {
         auto add_up = [&]() {
             sum = 0.0;
             row.each([&](int, const float (&v)[kChunk]) {
+                top = fmax_nan(top, chunk_max(v));
 #pragma unroll
-                for (int j = 0; j < kChunk; ++j) {
-                    top = fmax_nan(top, v[j]);
-                    sum += sm.weight(v[j]);
-                }
+                for (int j = 0; j < kChunk; ++j) sum += sm.weight(v[j]);
             });
         };
         add_up();
@@ -633,10 +658,7 @@ __global__ __launch_bounds__(T, 4) void klp_sample_kernel(SampleParams p) {
         return;
     }
     if constexpr (kFilters) {
-        row.each([&](int, const float (&v)[kChunk]) {
-#pragma unroll
-            for (int j = 0; j < kChunk; ++j) top = fmax_nan(top, v[j]);
-        });
+        row.each([&](int, const float (&v)[kChunk]) { top = fmax_nan(top, chunk_max(v)); });
         const float thread_top = top;
         if (!over_row()) return;
         sm.top = top + 0.0f;
@@ -648,7 +670,7 @@ __global__ __launch_bounds__(T, 4) void klp_sample_kernel(SampleParams p) {
         bool wide = false;  // top-p alone, with more than the list takes
         if (by_k) {
             sm.clear();
-            if (top_k <= T) {
+            if (top_k <= T / 4) {
                 if (thread_top != -INFINITY) atomicAdd(&s.count[sm.bucket(thread_top)], 1u);
             } else {
                 row.each([&](int, const float (&v)[kChunk]) {
