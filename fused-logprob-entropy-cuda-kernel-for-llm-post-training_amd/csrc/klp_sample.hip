@@ -117,8 +117,8 @@ struct Shared {
     // find()'s answer
     uint32_t at, at_count, above_count;
     unsigned long long above_mass;
-    // the token
-    int token, last;
+    // search()'s first and last thread with weight
+    int first, last;
 };
 
 __device__ __forceinline__ double wave_sum_d(double v) {
@@ -467,91 +467,98 @@ struct Sampler {
     }
 
     // The token of {key > tau, or one of the first keep_ties of {key == tau},
-    // with a weight of at least min_w}, by the parts set before.
+    // with a weight of at least min_w}, by the parts set before: the part whose
+    // running sum crosses the target, in it the thread whose run of elements
+    // does, and among those the element.  Where rounding (or u = 1) lets none
+    // cross, the last that has a weight.  The wave of that thread returns the
+    // token, the others -1.
     __device__ int search(float u, uint32_t tau, uint32_t keep_ties, double min_w, double& mass) {
+        const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
         double tau_w = keep_ties > 0 ? weight(value_of(tau)) : 0.0;
         if (tau_w < min_w) tau_w = 0.0;
         if (threadIdx.x == 0) {
-            s.token = 0x7FFFFFFF;
+            s.first = T;
             s.last = -1;
         }
         __syncthreads();
-        uint32_t ties_before = 0;
-        auto part_mass = [&](int i) {  // in order, from 0
-            const uint32_t n = s.wave_count[i];
-            const uint32_t left = keep_ties - min(keep_ties, ties_before);
-            ties_before += n;
-            return s.wave_sum[i] + min(n, left) * tau_w;
-        };
-        mass = 0.0;
-        for (int i = 0; i < kWaves; ++i) mass += part_mass(i);
+        // Lane i holds part i, in every wave.
+        uint32_t ties = lane < kWaves ? s.wave_count[lane] : 0, all_ties;
+        uint32_t rank = wave_before(ties, all_ties);
+        auto kept_ties = [&]() { return min(ties, keep_ties - min(keep_ties, rank)) * tau_w; };
+        double sum = (lane < kWaves ? s.wave_sum[lane] : 0.0) + kept_ties();
+        double pos = wave_before(sum, mass);
         const double target = static_cast<double>(u) * mass;
-        // The part in which the running sum crosses the target: the last one
-        // that holds anything if rounding (or u = 1) lets none.
-        int part = 0;
-        double base = 0.0, run = 0.0;
-        uint32_t base_ties = 0;
-        ties_before = 0;
-        for (int i = 0; i < kWaves; ++i) {
-            const uint32_t before = ties_before;
-            const double m = part_mass(i);
-            if (m > kNothing) {
-                part = i;
-                base = run;
-                base_ties = before;
-                if (run + m > target) break;
-            }
-            run += m;
-        }
+        auto choose = [&](bool has, bool crosses) {
+            const uint64_t c = __ballot(has && crosses), h = __ballot(has);
+            return c != 0 ? __ffsll(static_cast<unsigned long long>(c)) - 1
+                          : 63 - __clzll(static_cast<long long>(h));
+        };
+        const int part = choose(sum > kNothing, pos + sum > target);
+        if (part < 0) return wave == 0 ? 0 : -1;  // no weight at all: none of a row with a maximum
+        pos = __shfl(pos, part, 64);
+        rank = __shfl(rank, part, 64);
 
-        // That part again, 8 consecutive elements a thread.
-        const int begin = part * row.span;
-        int end = begin + row.span;
-        if (end > row.vocab) end = row.vocab;
-        for (int first = begin; first < end; first += T * kChunk) {
-            const int at = first + threadIdx.x * kChunk;
+        const int per = (row.span / kChunk + T - 1) / T * kChunk;  // elements a thread
+        const int end = min((part + 1) * row.span, row.vocab);
+        const int begin = part * row.span + static_cast<int>(threadIdx.x) * per;
+        sum = 0.0;
+        ties = 0;
+        for (int at = begin; at < begin + per && at < end; at += kChunk) {
             float v[kChunk];
-            double w[kChunk];
-            uint32_t tie = 0;  // a bit an element
-            row.load(at < end ? at : row.vocab, v);
+            row.load(at, v);
 #pragma unroll
             for (int j = 0; j < kChunk; ++j) {
+                if (at + j >= end) continue;
                 const uint32_t k = key_of(v[j]);
-                const bool in = at + j < end;
-                w[j] = in && k > tau ? weight(v[j]) : 0.0;
-                if (w[j] < min_w) w[j] = 0.0;
-                if (in && k == tau) tie |= 1u << j;
-            }
-            uint32_t all_ties = 0;
-            if (keep_ties > 0) {
-                uint32_t rank = base_ties + block_before<T>(s, static_cast<uint32_t>(__popc(tie)), all_ties);
-#pragma unroll
-                for (int j = 0; j < kChunk; ++j) {
-                    if (!(tie >> j & 1)) continue;
-                    if (rank < keep_ties) w[j] = tau_w;
-                    ++rank;
+                if (k > tau) {
+                    const double w = weight(v[j]);
+                    if (w >= min_w) sum += w;
                 }
-                base_ties += all_ties;
+                if (k == tau) ++ties;
             }
-            double sum = 0.0, all = 0.0;
-#pragma unroll
-            for (int j = 0; j < kChunk; ++j) sum += w[j];
-            double pos = base + block_before<T>(s, sum, all);
-            base += all;
-            int mine = 0x7FFFFFFF, last = -1;
-#pragma unroll
-            for (int j = 0; j < kChunk; ++j) {
-                pos += w[j];
-                if (w[j] > kNothing) {
-                    last = at + j;
-                    if (pos > target && mine == 0x7FFFFFFF) mine = at + j;
-                }
-            }
-            if (mine != 0x7FFFFFFF) atomicMin(&s.token, mine);
-            if (last >= 0) atomicMax(&s.last, last);
         }
+        double total;
+        if (keep_ties > 0) {
+            rank += block_before<T>(s, ties, all_ties);
+            sum += kept_ties();
+        }
+        pos += block_before<T>(s, sum, total);
+        const uint64_t has = __ballot(sum > kNothing);
+        const uint64_t crosses = __ballot(sum > kNothing && pos + sum > target);
+        if (lane == 0 && has != 0)
+            atomicMax(&s.last, wave * 64 + 63 - __clzll(static_cast<long long>(has)));
+        if (lane == 0 && crosses != 0)
+            atomicMin(&s.first, wave * 64 + __ffsll(static_cast<unsigned long long>(crosses)) - 1);
         __syncthreads();
-        return s.token != 0x7FFFFFFF ? s.token : s.last;
+        const int thread = s.first < T ? s.first : s.last;
+        if (thread < 0) return wave == 0 ? part * row.span : -1;
+        if (thread >> 6 != wave) return -1;
+        pos = __shfl(pos, thread & 63, 64);
+        rank = __shfl(rank, thread & 63, 64);
+
+        int token = -1;
+        const int first = __shfl(begin, thread & 63, 64), stop = min(first + per, end);
+        for (int from = first; from < stop; from += 64) {
+            const int at = from + lane;
+            const bool in = at < stop;
+            const float v = in ? to_f32<DT>(row.x[at]) : -INFINITY;
+            const uint32_t k = key_of(v);
+            double w = in && k > tau ? weight(v) : 0.0;
+            if (w < min_w) w = 0.0;
+            const uint64_t tie = __ballot(in && k == tau);
+            if (tie >> lane & 1) {
+                const uint32_t mine = rank + __popcll(tie & ((1ull << lane) - 1));
+                if (mine < keep_ties) w = tau_w;
+            }
+            rank += __popcll(tie);
+            const double before = pos + wave_before(w, total);
+            const int at_lane = choose(w > kNothing, before + w > target);
+            const bool found = __ballot(w > kNothing && before + w > target) != 0;
+            if (at_lane >= 0) token = from + at_lane;
+            if (found) break;
+            pos += total;
+        }
+        return token >= 0 ? token : first;
     }
 };
 
@@ -654,7 +661,7 @@ __global__ __launch_bounds__(T, kFilters ? 4 : KLP_OCC) void klp_sample_kernel(S
         sm.set_parts(sum, 0);
         double mass;
         const int token = sm.search(u, 0, 0, 0.0, mass);
-        if (threadIdx.x == 0) finish(token, mass, mass);
+        if (token >= 0 && lane == 0) finish(token, mass, mass);
         return;
     }
     if constexpr (kFilters) {
@@ -908,7 +915,7 @@ __global__ __launch_bounds__(T, kFilters ? 4 : KLP_OCC) void klp_sample_kernel(S
         sm.set_parts(kept, ties);
         double mass;
         const int token = sm.search(u, tau, keep_ties, min_w, mass);
-        if (threadIdx.x == 0) finish(token, all, mass);
+        if (token >= 0 && lane == 0) finish(token, all, mass);
     }
 }
 
