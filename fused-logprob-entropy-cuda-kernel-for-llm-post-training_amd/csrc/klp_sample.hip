@@ -49,15 +49,15 @@ constexpr int kMaxWaves = 16;
 constexpr int kBucketBits = 11;
 constexpr int kBuckets = 1 << kBucketBits;
 constexpr int kList = 4096;
-// What one wave sorts, a few entries a lane; longer lists go through histograms.
-constexpr int kSorted = 512;
-constexpr int kPerLane = kSorted / 64;
+// Lists whose entries are compared with each other; longer ones go through
+// histograms.
+constexpr int kRanked = 256;
 constexpr int kBatch = 4;  // chunks of a lane in flight
 // The histogram for top-p counts one of so many chunks, to foresee the list's length.
 constexpr int kCountEvery = 8;
-// Range of the first histogram, in units of log2 of the weight; lighter
-// elements share the last bucket.
-constexpr float kRangeBits = 44.0f;
+// Buckets of the first histogram to a factor of 2 of the weight; elements of
+// less than 2^-64 share the last bucket.
+constexpr int kPerBit = kBuckets / 64;
 constexpr double kLog2eD = 1.44269504088896340736;
 constexpr double kLn2D = 0.69314718055994530942;
 
@@ -121,59 +121,64 @@ struct Shared {
     int first, last;
 };
 
-__device__ __forceinline__ double wave_sum_d(double v) {
-#pragma unroll
-    for (int o = 32; o > 0; o >>= 1) v += __shfl_xor(v, o, 64);
+// v from the lane that DPP control Ctrl names, 0 where there is none.
+template <int Ctrl, int Rows>
+__device__ __forceinline__ uint32_t dpp_or_0(uint32_t v) {
+    return static_cast<uint32_t>(
+        __builtin_amdgcn_update_dpp(0, static_cast<int>(v), Ctrl, Rows, 0xF, false));
+}
+template <int Ctrl, int Rows>
+__device__ __forceinline__ unsigned long long dpp_or_0(unsigned long long v) {
+    const uint32_t lo = dpp_or_0<Ctrl, Rows>(static_cast<uint32_t>(v));
+    const uint32_t hi = dpp_or_0<Ctrl, Rows>(static_cast<uint32_t>(v >> 32));
+    return static_cast<unsigned long long>(hi) << 32 | lo;
+}
+template <int Ctrl, int Rows>
+__device__ __forceinline__ double dpp_or_0(double v) {
+    return __longlong_as_double(static_cast<long long>(
+        dpp_or_0<Ctrl, Rows>(static_cast<unsigned long long>(__double_as_longlong(v)))));
+}
+
+// What the lanes up to this one have of v: shifts within rows of 16 lanes,
+// then the first and third row's last lane to the row behind it, and the
+// second row's to the wave's second half.
+template <typename V>
+__device__ __forceinline__ V wave_scan(V v) {
+    v += dpp_or_0<0x111, 0xF>(v);
+    v += dpp_or_0<0x112, 0xF>(v);
+    v += dpp_or_0<0x114, 0xF>(v);
+    v += dpp_or_0<0x118, 0xF>(v);
+    v += dpp_or_0<0x142, 0xA>(v);
+    v += dpp_or_0<0x143, 0xC>(v);
     return v;
 }
-__device__ __forceinline__ uint32_t wave_sum_u(uint32_t v) {
-#pragma unroll
-    for (int o = 32; o > 0; o >>= 1) v += __shfl_xor(v, o, 64);
-    return v;
+// What the lanes before this one have of v; `total`: what the wave has.
+template <typename V>
+__device__ __forceinline__ V wave_before(V v, V& total) {
+    const V run = wave_scan(v);
+    total = __shfl(run, 63, 64);
+    return run - v;
+}
+template <typename V>
+__device__ __forceinline__ V wave_sum(V v) {
+    return __shfl(wave_scan(v), 63, 64);
 }
 
 // What the threads before this one have of v; `total`: what all have.
-template <int T, typename S>
-__device__ __forceinline__ double block_before(S& s, double v, double& total) {
+template <int T, typename V>
+__device__ __forceinline__ V block_before(V (&lds)[kMaxWaves], V v, V& total) {
     constexpr int kWaves = T / 64;
     const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
-    double run = v;
-#pragma unroll
-    for (int o = 1; o < 64; o <<= 1) {
-        const double x = __shfl_up(run, o, 64);
-        if (lane >= o) run += x;
-    }
+    const V run = wave_scan(v);
     __syncthreads();  // the last call's readers
-    if (lane == 63) s.wave_sum[wave] = run;
+    if (lane == 63) lds[wave] = run;
     __syncthreads();
-    double before = run - v;
-    total = 0.0;
-#pragma unroll
-    for (int i = 0; i < kWaves; ++i) {
-        if (i == wave) before += total;
-        total += s.wave_sum[i];
-    }
-    return before;
-}
-template <int T, typename S>
-__device__ __forceinline__ uint32_t block_before(S& s, uint32_t v, uint32_t& total) {
-    constexpr int kWaves = T / 64;
-    const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
-    uint32_t run = v;
-#pragma unroll
-    for (int o = 1; o < 64; o <<= 1) {
-        const uint32_t x = __shfl_up(run, o, 64);
-        if (lane >= o) run += x;
-    }
-    __syncthreads();
-    if (lane == 63) s.wave_count[wave] = run;
-    __syncthreads();
-    uint32_t before = run - v;
+    V before = run - v;
     total = 0;
 #pragma unroll
     for (int i = 0; i < kWaves; ++i) {
         if (i == wave) before += total;
-        total += s.wave_count[i];
+        total += lds[i];
     }
     return before;
 }
@@ -237,8 +242,7 @@ struct Row {
 // in it when none does.  Into s.at, with what lies before it.
 template <int T>
 __device__ void find(Shared<true>& s, bool by_mass, uint32_t count, double mass) {
-    constexpr int kWaves = T / 64, kPerThread = kBuckets / T;
-    const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
+    constexpr int kPerThread = kBuckets / T;
     const int first = threadIdx.x * kPerThread;
     uint32_t c[kPerThread], c_sum = 0;
     unsigned long long m[kPerThread], m_sum = 0;
@@ -249,35 +253,10 @@ __device__ void find(Shared<true>& s, bool by_mass, uint32_t count, double mass)
         c_sum += c[i];
         m_sum += m[i];
     }
-    uint32_t c_run = c_sum;
-    unsigned long long m_run = m_sum;
-#pragma unroll
-    for (int o = 1; o < 64; o <<= 1) {
-        const uint32_t cu = __shfl_up(c_run, o, 64);
-        const unsigned long long mu = __shfl_up(m_run, o, 64);
-        if (lane >= o) {
-            c_run += cu;
-            m_run += mu;
-        }
-    }
-    if (lane == 63) {
-        s.wave_count[wave] = c_run;
-        s.wave_mass[wave] = m_run;
-    }
-    __syncthreads();
-    uint32_t c_all = 0;
-    unsigned long long m_all = 0;
-    c_run -= c_sum;
-    m_run -= m_sum;
-#pragma unroll
-    for (int i = 0; i < kWaves; ++i) {
-        if (i == wave) {
-            c_run += c_all;
-            m_run += m_all;
-        }
-        c_all += s.wave_count[i];
-        m_all += s.wave_mass[i];
-    }
+    uint32_t c_all;
+    unsigned long long m_all;
+    uint32_t c_run = block_before<T>(s.wave_count, c_sum, c_all);
+    unsigned long long m_run = block_before<T>(s.wave_mass, m_sum, m_all);
     // A target that rounding left above the total is the total.
     const double want = fmin(mass, static_cast<double>(m_all));
     count = min(count, c_all);
@@ -296,48 +275,6 @@ __device__ void find(Shared<true>& s, bool by_mass, uint32_t count, double mass)
         m_run += m[i];
     }
     __syncthreads();
-}
-
-// What the lanes before this one have of v; `total`: what the wave has.
-template <typename V>
-__device__ __forceinline__ V wave_before(V v, V& total) {
-    const int lane = threadIdx.x & 63;
-    V run = v;
-#pragma unroll
-    for (int o = 1; o < 64; o <<= 1) {
-        const V x = __shfl_up(run, o, 64);
-        if (lane >= o) run += x;
-    }
-    total = __shfl(run, 63, 64);
-    return run - v;
-}
-
-// The first `n` <= kSorted entries of the list in order: a bitonic sort by one
-// wave, whose LDS accesses take effect in program order.
-__device__ void sort_list(Shared<true>& s, uint32_t n) {
-    const uint32_t lane = threadIdx.x & 63;
-    uint32_t size = 2;
-    while (size < n) size <<= 1;
-    for (uint32_t i = n + lane; i < size; i += 64)
-        s.list[i] = make_uint2(0xFFFFFFFFu, 0xFFFFFFFFu);
-    for (uint32_t width = 2; width <= size; width <<= 1) {
-        for (uint32_t step = width >> 1; step > 0; step >>= 1) {
-            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-            __builtin_amdgcn_wave_barrier();
-            for (uint32_t t = lane; t < size / 2; t += 64) {
-                const uint32_t i = 2 * t - (t & (step - 1));
-                const uint2 a = s.list[i], b = s.list[i + step];
-                const bool up = (i & width) == 0;
-                const bool less = b.x < a.x || (b.x == a.x && b.y < a.y);
-                if (less == up) {
-                    s.list[i] = b;
-                    s.list[i + step] = a;
-                }
-            }
-        }
-    }
-    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-    __builtin_amdgcn_wave_barrier();
 }
 
 struct Border {
@@ -371,12 +308,14 @@ struct Sampler {
         return static_cast<unsigned long long>(__double_as_longlong(w + fixed_one)) &
                ((1ull << 52) - 1);
     }
-    // -log2 of the weight in float32, and in buckets: monotone in x, so that
-    // equal logits share a bucket.
-    __device__ __forceinline__ float depth(float x) const { return (top - x) * c32; }
+    // By -log2 of the weight, which adding 1.5 2^52 / kPerBit rounds to whole
+    // buckets: monotone in x, so that equal logits share one.
+    __device__ __forceinline__ uint32_t bucket_of(double log2_w) const {
+        const int n = __double2loint(fmax(log2_w, -1000.0) + 0x1.8p52 / kPerBit);
+        return static_cast<uint32_t>(min(-n, kBuckets - 1));
+    }
     __device__ __forceinline__ uint32_t bucket(float x) const {
-        return static_cast<uint32_t>(
-            fminf(depth(x) * ((kBuckets - 1) / kRangeBits), kBuckets - 1.0f));
+        return bucket_of(log2_weight(x));
     }
     __device__ __forceinline__ void clear() {
 #pragma unroll
@@ -457,8 +396,8 @@ struct Sampler {
     // Each wave's part of the row: its sum of kept weights above the border,
     // and its count of ties.
     __device__ __forceinline__ void set_parts(double kept, uint32_t ties) {
-        kept = wave_sum_d(kept);
-        ties = wave_sum_u(ties);
+        kept = wave_sum(kept);
+        ties = wave_sum(ties);
         __syncthreads();
         if ((threadIdx.x & 63) == 0) {
             s.wave_sum[threadIdx.x >> 6] = kept;
@@ -519,10 +458,10 @@ struct Sampler {
         }
         double total;
         if (keep_ties > 0) {
-            rank += block_before<T>(s, ties, all_ties);
+            rank += block_before<T>(s.wave_count, ties, all_ties);
             sum += kept_ties();
         }
-        pos += block_before<T>(s, sum, total);
+        pos += block_before<T>(s.wave_sum, sum, total);
         const uint64_t has = __ballot(sum > kNothing);
         const uint64_t crosses = __ballot(sum > kNothing && pos + sum > target);
         if (lane == 0 && has != 0)
@@ -621,7 +560,7 @@ __global__ __launch_bounds__(T, kFilters ? 4 : KLP_OCC) void klp_sample_kernel(S
         return false;
     };
     auto over_waves = [&](double v) {
-        v = wave_sum_d(v);
+        v = wave_sum(v);
         __syncthreads();
         if (lane == 0) s.wave_all[wave] = v;
         __syncthreads();
@@ -630,11 +569,12 @@ __global__ __launch_bounds__(T, kFilters ? 4 : KLP_OCC) void klp_sample_kernel(S
         for (int i = 0; i < kWaves; ++i) v += s.wave_all[i];
         return v;
     };
-    auto finish = [&](int token, double all, double mass) {  // by one thread
+    // By an even lane and the next one, each with one of the logarithms.
+    auto finish = [&](int token, double all, double mass) {
         const double y = sm.log2_weight(to_f32<DT>(row.x[token])) * kLn2D;
-        p.tokens[r] = token;
-        p.logp[r] = static_cast<float>(y - log(all));
-        p.sample_logp[r] = static_cast<float>(y - log(mass));
+        const float out = static_cast<float>(y - log(lane & 1 ? mass : all));
+        (lane & 1 ? p.sample_logp : p.logp)[r] = out;
+        if (!(lane & 1)) p.tokens[r] = token;
     };
 
     if (!kFilters || (!by_k && !by_p && !by_m)) {
@@ -661,7 +601,7 @@ __global__ __launch_bounds__(T, kFilters ? 4 : KLP_OCC) void klp_sample_kernel(S
         sm.set_parts(sum, 0);
         double mass;
         const int token = sm.search(u, 0, 0, 0.0, mass);
-        if (token >= 0 && lane == 0) finish(token, mass, mass);
+        if (token >= 0 && lane < 2) finish(token, mass, mass);
         return;
     }
     if constexpr (kFilters) {
@@ -670,7 +610,6 @@ __global__ __launch_bounds__(T, kFilters ? 4 : KLP_OCC) void klp_sample_kernel(S
         if (!over_row()) return;
         sm.top = top + 0.0f;
         // What could be kept lies in buckets up to `bound`.
-        constexpr float kPerBit = (kBuckets - 1) / kRangeBits;
         uint32_t bound = kBuckets - 1, p_at = kBuckets;
         double all = 0.0, share = 0.0;
         unsigned long long p_above = 0;
@@ -695,8 +634,9 @@ __global__ __launch_bounds__(T, kFilters ? 4 : KLP_OCC) void klp_sample_kernel(S
                 const bool counted = (at / (64 * kChunk)) % kCountEvery == 0;
 #pragma unroll
                 for (int j = 0; j < kChunk; ++j) {
-                    const double w = sm.weight(v[j]);
-                    const uint32_t b = sm.bucket(v[j]);
+                    const double y = sm.log2_weight(v[j]);
+                    const double w = exp2_d(y);
+                    const uint32_t b = sm.bucket_of(y);
                     all += w;
                     atomicAdd(&s.mass[b], sm.fixed(w));
                     if (counted) atomicAdd(&s.count[b], 1u);
@@ -712,7 +652,7 @@ __global__ __launch_bounds__(T, kFilters ? 4 : KLP_OCC) void klp_sample_kernel(S
         }
         if (by_m && !(by_k && by_p)) {
             // One bucket on for the rounding of its border's logarithm.
-            const double b = -log2(min_w) * kPerBit + 1.0;
+            const double b = 1.0 - log2(min_w) * kPerBit;
             if (b < bound) {
                 bound = static_cast<uint32_t>(b);
                 wide = false;
@@ -740,9 +680,10 @@ __global__ __launch_bounds__(T, kFilters ? 4 : KLP_OCC) void klp_sample_kernel(S
                 uint32_t in = 0;
 #pragma unroll
                 for (int j = 0; j < kChunk; ++j) {
-                    const uint32_t b = sm.bucket(v[j]);
+                    const double y = sm.log2_weight(v[j]);
+                    const uint32_t b = sm.bucket_of(y);
                     if (b < bound) {
-                        const double w = sm.weight(v[j]);
+                        const double w = exp2_d(y);
                         if (w >= min_w) kept += w;
                     }
                     if (b == bound && at + j < vocab) in |= 1u << j;
@@ -751,81 +692,105 @@ __global__ __launch_bounds__(T, kFilters ? 4 : KLP_OCC) void klp_sample_kernel(S
             });
             __syncthreads();
         } else {
-            const float deep = bound < kBuckets - 1 ? static_cast<float>(bound + 1) : INFINITY;
-            const bool summed = !by_k && by_p;
-            row.each([&](int at, const float (&v)[kChunk]) {
-                float w[kChunk];
-                uint32_t in = 0;
+            // Float32 weights relative to 2^offset, offset the rounded log2 of
+            // the largest one's: sums of every token's weight serve logp
+            // alone.  And logits of the bound's bucket, or a little less.
+            const float offset = sm.top * sm.c32;
+            const float least =
+                bound < kBuckets - 1
+                    ? sm.top - static_cast<float>((bound + 1) / (kPerBit * c)) -
+                          fabsf(sm.top) * 0x1p-22f
+                    : -INFINITY;
+            bool summed = !by_k && by_p;
+            if (!summed && !(fabsf(offset) < 0x1p20f)) {  // a temperature near 0
+                row.each([&](int, const float (&v)[kChunk]) {
 #pragma unroll
-                for (int j = 0; j < kChunk; ++j) {
-                    const float d = sm.depth(v[j]);
-                    w[j] = exp2_hw(-d);
-                    if (d * kPerBit < deep && at + j < vocab) in |= 1u << j;
-                }
-                if (!summed)
+                    for (int j = 0; j < kChunk; ++j) all += sm.weight(v[j]);
+                });
+                all = over_waves(all);
+                summed = true;
+            }
+            row.each([&](int at, const float (&v)[kChunk]) {
+                if (!summed) {
+                    float w[kChunk];
+#pragma unroll
+                    for (int j = 0; j < kChunk; ++j) w[j] = exp2_hw(fmaf(v[j], sm.c32, -offset));
                     all += static_cast<double>(((w[0] + w[1]) + (w[2] + w[3])) +
                                                ((w[4] + w[5]) + (w[6] + w[7])));
+                }
+                if (chunk_max(v) < least) return;
+                uint32_t in = 0;
+#pragma unroll
+                for (int j = 0; j < kChunk; ++j)
+                    if (v[j] >= least && v[j] > -INFINITY) in |= 1u << j;
                 append(in, at, v);
             });
-            if (!summed) all = over_waves(all);
+            if (!summed)  // what the rounding of the offset left out
+                all = over_waves(all) *
+                      exp2_d(static_cast<double>(offset) -
+                             static_cast<double>(sm.top) * static_cast<double>(sm.c32));
             else __syncthreads();
         }
         const uint32_t n = s.n_list;
-        if (!wide && n <= kSorted) {
-            if (wave != 0) return;
-            // By falling value, then index: the kept ones are the first.
-            sort_list(s, n);
-            const uint32_t at = lane * kPerLane;
-            double w[kPerLane], sum = 0.0, total, mass;
-            uint2 e[kPerLane];
-#pragma unroll
-            for (int j = 0; j < kPerLane; ++j) {
-                const bool in = at + j < n && at + j < k_left;
-                e[j] = in ? s.list[at + j] : make_uint2(0xFFFFFFFFu, 0xFFFFFFFFu);
-                w[j] = in ? sm.weight(value_of(~e[j].x)) : 0.0;
-                sum += w[j];
+        if (!wide && n <= kRanked) {
+            // Every entry against every other, by a group of threads each: the
+            // mass before it in falling order decides whether it is kept, the
+            // kept mass before it by index whether it is drawn.  In fixed
+            // point, since the list's order depends on timing.
+            if (threadIdx.x < n) {
+                const double w = sm.weight(value_of(~s.list[threadIdx.x].x));
+                const unsigned long long f = sm.fixed(w);
+                s.mass[threadIdx.x] = f == 0 && w > kNothing ? 1 : f;
             }
-            double before = wave_before(sum, total);
-            const double most = p_left * (by_k ? total : all);
-            uint32_t count = 0, n_kept;
-#pragma unroll
-            for (int j = 0; j < kPerLane; ++j) {
-                const uint32_t i = at + j;
-                if (i < n && i < k_left &&
-                    (i == 0 || ((!by_p || before < most) && w[j] >= min_w)))
-                    ++count;
-                before += w[j];
+            if (threadIdx.x == 0) s.above_mass = 0;
+            __syncthreads();
+            uint32_t per = 64;  // threads an entry: 2 at least
+            while (per * n > T) per >>= 1;
+            const uint32_t i = threadIdx.x / per, g = threadIdx.x % per;
+            const uint2 e = i < n ? s.list[i] : make_uint2(0, 0);
+            const unsigned long long w = i < n ? s.mass[i] : 0;
+            const bool light = i >= n || sm.weight(value_of(~e.x)) < min_w;
+            auto over_group = [&](unsigned long long v) {
+                for (uint32_t o = per >> 1; o > 0; o >>= 1) v += __shfl_xor(v, o, 64);
+                return v;
+            };
+            unsigned long long rank = 0, before = 0;
+            for (uint32_t j = g; j < n; j += per) {
+                const uint2 o = s.list[j];
+                if (o.x < e.x || (o.x == e.x && o.y < e.y)) {
+                    ++rank;
+                    before += s.mass[j];
+                }
             }
-            wave_before(count, n_kept);
-            // By index.
-#pragma unroll
-            for (int j = 0; j < kPerLane; ++j)
-                if (at + j < n_kept) s.list[at + j] = make_uint2(e[j].y, e[j].x);
-            sort_list(s, n_kept);
-            sum = 0.0;
-#pragma unroll
-            for (int j = 0; j < kPerLane; ++j) {
-                const bool in = at + j < n_kept;
-                e[j] = in ? s.list[at + j] : make_uint2(0, 0);
-                w[j] = in ? sm.weight(value_of(~e[j].y)) : 0.0;
-                sum += w[j];
+            rank = over_group(rank);
+            before = over_group(before);
+            if (by_k && by_p) {
+                if (i < n && g == 0 && rank < k_left) atomicAdd(&s.above_mass, w);
+                __syncthreads();
+                share = p_left * static_cast<double>(s.above_mass);
             }
-            double pos = wave_before(sum, mass);
-            const double target = static_cast<double>(u) * mass;
-            int token = 0x7FFFFFFF, last = -1;
-#pragma unroll
-            for (int j = 0; j < kPerLane; ++j) {
-                pos += w[j];
-                if (w[j] <= kNothing) continue;
-                last = static_cast<int>(e[j].x);
-                if (pos > target) token = min(token, last);
+            const bool keep =
+                i < n && rank < k_left &&
+                (rank == 0 || ((!by_p || static_cast<double>(before) < share) && !light));
+            __syncthreads();
+            if (i < n && g == 0 && !keep) s.mass[i] = 0;
+            __syncthreads();
+            unsigned long long mass = 0;
+            before = 0;
+            for (uint32_t j = g; j < n; j += per) {
+                const unsigned long long m = s.mass[j];
+                mass += m;
+                if (s.list[j].y < e.y) before += m;
             }
-#pragma unroll
-            for (int o = 32; o > 0; o >>= 1) {
-                token = min(token, __shfl_xor(token, o, 64));
-                last = max(last, __shfl_xor(last, o, 64));
-            }
-            if (lane == 0) finish(token != 0x7FFFFFFF ? token : last, all, mass);
+            mass = over_group(mass);
+            before = over_group(before);
+            const double to = static_cast<double>(before + w);
+            const double target = static_cast<double>(u) * static_cast<double>(mass);
+            // One entry's: the first past the target, or the last for u = 1.
+            if (keep && w > 0 && static_cast<double>(before) <= target &&
+                (to > target || before + w == mass) && g < 2)
+                finish(static_cast<int>(e.y), all,
+                       static_cast<double>(mass) * ldexp(1.0, -frac));
             return;
         }
         const bool listed = n <= kList;
@@ -915,7 +880,7 @@ __global__ __launch_bounds__(T, kFilters ? 4 : KLP_OCC) void klp_sample_kernel(S
         sm.set_parts(kept, ties);
         double mass;
         const int token = sm.search(u, tau, keep_ties, min_w, mass);
-        if (token >= 0 && lane == 0) finish(token, all, mass);
+        if (token >= 0 && lane < 2) finish(token, all, mass);
     }
 }
 
