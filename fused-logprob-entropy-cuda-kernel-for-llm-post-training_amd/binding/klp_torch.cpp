@@ -791,6 +791,203 @@ std::optional<std::vector<at::Tensor>> fused_grpo_step(
     return std::vector<at::Tensor>{out[0], out[1], out[2]};
 }
 
+// ---------------------------------------------------------------------------
+// The norm in front of the LM head, 8-bit matrices and sampling: the views,
+// allocations and launches of kernel_opt.norm, kernel_opt.fp8 and
+// kernel_opt.sample after their argument checks, which stay in Python, and the
+// norm's autograd function.
+// ---------------------------------------------------------------------------
+constexpr int64_t kScaleBlock = 128;
+
+// t as rows of its last dim with unit stride (a view where its layout has
+// one), and their stride.
+struct Matrix {
+    at::Tensor t;
+    int64_t ld;
+};
+Matrix as_rows(const at::Tensor& t) {
+    const int64_t d = t.size(-1);
+    at::Tensor m = t.dim() == 2 ? t : t.reshape({d ? t.numel() / d : 0, d});
+    if (d > 1 && m.stride(-1) != 1) m = m.contiguous();
+    return Matrix{m, m.size(0) > 1 ? m.stride(0) : d};
+}
+void* data_or_null(const at::Tensor& t) { return t.defined() ? t.data_ptr() : nullptr; }
+std::vector<int64_t> scale_shape(const at::Tensor& t) {
+    std::vector<int64_t> shape = t.sizes().vec();
+    shape.back() = (shape.back() + kScaleBlock - 1) / kScaleBlock;
+    return shape;
+}
+hipStream_t current_stream(int dev) {
+    return c10::hip::getCurrentHIPStream(static_cast<c10::DeviceIndex>(dev)).stream();
+}
+
+struct NormForward {
+    at::Tensor y, scales, h, rstd;  // y: e4m3 codes with `fp8`
+};
+NormForward norm_forward(const at::Tensor& x, const at::Tensor& residual, const at::Tensor& weight,
+                         double eps, bool fp8) {
+    const int dev = x.get_device();
+    const c10::hip::HIPGuard guard(static_cast<c10::DeviceIndex>(dev));
+    const Matrix xm = as_rows(x);
+    const Matrix rm = residual.defined() ? as_rows(residual) : Matrix{at::Tensor(), 0};
+    const at::Tensor w = weight.contiguous();
+    const int64_t n = xm.t.size(0), d = xm.t.size(1);
+    const auto f32 = x.options().dtype(at::kFloat);
+    NormForward o;
+    if (residual.defined()) o.h = at::empty(x.sizes(), x.options());
+    const int code = dtype_code(x.scalar_type()), w_code = dtype_code(w.scalar_type());
+    const float e = static_cast<float>(eps);
+    hipStream_t stream = current_stream(dev);
+    if (fp8) {
+        o.y = at::empty(x.sizes(), x.options().dtype(at::kFloat8_e4m3fn));
+        o.scales = at::empty(scale_shape(x), f32);
+        check_status(klp_rms_norm_fp8(xm.t.data_ptr(), code, xm.ld, data_or_null(rm.t), rm.ld,
+                                      w.data_ptr(), w_code, n, d, e,
+                                      static_cast<uint8_t*>(o.y.data_ptr()), out_ptr(o.scales),
+                                      data_or_null(o.h), stream));
+        return o;
+    }
+    o.y = at::empty(x.sizes(), x.options());
+    o.rstd = at::empty({n}, f32);
+    check_status(klp_rms_norm(xm.t.data_ptr(), code, xm.ld, data_or_null(rm.t), rm.ld,
+                              w.data_ptr(), w_code, n, d, e, o.y.data_ptr(), data_or_null(o.h),
+                              out_ptr(o.rstd), stream));
+    return o;
+}
+
+class FusedRmsNorm : public torch::autograd::Function<FusedRmsNorm> {
+   public:
+    static variable_list forward(AutogradContext* ctx, const at::Tensor& x,
+                                 const std::optional<at::Tensor>& residual,
+                                 const at::Tensor& weight, double eps) {
+        NormForward o = norm_forward(x, residual.value_or(at::Tensor()), weight, eps, false);
+        ctx->save_for_backward({o.h.defined() ? o.h : x, weight, o.rstd});
+        ctx->set_materialize_grads(false);
+        if (o.h.defined()) return {o.y, o.h};
+        return {o.y};
+    }
+
+    static variable_list backward(AutogradContext* ctx, variable_list grads) {
+        const auto saved = ctx->get_saved_variables();
+        const at::Tensor &h = saved[0], &weight = saved[1], &rstd = saved[2];
+        const bool with_h = grads.size() > 1;
+        at::Tensor g_y = grads[0], g_h = with_h ? grads[1] : at::Tensor();
+        const bool need_x = ctx->needs_input_grad(0);
+        const bool need_r = with_h && ctx->needs_input_grad(1);
+        const bool need_w = ctx->needs_input_grad(with_h ? 2 : 1);
+        variable_list none(4);
+        if ((!g_y.defined() && !g_h.defined()) || !(need_x || need_r || need_w)) return none;
+        const int dev = h.get_device();
+        const c10::hip::HIPGuard guard(static_cast<c10::DeviceIndex>(dev));
+        hipStream_t stream = current_stream(dev);
+        hipStreamCaptureStatus status = hipStreamCaptureStatusNone;
+        if (hipStreamIsCapturing(stream, &status) != hipSuccess ||
+            status != hipStreamCaptureStatusNone)
+            throw std::runtime_error(
+                "kernel_opt: this backward belongs to a forward run outside graph capture and "
+                "cannot itself be captured; capture the forward with it");
+        if (!g_y.defined())  // only h was used
+            return {need_x ? g_h : at::Tensor(), need_r ? g_h : at::Tensor(),
+                    need_w ? at::zeros_like(weight) : at::Tensor(), at::Tensor()};
+        const Matrix hm = as_rows(h);
+        const int64_t n = hm.t.size(0), d = hm.t.size(1);
+        at::Tensor d_x = at::empty(h.sizes(), h.options()), d_w;
+        if (need_w) d_w = at::empty(weight.sizes(), weight.options());
+        if (n == 0) {
+            if (need_w) d_w.zero_();
+        } else {
+            g_y = g_y.contiguous();
+            if (g_h.defined()) g_h = g_h.contiguous();
+            const at::Tensor w = weight.contiguous();
+            const size_t bytes = need_w ? klp_rms_norm_bwd_workspace_bytes(n, d) : 0;
+            const at::Tensor ws =
+                need_w ? at::empty({static_cast<int64_t>(bytes)}, h.options().dtype(at::kByte))
+                       : at::Tensor();
+            check_status(klp_rms_norm_bwd(hm.t.data_ptr(), dtype_code(h.scalar_type()), hm.ld,
+                                          w.data_ptr(), dtype_code(w.scalar_type()), fptr(rstd),
+                                          g_y.data_ptr(), data_or_null(g_h), n, d, d_x.data_ptr(),
+                                          data_or_null(d_w), data_or_null(ws), bytes, stream));
+        }
+        return {need_x ? d_x : at::Tensor(), need_r ? d_x : at::Tensor(), d_w, at::Tensor()};
+    }
+};
+
+std::vector<at::Tensor> rms_norm(const at::Tensor& x, const std::optional<at::Tensor>& residual,
+                                 const at::Tensor& weight, double eps) {
+    decline_under_capture(x.get_device());
+    return FusedRmsNorm::apply(x, residual, weight, eps);
+}
+
+std::vector<at::Tensor> rms_norm_fp8(const at::Tensor& x, const std::optional<at::Tensor>& residual,
+                                     const at::Tensor& weight, double eps) {
+    decline_under_capture(x.get_device());
+    const at::AutoDispatchBelowADInplaceOrView below;
+    NormForward o = norm_forward(x, residual.value_or(at::Tensor()), weight, eps, true);
+    if (o.h.defined()) return {o.y, o.scales, o.h};
+    return {o.y, o.scales};
+}
+
+std::vector<at::Tensor> quantize_fp8(const at::Tensor& x, int64_t block_rows) {
+    const int dev = x.get_device();
+    decline_under_capture(dev);
+    const at::AutoDispatchBelowADInplaceOrView below;
+    const c10::hip::HIPGuard guard(static_cast<c10::DeviceIndex>(dev));
+    const Matrix m = as_rows(x);
+    std::vector<int64_t> shape = scale_shape(x);
+    if (block_rows != 1) shape[0] = (shape[0] + block_rows - 1) / block_rows;
+    at::Tensor q = at::empty(x.sizes(), x.options().dtype(at::kFloat8_e4m3fn));
+    at::Tensor scales = at::empty(shape, x.options().dtype(at::kFloat));
+    check_status(klp_quantize_fp8(m.t.data_ptr(), dtype_code(x.scalar_type()), m.ld, m.t.size(0),
+                                  m.t.size(1), static_cast<int>(block_rows),
+                                  static_cast<uint8_t*>(q.data_ptr()), out_ptr(scales),
+                                  current_stream(dev)));
+    return {q, scales};
+}
+
+at::Tensor fp8_linear(const at::Tensor& x, const at::Tensor& x_scale, const at::Tensor& weight,
+                      const at::Tensor& weight_scale, at::ScalarType out_dtype) {
+    const int dev = x.get_device();
+    decline_under_capture(dev);
+    const at::AutoDispatchBelowADInplaceOrView below;
+    const c10::hip::HIPGuard guard(static_cast<c10::DeviceIndex>(dev));
+    const Matrix xm = as_rows(x), wm = as_rows(weight);
+    const at::Tensor xs = x_scale.contiguous(), ws = weight_scale.contiguous();
+    std::vector<int64_t> shape = x.sizes().vec();
+    shape.back() = wm.t.size(0);
+    at::Tensor out = at::empty(shape, x.options().dtype(out_dtype));
+    check_status(klp_fp8_linear(static_cast<const uint8_t*>(xm.t.data_ptr()), xm.ld, fptr(xs),
+                                static_cast<const uint8_t*>(wm.t.data_ptr()), wm.ld, fptr(ws),
+                                xm.t.size(0), wm.t.size(0), wm.t.size(1), dtype_code(out_dtype),
+                                out.data_ptr(), wm.t.size(0), current_stream(dev)));
+    return out;
+}
+
+std::vector<at::Tensor> sample(const at::Tensor& logits, const at::Tensor& uniform, double t,
+                               const std::optional<at::Tensor>& ts, int64_t k,
+                               const std::optional<at::Tensor>& ks, double p,
+                               const std::optional<at::Tensor>& ps, double m,
+                               const std::optional<at::Tensor>& ms) {
+    const int dev = logits.get_device();
+    decline_under_capture(dev);
+    const at::AutoDispatchBelowADInplaceOrView below;
+    const c10::hip::HIPGuard guard(static_cast<c10::DeviceIndex>(dev));
+    const auto rows = row_layout(logits);
+    require(rows.has_value(), "logits must be contiguous");
+    const auto& L = *rows;
+    const at::Tensor u = uniform.contiguous();
+    at::Tensor tokens = at::empty(uniform.sizes(), uniform.options().dtype(at::kLong));
+    at::Tensor logp = at::empty(uniform.sizes(), uniform.options());
+    at::Tensor sample_logp = at::empty(uniform.sizes(), uniform.options());
+    const at::Tensor no;
+    check_status(klp_sample(
+        logits.data_ptr(), dtype_code(logits.scalar_type()), u.numel(), logits.size(-1), L[0], L[1],
+        L[2], fptr(u), static_cast<float>(t), fptr(ts.value_or(no)), static_cast<int32_t>(k),
+        static_cast<const int32_t*>(data_or_null(ks.value_or(no))), static_cast<float>(p),
+        fptr(ps.value_or(no)), static_cast<float>(m), fptr(ms.value_or(no)),
+        tokens.data_ptr<int64_t>(), out_ptr(logp), out_ptr(sample_logp), current_stream(dev)));
+    return {tokens, logp, sample_logp};
+}
+
 }  // namespace
 
 PYBIND11_MODULE(klp_torch, m) {
@@ -865,6 +1062,17 @@ PYBIND11_MODULE(klp_torch, m) {
           pybind11::arg("ref_logp"), pybind11::arg("temperature"), pybind11::arg("eps_low"),
           pybind11::arg("eps_high"), pybind11::arg("beta"), pybind11::arg("weight_kind"),
           pybind11::arg("weight_scale"), pybind11::arg("grad_scale") = 1.0);
+    // kernel_opt.norm, kernel_opt.fp8 and kernel_opt.sample
+    m.def("rms_norm", &rms_norm, pybind11::arg("x"), pybind11::arg("residual"),
+          pybind11::arg("weight"), pybind11::arg("eps"));
+    m.def("rms_norm_fp8", &rms_norm_fp8, pybind11::arg("x"), pybind11::arg("residual"),
+          pybind11::arg("weight"), pybind11::arg("eps"));
+    m.def("quantize_fp8", &quantize_fp8, pybind11::arg("x"), pybind11::arg("block_rows"));
+    m.def("fp8_linear", &fp8_linear, pybind11::arg("x"), pybind11::arg("x_scale"),
+          pybind11::arg("weight"), pybind11::arg("weight_scale"), pybind11::arg("out_dtype"));
+    m.def("sample", &sample, pybind11::arg("logits"), pybind11::arg("uniform"), pybind11::arg("t"),
+          pybind11::arg("ts"), pybind11::arg("k"), pybind11::arg("ks"), pybind11::arg("p"),
+          pybind11::arg("ps"), pybind11::arg("m"), pybind11::arg("ms"));
     m.def(
         "workspaces_cached",
         []() {

@@ -15,7 +15,8 @@ from __future__ import annotations
 
 import torch
 
-from ._library import DTYPE_CODES, check_status, device_guard, lib, ptr, stream_handle
+from ._library import (DTYPE_CODES, binding, check_status, device_guard, lib, ptr,
+                       stream_handle)
 from .norm import SCALE_BLOCK, _rows
 
 __all__ = ["quantize_fp8", "fp8_linear"]
@@ -38,7 +39,10 @@ def quantize_fp8(x: torch.Tensor, block_rows: int = 1):
     if x.dim() < 1 or x.size(-1) < 1 or (block_rows != 1 and x.dim() != 2):
         raise RuntimeError(f"x must be {'[..., dim]' if block_rows == 1 else '[N, dim]'} with "
                            f"dim >= 1, got {tuple(x.shape)}")
-    x = x.detach()
+    try:
+        return tuple(binding.quantize_fp8(x, int(block_rows)))
+    except binding.CaptureDeclined:
+        x = x.detach()
     dev = x.device
     D = x.size(-1)
     nb = -(-D // SCALE_BLOCK)
@@ -97,6 +101,10 @@ def fp8_linear(x: torch.Tensor, x_scale: torch.Tensor, weight: torch.Tensor,
     otherwise).  A NaN code or scale gives NaN in the outputs it enters.
     """
     _check_linear(x, x_scale, weight, weight_scale, out_dtype)
+    try:
+        return binding.fp8_linear(x, x_scale, weight, weight_scale, out_dtype)
+    except binding.CaptureDeclined:
+        pass
     dev = x.device
     x2, ld_x = _rows(x)
     w2, ld_w = _rows(weight)

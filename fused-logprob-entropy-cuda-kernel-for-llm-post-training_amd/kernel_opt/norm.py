@@ -13,12 +13,17 @@ those of the stored ``h``, all sums are float32, ``y`` is rounded once.
 ``fused_rms_norm_fp8`` / ``fused_add_rms_norm_fp8`` write the same ``y`` as
 e4m3 codes with a float32 scale for each 128 columns, the operand of
 :func:`kernel_opt.fp8_linear` (serving and scoring: no gradient).
+
+Calls run in the compiled binding (binding/klp_torch.cpp), the autograd function
+included; under graph capture, which it declines, the Python statement of them
+below runs.
 """
 from __future__ import annotations
 
 import torch
 
-from ._library import DTYPE_CODES, check_status, device_guard, lib, ptr, stream_handle
+from ._library import (DTYPE_CODES, binding, check_status, device_guard, lib, ptr,
+                       stream_handle)
 
 __all__ = ["fused_rms_norm", "fused_add_rms_norm", "fused_rms_norm_fp8", "fused_add_rms_norm_fp8"]
 
@@ -130,7 +135,10 @@ def fused_rms_norm(x: torch.Tensor, weight: torch.Tensor, eps: float = 1e-6):
         weight: ``[dim]``, of ``x``'s dtype or float32.
     """
     _check(x, None, weight, eps)
-    return _FusedRmsNorm.apply(x, None, weight, float(eps))
+    try:
+        return binding.rms_norm(x, None, weight, float(eps))[0]
+    except binding.CaptureDeclined:
+        return _FusedRmsNorm.apply(x, None, weight, float(eps))
 
 
 def fused_add_rms_norm(x: torch.Tensor, residual: torch.Tensor, weight: torch.Tensor,
@@ -139,7 +147,10 @@ def fused_add_rms_norm(x: torch.Tensor, residual: torch.Tensor, weight: torch.Te
     norm ``y`` as :func:`fused_rms_norm` gives it, differentiable in ``x``,
     ``residual`` and ``weight`` through both outputs."""
     _check(x, residual, weight, eps)
-    return _FusedRmsNorm.apply(x, residual, weight, float(eps))
+    try:
+        return tuple(binding.rms_norm(x, residual, weight, float(eps)))
+    except binding.CaptureDeclined:
+        return _FusedRmsNorm.apply(x, residual, weight, float(eps))
 
 
 def fused_rms_norm_fp8(x: torch.Tensor, weight: torch.Tensor, eps: float = 1e-6):
@@ -148,6 +159,10 @@ def fused_rms_norm_fp8(x: torch.Tensor, weight: torch.Tensor, eps: float = 1e-6)
     a = max |y|, ``scale = a / 448`` (1 where a is 0) and ``code = e4m3(y * (448
     / a))``.  A block with a NaN or an infinity stands for NaN.  No gradient."""
     _check(x, None, weight, eps)
+    try:
+        return tuple(binding.rms_norm_fp8(x, None, weight, float(eps)))
+    except binding.CaptureDeclined:
+        pass
     return _forward(x.detach(), None, weight.detach(), eps, True)[0]
 
 
@@ -156,5 +171,9 @@ def fused_add_rms_norm_fp8(x: torch.Tensor, residual: torch.Tensor, weight: torc
     """``(codes, scales, h)``: :func:`fused_rms_norm_fp8` of ``h = round(x +
     residual)``, and ``h``.  No gradient."""
     _check(x, residual, weight, eps)
+    try:
+        return tuple(binding.rms_norm_fp8(x, residual, weight, float(eps)))
+    except binding.CaptureDeclined:
+        pass
     y, h, _ = _forward(x.detach(), residual.detach(), weight.detach(), eps, True)
     return y[0], y[1], h

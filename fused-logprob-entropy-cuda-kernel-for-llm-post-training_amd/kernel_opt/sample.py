@@ -25,7 +25,8 @@ import math
 import torch
 
 from . import _C
-from ._library import DTYPE_CODES, check_status, device_guard, lib, ptr, stream_handle
+from ._library import (DTYPE_CODES, binding, check_status, device_guard, lib, ptr,
+                       stream_handle)
 
 __all__ = ["fused_sample"]
 
@@ -98,6 +99,10 @@ def fused_sample(logits: torch.Tensor, uniform: torch.Tensor, temperature=1.0, *
     k, ks = _parameter(top_k, "top_k", shape, dev, torch.int32, 0, 0, 2 ** 31 - 1)
     p, ps = _parameter(top_p, "top_p", shape, dev, torch.float32, 1.0, 0.0, 1.0)
     m, ms = _parameter(min_p, "min_p", shape, dev, torch.float32, 0.0, 0.0, 1.0)
+    try:
+        return tuple(binding.sample(logits, uniform, t, ts, k, ks, p, ps, m, ms))
+    except binding.CaptureDeclined:
+        pass
     u = uniform.detach().contiguous()
     tokens = torch.empty(shape, dtype=torch.int64, device=dev)
     logp = torch.empty(shape, dtype=torch.float32, device=dev)
