@@ -22,12 +22,15 @@
 //   No filter: one pass sums the weights, relative to one of the row's first
 // logits; the part whose running sum crosses the target is read again.
 //   Filters: one pass for the maximum, then one that collects, in LDS, every
-// logit that could be kept, and is followed by work on that list alone: sorted
-// by value it gives the kept set, sorted by index the token.  What could be
-// kept is bounded beforehand by a bucket of a scale that is linear in y: for
-// top-k the bucket of the k-th largest of the threads' maxima (k of the logits
-// are at least that large; for a k above a quarter of the threads a histogram
-// of the counts, since the k-th of few maxima is low), for min-p that of its border, for top-p without a
+// logit that could be kept, and is followed by work on that list alone: an
+// entry's rank, or the mass before it, in falling order says whether it is
+// kept, and the kept mass before it by index whether it is drawn.  Up to 256
+// entries are compared with each other; of more, those in the buckets of a
+// histogram that hold the borders.  What could be kept is bounded beforehand
+// by a bucket of a scale that is linear in y: for top-k the bucket of the k-th
+// largest of the threads' maxima (k of the logits are at least that large; for
+// a k above a quarter of the threads a histogram of the counts, since the k-th
+// of few maxima is low), for min-p that of its border, for top-p without a
 // top-k that in which a histogram of the masses, one more pass, reaches top_p.
 //   Where the list overflows (more than 4096 logits above the bound: a row of
 // equal logits, a wide nucleus) the kept set is {key > tau} and the first r of
@@ -107,7 +110,11 @@ template <bool kFilters>
 struct Shared {
     uint32_t count[kFilters ? kBuckets : 1];
     unsigned long long mass[kFilters ? kBuckets : 1];
-    uint2 list[kFilters ? kList : 1];  // x before y in the order of a sort
+    uint2 list[kFilters ? kList : 1];  // (~key, index): in falling order, x before y
+    uint2 few[kFilters ? kRanked : 1];  // those of one bucket
+    unsigned long long few_mass[kFilters ? kRanked : 1];
+    uint32_t few_kept[kFilters ? kRanked : 1];
+    uint32_t n_few;
     unsigned long long wave_mass[kMaxWaves];
     double wave_sum[kMaxWaves];
     double wave_all[kMaxWaves];
@@ -241,7 +248,7 @@ struct Row {
 // with by_mass, the running mass reaches `mass`); the last one with anything
 // in it when none does.  Into s.at, with what lies before it.
 template <int T>
-__device__ void find(Shared<true>& s, bool by_mass, uint32_t count, double mass) {
+__device__ void find(Shared<true>& s, bool by_mass, uint32_t count, unsigned long long mass) {
     constexpr int kPerThread = kBuckets / T;
     const int first = threadIdx.x * kPerThread;
     uint32_t c[kPerThread], c_sum = 0;
@@ -258,13 +265,12 @@ __device__ void find(Shared<true>& s, bool by_mass, uint32_t count, double mass)
     uint32_t c_run = block_before<T>(s.wave_count, c_sum, c_all);
     unsigned long long m_run = block_before<T>(s.wave_mass, m_sum, m_all);
     // A target that rounding left above the total is the total.
-    const double want = fmin(mass, static_cast<double>(m_all));
+    mass = min(mass, m_all);
     count = min(count, c_all);
 #pragma unroll
     for (int i = 0; i < kPerThread; ++i) {
-        const bool before = by_mass ? static_cast<double>(m_run) < want : c_run < count;
-        const bool here = by_mass ? static_cast<double>(m_run + m[i]) >= want
-                                  : c_run + c[i] >= count;
+        const bool before = by_mass ? m_run < mass : c_run < count;
+        const bool here = by_mass ? m_run + m[i] >= mass : c_run + c[i] >= count;
         if (before && here) {
             s.at = first + i;
             s.at_count = c[i];
@@ -326,6 +332,18 @@ struct Sampler {
         __syncthreads();
     }
 
+    // Threads that share one of n <= kRanked entries: 2 at least, neighbours.
+    static __device__ __forceinline__ uint32_t threads_for(uint32_t n) {
+        uint32_t per = 64;
+        while (per * n > T) per >>= 1;
+        return per;
+    }
+    static __device__ __forceinline__ unsigned long long over_group(unsigned long long v,
+                                                                    uint32_t per) {
+        for (uint32_t o = per >> 1; o > 0; o >>= 1) v += __shfl_xor(v, o, 64);
+        return v;
+    }
+
     // f(key) for every element of the list, or of the row.
     template <typename F>
     __device__ __forceinline__ void candidates(bool listed, F f) {
@@ -344,7 +362,7 @@ struct Sampler {
     // `above` elements and above_mass before the bucket.
     __device__ Border resolve(bool listed, uint32_t b, uint32_t floor, uint32_t above,
                               unsigned long long above_mass, bool by_mass, uint32_t count,
-                              double mass) {
+                              unsigned long long mass) {
         __syncthreads();
         if (threadIdx.x == 0) {
             s.key_count = 0;
@@ -380,8 +398,7 @@ struct Sampler {
                 if (by_mass) atomicAdd(&s.mass[i], fixed(weight(value_of(k))));
             });
             __syncthreads();
-            find<T>(s, by_mass, by_mass ? 0 : count - above,
-                    by_mass ? mass - static_cast<double>(above_mass) : 0.0);
+            find<T>(s, by_mass, by_mass ? 0 : count - above, by_mass ? mass - above_mass : 0);
             above += s.above_count;
             above_mass += s.above_mass;
             ties = s.at_count;
@@ -530,7 +547,12 @@ __global__ __launch_bounds__(T, kFilters ? 4 : KLP_OCC) void klp_sample_kernel(S
     const bool by_p = top_p < 1.0f;  // a NaN is no filter
     const bool by_m = min_p > 0.0f;
     const uint32_t k_left = by_k ? static_cast<uint32_t>(top_k) : 0xFFFFFFFFu;
-    const double p_left = static_cast<double>(fmaxf(top_p, 0.0f));
+    // A mass before which top-p keeps what it does, of whole masses: the first
+    // element always.
+    auto share_of = [&](double mass) {
+        const double m = ceil(static_cast<double>(fmaxf(top_p, 0.0f)) * mass);
+        return m > 1.0 ? static_cast<unsigned long long>(m) : 1ull;
+    };
     const double min_w = by_m ? fmin(static_cast<double>(min_p), 1.0) : 0.0;
 
     // Fixed point: sums of `vocab` weights of at most 1 stay below 2^63.
@@ -568,6 +590,10 @@ __global__ __launch_bounds__(T, kFilters ? 4 : KLP_OCC) void klp_sample_kernel(S
 #pragma unroll
         for (int i = 0; i < kWaves; ++i) v += s.wave_all[i];
         return v;
+    };
+    // A running sum of whole masses crosses uniform * mass where it exceeds this.
+    auto target_of = [&](unsigned long long mass) {
+        return static_cast<unsigned long long>(static_cast<double>(u) * static_cast<double>(mass));
     };
     // By an even lane and the next one, each with one of the logarithms.
     auto finish = [&](int token, double all, double mass) {
@@ -611,8 +637,8 @@ __global__ __launch_bounds__(T, kFilters ? 4 : KLP_OCC) void klp_sample_kernel(S
         sm.top = top + 0.0f;
         // What could be kept lies in buckets up to `bound`.
         uint32_t bound = kBuckets - 1, p_at = kBuckets;
-        double all = 0.0, share = 0.0;
-        unsigned long long p_above = 0;
+        double all = 0.0;
+        unsigned long long share = 0, p_above = 0;
         bool wide = false;  // top-p alone, with more than the list takes
         if (by_k) {
             sm.clear();
@@ -625,7 +651,7 @@ __global__ __launch_bounds__(T, kFilters ? 4 : KLP_OCC) void klp_sample_kernel(S
                 });
             }
             __syncthreads();
-            find<T>(s, false, k_left, 0.0);
+            find<T>(s, false, k_left, 0);
             // Fewer threads than top_k have a logit: no bound from them.
             if (s.above_count + s.at_count >= k_left) bound = s.at;
         } else if (by_p) {
@@ -643,8 +669,7 @@ __global__ __launch_bounds__(T, kFilters ? 4 : KLP_OCC) void klp_sample_kernel(S
                 }
             });
             all = over_waves(all);
-            // In fixed point; the first element is always kept.
-            share = fmax(p_left * all * ldexp(1.0, frac), 1.0);
+            share = share_of(all * ldexp(1.0, frac));
             find<T>(s, true, 0, share);
             bound = p_at = s.at;
             p_above = s.above_mass;
@@ -744,16 +769,11 @@ __global__ __launch_bounds__(T, kFilters ? 4 : KLP_OCC) void klp_sample_kernel(S
             }
             if (threadIdx.x == 0) s.above_mass = 0;
             __syncthreads();
-            uint32_t per = 64;  // threads an entry: 2 at least
-            while (per * n > T) per >>= 1;
+            const uint32_t per = sm.threads_for(n);
             const uint32_t i = threadIdx.x / per, g = threadIdx.x % per;
             const uint2 e = i < n ? s.list[i] : make_uint2(0, 0);
             const unsigned long long w = i < n ? s.mass[i] : 0;
             const bool light = i >= n || sm.weight(value_of(~e.x)) < min_w;
-            auto over_group = [&](unsigned long long v) {
-                for (uint32_t o = per >> 1; o > 0; o >>= 1) v += __shfl_xor(v, o, 64);
-                return v;
-            };
             unsigned long long rank = 0, before = 0;
             for (uint32_t j = g; j < n; j += per) {
                 const uint2 o = s.list[j];
@@ -762,16 +782,16 @@ __global__ __launch_bounds__(T, kFilters ? 4 : KLP_OCC) void klp_sample_kernel(S
                     before += s.mass[j];
                 }
             }
-            rank = over_group(rank);
-            before = over_group(before);
+            rank = sm.over_group(rank, per);
+            before = sm.over_group(before, per);
             if (by_k && by_p) {
                 if (i < n && g == 0 && rank < k_left) atomicAdd(&s.above_mass, w);
                 __syncthreads();
-                share = p_left * static_cast<double>(s.above_mass);
+                share = share_of(static_cast<double>(s.above_mass));
             }
             const bool keep =
                 i < n && rank < k_left &&
-                (rank == 0 || ((!by_p || static_cast<double>(before) < share) && !light));
+                (rank == 0 || ((!by_p || before < share) && !light));
             __syncthreads();
             if (i < n && g == 0 && !keep) s.mass[i] = 0;
             __syncthreads();
@@ -782,18 +802,141 @@ __global__ __launch_bounds__(T, kFilters ? 4 : KLP_OCC) void klp_sample_kernel(S
                 mass += m;
                 if (s.list[j].y < e.y) before += m;
             }
-            mass = over_group(mass);
-            before = over_group(before);
-            const double to = static_cast<double>(before + w);
-            const double target = static_cast<double>(u) * static_cast<double>(mass);
+            mass = sm.over_group(mass, per);
+            before = sm.over_group(before, per);
+            const unsigned long long target = target_of(mass);
             // One entry's: the first past the target, or the last for u = 1.
-            if (keep && w > 0 && static_cast<double>(before) <= target &&
-                (to > target || before + w == mass) && g < 2)
+            if (keep && w > 0 && before <= target && (before + w > target || before + w == mass) &&
+                g < 2)
                 finish(static_cast<int>(e.y), all,
                        static_cast<double>(mass) * ldexp(1.0, -frac));
             return;
         }
         const bool listed = n <= kList;
+        while (listed && !wide) {  // once; left where a bucket holds too many
+            // Up to kList / T entries a thread.  A border's bucket is found by
+            // histogram, its few entries are ranked; the token's likewise,
+            // with buckets of the index.
+            constexpr int kOwn = kList / T;
+            uint2 e[kOwn];
+            unsigned long long w[kOwn];
+            uint32_t b[kOwn];  // its bucket; kBuckets: not kept
+#pragma unroll
+            for (int j = 0; j < kOwn; ++j) {
+                const uint32_t i = threadIdx.x + j * T;
+                e[j] = i < n ? s.list[i] : make_uint2(0, 0);
+                const double y = i < n ? sm.log2_weight(value_of(~e[j].x)) : 0.0;
+                const double x = exp2_d(y);
+                const unsigned long long f = sm.fixed(x);
+                b[j] = i < n ? sm.bucket_of(y) : kBuckets;
+                w[j] = i < n ? (f == 0 && x > kNothing ? 1 : f) : 0;
+            }
+            // The few entries of bucket `at` in s.few, and each one's place.
+            uint32_t place[kOwn];
+            auto pick = [&](uint32_t at, auto bucket) {
+                __syncthreads();
+                if (threadIdx.x == 0) s.n_few = 0;
+                __syncthreads();
+#pragma unroll
+                for (int j = 0; j < kOwn; ++j) {
+                    place[j] = kRanked;
+                    if (b[j] == kBuckets || bucket(j) != at) continue;
+                    place[j] = atomicAdd(&s.n_few, 1u);
+                    if (place[j] >= kRanked) continue;
+                    s.few[place[j]] = e[j];
+                    s.few_mass[place[j]] = w[j];
+                }
+                __syncthreads();
+                return s.n_few <= kRanked;
+            };
+            auto own_bucket = [&](int j) { return b[j]; };
+            // Keeps what lies before the border in bucket `at`, of the entries
+            // in it `left` by count, or those before which less than `share` lies.
+            auto cut = [&](uint32_t at, bool by_mass, uint32_t left, unsigned long long share_left) {
+                if (!pick(at, own_bucket)) return false;
+                const uint32_t m = s.n_few, per = sm.threads_for(m);
+                const uint32_t i = threadIdx.x / per, g = threadIdx.x % per;
+                const uint2 o = i < m ? s.few[i] : make_uint2(0, 0);
+                unsigned long long rank = 0, before = 0;
+                for (uint32_t j = g; j < m; j += per) {
+                    const uint2 q = s.few[j];
+                    if (q.x < o.x || (q.x == o.x && q.y < o.y)) {
+                        ++rank;
+                        before += s.few_mass[j];
+                    }
+                }
+                rank = sm.over_group(rank, per);
+                before = sm.over_group(before, per);
+                if (i < m && g == 0)
+                    s.few_kept[i] = by_mass ? before < share_left : rank < left;
+                __syncthreads();
+#pragma unroll
+                for (int j = 0; j < kOwn; ++j)
+                    if (b[j] > at || (b[j] == at && !s.few_kept[place[j]])) b[j] = kBuckets;
+                return true;
+            };
+            if (by_k) {
+                sm.clear();
+#pragma unroll
+                for (int j = 0; j < kOwn; ++j)
+                    if (b[j] < kBuckets) atomicAdd(&s.count[b[j]], 1u);
+                __syncthreads();
+                find<T>(s, false, k_left, 0);
+                const uint32_t at = s.at, left = k_left - s.above_count;
+                if (!cut(at, false, left, 0)) break;
+            }
+            if (by_p && by_k) {
+                __syncthreads();
+                sm.clear();
+                unsigned long long own = 0, total;
+#pragma unroll
+                for (int j = 0; j < kOwn; ++j) {
+                    if (b[j] == kBuckets) continue;
+                    atomicAdd(&s.mass[b[j]], w[j]);
+                    own += w[j];
+                }
+                block_before<T>(s.wave_mass, own, total);
+                const unsigned long long part = share_of(static_cast<double>(total));
+                find<T>(s, true, 0, part);
+                const uint32_t at = s.at;
+                const unsigned long long left = part - s.above_mass;
+                if (!cut(at, true, 0, left)) break;
+            } else if (by_p && bound == p_at) {
+                if (!cut(p_at, true, 0, share - p_above)) break;
+            }
+            // By index.
+            const int shift = max(0, 32 - __clz(vocab - 1) - kBucketBits);
+            __syncthreads();
+            sm.clear();
+            unsigned long long own = 0, mass;
+#pragma unroll
+            for (int j = 0; j < kOwn; ++j) {
+                if (by_m && b[j] < kBuckets && sm.weight(value_of(~e[j].x)) < min_w)
+                    b[j] = kBuckets;
+                if (b[j] == kBuckets) continue;
+                atomicAdd(&s.mass[e[j].y >> shift], w[j]);
+                own += w[j];
+            }
+            block_before<T>(s.wave_mass, own, mass);
+            const unsigned long long target = target_of(mass);
+            find<T>(s, true, 0, target + 1);
+            const uint32_t at = s.at;
+            const unsigned long long above = s.above_mass;
+            if (!pick(at, [&](int j) { return e[j].y >> shift; })) break;
+            const uint32_t m = s.n_few, per = sm.threads_for(m);
+            const uint32_t i = threadIdx.x / per, g = threadIdx.x % per;
+            const uint2 o = i < m ? s.few[i] : make_uint2(0, 0);
+            const unsigned long long mine = i < m ? s.few_mass[i] : 0;
+            unsigned long long before = 0;
+            for (uint32_t j = g; j < m; j += per)
+                if (s.few[j].y < o.y) before += s.few_mass[j];
+            before = above + sm.over_group(before, per);
+            const unsigned long long to = before + mine;
+            if (mine > 0 && g < 2 && before <= target && (to > target || to == mass))
+                finish(static_cast<int>(o.y), all,
+                       static_cast<double>(mass) * ldexp(1.0, -frac));
+            return;
+        }
         uint32_t tau = 0, keep_ties = 0;
         if (by_k) {
             sm.clear();
@@ -801,9 +944,9 @@ __global__ __launch_bounds__(T, kFilters ? 4 : KLP_OCC) void klp_sample_kernel(S
                 atomicAdd(&s.count[sm.bucket(value_of(k))], 1u);
             });
             __syncthreads();
-            find<T>(s, false, k_left, 0.0);
+            find<T>(s, false, k_left, 0);
             const uint32_t b = s.at, above = s.above_count;
-            const Border k = sm.resolve(listed, b, 0, above, 0, false, k_left, 0.0);
+            const Border k = sm.resolve(listed, b, 0, above, 0, false, k_left, 0);
             tau = k.tau;
             // A list may end before top_k: what is not in it has no weight.
             keep_ties = min(k_left - k.above, k.ties);
@@ -826,7 +969,7 @@ __global__ __launch_bounds__(T, kFilters ? 4 : KLP_OCC) void klp_sample_kernel(S
                     part += keep_ties * w;
                     atomicAdd(&s.mass[sm.bucket(value_of(tau))], keep_ties * sm.fixed(w));
                 }
-                share = fmax(p_left * over_waves(part) * ldexp(1.0, frac), 1.0);
+                share = share_of(over_waves(part) * ldexp(1.0, frac));
                 find<T>(s, true, 0, share);
                 p_at = s.at;
                 p_above = s.above_mass;
@@ -834,7 +977,7 @@ __global__ __launch_bounds__(T, kFilters ? 4 : KLP_OCC) void klp_sample_kernel(S
             const Border q = sm.resolve(listed, p_at, floor, 0, p_above, true, 0, share);
             tau = q.tau;
             const double one = static_cast<double>(sm.fixed(sm.weight(value_of(tau))));
-            const double left = share - static_cast<double>(q.above_mass);
+            const double left = static_cast<double>(share - q.above_mass);
             const double need = one > 0.0 ? ceil(left / one) : 1.0;
             uint32_t limit = q.ties;
             if (by_k && tau == floor) limit = min(limit, most_ties);
