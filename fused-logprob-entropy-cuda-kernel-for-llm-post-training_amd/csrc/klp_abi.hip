@@ -1721,6 +1721,9 @@ int klp_fp8_linear(const uint8_t* x, int64_t ld_x, const float* x_scales, const 
                     "out must be non-null and aligned to its elements, with a row stride >= n");
     if (m > (1 << 20) || n > (int64_t{1} << 31) || k > (1 << 24))
         return fail(KLP_EINVAL, "m, n and k must not exceed 2^20, 2^31 and 2^24");
+    // The narrowest tiles: 128 x 64 outputs.
+    if (ceil_div(m, 64) * ceil_div(n, 128) > INT32_MAX / 2)
+        return fail(KLP_EINVAL, "too many output tiles");
     klp::Fp8LinearParams p{};
     p.x = x;
     p.ld_x = ld_x;

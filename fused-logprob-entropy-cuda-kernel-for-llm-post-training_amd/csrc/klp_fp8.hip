@@ -30,7 +30,7 @@ __global__ __launch_bounds__(kQuantThreads) void klp_quantize_rows_kernel(Quanti
     const uint32_t b = item - row * nb;
     const int64_t c = static_cast<int64_t>(b) * kScaleBlock + (threadIdx.x % kLanes) * kChunk;
     float x[kChunk];
-    load_chunk<DT>(static_cast<const elem*>(p.x) + row * p.ld_x + c, p.dim - c, 0.0f, x);
+    load_chunk<DT>(static_cast<const elem*>(p.x) + row * p.ld_x + c, p.dim - c, x);
     const E4m3Scale e = e4m3_scale(row_max16(chunk_amax(x)));
     store_codes(p.q + row * p.dim + c, p.dim - c, e4m3_pack8(x, e.inv));
     if (threadIdx.x % kLanes == 0) p.scales[item] = e.scale;
@@ -49,7 +49,7 @@ __global__ __launch_bounds__(kQuantThreads) void klp_quantize_tile_kernel(Quanti
     for (int i = 0; i < kTileRows; ++i) {
         const int64_t row = row0 + i * kRowsAtOnce;
         load_chunk<DT>(static_cast<const elem*>(p.x) + row * p.ld_x + c,
-                       row < p.rows ? p.dim - c : 0, 0.0f, x[i]);
+                       row < p.rows ? p.dim - c : 0, x[i]);
     }
     float a = chunk_amax(x[0]);
 #pragma unroll

@@ -13,9 +13,8 @@
 // Bound by memory: the forward reads x (and the residual) once and writes y
 // (and h) once, holding the row in registers between its two uses; the
 // backward reads h and the gradients once.  A row is held by a group of 64 to
-// 1024 threads, 8 elements (a chunk) a thread and pass, so that a thread has
-// at least two 16-byte loads in flight and a group at most 8 chunks a thread:
-// rows of up to 65536 elements.
+// 1024 threads, 8 elements (a chunk) a thread and pass, 1 to 8 chunks a
+// thread: rows of up to 65536 elements.
 //
 // dw: a group walks rows with a fixed stride and keeps its share of the sum
 // in registers; the shares, [groups, dim] float32 in a workspace, are added
@@ -50,13 +49,14 @@ template <bool kF32, int DT>
 __device__ __forceinline__ void load_weight(const void* w, int64_t at, int64_t left,
                                             float (&x)[kChunk]) {
     if constexpr (kF32)
-        load_chunk<kFP32>(static_cast<const uint32_t*>(w) + at, left, 0.0f, x);
+        load_chunk<kFP32>(static_cast<const uint32_t*>(w) + at, left, x);
     else
-        load_chunk<DT>(static_cast<const typename Traits<DT>::elem*>(w) + at, left, 0.0f, x);
+        load_chunk<DT>(static_cast<const typename Traits<DT>::elem*>(w) + at, left, x);
 }
 
 // T threads a row, N chunks a thread; kFp8: codes and scales instead of y.
-template <int DT, int T, int N, bool kResidual, bool kFp8>
+// kWF32: a float32 weight.
+template <int DT, int T, int N, bool kWF32, bool kResidual, bool kFp8>
 __global__ __launch_bounds__(T < kBlockThreads ? kBlockThreads : T) void klp_norm_kernel(
     NormParams p) {
     typedef typename Traits<DT>::elem elem;
@@ -73,7 +73,7 @@ __global__ __launch_bounds__(T < kBlockThreads ? kBlockThreads : T) void klp_nor
 #pragma unroll
     for (int i = 0; i < N; ++i) {
         const int c = (i * T + t) * kChunk;
-        load_chunk<DT>(x + c, dim - c, 0.0f, h[i]);
+        load_chunk<DT>(x + c, dim - c, h[i]);
     }
     if constexpr (kResidual) {
         elem* out = static_cast<elem*>(p.h) + row * p.dim;
@@ -81,7 +81,7 @@ __global__ __launch_bounds__(T < kBlockThreads ? kBlockThreads : T) void klp_nor
         for (int i = 0; i < N; ++i) {
             const int c = (i * T + t) * kChunk;
             float b[kChunk];
-            load_chunk<DT>(r + c, dim - c, 0.0f, b);
+            load_chunk<DT>(r + c, dim - c, b);
 #pragma unroll
             for (int j = 0; j < kChunk; ++j) h[i][j] = to_f32<DT>(from_f32<DT>(h[i][j] + b[j]));
             store_chunk<DT>(out + c, dim - c, h[i]);
@@ -100,8 +100,7 @@ __global__ __launch_bounds__(T < kBlockThreads ? kBlockThreads : T) void klp_nor
     for (int i = 0; i < N; ++i) {
         const int c = (i * T + t) * kChunk;
         float w[kChunk], y[kChunk];
-        if (p.weight_f32) load_weight<true, DT>(p.weight, c, dim - c, w);
-        else load_weight<false, DT>(p.weight, c, dim - c, w);
+        load_weight<kWF32, DT>(p.weight, c, dim - c, w);
 #pragma unroll
         for (int j = 0; j < kChunk; ++j) y[j] = h[i][j] * s * w[j];
         if constexpr (kFp8) {
@@ -118,7 +117,7 @@ __global__ __launch_bounds__(T < kBlockThreads ? kBlockThreads : T) void klp_nor
 }
 
 // The backward: group g of the grid takes rows g, g + groups, ...
-template <int DT, int T, int N, bool kWithH>
+template <int DT, int T, int N, bool kWF32, bool kWithH>
 __global__ __launch_bounds__(T < kBlockThreads ? kBlockThreads : T) void klp_norm_bwd_kernel(
     NormBwdParams p) {
     typedef typename Traits<DT>::elem elem;
@@ -129,60 +128,100 @@ __global__ __launch_bounds__(T < kBlockThreads ? kBlockThreads : T) void klp_nor
     const int64_t groups = static_cast<int64_t>(gridDim.x) * kGroups;
     const int dim = static_cast<int>(p.dim);
     const float inv_dim = 1.0f / static_cast<float>(dim);
+    uint32_t* share = reinterpret_cast<uint32_t*>(p.partials) + group * p.dim;
 
-    float dw[N][kChunk];
+    // dx of a chunk, from its h and gy w.
+    auto put = [&](int64_t row, int c, float s, float a, const float (&h)[kChunk],
+                   const float (&gw)[kChunk]) {
+        float d[kChunk];
+        if constexpr (kWithH)
+            load_chunk<DT>(static_cast<const elem*>(p.g_h) + row * p.dim + c, dim - c, d);
 #pragma unroll
-    for (int i = 0; i < N; ++i)
-#pragma unroll
-        for (int j = 0; j < kChunk; ++j) dw[i][j] = 0.0f;
-
-    for (int64_t row = group; row < p.rows; row += groups) {
-        const elem* hp = static_cast<const elem*>(p.h) + row * p.ld_h;
-        const elem* gp = static_cast<const elem*>(p.g_y) + row * p.dim;
-        const float s = p.rstd[row];
-        float h[N][kChunk], g[N][kChunk];
-        float dot = 0.0f;
-#pragma unroll
-        for (int i = 0; i < N; ++i) {
-            const int c = (i * T + t) * kChunk;
-            load_chunk<DT>(hp + c, dim - c, 0.0f, h[i]);
-            load_chunk<DT>(gp + c, dim - c, 0.0f, g[i]);
+        for (int j = 0; j < kChunk; ++j) {
+            const float v = fmaf(-a, h[j], gw[j]);
+            d[j] = kWithH ? fmaf(s, v, d[j]) : s * v;
         }
+        store_chunk<DT>(static_cast<elem*>(p.d_x) + row * p.dim + c, dim - c, d);
+    };
+
+    if constexpr (N <= 2 || T < 1024) {
+        float dw[N][kChunk];
 #pragma unroll
-        for (int i = 0; i < N; ++i) {
-            const int c = (i * T + t) * kChunk;
-            float w[kChunk];
-            if (p.weight_f32) load_weight<true, DT>(p.weight, c, dim - c, w);
-            else load_weight<false, DT>(p.weight, c, dim - c, w);
+        for (int i = 0; i < N; ++i)
 #pragma unroll
-            for (int j = 0; j < kChunk; ++j) {
-                dw[i][j] = fmaf(g[i][j] * s, h[i][j], dw[i][j]);
-                g[i][j] *= w[j];
-                dot = fmaf(g[i][j], h[i][j], dot);
+            for (int j = 0; j < kChunk; ++j) dw[i][j] = 0.0f;
+        for (int64_t row = group; row < p.rows; row += groups) {
+            const elem* hp = static_cast<const elem*>(p.h) + row * p.ld_h;
+            const elem* gp = static_cast<const elem*>(p.g_y) + row * p.dim;
+            const float s = p.rstd[row];
+            float h[N][kChunk], g[N][kChunk];
+            float dot = 0.0f;
+#pragma unroll
+            for (int i = 0; i < N; ++i) {
+                const int c = (i * T + t) * kChunk;
+                load_chunk<DT>(hp + c, dim - c, h[i]);
+                load_chunk<DT>(gp + c, dim - c, g[i]);
+            }
+#pragma unroll
+            for (int i = 0; i < N; ++i) {
+                const int c = (i * T + t) * kChunk;
+                float w[kChunk];
+                load_weight<kWF32, DT>(p.weight, c, dim - c, w);
+#pragma unroll
+                for (int j = 0; j < kChunk; ++j) {
+                    dw[i][j] = fmaf(g[i][j] * s, h[i][j], dw[i][j]);
+                    g[i][j] *= w[j];
+                    dot = fmaf(g[i][j], h[i][j], dot);
+                }
+            }
+            dot = group_sum<T>(dot, lds);
+            const float a = s * s * dot * inv_dim;
+#pragma unroll
+            for (int i = 0; i < N; ++i) put(row, (i * T + t) * kChunk, s, a, h[i], g[i]);
+        }
+        if (p.partials != nullptr) {
+#pragma unroll
+            for (int i = 0; i < N; ++i) {
+                const int c = (i * T + t) * kChunk;
+                store_chunk<kFP32>(share + c, dim - c, dw[i]);
             }
         }
-        dot = group_sum<T>(dot, lds);
-        const float a = s * s * dot * inv_dim;
+    } else {
+        // Rows beyond 16384 columns: h, gy w and the sums of dw do not fit the
+        // 128 registers that a thread of 1024 has.  h and gy are read twice,
+        // the second time from L2, and the sums are kept where they end up, in
+        // the group's share of the workspace, each column by one thread.
+        for (int64_t row = group; row < p.rows; row += groups) {
+            const elem* hp = static_cast<const elem*>(p.h) + row * p.ld_h;
+            const elem* gp = static_cast<const elem*>(p.g_y) + row * p.dim;
+            const float s = p.rstd[row];
+            float dot = 0.0f, h[kChunk], g[kChunk], w[kChunk];
+#pragma unroll 1
+            for (int c = t * kChunk; c < dim; c += T * kChunk) {
+                load_chunk<DT>(hp + c, dim - c, h);
+                load_chunk<DT>(gp + c, dim - c, g);
+                load_weight<kWF32, DT>(p.weight, c, dim - c, w);
+                if (p.partials != nullptr) {
+                    float dw[kChunk];
+                    load_chunk<kFP32>(share + c, row == group ? 0 : dim - c, dw);
 #pragma unroll
-        for (int i = 0; i < N; ++i) {
-            const int c = (i * T + t) * kChunk;
-            float d[kChunk];
-            if constexpr (kWithH)
-                load_chunk<DT>(static_cast<const elem*>(p.g_h) + row * p.dim + c, dim - c, 0.0f, d);
+                    for (int j = 0; j < kChunk; ++j) dw[j] = fmaf(g[j] * s, h[j], dw[j]);
+                    store_chunk<kFP32>(share + c, dim - c, dw);
+                }
 #pragma unroll
-            for (int j = 0; j < kChunk; ++j) {
-                const float v = fmaf(-a, h[i][j], g[i][j]);
-                d[j] = kWithH ? fmaf(s, v, d[j]) : s * v;
+                for (int j = 0; j < kChunk; ++j) dot = fmaf(g[j] * w[j], h[j], dot);
             }
-            store_chunk<DT>(static_cast<elem*>(p.d_x) + row * p.dim + c, dim - c, d);
-        }
-    }
-    if (p.partials != nullptr) {
+            dot = group_sum<T>(dot, lds);
+            const float a = s * s * dot * inv_dim;
+#pragma unroll 1
+            for (int c = t * kChunk; c < dim; c += T * kChunk) {
+                load_chunk<DT>(hp + c, dim - c, h);
+                load_chunk<DT>(gp + c, dim - c, g);
+                load_weight<kWF32, DT>(p.weight, c, dim - c, w);
 #pragma unroll
-        for (int i = 0; i < N; ++i) {
-            const int c = (i * T + t) * kChunk;
-            store_chunk<kFP32>(reinterpret_cast<uint32_t*>(p.partials) + group * p.dim + c,
-                               dim - c, dw[i]);
+                for (int j = 0; j < kChunk; ++j) g[j] *= w[j];
+                put(row, c, s, a, h, g);
+            }
         }
     }
 }
@@ -210,28 +249,30 @@ __global__ __launch_bounds__(kSumWaves * 64) void klp_norm_dw_kernel(NormBwdPara
     }
 }
 
-template <int DT, int T, int N>
+template <int DT, int T, int N, bool kWF32>
 hipError_t launch_norm_shape(const NormParams& p, hipStream_t stream) {
     constexpr int kGroups = T < kBlockThreads ? kBlockThreads / T : 1;
     const dim3 grid(static_cast<unsigned>((p.rows + kGroups - 1) / kGroups));
     const dim3 block(T < kBlockThreads ? kBlockThreads : T);
+    const auto launch = [&](auto kernel) {
+        return launch_kernel(kernel, grid, block, stream, p);
+    };
     if (p.q != nullptr)
-        return p.residual != nullptr
-                   ? launch_kernel(klp_norm_kernel<DT, T, N, true, true>, grid, block, stream, p)
-                   : launch_kernel(klp_norm_kernel<DT, T, N, false, true>, grid, block, stream, p);
-    return p.residual != nullptr
-               ? launch_kernel(klp_norm_kernel<DT, T, N, true, false>, grid, block, stream, p)
-               : launch_kernel(klp_norm_kernel<DT, T, N, false, false>, grid, block, stream, p);
+        return p.residual != nullptr ? launch(klp_norm_kernel<DT, T, N, kWF32, true, true>)
+                                     : launch(klp_norm_kernel<DT, T, N, kWF32, false, true>);
+    return p.residual != nullptr ? launch(klp_norm_kernel<DT, T, N, kWF32, true, false>)
+                                 : launch(klp_norm_kernel<DT, T, N, kWF32, false, false>);
 }
 
-template <int DT, int T, int N>
+template <int DT, int T, int N, bool kWF32>
 hipError_t launch_norm_bwd_shape(const NormBwdParams& p, hipStream_t stream) {
     constexpr int kGroups = T < kBlockThreads ? kBlockThreads / T : 1;
     const dim3 grid(static_cast<unsigned>(p.groups / kGroups));
     const dim3 block(T < kBlockThreads ? kBlockThreads : T);
     return p.g_h != nullptr
-               ? launch_kernel(klp_norm_bwd_kernel<DT, T, N, true>, grid, block, stream, p)
-               : launch_kernel(klp_norm_bwd_kernel<DT, T, N, false>, grid, block, stream, p);
+               ? launch_kernel(klp_norm_bwd_kernel<DT, T, N, kWF32, true>, grid, block, stream, p)
+               : launch_kernel(klp_norm_bwd_kernel<DT, T, N, kWF32, false>, grid, block, stream,
+                               p);
 }
 
 template <int V> using Int = std::integral_constant<int, V>;
@@ -252,13 +293,18 @@ hipError_t with_shape(int64_t dim, F f) {
 template <int DT>
 hipError_t launch_norm_dt(const NormParams& p, hipStream_t stream) {
     return with_shape(p.dim, [&](auto t, auto n) {
-        return launch_norm_shape<DT, decltype(t)::value, decltype(n)::value>(p, stream);
+        constexpr int T = decltype(t)::value, N = decltype(n)::value;
+        return DT == kFP32 || p.weight_f32 ? launch_norm_shape<DT, T, N, true>(p, stream)
+                                           : launch_norm_shape<DT, T, N, DT == kFP32>(p, stream);
     });
 }
 template <int DT>
 hipError_t launch_norm_bwd_dt(const NormBwdParams& p, hipStream_t stream) {
     return with_shape(p.dim, [&](auto t, auto n) {
-        return launch_norm_bwd_shape<DT, decltype(t)::value, decltype(n)::value>(p, stream);
+        constexpr int T = decltype(t)::value, N = decltype(n)::value;
+        return DT == kFP32 || p.weight_f32
+                   ? launch_norm_bwd_shape<DT, T, N, true>(p, stream)
+                   : launch_norm_bwd_shape<DT, T, N, DT == kFP32>(p, stream);
     });
 }
 
@@ -276,7 +322,11 @@ hipError_t launch_norm(int dtype, const NormParams& p, hipStream_t stream) {
 // Groups of the backward: enough workgroups to fill the chip, a multiple of
 // the groups of one, and no more shares of dw than rows.
 int64_t norm_bwd_groups(int64_t rows, int64_t dim) {
-    const int64_t threads = dim <= 2048 ? 64 : dim <= 4096 ? 256 : dim <= 8192 ? 512 : 1024;
+    int64_t threads = 0;
+    with_shape(dim, [&](auto t, auto) {
+        threads = decltype(t)::value;
+        return hipSuccess;
+    });
     const int64_t per = threads < kBlockThreads ? kBlockThreads / threads : 1;
     int64_t groups = kNormBwdThreads / threads;
     if (groups > rows) groups = rows;

@@ -16,19 +16,41 @@ struct __attribute__((packed, aligned(alignof(E)))) Unaligned16 {
     u32x4 v;
 };
 
-// x[j] = p[j] for j < left, `fill` behind; all 8 when left >= 8.
-template <int DT>
+// x[j] = p[j] for j < left, 0 (or with kNegInf -inf) behind; all 8 when left
+// >= 8.  Two branches of one side each, on conditions that the compiler cannot
+// join to an if and else: its registers are then written before either, and on
+// no path hold what another wave left.
+template <int DT, bool kNegInf = false>
 __device__ __forceinline__ void load_chunk(const typename Traits<DT>::elem* p, int64_t left,
-                                           float fill, float (&x)[kChunk]) {
+                                           float (&x)[kChunk]) {
     typedef typename Traits<DT>::elem elem;
+    constexpr int kVecs = DT == kFP32 ? 2 : 1;
+    constexpr uint32_t kFill = kNegInf ? Traits<DT>::kNegInfWord : 0;
+    u32x4 raw[kVecs];
+#pragma unroll
+    for (int k = 0; k < kVecs; ++k) raw[k] = u32x4{kFill, kFill, kFill, kFill};
     if (left >= kChunk) {
         const auto* v = reinterpret_cast<const Unaligned16<elem>*>(p);
-        unpack<DT>(v[0].v, x);
-        if constexpr (DT == kFP32) unpack<DT>(v[1].v, x + 4);
-    } else {
 #pragma unroll
-        for (int j = 0; j < kChunk; ++j) x[j] = j < left ? to_f32<DT>(p[j]) : fill;
+        for (int k = 0; k < kVecs; ++k) raw[k] = v[k].v;
     }
+#pragma unroll
+    for (int k = 0; k < kVecs; ++k) asm("" : "+v"(raw[k]));
+    int some = left > 0 && left < kChunk ? static_cast<int>(left) : 0;
+    asm("" : "+v"(some));
+    if (some > 0) {
+#pragma unroll
+        for (int j = 0; j < kChunk; ++j) {
+            const uint32_t e = p[j < some ? j : some - 1];
+            const uint32_t fill = DT == kFP32 ? kFill : kFill & 0xFFFFu;
+            const uint32_t w = j < some ? e : fill;
+            if constexpr (DT == kFP32) raw[j / 4][j % 4] = w;
+            else if (j & 1) raw[0][j / 2] |= w << 16;
+            else raw[0][j / 2] = w;
+        }
+    }
+    unpack<DT>(raw[0], x);
+    if constexpr (DT == kFP32) unpack<DT>(raw[1], x + 4);
 }
 
 // p[j] = round(x[j]) for j < left.

@@ -45,9 +45,6 @@ namespace klp {
 
 namespace {
 
-#ifndef KLP_OCC
-#define KLP_OCC 6
-#endif
 constexpr int kMaxWaves = 16;
 constexpr int kBucketBits = 11;
 constexpr int kBuckets = 1 << kBucketBits;
@@ -55,7 +52,6 @@ constexpr int kList = 4096;
 // Lists whose entries are compared with each other; longer ones go through
 // histograms.
 constexpr int kRanked = 256;
-constexpr int kBatch = 4;  // chunks of a lane in flight
 // The histogram for top-p counts one of so many chunks, to foresee the list's length.
 constexpr int kCountEvery = 8;
 // Buckets of the first histogram to a factor of 2 of the weight; elements of
@@ -196,9 +192,11 @@ struct Row {
     const elem* x;
     int vocab;
     int span;  // elements of a wave: a contiguous part of the row
+    // Chunks of a lane in flight.
+    static constexpr int kBatch = DT == kFP32 ? 2 : 4;
 
     __device__ __forceinline__ void load(int at, float (&v)[kChunk]) const {
-        load_chunk<DT>(x + at, vocab - at, -INFINITY, v);
+        load_chunk<DT, true>(x + at, vocab - at, v);
     }
     // f(first element, 8 values) for each chunk of this wave's part, the next
     // kBatch of them being loaded.  Values behind the row's end are -inf.
@@ -242,13 +240,28 @@ struct Row {
             f(at, v);
         }
     }
+    // The same for the passes that few rows take: a chunk at a time and f's
+    // code once, since all passes with theirs five times over are more than a
+    // branch of the kernel can span.
+    template <typename F>
+    __device__ __forceinline__ void each_small(F f) const {
+        const int begin = (threadIdx.x >> 6) * span;
+        const int end = min(begin + span, vocab);
+#pragma unroll 1
+        for (int at = begin + static_cast<int>(threadIdx.x & 63) * kChunk; at < end;
+             at += 64 * kChunk) {
+            float v[kChunk];
+            load(at, v);
+            f(at, v);
+        }
+    }
 };
 
 // The first bucket, in order, at which the running count reaches `count` (or,
 // with by_mass, the running mass reaches `mass`); the last one with anything
 // in it when none does.  Into s.at, with what lies before it.
 template <int T>
-__device__ void find(Shared<true>& s, bool by_mass, uint32_t count, unsigned long long mass) {
+__device__ __forceinline__ void find(Shared<true>& s, bool by_mass, uint32_t count, unsigned long long mass) {
     constexpr int kPerThread = kBuckets / T;
     const int first = threadIdx.x * kPerThread;
     uint32_t c[kPerThread], c_sum = 0;
@@ -351,7 +364,7 @@ struct Sampler {
             const uint32_t n = s.n_list;
             for (uint32_t i = threadIdx.x; i < n; i += T) f(~s.list[i].x);
         } else {
-            row.each([&](int, const float (&v)[kChunk]) {
+            row.each_small([&](int, const float (&v)[kChunk]) {
 #pragma unroll
                 for (int j = 0; j < kChunk; ++j) f(key_of(v[j]));
             });
@@ -360,7 +373,7 @@ struct Sampler {
 
     // The border inside first-histogram bucket b, among keys >= floor, with
     // `above` elements and above_mass before the bucket.
-    __device__ Border resolve(bool listed, uint32_t b, uint32_t floor, uint32_t above,
+    __device__ __forceinline__ Border resolve(bool listed, uint32_t b, uint32_t floor, uint32_t above,
                               unsigned long long above_mass, bool by_mass, uint32_t count,
                               unsigned long long mass) {
         __syncthreads();
@@ -428,7 +441,7 @@ struct Sampler {
     // does, and among those the element.  Where rounding (or u = 1) lets none
     // cross, the last that has a weight.  The wave of that thread returns the
     // token, the others -1.
-    __device__ int search(float u, uint32_t tau, uint32_t keep_ties, double min_w, double& mass) {
+    __device__ __forceinline__ int search(float u, uint32_t tau, uint32_t keep_ties, double min_w, double& mass) {
         const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
         double tau_w = keep_ties > 0 ? weight(value_of(tau)) : 0.0;
         if (tau_w < min_w) tau_w = 0.0;
@@ -520,7 +533,7 @@ struct Sampler {
 
 // kFilters: rows may have filters, or a temperature of 0.
 template <int DT, int T, bool kFilters>
-__global__ __launch_bounds__(T, kFilters ? 4 : KLP_OCC) void klp_sample_kernel(SampleParams p) {
+__global__ __launch_bounds__(T, kFilters ? 4 : 6) void klp_sample_kernel(SampleParams p) {
     constexpr int kWaves = T / 64;
     __shared__ Shared<kFilters> s;
     const int64_t r = blockIdx.x;
@@ -728,7 +741,7 @@ __global__ __launch_bounds__(T, kFilters ? 4 : KLP_OCC) void klp_sample_kernel(S
                     : -INFINITY;
             bool summed = !by_k && by_p;
             if (!summed && !(fabsf(offset) < 0x1p20f)) {  // a temperature near 0
-                row.each([&](int, const float (&v)[kChunk]) {
+                row.each_small([&](int, const float (&v)[kChunk]) {
 #pragma unroll
                     for (int j = 0; j < kChunk; ++j) all += sm.weight(v[j]);
                 });
@@ -1006,7 +1019,7 @@ __global__ __launch_bounds__(T, kFilters ? 4 : KLP_OCC) void klp_sample_kernel(S
             }
         } else {
             kept = 0.0;
-            row.each([&](int, const float (&v)[kChunk]) {
+            row.each_small([&](int, const float (&v)[kChunk]) {
 #pragma unroll
                 for (int j = 0; j < kChunk; ++j) {
                     const uint32_t k = key_of(v[j]);
@@ -1045,9 +1058,6 @@ hipError_t launch_sample_dt(const SampleParams& p, hipStream_t stream) {
                        p.min_ps == nullptr && p.temperature != 0.0f &&
                        !(p.top_k > 0 && p.top_k < p.vocab) && !(p.top_p < 1.0f) &&
                        !(p.min_p > 0.0f);
-#ifdef KLP_ST
-    return launch_sample_threads<DT, KLP_ST>(plain, p, stream);
-#endif
     if (p.n_rows > kHeadGemmCus) return launch_sample_threads<DT, 512>(plain, p, stream);
     return launch_sample_threads<DT, 1024>(plain, p, stream);
 }
