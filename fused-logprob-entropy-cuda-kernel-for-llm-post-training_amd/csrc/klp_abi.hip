@@ -705,6 +705,14 @@ int check_dtype3(int dtype, const char* name) {
     return fail(KLP_EDTYPE, "%s dtype must be bf16, fp16, or fp32", name);
 }
 
+// A launch has fewer than 2^32 threads.
+int check_threads(int64_t groups, int64_t threads, const char* what) {
+    if (groups > (int64_t{1} << 32) / threads - 1)
+        return fail(KLP_EINVAL, "too many %s for one launch: %lld", what,
+                    static_cast<long long>(groups));
+    return KLP_OK;
+}
+
 int check_norm(const void* x, int dtype, int64_t rows, int64_t dim, const void* weight,
                int weight_dtype) {
     int rc = check_dtype3(dtype, "x");
@@ -716,6 +724,9 @@ int check_norm(const void* x, int dtype, int64_t rows, int64_t dim, const void* 
         return fail(KLP_EINVAL, "dim must be in [1, %lld], got %lld",
                     static_cast<long long>(klp::kNormMaxDim), static_cast<long long>(dim));
     if (rows > INT32_MAX) return fail(KLP_EINVAL, "rows above 2^31-1 are not supported");
+    // Four rows of 64 threads share a workgroup.
+    if ((rc = check_threads(ceil_div(rows, 4) * 4, klp::norm_threads(dim), "rows")) != KLP_OK)
+        return rc;
     if (rows == 0) return KLP_OK;
     if (x == nullptr || !aligned(x, elem_bytes(dtype)))
         return fail(KLP_EINVAL, "x must be non-null and aligned to its elements");
@@ -1680,12 +1691,17 @@ int klp_quantize_fp8(const void* x, int dtype, int64_t ld_x, int64_t rows, int64
     if (q == nullptr) return fail(KLP_EINVAL, "q must be non-null");
     if ((rc = check_f32(scales, "scales")) != KLP_OK) return rc;
     const int64_t n_blocks = ceil_div(dim, klp::kScaleBlock);
-    // The grid: one 16-lane group per block of a row, or a workgroup per
-    // block with at most 65535 along the rows.
+    // The grid: one 16-lane group per block of a row, 16 a workgroup, or a
+    // workgroup per block with at most 65535 along the rows.
     if (n_blocks > INT32_MAX / rows ||
         (block_rows != 1 && ceil_div(rows, klp::kScaleBlock) > 65535))
         return fail(KLP_EINVAL, "too many scale blocks: %lld rows of %lld",
                     static_cast<long long>(rows), static_cast<long long>(n_blocks));
+    if ((rc = block_rows == 1
+                  ? check_threads(ceil_div(rows * n_blocks, 16) * 16, 16, "scale blocks")
+                  : check_threads(ceil_div(rows, klp::kScaleBlock) * n_blocks, 256,
+                                  "scale blocks")) != KLP_OK)
+        return rc;
     klp::QuantizeParams p{};
     p.x = x;
     p.ld_x = ld_x;
@@ -1721,9 +1737,12 @@ int klp_fp8_linear(const uint8_t* x, int64_t ld_x, const float* x_scales, const 
                     "out must be non-null and aligned to its elements, with a row stride >= n");
     if (m > (1 << 20) || n > (int64_t{1} << 31) || k > (1 << 24))
         return fail(KLP_EINVAL, "m, n and k must not exceed 2^20, 2^31 and 2^24");
-    // The narrowest tiles: 128 x 64 outputs.
-    if (ceil_div(m, 64) * ceil_div(n, 128) > INT32_MAX / 2)
-        return fail(KLP_EINVAL, "too many output tiles");
+    // The narrowest tiles, 128 x 64 outputs, and their grid's multiple of 8;
+    // or 16 weight rows and 64 tokens a workgroup, where row strides are long.
+    if ((rc = check_threads(ceil_div(m, 64) * ceil_div(n, 128) + 8, 512, "output tiles")) !=
+            KLP_OK ||
+        (rc = check_threads(ceil_div(n, 16), 256, "weight rows")) != KLP_OK)
+        return rc;
     klp::Fp8LinearParams p{};
     p.x = x;
     p.ld_x = ld_x;
@@ -1756,6 +1775,8 @@ int klp_sample(const void* logits, int dtype, int64_t n_rows, int64_t vocab, int
         return fail(KLP_EINVAL, "tokens must be non-null and 8-byte aligned");
     if (vocab > klp::kSampleMaxVocab)
         return fail(KLP_EINVAL, "vocab above 2^26 is not supported");
+    // A workgroup of 512 a row, of 1024 where rows are few.
+    if ((rc = check_threads(n_rows, 512, "rows")) != KLP_OK) return rc;
     if ((rc = check_f32(uniform, "uniform")) != KLP_OK) return rc;
     if ((rc = check_f32(logp, "logp")) != KLP_OK) return rc;
     if ((rc = check_f32(sample_logp, "sample_logp")) != KLP_OK) return rc;

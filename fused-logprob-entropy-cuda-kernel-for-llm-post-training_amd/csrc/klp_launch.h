@@ -324,6 +324,7 @@ struct NormBwdParams {
 };
 // Threads of the backward's grid: 1024 a CU.
 constexpr int64_t kNormBwdThreads = 256 * 1024;
+int64_t norm_threads(int64_t dim);  // of a row
 int64_t norm_bwd_groups(int64_t rows, int64_t dim);
 hipError_t launch_norm(int dtype, const NormParams& p, hipStream_t stream);
 hipError_t launch_norm_bwd(int dtype, const NormBwdParams& p, hipStream_t stream);

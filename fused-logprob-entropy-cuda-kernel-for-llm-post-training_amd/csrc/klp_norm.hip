@@ -319,14 +319,19 @@ hipError_t launch_norm(int dtype, const NormParams& p, hipStream_t stream) {
     }
 }
 
-// Groups of the backward: enough workgroups to fill the chip, a multiple of
-// the groups of one, and no more shares of dw than rows.
-int64_t norm_bwd_groups(int64_t rows, int64_t dim) {
+int64_t norm_threads(int64_t dim) {
     int64_t threads = 0;
     with_shape(dim, [&](auto t, auto) {
         threads = decltype(t)::value;
         return hipSuccess;
     });
+    return threads;
+}
+
+// Groups of the backward: enough workgroups to fill the chip, a multiple of
+// the groups of one, and no more shares of dw than rows.
+int64_t norm_bwd_groups(int64_t rows, int64_t dim) {
+    const int64_t threads = norm_threads(dim);
     const int64_t per = threads < kBlockThreads ? kBlockThreads / threads : 1;
     int64_t groups = kNormBwdThreads / threads;
     if (groups > rows) groups = rows;

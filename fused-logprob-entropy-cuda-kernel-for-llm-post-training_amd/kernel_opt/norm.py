@@ -8,7 +8,8 @@ compute, per row of ``dim`` elements,
 
 in one pass (csrc/klp_norm.hip), differentiable in ``x``, ``residual`` and
 ``weight``: the backward reads ``h`` and one float32 a row.  The statistics are
-those of the stored ``h``, all sums are float32, ``y`` is rounded once.
+those of the stored ``h``, all sums are float32, ``y`` is rounded once; a row
+whose sum of squares passes float32's range gives zeros.
 
 ``fused_rms_norm_fp8`` / ``fused_add_rms_norm_fp8`` write the same ``y`` as
 e4m3 codes with a float32 scale for each 128 columns, the operand of

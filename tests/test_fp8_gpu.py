@@ -240,3 +240,91 @@ def test_linear_graph_and_stream():
         g.replay()
         torch.cuda.synchronize()
         assert torch.equal(out, _ko().fp8_linear(xq, xs, wq, ws))
+
+
+def test_refusals():
+    ko = _ko()
+    x = torch.randn(4, 256, device=DEV)
+    with pytest.raises(ValueError, match="block_rows"):
+        ko.quantize_fp8(x, 64)
+    with pytest.raises(RuntimeError, match="bf16, fp16, or fp32"):
+        ko.quantize_fp8(x.double())
+    with pytest.raises(RuntimeError, match=r"\[N, dim\]"):
+        ko.quantize_fp8(x[None], 128)
+    with pytest.raises(RuntimeError, match="dim >= 1"):
+        ko.quantize_fp8(x[:, :0])
+    q, s = ko.quantize_fp8(x)
+    w, ws = ko.quantize_fp8(torch.randn(300, 256, device=DEV), 128)
+    good = (q, s, w, ws)
+
+    def refused(text, at=None, value=None, **kw):
+        args = list(good)
+        if at is not None:
+            args[at] = value
+        with pytest.raises(RuntimeError, match=text):
+            ko.fp8_linear(*args, **kw)
+
+    refused("GPU tensors", 1, s.cpu())
+    refused("float8_e4m3fn", 0, x)
+    refused("float8_e4m3fn", 2, w.view(torch.uint8))
+    refused("scales must be float32", 3, ws.bfloat16())
+    refused("out_dtype", out_dtype=torch.float64)
+    refused("x must be", 0, q[:, :128])
+    refused("x must be", 2, w[0])
+    refused("x must be", 2, w[:0])
+    refused("x_scale must be", 1, s[:3])
+    refused("x_scale must be", 1, s[:, :1])
+    refused("weight_scale must be", 3, ws[:2])
+    refused("no gradient", 1, s.clone().requires_grad_())
+    with torch.no_grad():
+        ko.fp8_linear(q, s.clone().requires_grad_(), w, ws)
+    with pytest.raises(RuntimeError, match="multiple of 16"):
+        ko.fp8_linear(q[:, :40], s[:, :1], w[:, :40], ws[:, :1])
+    # Rows that do not start at multiples of 16 bytes.
+    with pytest.raises(RuntimeError, match="16"):
+        ko.fp8_linear(q[:, 8:136], s[:, :1], w[:, 8:136], ws[:, :1])
+    odd = torch.zeros(4, 264, dtype=torch.uint8, device=DEV).view(torch.float8_e4m3fn)[:, :256]
+    with pytest.raises(RuntimeError, match="multiples of 16"):
+        ko.fp8_linear(odd, s, w, ws)
+
+
+def test_linear_beyond_32_bits():
+    """Weights and outputs of more than 2^32 bytes or 2^31 elements: the last
+    rows and columns are those of the product of these alone; a row that is
+    every row."""
+    ko = _ko()
+    g = torch.Generator(device=DEV).manual_seed(7)
+    byte = lambda *sh: torch.randint(0, 0x70, sh, dtype=torch.uint8, device=DEV,  # noqa: E731
+                                     generator=g).view(torch.float8_e4m3fn)
+    n, k = 2 ** 18 + 128, 2 ** 14 + 16
+    w = torch.zeros(n, k, dtype=torch.uint8, device=DEV).view(torch.float8_e4m3fn)
+    w[-256:] = byte(256, k)
+    nb = -(-k // 128)
+    ws = torch.rand(-(-n // 128), nb, device=DEV, generator=g)
+    for m in (3, 300):
+        x, xs = byte(m, k), torch.rand(m, nb, device=DEV, generator=g)
+        out = ko.fp8_linear(x, xs, w, ws)
+        # Another count of outputs may take another kernel: K is then added in
+        # another order, 130 blocks' sums of like size and all positive.
+        ref = ko.fp8_linear(x, xs, w[-256:], ws[-2:]).float()
+        tol = 2 * 2.0 ** -8 + 2 * 140 * 2.0 ** -24 + 7 * 2.0 ** -13
+        assert ((out[:, -256:].float() - ref).abs() <= tol * ref).all()
+    del w, out
+    n, m, k = 152064, 15000, 128
+    x, xs = byte(m, k), torch.rand(m, 1, device=DEV, generator=g)
+    w, ws = byte(n, k), torch.rand(n // 128, 1, device=DEV, generator=g)
+    out = ko.fp8_linear(x, xs, w, ws)
+    assert out.numel() > 2 ** 31
+    assert torch.equal(out[-300:], ko.fp8_linear(x[-300:], xs[-300:], w, ws))
+    same = ko.fp8_linear(x[-1:].expand(70, k), xs[-1:].expand(70, 1), w, ws)
+    assert torch.equal(same, out[-1:].expand(70, n))
+
+
+def test_quantize_beyond_32_bits():
+    ko = _ko()
+    x = torch.zeros(2 ** 20 + 3, 2056, dtype=torch.bfloat16, device=DEV)
+    x[-5:] = torch.randn(5, 2056, device=DEV)
+    q, s = ko.quantize_fp8(x)
+    q1, s1 = ko.quantize_fp8(x[-5:])
+    assert torch.equal(q[-5:].view(torch.uint8), q1.view(torch.uint8))
+    assert torch.equal(s[-5:], s1)

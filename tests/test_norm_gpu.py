@@ -120,6 +120,20 @@ def test_weight_gradient_over_many_rows(rows):
     _assert_grads(dx, dw, x, w, gy, None, torch.float32)
 
 
+@pytest.mark.parametrize("dim", [16392, 33001])
+@pytest.mark.parametrize("weight_dtype", [torch.bfloat16, torch.float32], ids=["w16", "w32"])
+def test_weight_gradient_over_many_wide_rows(dim, weight_dtype):
+    """More rows than groups, so that a group adds rows to its share."""
+    x, res, w, gy, gh = _data(523, dim, torch.bfloat16, dim, weight_dtype)
+    xs, rs, ws = (t.to(DEV).requires_grad_() for t in (x, res, w))
+    y, h = _ko().fused_add_rms_norm(xs, rs, ws, EPS)
+    dx, dw = torch.autograd.grad((y, h), (xs, ws), (gy.to(DEV), gh.to(DEV)))
+    _assert_grads(dx, dw, h.detach().cpu(), w, gy, gh, torch.bfloat16)
+    only_x, = torch.autograd.grad(_ko().fused_add_rms_norm(xs, rs, ws.detach(), EPS), xs,
+                                  (gy.to(DEV), gh.to(DEV)))
+    assert torch.equal(only_x, dx)
+
+
 def test_gradient_against_differences():
     """Central differences of <y, gy> + <h, gh> in float64 along random
     directions, with the oracle's forward; the kernel's gradient is float32."""
@@ -283,3 +297,47 @@ def test_streams_repeats_and_graph():
         torch.cuda.synchronize()
         assert all(torch.equal(a, b) for a, b in zip(out, step()))
 
+
+
+def test_refusals():
+    ko = _ko()
+    x = torch.zeros(4, 64, dtype=torch.bfloat16, device=DEV)
+    w = torch.ones(64, dtype=torch.bfloat16, device=DEV)
+    for f in (ko.fused_rms_norm, ko.fused_rms_norm_fp8):
+        for bad, text in ((w[:63], "weight must be"), (w.cpu(), "weight must be"),
+                          (w.half(), "weight must be float32"), (w[None], "weight must be")):
+            with pytest.raises(RuntimeError, match=text):
+                f(x, bad)
+        with pytest.raises(RuntimeError, match="eps"):
+            f(x, w, -1e-6)
+        with pytest.raises(RuntimeError, match="eps"):
+            f(x, w, float("nan"))
+        with pytest.raises(RuntimeError, match="bf16, fp16, or fp32"):
+            f(x.double(), w)
+        with pytest.raises(RuntimeError, match="last dim"):
+            f(torch.zeros(2, 65537, dtype=torch.bfloat16, device=DEV), w)
+        with pytest.raises(RuntimeError, match="last dim"):
+            f(torch.zeros(2, 0, dtype=torch.bfloat16, device=DEV), w[:0])
+    for f in (ko.fused_add_rms_norm, ko.fused_add_rms_norm_fp8):
+        for bad in (x[:3], x.half(), x.cpu(), x[:, :63]):
+            with pytest.raises(RuntimeError, match="residual must have"):
+                f(x, bad, w)
+
+
+def test_rows_beyond_32_bits():
+    """The last rows of 2^31 and more elements, and rows that share memory."""
+    ko = _ko()
+    g = torch.Generator(device=DEV).manual_seed(1)
+    rows, dim = 2 ** 19 + 5, 4104
+    x = torch.empty(rows, dim, dtype=torch.bfloat16, device=DEV)
+    x[-3:] = torch.randn(3, dim, generator=g, device=DEV)
+    w = torch.randn(dim, generator=g, device=DEV)
+    y = ko.fused_rms_norm(x, w, EPS)
+    assert torch.equal(y[-3:], ko.fused_rms_norm(x[-3:], w, EPS))
+    del y
+    q, s = ko.fused_rms_norm_fp8(x, w, EPS)
+    q1, s1 = ko.fused_rms_norm_fp8(x[-3:], w, EPS)
+    assert torch.equal(q[-3:].view(torch.uint8), q1.view(torch.uint8))
+    assert torch.equal(s[-3:], s1)
+    one = x[-1:].expand(9, dim)
+    assert torch.equal(ko.fused_rms_norm(one, w, EPS), ko.fused_rms_norm(one.contiguous(), w, EPS))

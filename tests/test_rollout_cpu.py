@@ -77,6 +77,26 @@ def test_norm_output_refusals():
     _refused(_norm8(scales=None), "KLP_EINVAL", "scales")
 
 
+def test_launches_of_too_many_threads_are_refused():
+    """2^32 threads or more: a row takes 64 to 1024 of the norm, a scale block
+    16 or 256, 16 weight rows 256, 128 x 64 outputs 512, a sampled row 512."""
+    L = _lib().lib
+    for dim, threads in ((8, 64), (2049, 256), (5000, 512), (65536, 1024)):
+        most = 2 ** 32 // threads
+        _refused(_norm(rows=most, dim=dim, ld=dim), "KLP_EINVAL", "too many rows")
+        _refused(_norm8(rows=most, dim=dim, ld=dim), "KLP_EINVAL", "too many rows")
+        _refused(L.klp_rms_norm_bwd(P, 0, dim, P, 0, P, P, None, most, dim, P, None, None, 0, None),
+                 "KLP_EINVAL", "too many rows")
+    _refused(L.klp_quantize_fp8(P, 0, 128, 2 ** 28, 128, 1, P, P, None), "KLP_EINVAL", "too many")
+    _refused(L.klp_quantize_fp8(P, 0, 128, 2 ** 22, 2 ** 16, 128, P, P, None), "KLP_EINVAL",
+             "too many")
+    for m, n in ((1, 2 ** 30), (2 ** 20, 2 ** 20)):
+        _refused(L.klp_fp8_linear(P, 16, P, P, 16, P, m, n, 16, 0, P, n, None), "KLP_EINVAL",
+                 "too many")
+    _refused(L.klp_sample(P, 0, 2 ** 23, 8, 2 ** 23, 0, 8, P, 1.0, None, 0, None, 1.0, None, 0.0,
+                          None, P, P, P, None), "KLP_EINVAL", "too many rows")
+
+
 def test_norm_backward_refusals():
     L = _lib()
     need = L.lib.klp_rms_norm_bwd_workspace_bytes(100, 64)

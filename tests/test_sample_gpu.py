@@ -269,3 +269,56 @@ def test_repeatable_stream_and_graph():
         torch.cuda.synchronize()
         assert all(torch.equal(a, b) for a, b in zip(out, ko.fused_sample(x, u, 0.8, **kw)))
         assert all(torch.equal(a, b) for a, b in zip(free, ko.fused_sample(x, u)))
+
+
+def test_refusals():
+    ko = _ko()
+    x = torch.zeros(4, 100, dtype=torch.bfloat16, device=DEV)
+    u = torch.zeros(4, device=DEV)
+    for bad in (u[:3], u.double(), u[None]):
+        with pytest.raises(RuntimeError, match="uniform must be"):
+            ko.fused_sample(x, bad)
+    with pytest.raises(RuntimeError, match="GPU tensors"):
+        ko.fused_sample(x, u.cpu())
+    with pytest.raises(RuntimeError, match="bf16, fp16, or fp32"):
+        ko.fused_sample(x.double(), u)
+    with pytest.raises(RuntimeError, match="contiguous"):
+        ko.fused_sample(x[:, ::2], u)
+    with pytest.raises(RuntimeError, match="vocab"):
+        ko.fused_sample(x[:, :0], u)
+    for t in (-1.0, float("inf"), float("nan")):
+        with pytest.raises(ValueError, match="temperature"):
+            ko.fused_sample(x, u, t)
+    with pytest.raises(ValueError, match="top_k"):
+        ko.fused_sample(x, u, top_k=1.5)
+    with pytest.raises(ValueError, match="top_p"):
+        ko.fused_sample(x, u, top_p=1.5)
+    with pytest.raises(ValueError, match="min_p"):
+        ko.fused_sample(x, u, min_p=-0.5)
+    for name in ("temperature", "top_k", "top_p", "min_p"):
+        with pytest.raises(RuntimeError, match=f"{name} must be"):
+            ko.fused_sample(x, u, **{name: u[:3]})
+    with pytest.raises(RuntimeError, match="top_k must hold integers"):
+        ko.fused_sample(x, u, top_k=u)
+
+
+def test_logits_beyond_32_bits():
+    """The last rows of more than 2^31 logits, and rows that share memory."""
+    ko = _ko()
+    rows, vocab = 16500, 131077
+    g = torch.Generator(device=DEV).manual_seed(3)
+    x = torch.empty(rows, vocab, dtype=torch.bfloat16, device=DEV)
+    x[:] = torch.randn(vocab, device=DEV, generator=g).to(torch.bfloat16)
+    x[-3:] = torch.randn(3, vocab, device=DEV, generator=g).to(torch.bfloat16)
+    u = torch.rand(rows, device=DEV, generator=g)
+    for how in ({}, {"top_k": 40}, {"top_p": 0.5}, {"min_p": 0.1}):
+        whole = ko.fused_sample(x, u, **how)
+        last = ko.fused_sample(x[-3:], u[-3:], **how)
+        assert torch.equal(whole[0][-3:], last[0])
+        # 512 or 1024 threads add the weights in another order.
+        for a, b in zip(whole[1:], last[1:]):
+            assert ((a[-3:] - b).abs() <= 4 * 2.0 ** -24 * (1 + b.abs())).all()
+    one = x[-1:].expand(9, vocab)
+    a = ko.fused_sample(one, u[:9], top_p=0.9)
+    b = ko.fused_sample(one.contiguous(), u[:9], top_p=0.9)
+    assert all(torch.equal(p, q) for p, q in zip(a, b))
