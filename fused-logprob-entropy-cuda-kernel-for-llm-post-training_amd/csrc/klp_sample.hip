@@ -12,10 +12,9 @@
 // Precision.  The token and the kept set are decided where a running sum over
 // the whole row crosses a border, and a row of 10^5 comparable weights has
 // 10^5 such borders: sums off by 10^-7 (float32) pick another token in one of
-// 100 rows.  So weights are computed in float64 (2^f by a polynomial of
-// degree 7, off by 10^-10 at most and, its error changing sign over f, far less
-// in a sum) and added in float64, or, in histograms,
-// as 64-bit integers of 2^-44, whose sums do not depend on the order of the
+// 100 rows.  So weights are computed in float64 (off by 1.5 10^-10 at most and,
+// since that error changes sign with the logit, far less in a sum) and added in
+// float64, or, in histograms, as 64-bit integers of 2^-44, whose sums do not depend on the order of the
 // atomics.
 //
 // A row is read by one workgroup, a contiguous part of it by each wave.
@@ -60,28 +59,45 @@ constexpr int kPerBit = kBuckets / 64;
 constexpr double kLog2eD = 1.44269504088896340736;
 constexpr double kLn2D = 0.69314718055994530942;
 
-// Weights below this one are none: exp2_d's smallest is 2^-1000, for a logit
+// Weights below this one are none: exp2's smallest is 2^-1000, for a logit
 // of -inf too, and a row of 2^26 of those sums to less than this.
 constexpr double kNothing = 0x1p-960;
 
-// 2^y for y < 1000: 2^f with f = y - rint(y) as 1 + f q(f), q interpolating
-// (2^f - 1) / f at the Chebyshev points of [-1/2, 1/2].  Adding 1.5 2^52
-// rounds to an integer and leaves it in the sum's low bits, from where it goes
-// into the result's exponent.
-__device__ __forceinline__ double exp2_d(double y) {
-    constexpr double kRound = 0x1.8p52;
-    y = fmax(y, -1000.0);
-    const double z = y + kRound;
-    const double f = y - (z - kRound);
-    double q = 0x1.00a581cp-16;
-    q = fma(q, f, 0x1.443fffc96db6ep-13);
-    q = fma(q, f, 0x1.5d879eac8p-10);
-    q = fma(q, f, 0x1.3b2a1b71525b6p-7);
-    q = fma(q, f, 0x1.c6b08d883e1b7p-5);
-    q = fma(q, f, 0x1.ebfbe045f4d3ep-3);
+// 2^y for |y| <= 1000 as t g: t = 2^(n / 32), n = rint(32 y), from a table of
+// 2^(i / 32), i < 32, and g = 2^f, f = y - n / 32, as 1 + f q(f), q
+// interpolating (2^f - 1) / f at the Chebyshev points of [-1/64, 1/64].
+// Adding kRound rounds to n / 32 and leaves n in the sum's low word.  An entry
+// lacks i 2^15 in its high word, which n 2^15 = (n / 32) 2^20 + (n % 32) 2^15
+// puts back along with the exponent.  32 entries of 8 bytes lie in different
+// LDS banks: a lookup is as fast as memory gives 64 lanes 8 bytes each, and
+// together with 3 products fewer than the 7 of a polynomial on [-1/2, 1/2]:
+// 80 against 90 us for 1024 rows of 128256 (fp16, unfiltered), where
+// arithmetic is the bound.
+constexpr double kRound = 0x1.8p47;
+constexpr int kExp2Entries = 32;
+__device__ const unsigned long long kExp2Table[kExp2Entries] = {
+    0x3ff0000000000000ull, 0x3fefd9b0d3158574ull, 0x3fefb5586cf9890full, 0x3fef9301d0125b51ull,
+    0x3fef72b83c7d517bull, 0x3fef54873168b9aaull, 0x3fef387a6e756238ull, 0x3fef1e9df51fdee1ull,
+    0x3fef06fe0a31b715ull, 0x3feef1a7373aa9cbull, 0x3feedea64c123422ull, 0x3feece086061892dull,
+    0x3feebfdad5362a27ull, 0x3feeb42b569d4f82ull, 0x3feeab07dd485429ull, 0x3feea47eb03a5585ull,
+    0x3feea09e667f3bcdull, 0x3fee9f75e8ec5f74ull, 0x3feea11473eb0187ull, 0x3feea589994cce13ull,
+    0x3feeace5422aa0dbull, 0x3feeb737b0cdc5e5ull, 0x3feec49182a3f090ull, 0x3feed503b23e255dull,
+    0x3feee89f995ad3adull, 0x3feeff76f2fb5e47ull, 0x3fef199bdd85529cull, 0x3fef3720dcef9069ull,
+    0x3fef5818dcfba487ull, 0x3fef7c97337b9b5full, 0x3fefa4afa2a490daull, 0x3fefd0765b6e4540ull};
+
+struct Exp2 {
+    double t, g;
+};
+__device__ __forceinline__ Exp2 exp2_parts(const unsigned long long* table, double y) {
+    const double rounded = y + kRound;
+    const double f = y - (rounded - kRound);
+    const int n = __double2loint(rounded);
+    const double t = __longlong_as_double(static_cast<long long>(table[n & (kExp2Entries - 1)]));
+    double q = 0x1.c6b110835b776p-5;
+    q = fma(q, f, 0x1.ebfccc586302fp-3);
     q = fma(q, f, 0x1.62e42fefa39efp-1);
-    const double r = fma(q, f, 1.0);
-    return __hiloint2double(__double2hiint(r) + (__double2loint(z) << 20), __double2loint(r));
+    return Exp2{__hiloint2double(__double2hiint(t) + (n << 15), __double2loint(t)),
+                fma(q, f, 1.0)};
 }
 
 // The largest, a NaN where there is one: three operands an instruction.
@@ -104,6 +120,7 @@ __device__ __forceinline__ float value_of(uint32_t key) {
 // workgroups of 512 threads a CU; without them registers set their number.
 template <bool kFilters>
 struct Shared {
+    unsigned long long exp2_table[kExp2Entries];
     uint32_t count[kFilters ? kBuckets : 1];
     unsigned long long mass[kFilters ? kBuckets : 1];
     uint2 list[kFilters ? kList : 1];  // (~key, index): in falling order, x before y
@@ -320,9 +337,14 @@ struct Sampler {
         if constexpr (DT == kFP32) return (static_cast<double>(x) - static_cast<double>(top)) * c;
         return fma(static_cast<double>(x), c, -static_cast<double>(top) * c);
     }
-    __device__ __forceinline__ double weight(float x) const {
-        return exp2_d(log2_weight(x));
+    __device__ __forceinline__ Exp2 parts(double log2_w) const {
+        return exp2_parts(s.exp2_table, fmax(log2_w, -1000.0));
     }
+    __device__ __forceinline__ double exp2(double log2_w) const {
+        const Exp2 e = parts(log2_w);
+        return e.t * e.g;
+    }
+    __device__ __forceinline__ double weight(float x) const { return exp2(log2_weight(x)); }
     __device__ __forceinline__ unsigned long long fixed(double w) const {
         return static_cast<unsigned long long>(__double_as_longlong(w + fixed_one)) &
                ((1ull << 52) - 1);
@@ -616,21 +638,26 @@ __global__ __launch_bounds__(T, kFilters ? 4 : 6) void klp_sample_kernel(SampleP
         if (!(lane & 1)) p.tokens[r] = token;
     };
 
+    if (threadIdx.x < kExp2Entries) s.exp2_table[threadIdx.x] = kExp2Table[threadIdx.x];
     if (!kFilters || (!by_k && !by_p && !by_m)) {
         // Weights relative to the largest of the first 64 logits; again, to the
         // row's largest, if that overflows (2^900 of them).
         float first = lane < vocab ? to_f32<DT>(row.x[lane]) : -INFINITY;
         first = xrow_max(row_max16(first));
-        sm.top = fabsf(first) < INFINITY ? first : 0.0f;
+        __syncthreads();
         double sum;
         auto add_up = [&]() {
             sum = 0.0;
             row.each([&](int, const float (&v)[kChunk]) {
                 top = fmax_nan(top, chunk_max(v));
 #pragma unroll
-                for (int j = 0; j < kChunk; ++j) sum += sm.weight(v[j]);
+                for (int j = 0; j < kChunk; ++j) {
+                    const Exp2 e = sm.parts(sm.log2_weight(v[j]));
+                    sum = fma(e.t, e.g, sum);
+                }
             });
         };
+        sm.top = fabsf(first) < INFINITY ? first : 0.0f;
         add_up();
         if (!over_row()) return;
         if (sm.log2_weight(top) > 900.0) {
@@ -674,7 +701,7 @@ __global__ __launch_bounds__(T, kFilters ? 4 : 6) void klp_sample_kernel(SampleP
 #pragma unroll
                 for (int j = 0; j < kChunk; ++j) {
                     const double y = sm.log2_weight(v[j]);
-                    const double w = exp2_d(y);
+                    const double w = sm.exp2(y);
                     const uint32_t b = sm.bucket_of(y);
                     all += w;
                     atomicAdd(&s.mass[b], sm.fixed(w));
@@ -721,7 +748,7 @@ __global__ __launch_bounds__(T, kFilters ? 4 : 6) void klp_sample_kernel(SampleP
                     const double y = sm.log2_weight(v[j]);
                     const uint32_t b = sm.bucket_of(y);
                     if (b < bound) {
-                        const double w = exp2_d(y);
+                        const double w = sm.exp2(y);
                         if (w >= min_w) kept += w;
                     }
                     if (b == bound && at + j < vocab) in |= 1u << j;
@@ -765,7 +792,7 @@ __global__ __launch_bounds__(T, kFilters ? 4 : 6) void klp_sample_kernel(SampleP
             });
             if (!summed)  // what the rounding of the offset left out
                 all = over_waves(all) *
-                      exp2_d(static_cast<double>(offset) -
+                      sm.exp2(static_cast<double>(offset) -
                              static_cast<double>(sm.top) * static_cast<double>(sm.c32));
             else __syncthreads();
         }
@@ -839,7 +866,7 @@ __global__ __launch_bounds__(T, kFilters ? 4 : 6) void klp_sample_kernel(SampleP
                 const uint32_t i = threadIdx.x + j * T;
                 e[j] = i < n ? s.list[i] : make_uint2(0, 0);
                 const double y = i < n ? sm.log2_weight(value_of(~e[j].x)) : 0.0;
-                const double x = exp2_d(y);
+                const double x = sm.exp2(y);
                 const unsigned long long f = sm.fixed(x);
                 b[j] = i < n ? sm.bucket_of(y) : kBuckets;
                 w[j] = i < n ? (f == 0 && x > kNothing ? 1 : f) : 0;
