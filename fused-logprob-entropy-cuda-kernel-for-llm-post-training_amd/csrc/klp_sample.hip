@@ -31,6 +31,9 @@
 // a k above a quarter of the threads a histogram of the counts, since the k-th
 // of few maxima is low), for min-p that of its border, for top-p without a
 // top-k that in which a histogram of the masses, one more pass, reaches top_p.
+//   Top-p alone: two passes.  A histogram of counts, in float32, whose masses
+// say near which bucket the border lies; then the float64 sums of what lies
+// before that bucket, and a list of what lies in it.
 //   Where the list overflows (more than 4096 logits above the bound: a row of
 // equal logits, a wide nucleus) the kept set is {key > tau} and the first r of
 // {key == tau}, key the logit's bits in order; tau is found with histograms of
@@ -56,6 +59,14 @@ constexpr int kCountEvery = 8;
 // Buckets of the first histogram to a factor of 2 of the weight; elements of
 // less than 2^-64 share the last bucket.
 constexpr int kPerBit = kBuckets / 64;
+constexpr uint32_t kAnyBucket = kBuckets;
+// A nucleus' border by a float32 histogram: buckets to a factor of 2, bits of
+// the place in a bucket, and the factors of 2 by which a logit may exceed the
+// one that the buckets are relative to.
+constexpr int kNear = kList;  // buckets, in the list's place
+constexpr int kNearPerBit = kNear / 64;
+constexpr int kNearBits = 8;
+constexpr int kNearRoom = 24;
 constexpr double kLog2eD = 1.44269504088896340736;
 constexpr double kLn2D = 0.69314718055994530942;
 
@@ -313,6 +324,13 @@ __device__ __forceinline__ void find(Shared<true>& s, bool by_mass, uint32_t cou
     __syncthreads();
 }
 
+// x cut to a whole number, 0 below 0 and for a NaN, 2^32 - 1 above that.
+__device__ __forceinline__ uint32_t whole_part(float x) {
+    uint32_t v;
+    asm("v_cvt_u32_f32 %0, %1" : "=v"(v) : "v"(x));
+    return v;
+}
+
 struct Border {
     uint32_t tau;        // key
     uint32_t ties;       // elements of that key
@@ -393,7 +411,7 @@ struct Sampler {
         }
     }
 
-    // The border inside first-histogram bucket b, among keys >= floor, with
+    // The border inside first-histogram bucket b (or kAnyBucket), among keys >= floor, with
     // `above` elements and above_mass before the bucket.
     __device__ __forceinline__ Border resolve(bool listed, uint32_t b, uint32_t floor, uint32_t above,
                               unsigned long long above_mass, bool by_mass, uint32_t count,
@@ -407,7 +425,7 @@ struct Sampler {
         __syncthreads();
         uint32_t lo = 0xFFFFFFFFu, hi = 0, n = 0;
         candidates(listed, [&](uint32_t k) {
-            if (k < floor || bucket(value_of(k)) != b) return;
+            if (k < floor || (b != kAnyBucket && bucket(value_of(k)) != b)) return;
             lo = min(lo, k);
             hi = max(hi, k);
             ++n;
@@ -553,10 +571,14 @@ struct Sampler {
     }
 };
 
-// kFilters: rows may have filters, or a temperature of 0.
-template <int DT, int T, bool kFilters>
-__global__ __launch_bounds__(T, kFilters ? 4 : 6) void klp_sample_kernel(SampleParams p) {
+// What rows may have: no filter and no temperature of 0; no filter but top-p;
+// any.  (In one kernel the passes of top-p alone would spill registers.)
+enum SampleMode { kPlain, kTopP, kAny };
+
+template <int DT, int T, int kMode>
+__global__ __launch_bounds__(T, kMode != kPlain ? 4 : 6) void klp_sample_kernel(SampleParams p) {
     constexpr int kWaves = T / 64;
+    constexpr bool kFilters = kMode != kPlain;
     __shared__ Shared<kFilters> s;
     const int64_t r = blockIdx.x;
     const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
@@ -567,7 +589,7 @@ __global__ __launch_bounds__(T, kFilters ? 4 : 6) void klp_sample_kernel(SampleP
     row.span = (vocab + kWaves * 64 * kChunk - 1) / (kWaves * 64 * kChunk) * 64 * kChunk;
 
     float t = p.temperatures != nullptr ? p.temperatures[r] : p.temperature;
-    const float top_p = p.top_ps != nullptr ? p.top_ps[r] : p.top_p;
+    float top_p = p.top_ps != nullptr ? p.top_ps[r] : p.top_p;
     const float min_p = p.min_ps != nullptr ? p.min_ps[r] : p.min_p;
     int top_k = p.top_ks != nullptr ? p.top_ks[r] : p.top_k;
     float u = p.uniform[r];
@@ -575,12 +597,13 @@ __global__ __launch_bounds__(T, kFilters ? 4 : 6) void klp_sample_kernel(SampleP
     if (t == 0.0f) {
         t = 1.0f;
         top_k = 1;
+        if (kMode == kTopP) top_p = 0.0f;  // keeps the same one
     }
     const bool bad_t = !(t > 0.0f && t < INFINITY);
     if (bad_t) t = 1.0f;
-    const bool by_k = top_k > 0 && top_k < vocab;
+    const bool by_k = kMode == kAny && top_k > 0 && top_k < vocab;
     const bool by_p = top_p < 1.0f;  // a NaN is no filter
-    const bool by_m = min_p > 0.0f;
+    const bool by_m = kMode == kAny && min_p > 0.0f;
     const uint32_t k_left = by_k ? static_cast<uint32_t>(top_k) : 0xFFFFFFFFu;
     // A mass before which top-p keeps what it does, of whole masses: the first
     // element always.
@@ -671,15 +694,179 @@ __global__ __launch_bounds__(T, kFilters ? 4 : 6) void klp_sample_kernel(SampleP
         return;
     }
     if constexpr (kFilters) {
+        uint32_t bound = 0, p_at = kBuckets;
+        double all = 0.0, kept = 0.0;
+        unsigned long long share = 0, p_above = 0;
+        uint32_t tau = 0, keep_ties = 0;
+        bool wide = false;  // what lies before p_at's bucket is kept, that one's elements listed
+        auto append = [&](uint32_t in, int at, const float (&v)[kChunk]) {
+            // Past kList only the count matters, and not how far.
+            if (in == 0 || *static_cast<volatile uint32_t*>(&s.n_list) > kList) return;
+            uint32_t i = atomicAdd(&s.n_list, static_cast<uint32_t>(__popc(in)));
+#pragma unroll
+            for (int j = 0; j < kChunk; ++j) {
+                if (!(in >> j & 1)) continue;
+                if (i < kList) s.list[i] = make_uint2(~key_of(v[j]), at + j);
+                ++i;
+            }
+        };
+
+        // Top-p alone: one pass finds the border's bucket in float32, another
+        // sums in float64 what lies before it and lists what lies in it.  The
+        // bucket's two ends count as the ends of x that they come to; that the
+        // border lies between them is checked with the float64 sums.  False
+        // where it does not, or the list overflows.  (The row's maximum, then
+        // an exact histogram, then this pass, as where top-p is not alone:
+        // 184 against 131 us for 200 rows of 262144 fp32, 114 against 88 for
+        // 256 of 152064 bf16; 18 against 22 for one of 32000.)
+        //   The histogram holds a bucket's count and its elements' summed
+        // places in it: its mass is the count times the weight of the mean
+        // place, up to the square of a bucket's width (10^-5).
+        auto nucleus = [&]() {
+            float near[kChunk];
+            row.load(wave * row.span + lane * kChunk, near);
+            float from = xrow_max(row_max16(chunk_max(near)));
+            if (lane == 0) s.wave_top[wave] = from;
+            __syncthreads();
+            for (int i = 0; i < kWaves; ++i) from = fmax_nan(from, s.wave_top[i]);
+            constexpr int kPlaces = 1 << kNearBits;
+            constexpr float kSteps = kNearPerBit * kPlaces;
+            constexpr uint32_t kLast = kNear * kPlaces - 1;
+            auto* bucket = reinterpret_cast<unsigned long long*>(s.list);
+            const float scale = sm.c32 * kSteps;
+            float offset;
+            for (;;) {
+                offset = fmaf(from, scale, kNearRoom * kSteps);
+                // No steps finer than float32's, no NaN, and no sum of places
+                // that reaches the count.
+                if (!(fabsf(offset) < 0x1p23f) || vocab > 1 << (32 - kNearBits)) return false;
+                __syncthreads();
+                for (int i = threadIdx.x; i < kNear; i += T) bucket[i] = 0;
+                __syncthreads();
+                top = -INFINITY;
+                row.each([&](int, const float (&v)[kChunk]) {
+                    top = fmax_nan(top, chunk_max(v));
+#pragma unroll
+                    for (int j = 0; j < kChunk; ++j) {
+                        const uint32_t at = min(whole_part(fmaf(-v[j], scale, offset)), kLast);
+                        atomicAdd(&bucket[at >> kNearBits],
+                                  (1ull << 32) + (at & (kPlaces - 1)));
+                    }
+                });
+                if (!over_row()) return true;
+                if ((top - from) * sm.c32 < kNearRoom - 1) break;
+                from = top;  // it exceeds the room: once more
+            }
+            sm.top = top + 0.0f;
+            // Masses in fixed point, as everywhere relative to the maximum; the
+            // first bucket begins at `first`.
+            constexpr int kOwn = kNear / T;
+            const double first = kNearRoom + frac - (static_cast<double>(top) - from) * c;
+            unsigned long long m[kOwn], own = 0, mass;
+            uint32_t k[kOwn], own_count = 0, total;
+#pragma unroll
+            for (int i = 0; i < kOwn; ++i) {
+                const int b = threadIdx.x * kOwn + i;
+                const uint32_t count = static_cast<uint32_t>(bucket[b] >> 32);
+                const double place =
+                    (static_cast<uint32_t>(bucket[b]) + 0.5 * count) / (kPlaces * max(count, 1u));
+                const double w = sm.exp2(first - (b + place) / kNearPerBit);
+                m[i] = static_cast<unsigned long long>(count * w);
+                own += m[i];
+                own_count += k[i] = count;
+            }
+            uint32_t run_count = block_before<T>(s.wave_count, own_count, total);
+            unsigned long long run = block_before<T>(s.wave_mass, own, mass);
+            const unsigned long long target = share_of(static_cast<double>(mass));
+            // What the sums may be off by: their fractions, a bucket's width.
+            const unsigned long long off = (mass >> 13) + kNear;
+#pragma unroll
+            for (int i = 0; i < kOwn; ++i) {
+                if (run < target && run + m[i] >= target) {
+                    s.at = threadIdx.x * kOwn + i;
+                    s.key_min = target - run <= off;
+                    s.key_max = run + m[i] <= target + off;
+                    s.at_count = run_count + k[i];
+                }
+                run += m[i];
+                run_count += k[i];
+            }
+            __syncthreads();
+            const uint32_t at = s.at;
+            const bool early = s.key_min, late = s.key_max;
+            if (at + late >= kNear - 1) return false;
+            // A list of all that could be kept, where it is short.
+            const bool whole = !late && s.at_count <= kRanked;
+            const float high = at == 0 || whole ? INFINITY : (offset - (at - early) * kPlaces) / scale;
+            const float low = (offset - (at + late + 1) * kPlaces) / scale;
+            __syncthreads();
+            if (threadIdx.x == 0) s.n_list = 0;
+            __syncthreads();
+            row.each([&](int first, const float (&v)[kChunk]) {
+                uint32_t in = 0;
+#pragma unroll
+                for (int j = 0; j < kChunk; ++j) {
+                    const double w = sm.weight(v[j]);
+                    all += w;
+                    kept += v[j] > high ? w : 0.0;
+                    if (v[j] <= high && v[j] >= low) in |= 1u << j;
+                }
+                // Added here, or the sums of 4 chunks wait in registers.
+                asm volatile("" : "+v"(all), "+v"(kept));
+                append(in, first, v);
+            });
+            all = over_waves(all);
+            const double before = over_waves(kept);
+            const uint32_t n = s.n_list;
+            if (n > kList) return false;
+            share = share_of(all * ldexp(1.0, frac));
+            p_above = static_cast<unsigned long long>(rint(before * ldexp(1.0, frac)));
+            own = 0;
+            for (uint32_t i = threadIdx.x; i < n; i += T)
+                own += sm.fixed(sm.weight(value_of(~s.list[i].x)));
+            block_before<T>(s.wave_mass, own, mass);
+            if (!(p_above < share && p_above + mass >= share)) return false;
+            if (whole) return n <= kRanked;
+            wide = true;
+            if (n > kRanked) {
+                bound = p_at = kAnyBucket;
+                return true;
+            }
+            // The border of a short list: the last entry before which less
+            // than the share lies, and those kept of its equals.
+            if (threadIdx.x < n)
+                s.few_mass[threadIdx.x] = sm.fixed(sm.weight(value_of(~s.list[threadIdx.x].x)));
+            if (threadIdx.x == 0) s.key_max = s.key_count = 0;
+            __syncthreads();
+            const uint32_t per = sm.threads_for(n);
+            const uint32_t i = threadIdx.x / per, g = threadIdx.x % per;
+            const uint2 e = i < n ? s.list[i] : make_uint2(0, 0);
+            own = 0;
+            for (uint32_t j = g; j < n; j += per) {
+                const uint2 o = s.list[j];
+                if (o.x < e.x || (o.x == e.x && o.y < e.y)) own += s.few_mass[j];
+            }
+            const bool keep = p_above + sm.over_group(own, per) < share && i < n && g == 0;
+            if (keep) atomicMax(&s.key_max, e.x);
+            __syncthreads();
+            if (keep && e.x == s.key_max) atomicAdd(&s.key_count, 1u);
+            __syncthreads();
+            tau = ~s.key_max;
+            keep_ties = s.key_count;
+            bound = 0;
+            return true;
+        };
+        if (kMode == kTopP && !bad_t && nucleus()) {
+            if (!(fabsf(top) < INFINITY)) return;  // no distribution
+        } else {
+        top = -INFINITY;
         row.each([&](int, const float (&v)[kChunk]) { top = fmax_nan(top, chunk_max(v)); });
         const float thread_top = top;
         if (!over_row()) return;
         sm.top = top + 0.0f;
         // What could be kept lies in buckets up to `bound`.
-        uint32_t bound = kBuckets - 1, p_at = kBuckets;
-        double all = 0.0;
-        unsigned long long share = 0, p_above = 0;
-        bool wide = false;  // top-p alone, with more than the list takes
+        bound = kBuckets - 1;
+        all = kept = 0.0;
         if (by_k) {
             sm.clear();
             if (top_k <= T / 4) {
@@ -726,18 +913,6 @@ __global__ __launch_bounds__(T, kFilters ? 4 : 6) void klp_sample_kernel(SampleP
         __syncthreads();
         if (threadIdx.x == 0) s.n_list = 0;
         __syncthreads();
-        auto append = [&](uint32_t in, int at, const float (&v)[kChunk]) {
-            // Past kList only the count matters, and not how far.
-            if (in == 0 || *static_cast<volatile uint32_t*>(&s.n_list) > kList) return;
-            uint32_t i = atomicAdd(&s.n_list, static_cast<uint32_t>(__popc(in)));
-#pragma unroll
-            for (int j = 0; j < kChunk; ++j) {
-                if (!(in >> j & 1)) continue;
-                if (i < kList) s.list[i] = make_uint2(~key_of(v[j]), at + j);
-                ++i;
-            }
-        };
-        double kept = 0.0;
         if (wide) {
             // What lies before the border's bucket is kept; the bucket's
             // elements are listed.
@@ -795,6 +970,7 @@ __global__ __launch_bounds__(T, kFilters ? 4 : 6) void klp_sample_kernel(SampleP
                       sm.exp2(static_cast<double>(offset) -
                              static_cast<double>(sm.top) * static_cast<double>(sm.c32));
             else __syncthreads();
+        }
         }
         const uint32_t n = s.n_list;
         if (!wide && n <= kRanked) {
@@ -977,7 +1153,6 @@ __global__ __launch_bounds__(T, kFilters ? 4 : 6) void klp_sample_kernel(SampleP
                        static_cast<double>(mass) * ldexp(1.0, -frac));
             return;
         }
-        uint32_t tau = 0, keep_ties = 0;
         if (by_k) {
             sm.clear();
             sm.candidates(listed, [&](uint32_t k) {
@@ -1072,21 +1247,26 @@ __global__ __launch_bounds__(T, kFilters ? 4 : 6) void klp_sample_kernel(SampleP
 namespace {
 
 template <int DT, int T>
-hipError_t launch_sample_threads(bool plain, const SampleParams& p, hipStream_t stream) {
-    const dim3 grid(static_cast<unsigned>(p.n_rows));
-    if (plain)
-        return launch_kernel(klp_sample_kernel<DT, T, false>, grid, dim3(T), stream, p);
-    return launch_kernel(klp_sample_kernel<DT, T, true>, grid, dim3(T), stream, p);
+hipError_t launch_sample_threads(const SampleParams& p, hipStream_t stream) {
+    const dim3 grid(static_cast<unsigned>(p.n_rows)), block(T);
+    const bool k = p.top_ks != nullptr || (p.top_k > 0 && p.top_k < p.vocab);
+    const bool m = p.min_ps != nullptr || p.min_p > 0.0f;
+    if (k || m) return launch_kernel(klp_sample_kernel<DT, T, kAny>, grid, block, stream, p);
+    if (p.top_ps != nullptr || p.top_p < 1.0f || p.temperatures != nullptr ||
+        p.temperature == 0.0f)
+        return launch_kernel(klp_sample_kernel<DT, T, kTopP>, grid, block, stream, p);
+    return launch_kernel(klp_sample_kernel<DT, T, kPlain>, grid, block, stream, p);
 }
 
+// A row's passes are short of arithmetic while its workgroup is alone on a CU,
+// so 1024 threads; with more rows than CUs two workgroups share one, and 512
+// leave fewer idle at a row's barriers.  (us, 1024 and 512 threads: 256 rows
+// of 152064 45 and 57, 1 row 39 and 45; 1024 rows of 32000 with min-p 126 and
+// 95.)
 template <int DT>
 hipError_t launch_sample_dt(const SampleParams& p, hipStream_t stream) {
-    const bool plain = p.temperatures == nullptr && p.top_ks == nullptr && p.top_ps == nullptr &&
-                       p.min_ps == nullptr && p.temperature != 0.0f &&
-                       !(p.top_k > 0 && p.top_k < p.vocab) && !(p.top_p < 1.0f) &&
-                       !(p.min_p > 0.0f);
-    if (p.n_rows > kHeadGemmCus) return launch_sample_threads<DT, 512>(plain, p, stream);
-    return launch_sample_threads<DT, 1024>(plain, p, stream);
+    if (p.n_rows > kHeadGemmCus) return launch_sample_threads<DT, 512>(p, stream);
+    return launch_sample_threads<DT, 1024>(p, stream);
 }
 
 }  // namespace

@@ -322,3 +322,37 @@ def test_logits_beyond_32_bits():
     a = ko.fused_sample(one, u[:9], top_p=0.9)
     b = ko.fused_sample(one.contiguous(), u[:9], top_p=0.9)
     assert all(torch.equal(p, q) for p, q in zip(a, b))
+
+
+@pytest.mark.parametrize("dtype", DTYPES, ids=IDS)
+def test_nucleus_alone(dtype):
+    """top_p without another filter: rows whose largest logit lies far above,
+    or behind, those that the buckets start from, rows too spread or too far
+    from zero for the buckets, masked rows, short and long nuclei."""
+    V = 70001
+    x, u = _logits(12, V, dtype, 61)
+    f = x.float()
+    f[1, 69000] += 40.0                       # a peak past the first logits of a wave's part
+    f[2] += 900.0 if dtype != torch.float16 else 300.0
+    f[3] = f[3] * 60.0                        # a spread of hundreds of factors of 2
+    f[4, ::2] = -math.inf
+    f[5, :60000] = -math.inf
+    f[6] = f[6] * 0.01                        # nearly flat: a list that overflows
+    f[7, 512:] = 0.0
+    f[8, 100] = math.inf
+    f[9, 65000] = math.nan
+    f[10] = -math.inf
+    f[11, 5000:9000] = 9.0                    # ties at the border
+    x = f.to(dtype)
+    for T, p in ((1.0, 0.9), (0.7, 0.5), (1.3, 0.99), (1.0, 0.999999), (1.0, 1e-6)):
+        got = _ko().fused_sample(x.to(DEV), u.to(DEV), T, top_p=p)
+        _check(x, u, got, T, 0, p)
+    t = [1.0, 0.0, 0.5, 1.5, 0.9, -1.0, 1.0, 1e-3, 1.0, 1.0, 1.0, 2.0]
+    p = [0.9, 0.5, 1.0, 2.0, math.nan, 0.5, 0.0, -1.0, 0.3, 0.3, 0.3, 0.7]
+    got = _ko().fused_sample(x.to(DEV), u.to(DEV), torch.tensor(t, device=DEV),
+                             top_p=torch.tensor(p, device=DEV))
+    _check(x, u, got, t, [0] * 12, [1.0 if math.isnan(q) else q for q in p], [0.0] * 12)
+    # 512 threads a row.
+    many = x.repeat(25, 1).to(DEV)
+    a = _ko().fused_sample(many, u.repeat(25).to(DEV), top_p=0.9)
+    _check(x, u, tuple(v[-12:] for v in a), 1.0, 0, 0.9)
