@@ -14,8 +14,8 @@
 // 10^5 such borders: sums off by 10^-7 (float32) pick another token in one of
 // 100 rows.  So weights are computed in float64 (off by 1.5 10^-10 at most and,
 // since that error changes sign with the logit, far less in a sum) and added in
-// float64, or, in histograms, as 64-bit integers of 2^-44, whose sums do not depend on the order of the
-// atomics.
+// float64, or, in histograms, as 64-bit integers of 2^-44, whose sums do not
+// depend on the order of the atomics.
 //
 // A row is read by one workgroup, a contiguous part of it by each wave.
 //   No filter: one pass sums the weights, relative to one of the row's first
@@ -289,7 +289,8 @@ struct Row {
 // with by_mass, the running mass reaches `mass`); the last one with anything
 // in it when none does.  Into s.at, with what lies before it.
 template <int T>
-__device__ __forceinline__ void find(Shared<true>& s, bool by_mass, uint32_t count, unsigned long long mass) {
+__device__ __forceinline__ void find(Shared<true>& s, bool by_mass, uint32_t count,
+                                     unsigned long long mass) {
     constexpr int kPerThread = kBuckets / T;
     const int first = threadIdx.x * kPerThread;
     uint32_t c[kPerThread], c_sum = 0;
@@ -413,9 +414,10 @@ struct Sampler {
 
     // The border inside first-histogram bucket b (or kAnyBucket), among keys >= floor, with
     // `above` elements and above_mass before the bucket.
-    __device__ __forceinline__ Border resolve(bool listed, uint32_t b, uint32_t floor, uint32_t above,
-                              unsigned long long above_mass, bool by_mass, uint32_t count,
-                              unsigned long long mass) {
+    __device__ __forceinline__ Border resolve(bool listed, uint32_t b, uint32_t floor,
+                                              uint32_t above, unsigned long long above_mass,
+                                              bool by_mass, uint32_t count,
+                                              unsigned long long mass) {
         __syncthreads();
         if (threadIdx.x == 0) {
             s.key_count = 0;
@@ -481,7 +483,8 @@ struct Sampler {
     // does, and among those the element.  Where rounding (or u = 1) lets none
     // cross, the last that has a weight.  The wave of that thread returns the
     // token, the others -1.
-    __device__ __forceinline__ int search(float u, uint32_t tau, uint32_t keep_ties, double min_w, double& mass) {
+    __device__ __forceinline__ int search(float u, uint32_t tau, uint32_t keep_ties, double min_w,
+                                          double& mass) {
         const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
         double tau_w = keep_ties > 0 ? weight(value_of(tau)) : 0.0;
         if (tau_w < min_w) tau_w = 0.0;
@@ -797,7 +800,8 @@ __global__ __launch_bounds__(T, kMode != kPlain ? 4 : 6) void klp_sample_kernel(
             if (at + late >= kNear - 1) return false;
             // A list of all that could be kept, where it is short.
             const bool whole = !late && s.at_count <= kRanked;
-            const float high = at == 0 || whole ? INFINITY : (offset - (at - early) * kPlaces) / scale;
+            const float high =
+                at == 0 || whole ? INFINITY : (offset - (at - early) * kPlaces) / scale;
             const float low = (offset - (at + late + 1) * kPlaces) / scale;
             __syncthreads();
             if (threadIdx.x == 0) s.n_list = 0;
@@ -1068,7 +1072,8 @@ __global__ __launch_bounds__(T, kMode != kPlain ? 4 : 6) void klp_sample_kernel(
             auto own_bucket = [&](int j) { return b[j]; };
             // Keeps what lies before the border in bucket `at`, of the entries
             // in it `left` by count, or those before which less than `share` lies.
-            auto cut = [&](uint32_t at, bool by_mass, uint32_t left, unsigned long long share_left) {
+            auto cut = [&](uint32_t at, bool by_mass, uint32_t left,
+                           unsigned long long share_left) {
                 if (!pick(at, own_bucket)) return false;
                 const uint32_t m = s.n_few, per = sm.threads_for(m);
                 const uint32_t i = threadIdx.x / per, g = threadIdx.x % per;
@@ -1261,8 +1266,9 @@ hipError_t launch_sample_threads(const SampleParams& p, hipStream_t stream) {
 // A row's passes are short of arithmetic while its workgroup is alone on a CU,
 // so 1024 threads; with more rows than CUs two workgroups share one, and 512
 // leave fewer idle at a row's barriers.  (us, 1024 and 512 threads: 256 rows
-// of 152064 45 and 57, 1 row 39 and 45; 1024 rows of 32000 with min-p 126 and
-// 95.)
+// of 152064 unfiltered 28 and 31, 200 of 262144 fp32 with top-p 131 and 143;
+// 300 rows of 32000 unfiltered 18 and 15, 1024 of 128256 fp16 with top-p 283
+// and 212.)
 template <int DT>
 hipError_t launch_sample_dt(const SampleParams& p, hipStream_t stream) {
     if (p.n_rows > kHeadGemmCus) return launch_sample_threads<DT, 512>(p, stream);
