@@ -16,6 +16,11 @@
 // 1024 threads, 8 elements (a chunk) a thread and pass, 1 to 8 chunks a
 // thread: rows of up to 65536 elements.
 //
+// Measured: 8192 rows of 4096 bf16 with a residual 48 us forward (5.55 TB/s),
+// 55.6 backward (h and two gradients in, one out: 4.8 TB/s, 5.1 with the
+// shares) and 4.8 for the sum of the shares; 16384 rows of 3584 to e4m3 74 us
+// (5.56 TB/s); a copy of this size runs at 5.9.  64 rows: 4 us, the launch's.
+//
 // dw: a group walks rows with a fixed stride and keeps its share of the sum
 // in registers; the shares, [groups, dim] float32 in a workspace, are added
 // in group order by a second kernel, so that the result depends on nothing

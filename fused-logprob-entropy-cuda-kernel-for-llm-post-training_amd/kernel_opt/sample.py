@@ -4,7 +4,8 @@
 one token a row by inverse transform of a given uniform number and returns the
 token with its log-probability under the whole and under the filtered
 distribution (csrc/klp_sample.hip: no sort, float64 sums, results that do not
-depend on timing).
+depend on timing; with a top_k, or a min_p and no top_p, the sum behind ``logp``
+is of float32 weights).
 
 Per row, with y = (x - max x) / T, w = exp(y) and the vocabulary ordered by
 falling x (equal logits by index):

@@ -543,7 +543,9 @@ int klp_head_dhidden(int dtype, const void* d_logits, int64_t ld_d, int64_t n_to
  * stride along dim (row strides in elements, any value >= 0); weight [dim] is
  * of `dtype` or KLP_FP32 (`weight_dtype`); y, h [rows, dim] are dense.  rstd
  * (nullable, float32 [rows]) is what the backward needs.  Sums are float32;
- * the statistics are those of the rounded h.  dim is at most 65536.
+ * the statistics are those of the rounded h, and a row whose sum of squares
+ * passes float32's range gives zeros.  dim is at most 65536, and a row's 64 to
+ * 1024 threads times rows below 2^32 (KLP_EINVAL).
  */
 int klp_rms_norm(const void* x, int dtype, int64_t ld_x, const void* residual,
                  int64_t ld_residual, const void* weight, int weight_dtype, int64_t rows,
@@ -594,7 +596,13 @@ int klp_quantize_fp8(const void* x, int dtype, int64_t ld_x, int64_t rows, int64
  * x [m, ld_x], w [n, ld_w] (16-byte aligned, row strides multiples of 16; k a
  * positive multiple of 16), x_scales [m, ceil(k / 128)], w_scales
  * [ceil(n / 128), ceil(k / 128)] dense, out [m, ld_out] of out_dtype.
- * Products and sums are float32.  m <= 2^20, n <= 2^31, k <= 2^24.
+ * A float32 output has exact products and float32 sums (the bf16 matrix
+ * instruction on the codes).  A 16-bit one takes the e4m3 instruction, which
+ * aligns the products of 8 consecutive k to the largest of them and cuts what
+ * lies more than 13 bits below that: off by up to 7 2^-13 of that product a
+ * group, 5 10^-5 of a result (2-norm) on normal data.  Which kernel adds the
+ * blocks, and so their order, depends on m, n and k.  m <= 2^20, n < 2^28,
+ * k <= 2^24 and ceil(m / 64) ceil(n / 128) < 2^23 - 8 (KLP_EINVAL).
  */
 int klp_fp8_linear(const uint8_t* x, int64_t ld_x, const float* x_scales, const uint8_t* w,
                    int64_t ld_w, const float* w_scales, int64_t m, int64_t n, int64_t k,
@@ -608,7 +616,11 @@ int klp_fp8_linear(const uint8_t* x, int64_t ld_x, const float* x_scales, const 
  * P with w >= min_p; the first always stays.  tokens[row] is the lowest index
  * whose running sum (in index order) of M's weights exceeds uniform * mass(M),
  *   logp = y - ln sum w,   sample_logp = y - ln mass(M)
- * of that token, the sums in float64.
+ * of that token.  Sums that decide the token, and sample_logp's, are float64
+ * or whole numbers of 2^-44 and do not depend on timing; with a top_k, or a
+ * min_p and no top_p, the sum behind logp is of float32 weights.  Weights
+ * below 2^-960 of the first 64 logits' largest (of the row's largest, with a
+ * filter) count as none.
  * Each parameter is one value, or with its array non-null one per row
  * (float32, top_k int32; [n_rows]).  top_k <= 0 or >= vocab, top_p >= 1 and
  * min_p <= 0 (or NaN) are off.  T = 0 takes the largest logit (lowest index),
@@ -616,7 +628,8 @@ int klp_fp8_linear(const uint8_t* x, int64_t ld_x, const float* x_scales, const 
  * from 1 on takes M's last token with a weight above 0.
  * A row without a distribution has token -1: with every logit -inf its
  * log-probabilities are -inf, with a NaN or +inf logit, or a temperature in
- * the array that is negative or not finite, NaN.  vocab <= 2^26.
+ * the array that is negative or not finite, NaN.  vocab <= 2^26, n_rows below
+ * 2^23 (KLP_EINVAL).
  */
 int klp_sample(const void* logits, int dtype, int64_t n_rows, int64_t vocab, int64_t rows_inner,
                int64_t stride_outer, int64_t stride_inner, const float* uniform,
