@@ -5,7 +5,9 @@
 // Blocks are 128 elements of a row (activations: 16 lanes a block, one pass)
 // or 128 x 128 elements (weights: a workgroup a block, held in registers
 // between its maximum and its codes).  Bound by memory: every element is read
-// once and its code written once.
+// once and its code written once.  Measured: 152064 x 3584 bf16 in 128 x 128
+// blocks 293 us (5.6 TB/s), 4096 x 3584 fp16 in rows 9.2 us (4.8 TB/s); a copy
+// runs at 5.9.
 #include "klp_launch.h"
 #include "klp_rows.h"
 
