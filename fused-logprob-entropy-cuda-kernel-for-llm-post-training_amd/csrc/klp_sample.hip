@@ -575,8 +575,8 @@ struct Sampler {
     }
 };
 
-// What rows may have: no filter and no temperature of 0; no filter but top-p;
-// any.  (In one kernel the passes of top-p alone would spill registers.)
+// What rows may have: no filter and no temperature of 0; no filter but top-p
+// (a row's temperature of 0 is then a top-p of 0); any.  (In one kernel the passes of top-p alone would spill registers.)
 enum SampleMode { kPlain, kTopP, kAny };
 
 template <int DT, int T, int kMode>
@@ -1257,10 +1257,12 @@ hipError_t launch_sample_threads(const SampleParams& p, hipStream_t stream) {
     const dim3 grid(static_cast<unsigned>(p.n_rows)), block(T);
     const bool k = p.top_ks != nullptr || (p.top_k > 0 && p.top_k < p.vocab);
     const bool m = p.min_ps != nullptr || p.min_p > 0.0f;
-    if (k || m) return launch_kernel(klp_sample_kernel<DT, T, kAny>, grid, block, stream, p);
-    if (p.top_ps != nullptr || p.top_p < 1.0f || p.temperatures != nullptr ||
-        p.temperature == 0.0f)
+    const bool greedy = p.temperatures == nullptr && p.temperature == 0.0f;
+    const bool by_p = p.top_ps != nullptr || p.top_p < 1.0f;
+    if (by_p && !k && !m && !greedy)
         return launch_kernel(klp_sample_kernel<DT, T, kTopP>, grid, block, stream, p);
+    if (by_p || k || m || greedy || p.temperatures != nullptr)
+        return launch_kernel(klp_sample_kernel<DT, T, kAny>, grid, block, stream, p);
     return launch_kernel(klp_sample_kernel<DT, T, kPlain>, grid, block, stream, p);
 }
 

@@ -356,3 +356,21 @@ def test_nucleus_alone(dtype):
     many = x.repeat(25, 1).to(DEV)
     a = _ko().fused_sample(many, u.repeat(25).to(DEV), top_p=0.9)
     _check(x, u, tuple(v[-12:] for v in a), 1.0, 0, 0.9)
+
+
+def test_greedy_with_a_nucleus():
+    """A temperature of 0, one for all or a row's, next to a top_p."""
+    x, u = _logits(6, 30011, torch.bfloat16, 91)
+    x[2, 7] = x[2, 29000] = 25.0
+    want = x.float().argmax(-1)
+    for t in (0.0, torch.zeros(6, device=DEV)):
+        for p in (None, 0.9, 1.0):
+            tok, logp, slogp = _ko().fused_sample(x.to(DEV), u.to(DEV), t, top_p=p)
+            assert torch.equal(tok.cpu(), want) and not slogp.any()
+    _check(x, u, (tok, logp, slogp), 0.0)
+
+
+@pytest.mark.parametrize("filters", [{}, {"top_p": 0.4}, {"top_k": 900}], ids=["none", "p", "k"])
+def test_a_vocabulary_past_the_histograms_counts(filters):
+    x, u = _logits(2, 2 ** 24 + 5, torch.bfloat16, 92)
+    _check(x, u, _ko().fused_sample(x.to(DEV), u.to(DEV), **filters), **filters)
