@@ -12,7 +12,7 @@
 // Precision.  The token and the kept set are decided where a running sum over
 // the whole row crosses a border, and a row of 10^5 comparable weights has
 // 10^5 such borders: sums off by 10^-7 (float32) pick another token in one of
-// 100 rows.  So weights are computed in float64 (off by 1.5 10^-10 at most and,
+// 100 rows.  So weights are computed in float64 (off by 1.04 10^-10 at most and,
 // since that error changes sign with the logit, far less in a sum) and added in
 // float64, or, in histograms, as 64-bit integers of 2^-44, whose sums do not
 // depend on the order of the atomics.
@@ -74,27 +74,85 @@ constexpr double kLn2D = 0.69314718055994530942;
 // of -inf too, and a row of 2^26 of those sums to less than this.
 constexpr double kNothing = 0x1p-960;
 
-// 2^y for |y| <= 1000 as t g: t = 2^(n / 32), n = rint(32 y), from a table of
-// 2^(i / 32), i < 32, and g = 2^f, f = y - n / 32, as 1 + f q(f), q
-// interpolating (2^f - 1) / f at the Chebyshev points of [-1/64, 1/64].
-// Adding kRound rounds to n / 32 and leaves n in the sum's low word.  An entry
-// lacks i 2^15 in its high word, which n 2^15 = (n / 32) 2^20 + (n % 32) 2^15
-// puts back along with the exponent.  32 entries of 8 bytes lie in different
-// LDS banks: a lookup is as fast as memory gives 64 lanes 8 bytes each, and
-// together with 3 products fewer than the 7 of a polynomial on [-1/2, 1/2]:
-// 80 against 90 us for 1024 rows of 128256 (fp16, unfiltered), where
-// arithmetic is the bound.
-constexpr double kRound = 0x1.8p47;
-constexpr int kExp2Entries = 32;
+// 2^y for |y| <= 1000 as t g: t = 2^(n / 256), n = rint(256 y), from a table
+// of 2^(i / 256), i < 256, and g = 2^f, f = y - n / 256, as 1 + f q(f), q
+// interpolating (2^f - 1) / f where the cubic Chebyshev polynomial of [-1/512,
+// 1/512] is 0 (besides f = 0): g is off by (ln 2 / 512)^3 / 24, 1.04 10^-10
+// with the terms behind.
+// Adding kRound rounds to n / 256 and leaves n in the sum's low word.  An entry
+// lacks i 2^12 in its high word, which n 2^12 = (n / 256) 2^20 + (n % 256) 2^12
+// puts back along with the exponent.  256 entries: n's low byte is an operand
+// of its own, so one shift makes it an address, and 2 products suffice.
+// Arithmetic is the bound, and LDS has the room: 1024 rows of 128256 (fp16,
+// unfiltered) 81.5 us, with 32 entries (in different banks, 3 products, one
+// operation more for the address) 89, with a polynomial of degree 7 100.
+constexpr double kRound = 0x1.8p44;
+constexpr int kExp2Entries = 256;
 __device__ const unsigned long long kExp2Table[kExp2Entries] = {
-    0x3ff0000000000000ull, 0x3fefd9b0d3158574ull, 0x3fefb5586cf9890full, 0x3fef9301d0125b51ull,
-    0x3fef72b83c7d517bull, 0x3fef54873168b9aaull, 0x3fef387a6e756238ull, 0x3fef1e9df51fdee1ull,
-    0x3fef06fe0a31b715ull, 0x3feef1a7373aa9cbull, 0x3feedea64c123422ull, 0x3feece086061892dull,
-    0x3feebfdad5362a27ull, 0x3feeb42b569d4f82ull, 0x3feeab07dd485429ull, 0x3feea47eb03a5585ull,
-    0x3feea09e667f3bcdull, 0x3fee9f75e8ec5f74ull, 0x3feea11473eb0187ull, 0x3feea589994cce13ull,
-    0x3feeace5422aa0dbull, 0x3feeb737b0cdc5e5ull, 0x3feec49182a3f090ull, 0x3feed503b23e255dull,
-    0x3feee89f995ad3adull, 0x3feeff76f2fb5e47ull, 0x3fef199bdd85529cull, 0x3fef3720dcef9069ull,
-    0x3fef5818dcfba487ull, 0x3fef7c97337b9b5full, 0x3fefa4afa2a490daull, 0x3fefd0765b6e4540ull};
+    0x3ff0000000000000ull, 0x3feffb1afa5abcbfull, 0x3feff63da9fb3335ull, 0x3feff168143b0281ull,
+    0x3fefec9a3e778061ull, 0x3fefe7d42e11bbccull, 0x3fefe315e86e7f85ull, 0x3fefde5f72f654b1ull,
+    0x3fefd9b0d3158574ull, 0x3fefd50a0e3c1f89ull, 0x3fefd06b29ddf6deull, 0x3fefcbd42b72a836ull,
+    0x3fefc74518759bc8ull, 0x3fefc2bdf66607e0ull, 0x3fefbe3ecac6f383ull, 0x3fefb9c79b1f3919ull,
+    0x3fefb5586cf9890full, 0x3fefb0f145e46c85ull, 0x3fefac922b7247f7ull, 0x3fefa83b23395decull,
+    0x3fefa3ec32d3d1a2ull, 0x3fef9fa55fdfa9c5ull, 0x3fef9b66affed31bull, 0x3fef973028d7233eull,
+    0x3fef9301d0125b51ull, 0x3fef8edbab5e2ab6ull, 0x3fef8abdc06c31ccull, 0x3fef86a814f204abull,
+    0x3fef829aaea92de0ull, 0x3fef7e95934f312eull, 0x3fef7a98c8a58e51ull, 0x3fef76a45471c3c2ull,
+    0x3fef72b83c7d517bull, 0x3fef6ed48695bbc0ull, 0x3fef6af9388c8deaull, 0x3fef672658375d2full,
+    0x3fef635beb6fcb75ull, 0x3fef5f99f8138a1cull, 0x3fef5be084045cd4ull, 0x3fef582f95281c6bull,
+    0x3fef54873168b9aaull, 0x3fef50e75eb44027ull, 0x3fef4d5022fcd91dull, 0x3fef49c18438ce4dull,
+    0x3fef463b88628cd6ull, 0x3fef42be3578a819ull, 0x3fef3f49917ddc96ull, 0x3fef3bdda27912d1ull,
+    0x3fef387a6e756238ull, 0x3fef351ffb82140aull, 0x3fef31ce4fb2a63full, 0x3fef2e85711ece75ull,
+    0x3fef2b4565e27cddull, 0x3fef280e341ddf29ull, 0x3fef24dfe1f56381ull, 0x3fef21ba7591bb70ull,
+    0x3fef1e9df51fdee1ull, 0x3fef1b8a66d10f13ull, 0x3fef187fd0dad990ull, 0x3fef157e39771b2full,
+    0x3fef1285a6e4030bull, 0x3fef0f961f641589ull, 0x3fef0cafa93e2f56ull, 0x3fef09d24abd886bull,
+    0x3fef06fe0a31b715ull, 0x3fef0432edeeb2fdull, 0x3fef0170fc4cd831ull, 0x3feefeb83ba8ea32ull,
+    0x3feefc08b26416ffull, 0x3feef96266e3fa2dull, 0x3feef6c55f929ff1ull, 0x3feef431a2de883bull,
+    0x3feef1a7373aa9cbull, 0x3feeef26231e754aull, 0x3feeecae6d05d866ull, 0x3feeea401b7140efull,
+    0x3feee7db34e59ff7ull, 0x3feee57fbfec6cf4ull, 0x3feee32dc313a8e5ull, 0x3feee0e544ede173ull,
+    0x3feedea64c123422ull, 0x3feedc70df1c5175ull, 0x3feeda4504ac801cull, 0x3feed822c367a024ull,
+    0x3feed60a21f72e2aull, 0x3feed3fb2709468aull, 0x3feed1f5d950a897ull, 0x3feecffa3f84b9d4ull,
+    0x3feece086061892dull, 0x3feecc2042a7d232ull, 0x3feeca41ed1d0057ull, 0x3feec86d668b3237ull,
+    0x3feec6a2b5c13cd0ull, 0x3feec4e1e192aed2ull, 0x3feec32af0d7d3deull, 0x3feec17dea6db7d7ull,
+    0x3feebfdad5362a27ull, 0x3feebe41b817c114ull, 0x3feebcb299fddd0dull, 0x3feebb2d81d8abffull,
+    0x3feeb9b2769d2ca7ull, 0x3feeb8417f4531eeull, 0x3feeb6daa2cf6642ull, 0x3feeb57de83f4eefull,
+    0x3feeb42b569d4f82ull, 0x3feeb2e2f4f6ad27ull, 0x3feeb1a4ca5d920full, 0x3feeb070dde910d2ull,
+    0x3feeaf4736b527daull, 0x3feeae27dbe2c4cfull, 0x3feead12d497c7fdull, 0x3feeac0827ff07ccull,
+    0x3feeab07dd485429ull, 0x3feeaa11fba87a03ull, 0x3feea9268a5946b7ull, 0x3feea84590998b93ull,
+    0x3feea76f15ad2148ull, 0x3feea6a320dceb71ull, 0x3feea5e1b976dc09ull, 0x3feea52ae6cdf6f4ull,
+    0x3feea47eb03a5585ull, 0x3feea3dd1d1929fdull, 0x3feea34634ccc320ull, 0x3feea2b9febc8fb7ull,
+    0x3feea23882552225ull, 0x3feea1c1c70833f6ull, 0x3feea155d44ca973ull, 0x3feea0f4b19e9538ull,
+    0x3feea09e667f3bcdull, 0x3feea052fa75173eull, 0x3feea012750bdabfull, 0x3fee9fdcddd47645ull,
+    0x3fee9fb23c651a2full, 0x3fee9f9298593ae5ull, 0x3fee9f7df9519484ull, 0x3fee9f7466f42e87ull,
+    0x3fee9f75e8ec5f74ull, 0x3fee9f8286ead08aull, 0x3fee9f9a48a58174ull, 0x3fee9fbd35d7cbfdull,
+    0x3fee9feb564267c9ull, 0x3feea024b1ab6e09ull, 0x3feea0694fde5d3full, 0x3feea0b938ac1cf6ull,
+    0x3feea11473eb0187ull, 0x3feea17b0976cfdbull, 0x3feea1ed0130c132ull, 0x3feea26a62ff86f0ull,
+    0x3feea2f336cf4e62ull, 0x3feea3878491c491ull, 0x3feea427543e1a12ull, 0x3feea4d2add106d9ull,
+    0x3feea589994cce13ull, 0x3feea64c1eb941f7ull, 0x3feea71a4623c7adull, 0x3feea7f4179f5b21ull,
+    0x3feea8d99b4492edull, 0x3feea9cad931a436ull, 0x3feeaac7d98a6699ull, 0x3feeabd0a478580full,
+    0x3feeace5422aa0dbull, 0x3feeae05bad61778ull, 0x3feeaf3216b5448cull, 0x3feeb06a5e0866d9ull,
+    0x3feeb1ae99157736ull, 0x3feeb2fed0282c8aull, 0x3feeb45b0b91ffc6ull, 0x3feeb5c353aa2fe2ull,
+    0x3feeb737b0cdc5e5ull, 0x3feeb8b82b5f98e5ull, 0x3feeba44cbc8520full, 0x3feebbdd9a7670b3ull,
+    0x3feebd829fde4e50ull, 0x3feebf33e47a22a2ull, 0x3feec0f170ca07baull, 0x3feec2bb4d53fe0dull,
+    0x3feec49182a3f090ull, 0x3feec674194bb8d5ull, 0x3feec86319e32323ull, 0x3feeca5e8d07f29eull,
+    0x3feecc667b5de565ull, 0x3feece7aed8eb8bbull, 0x3feed09bec4a2d33ull, 0x3feed2c980460ad8ull,
+    0x3feed503b23e255dull, 0x3feed74a8af46052ull, 0x3feed99e1330b358ull, 0x3feedbfe53c12e59ull,
+    0x3feede6b5579fdbfull, 0x3feee0e521356ebaull, 0x3feee36bbfd3f37aull, 0x3feee5ff3a3c2774ull,
+    0x3feee89f995ad3adull, 0x3feeeb4ce622f2ffull, 0x3feeee07298db666ull, 0x3feef0ce6c9a8952ull,
+    0x3feef3a2b84f15fbull, 0x3feef68415b749b1ull, 0x3feef9728de5593aull, 0x3feefc6e29f1c52aull,
+    0x3feeff76f2fb5e47ull, 0x3fef028cf22749e4ull, 0x3fef05b030a1064aull, 0x3fef08e0b79a6f1full,
+    0x3fef0c1e904bc1d2ull, 0x3fef0f69c3f3a207ull, 0x3fef12c25bd71e09ull, 0x3fef16286141b33dull,
+    0x3fef199bdd85529cull, 0x3fef1d1cd9fa652cull, 0x3fef20ab5fffd07aull, 0x3fef244778fafb22ull,
+    0x3fef27f12e57d14bull, 0x3fef2ba88988c933ull, 0x3fef2f6d9406e7b5ull, 0x3fef33405751c4dbull,
+    0x3fef3720dcef9069ull, 0x3fef3b0f2e6d1675ull, 0x3fef3f0b555dc3faull, 0x3fef43155b5bab74ull,
+    0x3fef472d4a07897cull, 0x3fef4b532b08c968ull, 0x3fef4f87080d89f2ull, 0x3fef53c8eacaa1d6ull,
+    0x3fef5818dcfba487ull, 0x3fef5c76e862e6d3ull, 0x3fef60e316c98398ull, 0x3fef655d71ff6075ull,
+    0x3fef69e603db3285ull, 0x3fef6e7cd63a8315ull, 0x3fef7321f301b460ull, 0x3fef77d5641c0658ull,
+    0x3fef7c97337b9b5full, 0x3fef81676b197d17ull, 0x3fef864614f5a129ull, 0x3fef8b333b16ee12ull,
+    0x3fef902ee78b3ff6ull, 0x3fef953924676d76ull, 0x3fef9a51fbc74c83ull, 0x3fef9f7977cdb740ull,
+    0x3fefa4afa2a490daull, 0x3fefa9f4867cca6eull, 0x3fefaf482d8e67f1ull, 0x3fefb4aaa2188510ull,
+    0x3fefba1bee615a27ull, 0x3fefbf9c1cb6412aull, 0x3fefc52b376bba97ull, 0x3fefcac948dd7274ull,
+    0x3fefd0765b6e4540ull, 0x3fefd632798844f8ull, 0x3fefdbfdad9cbe14ull, 0x3fefe1d802243c89ull,
+    0x3fefe7c1819e90d8ull, 0x3fefedba3692d514ull, 0x3feff3c22b8f71f1ull, 0x3feff9d96b2a23d9ull};
 
 struct Exp2 {
     double t, g;
@@ -104,10 +162,8 @@ __device__ __forceinline__ Exp2 exp2_parts(const unsigned long long* table, doub
     const double f = y - (rounded - kRound);
     const int n = __double2loint(rounded);
     const double t = __longlong_as_double(static_cast<long long>(table[n & (kExp2Entries - 1)]));
-    double q = 0x1.c6b110835b776p-5;
-    q = fma(q, f, 0x1.ebfccc586302fp-3);
-    q = fma(q, f, 0x1.62e42fefa39efp-1);
-    return Exp2{__hiloint2double(__double2hiint(t) + (n << 15), __double2loint(t)),
+    const double q = fma(0x1.ebfbe3a9ac80bp-3, f, 0x1.62e43543b54d7p-1);
+    return Exp2{__hiloint2double(__double2hiint(t) + (n << 12), __double2loint(t)),
                 fma(q, f, 1.0)};
 }
 
