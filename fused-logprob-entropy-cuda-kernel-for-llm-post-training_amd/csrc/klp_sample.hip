@@ -867,9 +867,12 @@ __global__ __launch_bounds__(T, kMode != kPlain ? 4 : 6) void klp_sample_kernel(
                 uint32_t in = 0;
 #pragma unroll
                 for (int j = 0; j < kChunk; ++j) {
-                    const double w = sm.weight(v[j]);
-                    all += w;
-                    kept += v[j] > high ? w : 0.0;
+                    // Without its high word a weight is less than 2^-1042.
+                    const Exp2 e = sm.parts(sm.log2_weight(v[j]));
+                    all = fma(e.t, e.g, all);
+                    kept = fma(__hiloint2double(v[j] > high ? __double2hiint(e.t) : 0,
+                                                __double2loint(e.t)),
+                               e.g, kept);
                     if (v[j] <= high && v[j] >= low) in |= 1u << j;
                 }
                 // Added here, or the sums of 4 chunks wait in registers.
