@@ -3,9 +3,12 @@ the scoring of what was sampled; the pieces against their composition, and the
 composition against a plain one in 64 bits."""
 from __future__ import annotations
 
+import threading
+
 import numpy as np
 import pytest
 import torch
+from torch.utils.checkpoint import checkpoint
 
 from oracle import fp8_oracle, norm_oracle
 from oracle.sample_oracle import sample_row
@@ -118,3 +121,55 @@ def test_norm_in_front_of_the_fused_grpo_step():
     assert torch.equal(x.grad, res.grad)
     assert (np.abs(x.grad.double().cpu().numpy().reshape(-1, D) - dx) <= tol * size).all()
     assert (np.abs(nw.grad.double().cpu().numpy() - dw) <= tol * dw_size).all()
+
+
+def _tail(x, res, nw, head, head_scale, u):
+    ko = _ko()
+    y, h = ko.fused_add_rms_norm(x, res, nw)
+    logits = ko.fp8_linear(*ko.fused_rms_norm_fp8(h, nw), head, head_scale)
+    return (y, h, logits, *ko.fused_sample(logits, u, 0.9, top_p=0.9),
+            *ko.sample_hidden(x, nw, head, head_scale, u, residual=res, top_k=20))
+
+
+def test_threads_with_streams_of_their_own():
+    """Four threads, a stream each, calling at once: the bits of one alone."""
+    x, res, nw, w, u = _model(40, 512, 3001, 5)
+    head, head_scale = _ko().quantize_fp8(w, block_rows=128)
+    want = _tail(x, res, nw, head, head_scale, u)
+    torch.cuda.synchronize()
+    got = [None] * 4
+
+    def work(i):
+        stream = torch.cuda.Stream()
+        with torch.cuda.stream(stream):
+            for _ in range(20):
+                got[i] = _tail(x, res, nw, head, head_scale, u)
+        stream.synchronize()
+
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(4)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    for g in got:
+        assert all(torch.equal(a, b) for a, b in zip(g, want))
+
+
+def test_inference_mode_autocast_and_checkpoint():
+    x, res, nw, w, u = _model(30, 272, 900, 6)
+    head, head_scale = _ko().quantize_fp8(w, block_rows=128)
+    want = _tail(x, res, nw, head, head_scale, u)
+    with torch.inference_mode():
+        assert all(torch.equal(a, b)
+                   for a, b in zip(_tail(x, res, nw, head, head_scale, u), want))
+    with torch.autocast("cuda", dtype=torch.float16):
+        assert all(torch.equal(a, b)
+                   for a, b in zip(_tail(x, res, nw, head, head_scale, u), want))
+    leaf = x.float().requires_grad_()
+    weight = nw.float().requires_grad_()
+    grads = []
+    for again in (False, True):
+        f = lambda t: _ko().fused_rms_norm(t, weight)  # noqa: E731
+        y = checkpoint(f, leaf, use_reentrant=False) if again else f(leaf)
+        grads.append(torch.autograd.grad(y.square().sum(), (leaf, weight)))
+    assert all(torch.equal(a, b) for a, b in zip(*grads))
