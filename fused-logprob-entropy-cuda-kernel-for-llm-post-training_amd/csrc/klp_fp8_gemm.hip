@@ -269,7 +269,9 @@ __device__ __forceinline__ void copy_dwords_to_lds(u32x4 rsrc, uint32_t lds, uin
 }
 
 template <int DT, typename Shape>
-__global__ __launch_bounds__(kTileThreads, Shape::kSmall && DT != kFP32 ? 4 : 2) void klp_fp8_tile_kernel(Fp8LinearParams p) {
+__global__
+__launch_bounds__(kTileThreads, Shape::kSmall && DT != kFP32 ? 4 : 2) void klp_fp8_tile_kernel(
+    Fp8LinearParams p) {
     using namespace mfma;
     constexpr int VB = Shape::VB, MB = Shape::MB;
     __shared__ __attribute__((aligned(1024))) unsigned char lds[Shape::kLds];
@@ -316,13 +318,15 @@ __global__ __launch_bounds__(kTileThreads, Shape::kSmall && DT != kFP32 ? 4 : 2)
     // Copies of block b into slot b % 2.  Chunks past K, and all of a block
     // past the last, come from past the descriptors: zeros, and the count of
     // copies in flight stays the same.
-    const u32x4 rs_v = bytes_rsrc(p.w + v0 * p.ld_w, (rows_v - 1) * ld_v + static_cast<uint32_t>(p.k));
-    const u32x4 rs_m = bytes_rsrc(p.x + t0 * p.ld_x, (rows_m - 1) * ld_m + static_cast<uint32_t>(p.k));
+    const uint32_t k = static_cast<uint32_t>(p.k);
+    const u32x4 rs_v = bytes_rsrc(p.w + v0 * p.ld_w, (rows_v - 1) * ld_v + k);
+    const u32x4 rs_m = bytes_rsrc(p.x + t0 * p.ld_x, (rows_m - 1) * ld_m + k);
     const u32x4 rs_s = bytes_rsrc(p.xs + t0 * p.n_blocks, static_cast<uint32_t>(rows_m) * nb * 4);
     const uint32_t lane_v = static_cast<uint32_t>(wrow + (lane >> 3)) * ld_v + cchunk * 16;
     const uint32_t lane_m = static_cast<uint32_t>(crow) * ld_m + cchunk * 16;
     const uint32_t lane_s = stok * static_cast<uint32_t>(nb) * 4;
-    const int chunks = static_cast<int>((p.k - cchunk * 16 + kK - 1) / kK);  // blocks with this chunk
+    // Blocks with this chunk.
+    const int chunks = static_cast<int>((p.k - cchunk * 16 + kK - 1) / kK);
     int block[2] = {0, 0};  // the first and second copies' next
     auto copy_v = [&](int half, int j) {
         const int b = block[half];
@@ -363,8 +367,12 @@ __global__ __launch_bounds__(kTileThreads, Shape::kSmall && DT != kFP32 ? 4 : 2)
         u.h[1] = *reinterpret_cast<const u32x4*>(lds + at + (lchunk ^ 64));
         return Operand<DT == kFP32>::from(u.v);
     };
-    auto read_v = [&](int slot, int i) { return read(slot * Shape::kSlotV + base_v + i * 16 * kK); };
-    auto read_m = [&](int slot, int j) { return read(slot * Shape::kSlotM + base_m + j * 16 * kK); };
+    auto read_v = [&](int slot, int i) {
+        return read(slot * Shape::kSlotV + base_v + i * 16 * kK);
+    };
+    auto read_m = [&](int slot, int j) {
+        return read(slot * Shape::kSlotM + base_m + j * 16 * kK);
+    };
     auto read_s = [&](int slot, int j) {
         return *reinterpret_cast<const float*>(lds + kAt_s + slot * Shape::kSlotS +
                                                (wm * 16 * MB + 16 * j + lrow) * 4);
@@ -374,7 +382,8 @@ __global__ __launch_bounds__(kTileThreads, Shape::kSmall && DT != kFP32 ? 4 : 2)
     // Constant memory: a scalar load.  A vector load's wait would also wait for
     // the copies before it.
     typedef __attribute__((address_space(4))) const float const_float;
-    const const_float* ws = (const const_float*)(uintptr_t)(p.ws + first_row / kScaleBlock * p.n_blocks);
+    const const_float* ws =
+        (const const_float*)(uintptr_t)(p.ws + first_row / kScaleBlock * p.n_blocks);
 
     f32x4 acc[VB][MB];
 #pragma unroll
@@ -487,7 +496,8 @@ hipError_t launch_stream(const Fp8LinearParams& p, hipStream_t stream) {
 
 template <typename Shape>
 int64_t tiles_of(const Fp8LinearParams& p) {
-    return ((p.n + Shape::kRowsV - 1) / Shape::kRowsV) * ((p.m + Shape::kRowsM - 1) / Shape::kRowsM);
+    return ((p.n + Shape::kRowsV - 1) / Shape::kRowsV) *
+           ((p.m + Shape::kRowsM - 1) / Shape::kRowsM);
 }
 // Rounds of one tile a CU, times a round's time.
 template <typename Shape>

@@ -875,7 +875,7 @@ __global__ __launch_bounds__(T, kMode != kPlain ? 4 : 6) void klp_sample_kernel(
                                e.g, kept);
                     if (v[j] <= high && v[j] >= low) in |= 1u << j;
                 }
-                // Added here, or the sums of 4 chunks wait in registers.
+                // Added here, or the sums of several chunks wait in registers.
                 asm volatile("" : "+v"(all), "+v"(kept));
                 append(in, first, v);
             });
