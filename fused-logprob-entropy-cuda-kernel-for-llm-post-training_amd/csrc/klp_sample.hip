@@ -19,7 +19,9 @@
 //
 // A row is read by one workgroup, a contiguous part of it by each wave.
 //   No filter: one pass sums the weights, relative to one of the row's first
-// logits; the part whose running sum crosses the target is read again.
+// logits (or, where those are masked or far below the row's largest, a second
+// one relative to that); the part whose running sum crosses the target is read
+// again.
 //   Filters: one pass for the maximum, then one that collects, in LDS, every
 // logit that could be kept, and is followed by work on that list alone: an
 // entry's rank, or the mass before it, in falling order says whether it is
@@ -563,7 +565,9 @@ struct Sampler {
                           : 63 - __clzll(static_cast<long long>(h));
         };
         const int part = choose(sum > kNothing, pos + sum > target);
-        if (part < 0) return wave == 0 ? 0 : -1;  // no weight at all: none of a row with a maximum
+        // Weights are relative to a logit of at most the row's largest, whose own
+        // is then at least 1: there is such a part.
+        if (part < 0) return wave == 0 ? 0 : -1;
         pos = __shfl(pos, part, 64);
         rank = __shfl(rank, part, 64);
 
@@ -723,8 +727,10 @@ __global__ __launch_bounds__(T, kMode != kPlain ? 4 : 6) void klp_sample_kernel(
 
     if (threadIdx.x < kExp2Entries) s.exp2_table[threadIdx.x] = kExp2Table[threadIdx.x];
     if (!kFilters || (!by_k && !by_p && !by_m)) {
-        // Weights relative to the largest of the first 64 logits; again, to the
-        // row's largest, if that overflows (2^900 of them).
+        // Weights relative to the largest of the first 64 logits, or to 0 where
+        // those are all masked; again, to the row's largest, where that
+        // outranges float64 (by 2^900) or lies below such a 0, from which the
+        // row's own weights would count as none.
         float first = lane < vocab ? to_f32<DT>(row.x[lane]) : -INFINITY;
         first = xrow_max(row_max16(first));
         __syncthreads();
@@ -743,7 +749,8 @@ __global__ __launch_bounds__(T, kMode != kPlain ? 4 : 6) void klp_sample_kernel(
         sm.top = fabsf(first) < INFINITY ? first : 0.0f;
         add_up();
         if (!over_row()) return;
-        if (sm.log2_weight(top) > 900.0) {
+        const double ahead = sm.log2_weight(top);
+        if (ahead > 900.0 || ahead < 0.0) {
             sm.top = top;
             add_up();
         }
