@@ -855,6 +855,23 @@ NormForward norm_forward(const at::Tensor& x, const at::Tensor& residual, const 
     return o;
 }
 
+// The norm's gradients as functions of what they depend on, whose own gradient
+// is refused: left without a graph they would count as constants in a second
+// derivative.
+class FirstOrder : public torch::autograd::Function<FirstOrder> {
+   public:
+    static variable_list forward(AutogradContext*, const at::Tensor& d_x,
+                                 const std::optional<at::Tensor>& d_w, const at::Tensor&,
+                                 const at::Tensor&, const at::Tensor&,
+                                 const std::optional<at::Tensor>&) {
+        if (d_w.has_value()) return {d_x, *d_w};
+        return {d_x};
+    }
+    static variable_list backward(AutogradContext*, variable_list) {
+        throw std::runtime_error("kernel_opt: the root-mean-square norms have no second derivative");
+    }
+};
+
 class FusedRmsNorm : public torch::autograd::Function<FusedRmsNorm> {
    public:
     static variable_list forward(AutogradContext* ctx, const at::Tensor& x,
@@ -907,6 +924,14 @@ class FusedRmsNorm : public torch::autograd::Function<FusedRmsNorm> {
                                           w.data_ptr(), dtype_code(w.scalar_type()), fptr(rstd),
                                           g_y.data_ptr(), data_or_null(g_h), n, d, d_x.data_ptr(),
                                           data_or_null(d_w), data_or_null(ws), bytes, stream));
+        }
+        if (at::GradMode::is_enabled()) {  // create_graph
+            const auto opt = [](const at::Tensor& t) {
+                return t.defined() ? std::optional<at::Tensor>(t) : std::nullopt;
+            };
+            const variable_list d = FirstOrder::apply(d_x, opt(d_w), h, weight, g_y, opt(g_h));
+            d_x = d[0];
+            if (need_w) d_w = d[1];
         }
         return {need_x ? d_x : at::Tensor(), need_r ? d_x : at::Tensor(), d_w, at::Tensor()};
     }

@@ -7,7 +7,9 @@ compute, per row of ``dim`` elements,
     y = round(h * (mean(h^2) + eps)^-1/2 * weight)
 
 in one pass (csrc/klp_norm.hip), differentiable in ``x``, ``residual`` and
-``weight``: the backward reads ``h`` and one float32 a row.  The statistics are
+``weight``: the backward reads ``h`` and one float32 a row.  The gradient is of
+first order: with ``create_graph=True`` a second derivative through it raises
+RuntimeError (what flows through ``h`` alone has one).  The statistics are
 those of the stored ``h``, all sums are float32, ``y`` is rounded once; a row
 whose sum of squares passes float32's range gives zeros.
 
@@ -88,6 +90,20 @@ def _forward(x, residual, weight, eps, fp8):
     return y, h, rstd
 
 
+class _FirstOrder(torch.autograd.Function):
+    """The norm's gradients as functions of what they depend on (``of``), whose
+    own gradient is refused: left without a graph they would count as constants
+    in a second derivative."""
+
+    @staticmethod
+    def forward(ctx, d_x, d_w, *of):
+        return d_x, d_w
+
+    @staticmethod
+    def backward(ctx, *grads):
+        raise RuntimeError("kernel_opt: the root-mean-square norms have no second derivative")
+
+
 class _FusedRmsNorm(torch.autograd.Function):
 
     @staticmethod
@@ -124,6 +140,8 @@ class _FusedRmsNorm(torch.autograd.Function):
                 ptr(h2), DTYPE_CODES[h.dtype], ld_h, ptr(w), DTYPE_CODES[w.dtype], ptr(rstd),
                 ptr(g_y), ptr(g_h), N, D, ptr(d_x), ptr(d_w), ptr(ws), nbytes,
                 stream_handle(dev.index)))
+        if torch.is_grad_enabled():  # create_graph
+            d_x, d_w = _FirstOrder.apply(d_x, d_w, h, weight, g_y, g_h)
         return d_x if need_x else None, d_x if need_r else None, d_w, None
 
 
