@@ -47,7 +47,8 @@ def _parameter(value, name, shape, device, dtype, off, low, high):
             value = value.clamp(0, 2 ** 31 - 1)
         return off, value.detach().to(dtype).contiguous()
     if dtype == torch.int32:
-        if isinstance(value, bool) or int(value) != value:
+        # value - value: NaN for an infinity or a NaN.
+        if isinstance(value, bool) or value - value != 0 or int(value) != value:
             raise ValueError(f"{name} must be an integer, got {value!r}")
         value = int(value)
     else:
@@ -69,12 +70,15 @@ def fused_sample(logits: torch.Tensor, uniform: torch.Tensor, temperature=1.0, *
         temperature: T >= 0; 0 takes the largest logit (the lowest index of
             equal ones), with ``logp`` at T = 1 and ``sample_logp`` 0.
         top_k, top_p, min_p: filters, in this order; None turns one off, and
-            so do ``top_k`` <= 0 or >= V, ``top_p`` >= 1 and ``min_p`` <= 0.
+            so do ``top_k`` <= 0 or >= V, ``top_p`` 1 and ``min_p`` 0.
 
     Every parameter is a number or a tensor shaped like ``uniform`` with one
-    value a row (read as float32, ``top_k`` as int32).  A tensor's values are
-    not checked: a row whose temperature is negative or not finite gets token
-    -1, as do rows without a distribution, below.
+    value a row (read as float32, ``top_k`` as int32).  A number that is not in
+    range raises ValueError: T >= 0 and finite, ``top_k`` an integer, ``top_p``
+    and ``min_p`` in [0, 1].  A tensor's values are not checked: a row whose
+    temperature is negative or not finite gets token -1, as do rows without a
+    distribution, below; a ``top_p`` above 1 and a ``min_p`` below 0, or a NaN
+    of either, is off, a ``top_p`` below 0 counts as 0, a ``min_p`` above 1 as 1.
 
     Returns:
         ``(tokens, logp, sample_logp)``, int64 and twice float32, each
@@ -97,7 +101,8 @@ def fused_sample(logits: torch.Tensor, uniform: torch.Tensor, temperature=1.0, *
                            f"{uniform.dtype} {tuple(shape)} on {uniform.device}")
     inf = math.inf
     t, ts = _parameter(temperature, "temperature", shape, dev, torch.float32, 1.0, 0.0, inf)
-    k, ks = _parameter(top_k, "top_k", shape, dev, torch.int32, 0, 0, 2 ** 31 - 1)
+    k, ks = _parameter(top_k, "top_k", shape, dev, torch.int32, 0, -inf, inf)
+    k = min(max(k, 0), 2 ** 31 - 1)
     p, ps = _parameter(top_p, "top_p", shape, dev, torch.float32, 1.0, 0.0, 1.0)
     m, ms = _parameter(min_p, "min_p", shape, dev, torch.float32, 0.0, 0.0, 1.0)
     try:
