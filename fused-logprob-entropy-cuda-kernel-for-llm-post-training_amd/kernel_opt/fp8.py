@@ -25,6 +25,8 @@ from .norm import SCALE_BLOCK, _rows
 
 __all__ = ["quantize_fp8", "fp8_linear"]
 
+MAX_ROWS = 2 ** 20  # of one product's x
+
 
 def quantize_fp8(x: torch.Tensor, block_rows: int = 1):
     """``(codes, scales)`` of ``x`` ``[..., dim]`` (bf16 / fp16 / fp32, GPU).
@@ -96,7 +98,7 @@ def fp8_linear(x: torch.Tensor, x_scale: torch.Tensor, weight: torch.Tensor,
     ``out_dtype``.
 
     Args:
-        x: ``[..., K]`` float8_e4m3fn, K a multiple of 16.
+        x: ``[..., K]`` float8_e4m3fn, K a multiple of 16, at most 2**20 rows.
         x_scale: ``[..., ceil(K / 128)]`` float32.
         weight: ``[N, K]`` float8_e4m3fn.
         weight_scale: ``[ceil(N / 128), ceil(K / 128)]`` float32.

@@ -14,7 +14,7 @@ from __future__ import annotations
 
 import torch
 
-from .fp8 import fp8_linear
+from .fp8 import MAX_ROWS, fp8_linear
 from .linear_grpo import default_chunk_tokens
 from .norm import fused_add_rms_norm_fp8, fused_rms_norm_fp8
 from .ops import fused_logprob_entropy_forward
@@ -41,7 +41,8 @@ def sample_hidden(hidden: torch.Tensor, norm_weight: torch.Tensor, head: torch.T
             :func:`fused_rms_norm` takes it.
         head, head_scale: ``[V, dim]`` float8_e4m3fn and its scales
             (``quantize_fp8(weight, block_rows=128)``); dim a multiple of 16.
-        uniform, temperature, top_k, top_p, min_p: :func:`fused_sample`'s.
+        uniform, temperature, top_k, top_p, min_p: :func:`fused_sample`'s; at
+            most 2**20 rows.
         logits_dtype: dtype the logits are rounded to.
 
     Returns:
@@ -64,8 +65,8 @@ def score_hidden(hidden: torch.Tensor, norm_weight: torch.Tensor, head: torch.Te
 
     Args:
         targets: ``[...]`` int64, ``hidden``'s leading shape.
-        chunk_tokens: tokens whose logits are held at a time; by default the
-            fewest equal chunks of at most 4 GiB of logits.
+        chunk_tokens: tokens whose logits are held at a time, at most 2**20 of
+            them; by default the fewest equal chunks of at most 4 GiB of logits.
     """
     if targets.dtype != torch.int64:
         raise RuntimeError("targets must be int64")
@@ -81,6 +82,7 @@ def score_hidden(hidden: torch.Tensor, norm_weight: torch.Tensor, head: torch.Te
     n = t.numel()
     size = 4 if logits_dtype == torch.float32 else 2
     chunk = default_chunk_tokens(n, head.size(0), size) if chunk_tokens is None else chunk_tokens
+    chunk = min(chunk, MAX_ROWS)
     out = torch.empty(3, n, dtype=torch.float32, device=hidden.device)
     for i in range(0, n, chunk):
         logits = fp8_linear(q[i:i + chunk], s[i:i + chunk], head, head_scale, logits_dtype)
