@@ -19,7 +19,8 @@ e4m3 codes with a float32 scale for each 128 columns, the operand of
 
 Calls run in the compiled binding (binding/klp_torch.cpp), the autograd function
 included; under graph capture, which it declines, the Python statement of them
-below runs.
+below runs, and under ``torch.compile`` the two differentiable ones go through
+the registered op ``torch.ops.kernel_opt.rms_norm`` (no graph break).
 """
 from __future__ import annotations
 
@@ -90,6 +91,28 @@ def _forward(x, residual, weight, eps, fp8):
     return y, h, rstd
 
 
+def _backward(h, weight, rstd, g_y, g_h, need_w):
+    """(d_x, d_weight or None) into new dense tensors."""
+    dev = h.device
+    h2, ld_h = _rows(h)
+    N, D = h2.shape
+    d_x = torch.empty(h.shape, dtype=h.dtype, device=dev)
+    d_w = torch.empty_like(weight, memory_format=torch.contiguous_format) if need_w else None
+    if N == 0:
+        return d_x, d_w.zero_() if need_w else None
+    g_y = g_y.contiguous()
+    g_h = None if g_h is None else g_h.contiguous()
+    nbytes = lib.klp_rms_norm_bwd_workspace_bytes(N, D) if need_w else 0
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=dev) if need_w else None
+    w = weight.contiguous()
+    with device_guard(dev.index):
+        check_status(lib.klp_rms_norm_bwd(
+            ptr(h2), DTYPE_CODES[h.dtype], ld_h, ptr(w), DTYPE_CODES[w.dtype], ptr(rstd),
+            ptr(g_y), ptr(g_h), N, D, ptr(d_x), ptr(d_w), ptr(ws), nbytes,
+            stream_handle(dev.index)))
+    return d_x, d_w
+
+
 class _FirstOrder(torch.autograd.Function):
     """The norm's gradients as functions of what they depend on (``of``), whose
     own gradient is refused: left without a graph they would count as constants
@@ -104,6 +127,19 @@ class _FirstOrder(torch.autograd.Function):
         raise RuntimeError("kernel_opt: the root-mean-square norms have no second derivative")
 
 
+def _gradients(ctx, g_y, g_h, backward):
+    """Gradients of (x, residual, weight), by ``backward`` where y's is given."""
+    h, weight, rstd = ctx.saved_tensors
+    need_x, need_r, need_w = ctx.needs_input_grad[:3]
+    if (g_y is None and g_h is None) or not (need_x or need_r or need_w):
+        return None, None, None
+    if g_y is None:  # only h was used
+        d_w = torch.zeros_like(weight) if need_w else None
+        return g_h if need_x else None, g_h if need_r else None, d_w
+    d_x, d_w = backward(h, weight, rstd, g_y, g_h, need_w)
+    return d_x if need_x else None, d_x if need_r else None, d_w
+
+
 class _FusedRmsNorm(torch.autograd.Function):
 
     @staticmethod
@@ -115,34 +151,64 @@ class _FusedRmsNorm(torch.autograd.Function):
 
     @staticmethod
     def backward(ctx, g_y, g_h=None):
-        h, weight, rstd = ctx.saved_tensors
-        need_x, need_r, need_w = ctx.needs_input_grad[:3]
-        if (g_y is None and g_h is None) or not (need_x or need_r or need_w):
-            return None, None, None, None
-        if g_y is None:  # only h was used
-            d_w = torch.zeros_like(weight) if need_w else None
-            return g_h if need_x else None, g_h if need_r else None, d_w, None
-        dev = h.device
-        h2, ld_h = _rows(h)
-        N, D = h2.shape
-        d_x = torch.empty(h.shape, dtype=h.dtype, device=dev)
-        d_w = torch.empty_like(weight, memory_format=torch.contiguous_format) if need_w else None
-        if N == 0:
-            return d_x if need_x else None, d_x if need_r else None, d_w.zero_() if need_w else None, \
-                None
-        g_y = g_y.contiguous()
-        g_h = None if g_h is None else g_h.contiguous()
-        nbytes = lib.klp_rms_norm_bwd_workspace_bytes(N, D) if need_w else 0
-        ws = torch.empty(nbytes, dtype=torch.uint8, device=dev) if need_w else None
-        w = weight.contiguous()
-        with device_guard(dev.index):
-            check_status(lib.klp_rms_norm_bwd(
-                ptr(h2), DTYPE_CODES[h.dtype], ld_h, ptr(w), DTYPE_CODES[w.dtype], ptr(rstd),
-                ptr(g_y), ptr(g_h), N, D, ptr(d_x), ptr(d_w), ptr(ws), nbytes,
-                stream_handle(dev.index)))
-        if torch.is_grad_enabled():  # create_graph
-            d_x, d_w = _FirstOrder.apply(d_x, d_w, h, weight, g_y, g_h)
-        return d_x if need_x else None, d_x if need_r else None, d_w, None
+        def first_order(h, weight, rstd, g_y, g_h, need_w):
+            d_x, d_w = _backward(h, weight, rstd, g_y, g_h, need_w)
+            if torch.is_grad_enabled():  # create_graph
+                d_x, d_w = _FirstOrder.apply(d_x, d_w, h, weight, g_y, g_h)
+            return d_x, d_w
+
+        return *_gradients(ctx, g_y, g_h, first_order), None
+
+
+# ---------------------------------------------------------------------------
+# torch.library registration, for torch.compile: the norm traces without a
+# graph break.  Eager calls take the compiled autograd function.
+# ---------------------------------------------------------------------------
+@torch.library.custom_op("kernel_opt::rms_norm", mutates_args=(), device_types="cuda")
+def _op_forward(x: torch.Tensor, residual: torch.Tensor | None, weight: torch.Tensor,
+                eps: float) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+    y, h, rstd = _forward(x, residual, weight, eps, False)
+    return y, x.new_empty(0) if h is None else h, rstd
+
+
+@_op_forward.register_fake
+def _(x, residual, weight, eps):
+    y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    rstd = x.new_empty(x.numel() // x.size(-1), dtype=torch.float32)
+    return y, x.new_empty(0) if residual is None else torch.empty_like(y), rstd
+
+
+@torch.library.custom_op("kernel_opt::rms_norm_backward", mutates_args=(), device_types="cuda")
+def _op_backward(h: torch.Tensor, weight: torch.Tensor, rstd: torch.Tensor, g_y: torch.Tensor,
+                 g_h: torch.Tensor | None, need_w: bool) -> tuple[torch.Tensor, torch.Tensor]:
+    d_x, d_w = _backward(h, weight, rstd, g_y, g_h, need_w)
+    return d_x, d_w if need_w else weight.new_empty(0)
+
+
+@_op_backward.register_fake
+def _(h, weight, rstd, g_y, g_h, need_w):
+    d_x = torch.empty(h.shape, dtype=h.dtype, device=h.device)
+    return d_x, weight.new_empty(weight.shape if need_w else 0)
+
+
+def _op_setup_context(ctx, inputs, output):
+    x, residual, weight, _eps = inputs
+    _y, h, rstd = output
+    ctx.has_h = residual is not None
+    ctx.save_for_backward(h if ctx.has_h else x, weight, rstd)
+    ctx.mark_non_differentiable(rstd)
+    ctx.set_materialize_grads(False)
+
+
+def _op_backward_rule(ctx, g_y, g_h, _g_rstd):
+    def backward(h, weight, rstd, g_y, g_h, need_w):
+        d_x, d_w = _op_backward(h, weight, rstd, g_y, g_h, need_w)
+        return d_x, d_w if need_w else None
+
+    return *_gradients(ctx, g_y, g_h if ctx.has_h else None, backward), None
+
+
+_op_forward.register_autograd(_op_backward_rule, setup_context=_op_setup_context)
 
 
 def fused_rms_norm(x: torch.Tensor, weight: torch.Tensor, eps: float = 1e-6):
@@ -154,6 +220,8 @@ def fused_rms_norm(x: torch.Tensor, weight: torch.Tensor, eps: float = 1e-6):
         weight: ``[dim]``, of ``x``'s dtype or float32.
     """
     _check(x, None, weight, eps)
+    if torch.compiler.is_compiling():
+        return torch.ops.kernel_opt.rms_norm(x, None, weight, float(eps))[0]
     try:
         return binding.rms_norm(x, None, weight, float(eps))[0]
     except binding.CaptureDeclined:
@@ -166,6 +234,8 @@ def fused_add_rms_norm(x: torch.Tensor, residual: torch.Tensor, weight: torch.Te
     norm ``y`` as :func:`fused_rms_norm` gives it, differentiable in ``x``,
     ``residual`` and ``weight`` through both outputs."""
     _check(x, residual, weight, eps)
+    if torch.compiler.is_compiling():
+        return torch.ops.kernel_opt.rms_norm(x, residual, weight, float(eps))[:2]
     try:
         return tuple(binding.rms_norm(x, residual, weight, float(eps)))
     except binding.CaptureDeclined:
