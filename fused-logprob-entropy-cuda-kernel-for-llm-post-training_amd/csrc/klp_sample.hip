@@ -565,8 +565,7 @@ struct Sampler {
                           : 63 - __clzll(static_cast<long long>(h));
         };
         const int part = choose(sum > kNothing, pos + sum > target);
-        // Weights are relative to a logit of at most the row's largest, whose own
-        // is then at least 1: there is such a part.
+        // The row's largest weighs 2^-300 at least: there is such a part.
         if (part < 0) return wave == 0 ? 0 : -1;
         pos = __shfl(pos, part, 64);
         rank = __shfl(rank, part, 64);
@@ -729,8 +728,9 @@ __global__ __launch_bounds__(T, kMode != kPlain ? 4 : 6) void klp_sample_kernel(
     if (!kFilters || (!by_k && !by_p && !by_m)) {
         // Weights relative to the largest of the first 64 logits, or to 0 where
         // those are all masked; again, to the row's largest, where that
-        // outranges float64 (by 2^900) or lies below such a 0, from which the
-        // row's own weights would count as none.
+        // outranges float64 (by 2^900) or lies so far below such a 0 (2^300)
+        // that the row's own weights would come near to counting as none.
+        // (1024 rows of 128256 fp16, the first 64 masked: 86 us, 132 twice.)
         float first = lane < vocab ? to_f32<DT>(row.x[lane]) : -INFINITY;
         first = xrow_max(row_max16(first));
         __syncthreads();
@@ -750,7 +750,7 @@ __global__ __launch_bounds__(T, kMode != kPlain ? 4 : 6) void klp_sample_kernel(
         add_up();
         if (!over_row()) return;
         const double ahead = sm.log2_weight(top);
-        if (ahead > 900.0 || ahead < 0.0) {
+        if (ahead > 900.0 || ahead < -300.0) {
             sm.top = top;
             add_up();
         }

@@ -619,7 +619,7 @@ int klp_fp8_linear(const uint8_t* x, int64_t ld_x, const float* x_scales, const 
  * of that token.  Sums that decide the token, and sample_logp's, are float64
  * or whole numbers of 2^-44 and do not depend on timing; with a top_k, or a
  * min_p and no top_p, the sum behind logp is of float32 weights.  Weights
- * below 2^-960 of the row's largest may count as none.
+ * below 2^-660 of the row's largest may count as none.
  * Each parameter is one value, or with its array non-null one per row
  * (float32, top_k int32; [n_rows]).  top_k <= 0 or >= vocab, top_p >= 1 and
  * min_p <= 0 (or NaN) are off.  T = 0 takes the largest logit (lowest index),

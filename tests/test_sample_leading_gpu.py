@@ -43,8 +43,9 @@ def _check(x, u, got, temperature):
 
 # (largest logit, temperature): quotients from -0.5 to -50000, past the ends of
 # float64's exponents (-708), of the weights that count (-665) and of those
-# before light tokens go (-624); and above zero.
-TOPS = [(-0.5, 1.0), (-7.0, 0.01), (-14.0, 0.02), (-10.0, 0.01), (-640.0, 1.0), (-6.3, 0.01),
+# before light tokens go (-624), around the -208 from which on they are taken
+# relative to the row's largest; and above zero.
+TOPS = [(-0.5, 1.0), (-2.0, 0.01), (-2.2, 0.01), (-207.0, 1.0), (-209.0, 1.0), (-7.0, 0.01), (-14.0, 0.02), (-10.0, 0.01), (-640.0, 1.0), (-6.3, 0.01),
         (-700.0, 1.0), (-5000.0, 1.0), (-50.0, 1e-3), (9.0, 0.01), (700.0, 1.0), (0.0, 0.005)]
 
 
