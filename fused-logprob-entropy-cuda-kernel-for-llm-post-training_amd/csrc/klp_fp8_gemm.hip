@@ -234,13 +234,15 @@ __global__ __launch_bounds__(64 * kSplit) void klp_fp8_stream_kernel(Fp8LinearPa
 // the second half's weight rows.  The meetings wait for the copies that the
 // next half reads, which were started one and a half stages before.
 //
-// Bound by LDS and, at large sizes, the clock: a stage of a 256 x 256 tile
-// reads 192 KB (128 bytes a clock) and receives 64 KB (64 a clock), 2560
-// clocks against 2048 of matrix instructions, beside which the four FMAs of a
-// scale run for nothing (4780 TFLOP/s for a loop of one and four).  4096
-// tokens of a [152064, 3584] head: 2190 us, 2040 TFLOP/s, matrix units 56%
-// busy at 1.83 GHz; without its stores 2016 us, without its copies 1717.  16
-// tokens: 100 us, the weight read at 5.5 TB/s.
+// LDS is the bound that can be counted: a stage of a 256 x 256 tile reads 192
+// KB (128 bytes a clock) and receives 64 KB (64 a clock), 2560 clocks against
+// 2048 of matrix instructions, beside which the four FMAs of a scale run for
+// nothing (4780 TFLOP/s for a loop of one and four).  4096 tokens of a [152064,
+// 3584] head: 2150 us, 2.08 PFLOP/s, 58 us a tile of which that makes 39 at
+// 1.83 GHz; matrix units 56% busy, 80% if it were all.  The rest is not
+// accounted for: one workgroup fills a CU's LDS, so nothing runs under a tile's
+// first copies and its stores (without stores 2016 us, without copies 1717).
+// 16 tokens: 100 us, the weight read at 5.5 TB/s.
 template <int VB_, int MB_, int kTokenWaves_>
 struct TileShape {
     static constexpr int VB = VB_, MB = MB_, kTokenWaves = kTokenWaves_;

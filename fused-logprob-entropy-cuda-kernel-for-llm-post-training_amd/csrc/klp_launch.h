@@ -344,7 +344,7 @@ struct QuantizeParams {
 };
 hipError_t launch_quantize(int dtype, const QuantizeParams& p, hipStream_t stream);
 
-// Product of e4m3 matrices with a scale for each 128 of K (klp_fp8.hip):
+// Product of e4m3 matrices with a scale for each 128 of K (klp_fp8_gemm.hip):
 // out[m, n] = sum_b xs[m, b] ws[n / 128, b] sum_{k in b} x[m, k] w[n, k].
 struct Fp8LinearParams {
     const uint8_t* x;   // [m, ld_x]

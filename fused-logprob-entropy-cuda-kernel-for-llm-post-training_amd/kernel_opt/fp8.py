@@ -34,7 +34,8 @@ def quantize_fp8(x: torch.Tensor, block_rows: int = 1):
     ``block_rows=1``: scales ``[..., ceil(dim / 128)]``, 128 columns of a row
     each.  ``block_rows=128`` (a weight ``[N, dim]``): scales ``[ceil(N / 128),
     ceil(dim / 128)]``, 128 x 128 elements each.  A block with a NaN or an
-    infinity stands for NaN.
+    infinity stands for NaN.  No gradient: the outputs are detached from an
+    ``x`` that requires one.
     """
     if not x.is_cuda:
         raise RuntimeError("x must be a GPU tensor")
@@ -104,7 +105,9 @@ def fp8_linear(x: torch.Tensor, x_scale: torch.Tensor, weight: torch.Tensor,
         weight_scale: ``[ceil(N / 128), ceil(K / 128)]`` float32.
 
     Rows of ``x`` and ``weight`` start at multiples of 16 bytes (RuntimeError
-    otherwise).  A NaN code or scale gives NaN in the outputs it enters.
+    otherwise).  A NaN code or scale gives NaN in the outputs it enters.  The
+    two scales of a block are multiplied first, in float32: their product has
+    to stay in its range.
     """
     _check_linear(x, x_scale, weight, weight_scale, out_dtype)
     try:

@@ -246,7 +246,8 @@ def fused_rms_norm_fp8(x: torch.Tensor, weight: torch.Tensor, eps: float = 1e-6)
     """``(codes, scales)`` of :func:`fused_rms_norm`'s unrounded output: e4m3
     ``[..., dim]`` and float32 ``[..., ceil(dim / 128)]``; per 128 columns with
     a = max |y|, ``scale = a / 448`` (1 where a is 0) and ``code = e4m3(y * (448
-    / a))``.  A block with a NaN or an infinity stands for NaN.  No gradient."""
+    / a))``.  A block with a NaN or an infinity stands for NaN.  No gradient:
+    the outputs are detached from inputs that require one."""
     _check(x, None, weight, eps)
     try:
         return tuple(binding.rms_norm_fp8(x, None, weight, float(eps)))
@@ -258,7 +259,8 @@ def fused_rms_norm_fp8(x: torch.Tensor, weight: torch.Tensor, eps: float = 1e-6)
 def fused_add_rms_norm_fp8(x: torch.Tensor, residual: torch.Tensor, weight: torch.Tensor,
                            eps: float = 1e-6):
     """``(codes, scales, h)``: :func:`fused_rms_norm_fp8` of ``h = round(x +
-    residual)``, and ``h``.  No gradient."""
+    residual)``, and ``h``.  No gradient: the outputs, ``h`` among them, are
+    detached from inputs that require one."""
     _check(x, residual, weight, eps)
     try:
         return tuple(binding.rms_norm_fp8(x, residual, weight, float(eps)))

@@ -602,7 +602,9 @@ int klp_quantize_fp8(const void* x, int dtype, int64_t ld_x, int64_t rows, int64
  * lies more than 13 bits below that: off by up to 7 2^-13 of that product a
  * group, 5 10^-5 of a result (2-norm) on normal data.  Which kernel adds the
  * blocks, and so their order, depends on m, n and k.  m <= 2^20, n < 2^28,
- * k <= 2^24 and ceil(m / 64) ceil(n / 128) < 2^23 - 8 (KLP_EINVAL).
+ * k <= 2^24 and ceil(m / 64) ceil(n / 128) < 2^23 - 8 (KLP_EINVAL).  A block's
+ * two scales are multiplied first, in float32: a product of theirs past
+ * float32's range gives infinities or NaN, one below it zeros.
  */
 int klp_fp8_linear(const uint8_t* x, int64_t ld_x, const float* x_scales, const uint8_t* w,
                    int64_t ld_w, const float* w_scales, int64_t m, int64_t n, int64_t k,
