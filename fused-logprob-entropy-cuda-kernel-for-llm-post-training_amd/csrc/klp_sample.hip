@@ -41,7 +41,10 @@
 // {key == tau}, key the logit's bits in order; tau is found with histograms of
 // counts and masses, first over the linear buckets, then inside the bucket
 // that holds the border over the key's bits, 11 at a time, and the kept
-// weights are summed and searched as those of an unfiltered row.
+// weights are summed and searched as those of an unfiltered row.  64 rows of
+// 152064 bf16 with top_k = 50 take 23 us at T = 0.7 (greedy: 21), but 135 at T
+// = 0.3 and 247 at 0.1: where the k-th largest weighs less than 2^-63 no bucket
+// bounds it and the whole row is listed.
 #include "klp_launch.h"
 #include "klp_rows.h"
 
