@@ -165,22 +165,25 @@ struct Workspace {
 // would run after the caching allocator is gone.
 std::mutex g_ws_mutex;
 std::list<Workspace>& g_ws = *new std::list<Workspace>();  // most recently used first
+// klp_fwd_top's, which leaves other words zero than klp_fwd does.
+std::list<Workspace>& g_top_ws = *new std::list<Workspace>();
 constexpr size_t kWorkspacesKept = 16;
 
-at::Tensor workspace(int device, hipStream_t stream, size_t nbytes) {
+at::Tensor workspace(int device, hipStream_t stream, size_t nbytes,
+                     std::list<Workspace>& kept = g_ws) {
     if (nbytes == 0) return at::Tensor();
     const auto opts = at::TensorOptions().dtype(at::kByte).device(at::kCUDA, device);
     std::lock_guard<std::mutex> lock(g_ws_mutex);
-    for (auto it = g_ws.begin(); it != g_ws.end(); ++it) {
+    for (auto it = kept.begin(); it != kept.end(); ++it) {
         if (it->device != device || it->stream != stream) continue;
         if (static_cast<size_t>(it->buf.numel()) < nbytes)
             it->buf = at::zeros({static_cast<int64_t>(nbytes)}, opts);
-        g_ws.splice(g_ws.begin(), g_ws, it);
-        return g_ws.front().buf;
+        kept.splice(kept.begin(), kept, it);
+        return kept.front().buf;
     }
-    g_ws.push_front(Workspace{device, stream, at::zeros({static_cast<int64_t>(nbytes)}, opts)});
-    while (g_ws.size() > kWorkspacesKept) g_ws.pop_back();
-    return g_ws.front().buf;
+    kept.push_front(Workspace{device, stream, at::zeros({static_cast<int64_t>(nbytes)}, opts)});
+    while (kept.size() > kWorkspacesKept) kept.pop_back();
+    return kept.front().buf;
 }
 
 // ---------------------------------------------------------------------------
@@ -1013,6 +1016,123 @@ std::vector<at::Tensor> sample(const at::Tensor& logits, const at::Tensor& unifo
     return {tokens, logp, sample_logp};
 }
 
+// ---------------------------------------------------------------------------
+// Log-probabilities with alternatives, and the norms around a block: the
+// autograd functions of kernel_opt.top and kernel_opt.block after their argument
+// checks, which stay in Python.
+// ---------------------------------------------------------------------------
+void refuse_captured_backward(hipStream_t stream) {
+    hipStreamCaptureStatus status = hipStreamCaptureStatusNone;
+    if (hipStreamIsCapturing(stream, &status) != hipSuccess ||
+        status != hipStreamCaptureStatusNone)
+        throw std::runtime_error(
+            "kernel_opt: this backward belongs to a forward run outside graph capture and "
+            "cannot itself be captured; capture the forward with it");
+}
+std::optional<at::Tensor> optional_tensor(const at::Tensor& t) {
+    return t.defined() ? std::optional<at::Tensor>(t) : std::nullopt;
+}
+
+// kernel_opt._order: a gradient as a function of what it depends on, whose own
+// gradient is refused.
+class Once : public torch::autograd::Function<Once> {
+   public:
+    static variable_list forward(AutogradContext* ctx, const at::Tensor& grad,
+                                 const std::string& name, const std::optional<at::Tensor>&,
+                                 const std::optional<at::Tensor>&,
+                                 const std::optional<at::Tensor>&,
+                                 const std::optional<at::Tensor>&,
+                                 const std::optional<at::Tensor>&,
+                                 const std::optional<at::Tensor>&,
+                                 const std::optional<at::Tensor>&) {
+        ctx->saved_data["name"] = name;
+        return {grad};
+    }
+    static variable_list backward(AutogradContext* ctx, variable_list) {
+        throw std::runtime_error("kernel_opt: " + ctx->saved_data["name"].toStringRef() +
+                                 " has no second derivative");
+    }
+};
+void first_order(const char* name, std::vector<at::Tensor*> grads, const variable_list& of) {
+    if (!at::GradMode::is_enabled()) return;  // create_graph
+    std::array<std::optional<at::Tensor>, 7> o;
+    for (size_t i = 0; i < of.size() && i < o.size(); ++i) o[i] = optional_tensor(of[i]);
+    for (at::Tensor* g : grads)
+        if (g->defined())
+            *g = Once::apply(*g, std::string(name), o[0], o[1], o[2], o[3], o[4], o[5], o[6])[0];
+}
+
+class FusedTopLogprobs : public torch::autograd::Function<FusedTopLogprobs> {
+   public:
+    static variable_list forward(AutogradContext* ctx, const at::Tensor& logits,
+                                 const at::Tensor& targets, int64_t k, double temperature) {
+        const int dev = logits.get_device();
+        const c10::hip::HIPGuard guard(static_cast<c10::DeviceIndex>(dev));
+        hipStream_t stream = current_stream(dev);
+        const at::Tensor t = targets.contiguous();
+        const auto L = row_layout(logits);
+        require(L.has_value(), "logits must be contiguous");
+        std::vector<int64_t> shape = t.sizes().vec();
+        const auto f32 = t.options().dtype(at::kFloat);
+        at::Tensor logprob = at::empty(shape, f32), entropy = at::empty(shape, f32),
+                   lse = at::empty(shape, f32), rank = at::empty(shape, t.options());
+        shape.push_back(k);
+        at::Tensor ids = at::empty(shape, t.options()), top = at::empty(shape, f32);
+        const int code = dtype_code(logits.scalar_type());
+        const int64_t n = t.numel(), v = logits.size(-1);
+        const at::Tensor ws = workspace(
+            dev, stream, klp_fwd_top_workspace_bytes(code, n, v, static_cast<int>(k)), g_top_ws);
+        check_status(klp_fwd_top(
+            logits.data_ptr(), code, n, v, (*L)[0], (*L)[1], (*L)[2], t.data_ptr<int64_t>(),
+            static_cast<float>(temperature), static_cast<int>(k), out_ptr(logprob),
+            out_ptr(entropy), out_ptr(lse), rank.data_ptr<int64_t>(), ids.data_ptr<int64_t>(),
+            out_ptr(top), data_or_null(ws), ws.defined() ? static_cast<size_t>(ws.numel()) : 0,
+            stream));
+        ctx->save_for_backward({logits, t, entropy, lse, ids});
+        ctx->saved_data["temperature"] = temperature;
+        ctx->mark_non_differentiable({rank, ids});
+        ctx->set_materialize_grads(false);
+        return {logprob, entropy, lse, rank, ids, top};
+    }
+
+    static variable_list backward(AutogradContext* ctx, variable_list grads) {
+        variable_list none(4);
+        if (!ctx->needs_input_grad(0)) return none;
+        auto prep = [](const at::Tensor& g) {
+            return g.defined() ? g.to(at::kFloat).contiguous() : at::Tensor();
+        };
+        const at::Tensor g_logp = prep(grads[0]), g_ent = prep(grads[1]), g_lse = prep(grads[2]),
+                         g_top = prep(grads[5]);
+        if (!(g_logp.defined() || g_ent.defined() || g_lse.defined() || g_top.defined()))
+            return none;
+        const auto saved = ctx->get_saved_variables();
+        const at::Tensor &logits = saved[0], &t = saved[1], &entropy = saved[2], &lse = saved[3],
+                         &ids = saved[4];
+        const int dev = logits.get_device();
+        const c10::hip::HIPGuard guard(static_cast<c10::DeviceIndex>(dev));
+        hipStream_t stream = current_stream(dev);
+        refuse_captured_backward(stream);
+        const auto L = row_layout(logits);
+        require(L.has_value(), "logits must be contiguous");
+        at::Tensor d = at::empty(logits.sizes(), logits.options());
+        check_status(klp_bwd_top(
+            logits.data_ptr(), dtype_code(logits.scalar_type()), t.numel(), logits.size(-1),
+            (*L)[0], (*L)[1], (*L)[2], t.data_ptr<int64_t>(),
+            static_cast<float>(ctx->saved_data["temperature"].toDouble()),
+            static_cast<int>(ids.size(-1)), ids.data_ptr<int64_t>(), fptr(lse), fptr(entropy),
+            fptr(g_logp), fptr(g_ent), fptr(g_lse), fptr(g_top), d.data_ptr(), stream));
+        first_order("fused_top_logprobs", {&d}, {logits, g_logp, g_ent, g_lse, g_top});
+        none[0] = d;
+        return none;
+    }
+};
+
+std::vector<at::Tensor> top_logprobs(const at::Tensor& logits, const at::Tensor& targets,
+                                     int64_t k, double temperature) {
+    decline_under_capture(logits.get_device());
+    return FusedTopLogprobs::apply(logits, targets, k, temperature);
+}
+
 }  // namespace
 
 PYBIND11_MODULE(klp_torch, m) {
@@ -1095,6 +1215,8 @@ PYBIND11_MODULE(klp_torch, m) {
     m.def("quantize_fp8", &quantize_fp8, pybind11::arg("x"), pybind11::arg("block_rows"));
     m.def("fp8_linear", &fp8_linear, pybind11::arg("x"), pybind11::arg("x_scale"),
           pybind11::arg("weight"), pybind11::arg("weight_scale"), pybind11::arg("out_dtype"));
+    m.def("top_logprobs", &top_logprobs, pybind11::arg("logits"), pybind11::arg("targets"),
+          pybind11::arg("k"), pybind11::arg("temperature"));
     m.def("sample", &sample, pybind11::arg("logits"), pybind11::arg("uniform"), pybind11::arg("t"),
           pybind11::arg("ts"), pybind11::arg("k"), pybind11::arg("ks"), pybind11::arg("p"),
           pybind11::arg("ps"), pybind11::arg("m"), pybind11::arg("ms"));

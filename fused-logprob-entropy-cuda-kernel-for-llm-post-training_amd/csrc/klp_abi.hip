@@ -94,6 +94,8 @@ int check_rows(const void* logits, int dtype, int64_t n_rows, int64_t vocab, int
     return KLP_OK;
 }
 
+int check_threads(int64_t groups, int64_t threads, const char* what);
+
 int check_f32(const float* p, const char* name) {
     if (p == nullptr) return fail(KLP_EINVAL, "%s must be non-null", name);
     if (!aligned(p, 4)) return fail(KLP_EINVAL, "%s is not 4-byte aligned", name);
@@ -378,7 +380,8 @@ int fwd_impl(const void* logits, int dtype, int64_t n_rows, int64_t vocab, int64
 int bwd_impl(const void* logits, int dtype, int64_t n_rows, int64_t vocab, int64_t rows_inner,
              int64_t stride_outer, int64_t stride_inner, const int64_t* targets, const float* lse,
              const float* entropy, const float* g_logp, const float* g_ent, const float* g_lse,
-             void* d_logits, klp::BwdConfig cfg, float scale, void* stream) {
+             void* d_logits, klp::BwdConfig cfg, float scale, void* stream,
+             const int64_t* top_ids = nullptr, const float* g_top = nullptr, int k = 0) {
     int rc = check_rows(logits, dtype, n_rows, vocab, rows_inner, stride_outer, stride_inner,
                         targets);
     if (rc != KLP_OK) return rc;
@@ -416,9 +419,51 @@ int bwd_impl(const void* logits, int dtype, int64_t n_rows, int64_t vocab, int64
     p.d_logits = d_logits;
     p.splits = cfg.splits;
     p.scale = scale;
+    p.top_ids = top_ids;
+    p.g_top = g_top;
+    p.k = k;
     if (injected_failure("backward")) return KLP_ELAUNCH;
     return after_launch(klp::launch_bwd(dtype, p, cfg, static_cast<hipStream_t>(stream)),
                         "backward");
+}
+
+// Launch shape of the log-probabilities with alternatives: workgroups of 8
+// waves for rows of at least 16 vectors a thread, else of 4 (a thread's
+// maximum is one of the k that bound the row's, so that 4 waves are the least
+// for k = 256); few long rows in pieces, as the forward's, whose lists
+// together hold at most kTopMergeKeys.
+struct TopConfig {
+    int waves;
+    int splits;
+};
+TopConfig top_config(int dtype, int64_t n_rows, int64_t vocab, int k) {
+    TopConfig c{4, 1};
+    const int64_t nvec = body_vectors(dtype, vocab);
+    if (nvec >= int64_t{8} * 64 * 8) c.waves = 8;
+    int s = 1;
+    while (s < kMaxSplits && n_rows * 2 * s <= kFwdSplitGrid &&
+           nvec >= int64_t{3} * c.waves * 64 * 2 * s && 2 * s * k <= klp::kTopMergeKeys)
+        s *= 2;
+    c.splits = s;
+    return c;
+}
+// Arrival counters, a fixed region so that no call's states lie where another's
+// counters do; then the pieces' states, then their keys.
+constexpr size_t kTopCounterBytes = kFwdSplitGrid * sizeof(unsigned int);
+size_t top_state_bytes(int64_t n_rows, const TopConfig& c) {
+    return static_cast<size_t>(n_rows) * c.splits * 4 * sizeof(float);
+}
+size_t top_workspace(int64_t n_rows, int k, const TopConfig& c) {
+    if (c.splits == 1) return 0;
+    return kTopCounterBytes + top_state_bytes(n_rows, c) +
+           static_cast<size_t>(n_rows) * c.splits * k * sizeof(unsigned long long);
+}
+
+int check_top(int64_t vocab, int64_t n_rows, int k) {
+    if (k < 1 || k > klp::kTopMax)
+        return fail(KLP_EINVAL, "k must be in [1, %d], got %d", klp::kTopMax, k);
+    if (vocab > klp::kTopMaxVocab) return fail(KLP_EINVAL, "vocab above 2^26 is not supported");
+    return check_threads(n_rows, 512, "rows");
 }
 
 size_t grpo_workspace_bytes(int64_t n_seqs) {
@@ -1759,6 +1804,88 @@ int klp_fp8_linear(const uint8_t* x, int64_t ld_x, const float* x_scales, const 
     if (injected_failure("fp8 linear")) return KLP_ELAUNCH;
     return after_launch(klp::launch_fp8_linear(out_dtype, p, static_cast<hipStream_t>(stream)),
                         "fp8 linear");
+}
+
+size_t klp_fwd_top_workspace_bytes(int dtype, int64_t n_rows, int64_t vocab, int k) {
+    if ((dtype != KLP_BF16 && dtype != KLP_FP16 && dtype != KLP_FP32) || n_rows < 1 || vocab < 1 ||
+        k < 1 || k > klp::kTopMax)
+        return 0;
+    return top_workspace(n_rows, k, top_config(dtype, n_rows, vocab, k));
+}
+
+int klp_fwd_top(const void* logits, int dtype, int64_t n_rows, int64_t vocab, int64_t rows_inner,
+                int64_t stride_outer, int64_t stride_inner, const int64_t* targets,
+                float temperature, int k, float* logprob, float* entropy, float* lse,
+                int64_t* rank, int64_t* top_ids, float* top_logprob, void* workspace,
+                size_t workspace_bytes, void* stream) {
+    int rc = check_rows(logits, dtype, n_rows, vocab, rows_inner, stride_outer, stride_inner,
+                        targets);
+    if (rc != KLP_OK) return rc;
+    klp::TopParams p{};
+    if (!scale_from_temperature(temperature, &p.inv_t)) return KLP_EINVAL;
+    if ((rc = check_top(vocab, n_rows, k)) != KLP_OK) return rc;
+    if (n_rows == 0) return ok();
+    if ((rc = check_f32(logprob, "logprob")) != KLP_OK) return rc;
+    if ((rc = check_f32(entropy, "entropy")) != KLP_OK) return rc;
+    if ((rc = check_f32(lse, "lse")) != KLP_OK) return rc;
+    if ((rc = check_f32(top_logprob, "top_logprob")) != KLP_OK) return rc;
+    if (rank == nullptr || !aligned(rank, 8) || top_ids == nullptr || !aligned(top_ids, 8))
+        return fail(KLP_EINVAL, "rank and top_ids must be non-null and 8-byte aligned");
+    TopConfig c = top_config(dtype, n_rows, vocab, k);
+    if (c.splits > 1) {
+        const size_t need = top_workspace(n_rows, k, c);
+        if (workspace == nullptr) {
+            c.splits = 1;  // no workspace: one workgroup per row
+        } else if (workspace_bytes < need || !aligned(workspace, 16)) {
+            return fail(KLP_EWORKSPACE,
+                        "workspace too small or not 16-byte aligned: have %zu bytes, need %zu",
+                        workspace_bytes, need);
+        }
+    }
+    p.logits = logits;
+    p.rm = klp::RowMap{rows_inner, stride_outer, stride_inner};
+    p.n_rows = n_rows;
+    p.vocab = vocab;
+    p.targets = targets;
+    p.k = k;
+    p.factor = static_cast<float>(1.4426950408889634074 / static_cast<double>(temperature));
+    p.waves = c.waves;
+    p.splits = c.splits;
+    if (c.splits > 1) {
+        unsigned char* w = static_cast<unsigned char*>(workspace);
+        p.counters = reinterpret_cast<unsigned int*>(w);
+        p.states = reinterpret_cast<float*>(w + kTopCounterBytes);
+        p.keys = reinterpret_cast<unsigned long long*>(w + kTopCounterBytes +
+                                                       top_state_bytes(n_rows, c));
+    }
+    p.logprob = logprob;
+    p.entropy = entropy;
+    p.lse = lse;
+    p.rank = rank;
+    p.top_ids = top_ids;
+    p.top_logprob = top_logprob;
+    if (injected_failure("top log-probabilities")) return KLP_ELAUNCH;
+    return after_launch(klp::launch_top(dtype, p, static_cast<hipStream_t>(stream)),
+                        "top log-probabilities");
+}
+
+int klp_bwd_top(const void* logits, int dtype, int64_t n_rows, int64_t vocab, int64_t rows_inner,
+                int64_t stride_outer, int64_t stride_inner, const int64_t* targets,
+                float temperature, int k, const int64_t* top_ids, const float* lse,
+                const float* entropy, const float* g_logp, const float* g_ent,
+                const float* g_lse, const float* g_top, void* d_logits, void* stream) {
+    float scale;
+    if (!scale_from_temperature(temperature, &scale)) return KLP_EINVAL;
+    int rc = check_top(vocab, n_rows, k);
+    if (rc != KLP_OK) return rc;
+    if (n_rows > 0 && g_top != nullptr &&
+        (!aligned(g_top, 4) || top_ids == nullptr || !aligned(top_ids, 8)))
+        return fail(KLP_EINVAL, "g_top must be 4-byte aligned, and top_ids with it non-null and "
+                                "8-byte aligned");
+    return bwd_impl(logits, dtype, n_rows, vocab, rows_inner, stride_outer, stride_inner, targets,
+                    lse, entropy, g_logp, g_ent, g_lse, d_logits,
+                    default_bwd_config(dtype, n_rows, vocab), scale, stream,
+                    g_top != nullptr ? top_ids : nullptr, g_top, k);
 }
 
 int klp_sample(const void* logits, int dtype, int64_t n_rows, int64_t vocab, int64_t rows_inner,

@@ -15,6 +15,12 @@
 //
 // With a temperature T (BwdParams::scale = 1/T != 1) the logits are scaled by
 // 1/T on load, as in the forward, and the gradient is multiplied by 1/T.
+//
+// With alternatives (kTop: klp_bwd_top) each of their log-probabilities adds
+//   g_top[j] ((v == id_j) - p)
+// so that c0 loses the sum of g_top, and a workgroup, its vectors written and
+// acknowledged, writes its piece's few elements id_j once more, with the whole
+// sum rounded once.
 #include "klp_device.h"
 #include "klp_launch.h"
 
@@ -99,7 +105,42 @@ __device__ __forceinline__ void bwd_piece(const BwdParams& p, const u32x4* vin, 
 // 2001 11.7 / 10.0; fp32 4096 x 1001 9.0 / 9.4, 4096 x 1501 11.2 / 10.5.
 constexpr int64_t kBwdElementRow = 1024;
 
-template <int DT, int WAVES, int U, bool kNtStore, bool kScaled>
+// Sum of the row's gradients of its alternatives (those that exist), every
+// wave for itself.
+__device__ __forceinline__ float top_sum(const BwdParams& p, int64_t row) {
+    const int64_t* ids = p.top_ids + row * p.k;
+    const float* g = p.g_top + row * p.k;
+    float s = 0.0f;
+    for (int j = threadIdx.x & 63; j < p.k; j += 64) s += ids[j] >= 0 ? g[j] : 0.0f;
+    return xrow_sum(row_sum16(s));
+}
+
+// The gradients of the alternatives that `mine` says are this workgroup's,
+// over what its vectors wrote there.
+template <int DT, int WAVES, bool kScaled, typename F>
+__device__ __forceinline__ void put_top(const BwdParams& p, int64_t row,
+                                        const typename Traits<DT>::elem* rp,
+                                        typename Traits<DT>::elem* dp, int64_t tgt,
+                                        const RowGrad& g, F mine) {
+    // Two stores to one address by two waves: the first has to be done.
+    __atomic_signal_fence(__ATOMIC_SEQ_CST);
+    __builtin_amdgcn_s_waitcnt(kWaitVmcnt0);
+    __atomic_signal_fence(__ATOMIC_SEQ_CST);
+    __syncthreads();
+    for (int j = threadIdx.x; j < p.k; j += WAVES * 64) {
+        const int64_t v = p.top_ids[row * p.k + j];
+        if (v < 0 || v >= p.vocab || !mine(v)) continue;
+        float x = to_f32<DT>(rp[v]);
+        if (kScaled) x *= p.scale;
+        float d = g.lse >= 0.0f ? grad_elem<DT, true>(x, g) : grad_elem<DT, false>(x, g);
+        if (v == tgt) d += g.g_logp;
+        d += p.g_top[row * p.k + j];
+        if (kScaled) d *= p.scale;
+        dp[v] = from_f32<DT>(d);
+    }
+}
+
+template <int DT, int WAVES, int U, bool kNtStore, bool kScaled, bool kTop>
 __global__ __launch_bounds__(WAVES * 64) void klp_bwd_kernel(BwdParams p) {
     typedef typename Traits<DT>::elem elem;
     constexpr int EPV = Traits<DT>::kPerVec;
@@ -114,8 +155,9 @@ __global__ __launch_bounds__(WAVES * 64) void klp_bwd_kernel(BwdParams p) {
     elem* dp = static_cast<elem*>(p.d_logits) + row * vocab;
     const int64_t tgt = p.targets[row];
 
-    const RowGrad g = row_grad(p.lse[row], p.entropy[row], p.g_logp ? p.g_logp[row] : 0.0f,
-                               p.g_ent ? p.g_ent[row] : 0.0f, p.g_lse ? p.g_lse[row] : 0.0f);
+    RowGrad g = row_grad(p.lse[row], p.entropy[row], p.g_logp ? p.g_logp[row] : 0.0f,
+                         p.g_ent ? p.g_ent[row] : 0.0f, p.g_lse ? p.g_lse[row] : 0.0f);
+    if constexpr (kTop) g.c0 -= top_sum(p, row);
 
     const uintptr_t in_addr = reinterpret_cast<uintptr_t>(rp);
     const uintptr_t out_addr = reinterpret_cast<uintptr_t>(dp);
@@ -131,6 +173,9 @@ __global__ __launch_bounds__(WAVES * 64) void klp_bwd_kernel(BwdParams p) {
             if (kScaled) d *= p.scale;
             dp[v] = from_f32<DT>(d);
         }
+        if constexpr (kTop)
+            put_top<DT, WAVES, kScaled>(p, row, rp, dp, tgt, g,
+                                        [&](int64_t v) { return v >= b && v < e; });
         return;
     }
 
@@ -183,15 +228,20 @@ __global__ __launch_bounds__(WAVES * 64) void klp_bwd_kernel(BwdParams p) {
     else
         bwd_piece<DT, WAVES, U, kNtStore, kScaled, true>(p, vin, vout, vb, ve, t_vec,
                                                          t_lane_elem, g);
+    if constexpr (kTop)
+        put_top<DT, WAVES, kScaled>(p, row, rp, dp, tgt, g, [&](int64_t v) {
+            return v < head || v >= tail_begin ? split == 0
+                                               : v >= head + vb * EPV && v < head + ve * EPV;
+        });
 }
 
-template <int DT, int WAVES, int U, bool kNtStore>
+template <int DT, int WAVES, int U, bool kNtStore, bool kTop>
 static hipError_t launch_bwd_t(const BwdParams& p, hipStream_t stream) {
     if (p.scale != 1.0f)
-        return launch_kernel(klp_bwd_kernel<DT, WAVES, U, kNtStore, true>,
+        return launch_kernel(klp_bwd_kernel<DT, WAVES, U, kNtStore, true, kTop>,
                              dim3(static_cast<unsigned>(p.n_rows * p.splits)),
                              dim3(WAVES * 64), stream, p);
-    return launch_kernel(klp_bwd_kernel<DT, WAVES, U, kNtStore, false>,
+    return launch_kernel(klp_bwd_kernel<DT, WAVES, U, kNtStore, false, kTop>,
                          dim3(static_cast<unsigned>(p.n_rows * p.splits)), dim3(WAVES * 64),
                          stream, p);
 }
@@ -199,10 +249,21 @@ static hipError_t launch_bwd_t(const BwdParams& p, hipStream_t stream) {
 template <int DT>
 static hipError_t launch_bwd_dt(const BwdParams& p, const BwdConfig& c, hipStream_t stream) {
     const bool nt = (c.flags & kFlagNtStore) != 0;
+    // Alternatives come with the default shapes only.
+    if (p.top_ids != nullptr) {
+#define KLP_BWD_TOP_CASE(W)                                                    \
+    if (c.waves == W && c.unroll == 2 && nt)                                   \
+        return launch_bwd_t<DT, W, 2, true, true>(p, stream);
+        KLP_BWD_TOP_CASE(4)
+        KLP_BWD_TOP_CASE(8)
+        KLP_BWD_TOP_CASE(16)
+#undef KLP_BWD_TOP_CASE
+        return hipErrorInvalidValue;
+    }
 #define KLP_BWD_CASE(W, U)                                                     \
     if (c.waves == W && c.unroll == U)                                         \
-        return nt ? launch_bwd_t<DT, W, U, true>(p, stream)                \
-                  : launch_bwd_t<DT, W, U, false>(p, stream);
+        return nt ? launch_bwd_t<DT, W, U, true, false>(p, stream)         \
+                  : launch_bwd_t<DT, W, U, false, false>(p, stream);
     KLP_BWD_CASE(4, 2)
     KLP_BWD_CASE(4, 4)
     KLP_BWD_CASE(8, 2)

@@ -84,6 +84,11 @@ struct BwdParams {
     void* d_logits;       // dense [n_rows, vocab]
     int splits;
     float scale;          // 1 / temperature (gradient is w.r.t. the unscaled logits)
+    // klp_bwd_top: the alternatives and the gradients of their
+    // log-probabilities, [n_rows, k]; null for every other call.
+    const int64_t* top_ids;
+    const float* g_top;
+    int k;
 };
 
 // Launch shape: `waves` wave64s per workgroup, `unroll` 16-byte loads per
@@ -380,6 +385,36 @@ struct SampleParams {
     float* sample_logp;         // [n_rows]
 };
 hipError_t launch_sample(int dtype, const SampleParams& p, hipStream_t stream);
+
+// Log-probabilities with alternatives (klp_top.hip).
+constexpr int64_t kTopMaxVocab = int64_t{1} << 26;
+constexpr int kTopMax = 256;            // alternatives of a row at most
+constexpr int kTopMergeKeys = 4096;     // splits * k at most
+struct TopParams {
+    const void* logits;
+    RowMap rm;
+    int64_t n_rows;
+    int64_t vocab;
+    const int64_t* targets;
+    int k;
+    float factor;          // log2(e) / temperature
+    float inv_t;           // 1 / temperature
+    int waves;             // of a workgroup: 4 or 8
+    int splits;            // workgroups of a row, at most 64
+    // Pieces (splits > 1): arrival counters [n_rows], zero before the launch
+    // and left zero by it; states [n_rows, splits] float4 and keys [n_rows,
+    // splits, k] of any contents.
+    unsigned int* counters;
+    float* states;
+    unsigned long long* keys;
+    float* logprob;
+    float* entropy;
+    float* lse;
+    int64_t* rank;
+    int64_t* top_ids;      // [n_rows, k]
+    float* top_logprob;    // [n_rows, k]
+};
+hipError_t launch_top(int dtype, const TopParams& p, hipStream_t stream);
 
 // Calibration kernels (klp_ceiling.hip): rows of `row_bytes` (a multiple of
 // 16) at `src` (and `dst`), 16-byte aligned and contiguous; `splits`

@@ -27,6 +27,7 @@ from .norm import (  # noqa: F401
 )
 from .fp8 import fp8_linear, quantize_fp8  # noqa: F401
 from .sample import fused_sample  # noqa: F401
+from .top import fused_top_logprobs  # noqa: F401
 from .rollout import sample_hidden, score_hidden  # noqa: F401
 
 

@@ -103,6 +103,9 @@ SIGNATURES = {
                               _vp]),
     "klp_sample": (_i32, _ROWS + [_vp, ctypes.c_float, _vp, ctypes.c_int32, _vp, ctypes.c_float,
                                   _vp, ctypes.c_float, _vp, _vp, _vp, _vp, _vp]),
+    "klp_fwd_top_workspace_bytes": (_sz, [_i32, _i64, _i64, _i32]),
+    "klp_fwd_top": (_i32, _ROWS + [_vp, ctypes.c_float, _i32] + [_vp] * 7 + [_sz, _vp]),
+    "klp_bwd_top": (_i32, _ROWS + [_vp, ctypes.c_float, _i32] + [_vp] * 9),
     # include/kernel_opt_hip_tuning.h
     "klp_grpo_step_persistent_min_rows": (_i64, [_i32, _i64, _i32]),
     "klp_fwd_workspace_bytes_ex": (_sz, [_i64, _i32]),

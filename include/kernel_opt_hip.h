@@ -639,6 +639,48 @@ int klp_sample(const void* logits, int dtype, int64_t n_rows, int64_t vocab, int
                int64_t* tokens, float* logp, float* sample_logp, void* stream);
 
 /*
+ * Log-probabilities of given tokens with alternatives, in one read of the
+ * logits (row addressing and targets as above).  With y = x / T and the row
+ * ordered by falling x (equal ones by index, -0 equal to +0):
+ *   logprob, entropy, lse   as klp_fwd_temp's,
+ *   rank                    tokens before the target in the order, -1 for a
+ *                           target outside [0, vocab),
+ *   top_ids, top_logprob    [n_rows, k]: the order's first k tokens, with
+ *                           y - lse.  -inf logits are not listed: the places
+ *                           left over hold -1 and -inf.
+ * Log-probabilities are (x - max) / T - ln sum, differences that keep their
+ * precision next to 0 (klp_fwd's are x / T - lse), and the same for the same
+ * logits wherever the row lies and whatever the other rows are, but for the
+ * order of float32 sums.  A row with a NaN or +inf logit has rank -1, top_ids
+ * -1 and NaN otherwise; one of -inf logits lse -inf, logprob and entropy NaN.
+ * k in [1, 256], vocab <= 2^26, n_rows below 2^23 (KLP_EINVAL).
+ *
+ * The workspace (klp_fwd_top_workspace_bytes; 0 for calls that need none) is
+ * for few rows, cut into pieces; NULL leaves them whole.  Its first 1024 bytes
+ * must be zero before its first use and every call leaves them zero (other
+ * entry points do not: it is not to be shared with them); calls that share it
+ * must be ordered on one stream.
+ */
+size_t klp_fwd_top_workspace_bytes(int dtype, int64_t n_rows, int64_t vocab, int k);
+int klp_fwd_top(const void* logits, int dtype, int64_t n_rows, int64_t vocab, int64_t rows_inner,
+                int64_t stride_outer, int64_t stride_inner, const int64_t* targets,
+                float temperature, int k, float* logprob, float* entropy, float* lse,
+                int64_t* rank, int64_t* top_ids, float* top_logprob, void* workspace,
+                size_t workspace_bytes, void* stream);
+
+/*
+ * Its backward, from the saved top_ids, lse and entropy: klp_bwd_temp's
+ * gradient with, for each alternative, g_top[j] ([v == top_ids[j]] - p_v) / T
+ * (top_ids of -1 have no gradient; the ids of a row differ).  Null gradients
+ * count as zeros; with g_top NULL top_ids is not read.
+ */
+int klp_bwd_top(const void* logits, int dtype, int64_t n_rows, int64_t vocab, int64_t rows_inner,
+                int64_t stride_outer, int64_t stride_inner, const int64_t* targets,
+                float temperature, int k, const int64_t* top_ids, const float* lse,
+                const float* entropy, const float* g_logp, const float* g_ent,
+                const float* g_lse, const float* g_top, void* d_logits, void* stream);
+
+/*
  * Test hook with no counterpart in the reference: the next `count` compute
  * calls on the calling thread return KLP_ELAUNCH without launching anything,
  * as if hipGetLastError() had reported a failure.  Lets the error path be
