@@ -18,13 +18,26 @@
 //
 // With alternatives (kTop: klp_bwd_top) each of their log-probabilities adds
 //   g_top[j] ((v == id_j) - p)
-// so that c0 loses the sum of g_top, and a workgroup, its vectors written and
-// acknowledged, writes its piece's few elements id_j once more, with the whole
-// sum rounded once.
+// so that c0 loses the sum of g_top, and the few id_j that lie in a
+// workgroup's piece are listed in LDS while its first vectors are on their
+// way; every vector looks the list through before it is rounded.
 #include "klp_device.h"
 #include "klp_launch.h"
 
 namespace klp {
+
+// The alternatives of a workgroup's piece: their vector of the piece (-1: an
+// element of the row's edges), their element of it (of the row), and their
+// gradient.
+struct TopHits {
+    int n;
+    int vec[kTopMax];
+    int elem[kTopMax];
+    float grad[kTopMax];
+    float sum[16];  // of the waves' g_top
+};
+template <bool kTop> struct TopOf {};
+template <> struct TopOf<true> { TopHits h; };
 
 // A 16-byte vector at the alignment of the shortest element.
 typedef u32x4 u32x4_elem_aligned __attribute__((aligned(2)));
@@ -32,10 +45,12 @@ typedef u32x4 u32x4_elem_aligned __attribute__((aligned(2)));
 // The piece's 16-byte vectors [vb, ve) (the body of klp_bwd_kernel).  `vout`
 // is 16-byte aligned; `vin` is too, or, with kInAligned false, only as an
 // element is.
-template <int DT, int WAVES, int U, bool kNtStore, bool kScaled, bool kInAligned, bool kLseNonNeg>
+template <int DT, int WAVES, int U, bool kNtStore, bool kScaled, bool kInAligned, bool kLseNonNeg,
+          bool kTop>
 __device__ __forceinline__ void bwd_vectors(const BwdParams& p, const u32x4* vin, u32x4* vout,
                                             int64_t vb, int64_t ve, int64_t t_vec,
-                                            int t_lane_elem, const RowGrad& g) {
+                                            int t_lane_elem, const RowGrad& g,
+                                            const TopOf<kTop>& top) {
     constexpr int NTHREADS = WAVES * 64;
     constexpr int EPV = Traits<DT>::kPerVec;
     const int tid = threadIdx.x;
@@ -73,6 +88,15 @@ __device__ __forceinline__ void bwd_vectors(const BwdParams& p, const u32x4* vin
                     for (int j = 0; j < EPV; ++j)
                         if (j == t_lane_elem) x[j] += g.g_logp;
                 }
+                if constexpr (kTop) {
+                    for (int h = 0; h < top.h.n; ++h) {
+                        if (top.h.vec[h] != static_cast<int>(idx - vb)) continue;
+                        const int e = top.h.elem[h];
+#pragma unroll
+                        for (int j = 0; j < EPV; ++j)
+                            if (j == e) x[j] += top.h.grad[h];
+                    }
+                }
                 if (kScaled) {
 #pragma unroll
                     for (int j = 0; j < EPV; ++j) x[j] *= p.scale;
@@ -86,16 +110,16 @@ __device__ __forceinline__ void bwd_vectors(const BwdParams& p, const u32x4* vin
 
 // fp32 rows take their Fast2Sum operand order from the sign of lse
 // (grad_one_fp32): one branch per row, outside the element loop.
-template <int DT, int WAVES, int U, bool kNtStore, bool kScaled, bool kInAligned>
+template <int DT, int WAVES, int U, bool kNtStore, bool kScaled, bool kInAligned, bool kTop>
 __device__ __forceinline__ void bwd_piece(const BwdParams& p, const u32x4* vin, u32x4* vout,
                                           int64_t vb, int64_t ve, int64_t t_vec, int t_lane_elem,
-                                          const RowGrad& g) {
+                                          const RowGrad& g, const TopOf<kTop>& top) {
     if (DT != kFP32 || g.lse >= 0.0f)
-        bwd_vectors<DT, WAVES, U, kNtStore, kScaled, kInAligned, true>(p, vin, vout, vb, ve,
-                                                                       t_vec, t_lane_elem, g);
+        bwd_vectors<DT, WAVES, U, kNtStore, kScaled, kInAligned, true, kTop>(
+            p, vin, vout, vb, ve, t_vec, t_lane_elem, g, top);
     else
-        bwd_vectors<DT, WAVES, U, kNtStore, kScaled, kInAligned, false>(p, vin, vout, vb, ve,
-                                                                        t_vec, t_lane_elem, g);
+        bwd_vectors<DT, WAVES, U, kNtStore, kScaled, kInAligned, false, kTop>(
+            p, vin, vout, vb, ve, t_vec, t_lane_elem, g, top);
 }
 
 // Rows of up to this many elements whose input and output sit at different
@@ -105,39 +129,43 @@ __device__ __forceinline__ void bwd_piece(const BwdParams& p, const u32x4* vin, 
 // 2001 11.7 / 10.0; fp32 4096 x 1001 9.0 / 9.4, 4096 x 1501 11.2 / 10.5.
 constexpr int64_t kBwdElementRow = 1024;
 
-// Sum of the row's gradients of its alternatives (those that exist), every
-// wave for itself.
-__device__ __forceinline__ float top_sum(const BwdParams& p, int64_t row) {
+// The alternatives that place(id, &vec, &elem) finds in the workgroup's part,
+// into `h`; returns the sum of the gradients of all that exist.  The ids of a
+// row differ, so that the list's order is of no consequence.
+template <int WAVES, typename F>
+__device__ __forceinline__ float list_top(const BwdParams& p, int64_t row, TopHits& h, F place) {
+    static_assert(WAVES <= 16, "the waves' sums");
     const int64_t* ids = p.top_ids + row * p.k;
-    const float* g = p.g_top + row * p.k;
-    float s = 0.0f;
-    for (int j = threadIdx.x & 63; j < p.k; j += 64) s += ids[j] >= 0 ? g[j] : 0.0f;
-    return xrow_sum(row_sum16(s));
-}
-
-// The gradients of the alternatives that `mine` says are this workgroup's,
-// over what its vectors wrote there.
-template <int DT, int WAVES, bool kScaled, typename F>
-__device__ __forceinline__ void put_top(const BwdParams& p, int64_t row,
-                                        const typename Traits<DT>::elem* rp,
-                                        typename Traits<DT>::elem* dp, int64_t tgt,
-                                        const RowGrad& g, F mine) {
-    // Two stores to one address by two waves: the first has to be done.
-    __atomic_signal_fence(__ATOMIC_SEQ_CST);
-    __builtin_amdgcn_s_waitcnt(kWaitVmcnt0);
-    __atomic_signal_fence(__ATOMIC_SEQ_CST);
+    const float* grads = p.g_top + row * p.k;
+    if (threadIdx.x == 0) h.n = 0;
     __syncthreads();
+    float s = 0.0f;
     for (int j = threadIdx.x; j < p.k; j += WAVES * 64) {
-        const int64_t v = p.top_ids[row * p.k + j];
-        if (v < 0 || v >= p.vocab || !mine(v)) continue;
-        float x = to_f32<DT>(rp[v]);
-        if (kScaled) x *= p.scale;
-        float d = g.lse >= 0.0f ? grad_elem<DT, true>(x, g) : grad_elem<DT, false>(x, g);
-        if (v == tgt) d += g.g_logp;
-        d += p.g_top[row * p.k + j];
-        if (kScaled) d *= p.scale;
-        dp[v] = from_f32<DT>(d);
+        const int64_t id = ids[j];
+        const float g = grads[j];
+        if (id < 0 || id >= p.vocab) continue;
+        s += g;
+        int vec, elem;
+        if (!place(id, &vec, &elem)) continue;
+        const int at = atomicAdd(&h.n, 1);
+        h.vec[at] = vec;
+        h.elem[at] = elem;
+        h.grad[at] = g;
     }
+    s = xrow_sum(row_sum16(s));
+    if ((threadIdx.x & 63) == 0) h.sum[threadIdx.x >> 6] = s;
+    __syncthreads();
+    s = h.sum[0];
+#pragma unroll
+    for (int w = 1; w < WAVES; ++w) s += h.sum[w];
+    return s;
+}
+// What an element of the edges (or of a row taken element by element) gets.
+__device__ __forceinline__ float top_at(const TopHits& h, int64_t v) {
+    float g = 0.0f;
+    for (int i = 0; i < h.n; ++i)
+        if (h.vec[i] < 0 && h.elem[i] == static_cast<int>(v)) g = h.grad[i];
+    return g;
 }
 
 template <int DT, int WAVES, int U, bool kNtStore, bool kScaled, bool kTop>
@@ -157,7 +185,7 @@ __global__ __launch_bounds__(WAVES * 64) void klp_bwd_kernel(BwdParams p) {
 
     RowGrad g = row_grad(p.lse[row], p.entropy[row], p.g_logp ? p.g_logp[row] : 0.0f,
                          p.g_ent ? p.g_ent[row] : 0.0f, p.g_lse ? p.g_lse[row] : 0.0f);
-    if constexpr (kTop) g.c0 -= top_sum(p, row);
+    __shared__ TopOf<kTop> top;
 
     const uintptr_t in_addr = reinterpret_cast<uintptr_t>(rp);
     const uintptr_t out_addr = reinterpret_cast<uintptr_t>(dp);
@@ -165,17 +193,21 @@ __global__ __launch_bounds__(WAVES * 64) void klp_bwd_kernel(BwdParams p) {
         const int64_t per = (vocab + p.splits - 1) / p.splits;
         const int64_t b = static_cast<int64_t>(split) * per;
         const int64_t e = b + per < vocab ? b + per : vocab;
+        if constexpr (kTop)
+            g.c0 -= list_top<WAVES>(p, row, top.h, [&](int64_t id, int* vec, int* elem) {
+                *vec = -1;
+                *elem = static_cast<int>(id);
+                return id >= b && id < e;
+            });
         for (int64_t v = b + tid; v < e; v += WAVES * 64) {
             float x = to_f32<DT>(rp[v]);
             if (kScaled) x *= p.scale;
             float d = g.lse >= 0.0f ? grad_elem<DT, true>(x, g) : grad_elem<DT, false>(x, g);
             if (v == tgt) d += g.g_logp;
+            if constexpr (kTop) d += top_at(top.h, v);
             if (kScaled) d *= p.scale;
             dp[v] = from_f32<DT>(d);
         }
-        if constexpr (kTop)
-            put_top<DT, WAVES, kScaled>(p, row, rp, dp, tgt, g,
-                                        [&](int64_t v) { return v >= b && v < e; });
         return;
     }
 
@@ -183,19 +215,6 @@ __global__ __launch_bounds__(WAVES * 64) void klp_bwd_kernel(BwdParams p) {
     if (head > vocab) head = vocab;
     const int64_t nvec = (vocab - head) / EPV;
     const int64_t tail_begin = head + nvec * EPV;
-
-    if (split == 0) {
-        const int64_t n_edge = head + (vocab - tail_begin);
-        if (tid < n_edge) {
-            const int64_t v = (tid < head) ? tid : tail_begin + (tid - head);
-            float x = to_f32<DT>(rp[v]);
-            if (kScaled) x *= p.scale;
-            float d = g.lse >= 0.0f ? grad_elem<DT, true>(x, g) : grad_elem<DT, false>(x, g);
-            if (v == tgt) d += g.g_logp;
-            if (kScaled) d *= p.scale;
-            dp[v] = from_f32<DT>(d);
-        }
-    }
 
     const u32x4* vin = reinterpret_cast<const u32x4*>(rp + head);
     u32x4* vout = reinterpret_cast<u32x4*>(dp + head);
@@ -209,6 +228,33 @@ __global__ __launch_bounds__(WAVES * 64) void klp_bwd_kernel(BwdParams p) {
     int64_t ve = vb + per;
     if (vb > nvec) vb = nvec;
     if (ve > nvec) ve = nvec;
+
+    if constexpr (kTop)
+        g.c0 -= list_top<WAVES>(p, row, top.h, [&](int64_t id, int* vec, int* elem) {
+            if (id < head || id >= tail_begin) {
+                *vec = -1;
+                *elem = static_cast<int>(id);
+                return split == 0;
+            }
+            const int64_t v = (id - head) / EPV;
+            *vec = static_cast<int>(v - vb);
+            *elem = static_cast<int>(id - head - v * EPV);
+            return v >= vb && v < ve;
+        });
+
+    if (split == 0) {
+        const int64_t n_edge = head + (vocab - tail_begin);
+        if (tid < n_edge) {
+            const int64_t v = (tid < head) ? tid : tail_begin + (tid - head);
+            float x = to_f32<DT>(rp[v]);
+            if (kScaled) x *= p.scale;
+            float d = g.lse >= 0.0f ? grad_elem<DT, true>(x, g) : grad_elem<DT, false>(x, g);
+            if (v == tgt) d += g.g_logp;
+            if constexpr (kTop) d += top_at(top.h, v);
+            if (kScaled) d *= p.scale;
+            dp[v] = from_f32<DT>(d);
+        }
+    }
 
     // Vector index holding the target's one-hot term (or -1).
     const int64_t t_rel = tgt - head;
@@ -224,15 +270,10 @@ __global__ __launch_bounds__(WAVES * 64) void klp_bwd_kernel(BwdParams p) {
     // 299 us (2.8 TB/s).
     if (((in_addr ^ out_addr) & 15u) != 0)
         bwd_piece<DT, WAVES, U, kNtStore, kScaled, false>(p, vin, vout, vb, ve, t_vec,
-                                                          t_lane_elem, g);
+                                                          t_lane_elem, g, top);
     else
         bwd_piece<DT, WAVES, U, kNtStore, kScaled, true>(p, vin, vout, vb, ve, t_vec,
-                                                         t_lane_elem, g);
-    if constexpr (kTop)
-        put_top<DT, WAVES, kScaled>(p, row, rp, dp, tgt, g, [&](int64_t v) {
-            return v < head || v >= tail_begin ? split == 0
-                                               : v >= head + vb * EPV && v < head + ve * EPV;
-        });
+                                                         t_lane_elem, g, top);
 }
 
 template <int DT, int WAVES, int U, bool kNtStore, bool kTop>

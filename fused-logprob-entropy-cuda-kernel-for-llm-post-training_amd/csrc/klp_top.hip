@@ -33,7 +33,6 @@ namespace klp {
 namespace {
 
 constexpr int kRecords = 16;           // a thread's records at most
-constexpr int kWork = 1024;            // records read again at most
 constexpr int kTopList = 1024;         // elements ranked at most (unsplit)
 constexpr unsigned long long kNoKey = 0;
 
@@ -47,6 +46,18 @@ __device__ __forceinline__ float from_ordered(uint32_t k) {
 }
 constexpr uint32_t kOrderedNegInf = 0x007FFFFFu;
 
+// A record: the upper half of a float that is its maximum (bf16 logits) or the
+// next one up.
+template <int DT>
+__device__ __forceinline__ uint16_t record_of(float x) {
+    uint32_t b = __float_as_uint(x);
+    if constexpr (DT != kBF16) b += ~(static_cast<int32_t>(b) >> 31) & 0xFFFF;
+    return static_cast<uint16_t>(b >> 16);
+}
+__device__ __forceinline__ float record_value(uint16_t r) {
+    return __uint_as_float(static_cast<uint32_t>(r) << 16);
+}
+
 // The order's key of element `index` with value x: larger comes first.
 __device__ __forceinline__ unsigned long long order_key(float x, uint32_t index) {
     return static_cast<unsigned long long>(ordered(x)) << 32 | (0xFFFFFFFFu - index);
@@ -58,23 +69,26 @@ __device__ __forceinline__ uint32_t key_index(unsigned long long k) {
     return 0xFFFFFFFFu - static_cast<uint32_t>(k);
 }
 
-// absorb() of klp_device.h with a base-2 factor: K values into the state, and
-// their maximum.  -inf values add nothing (their exponent is clamped).
+// A thread's sums: klp_device.h's Stat with its offset o = RN(m S).
+struct Sums {
+    float m, o, z, t;
+};
+__device__ __forceinline__ Sums sums_empty() { return Sums{-INFINITY, -INFINITY, 0.0f, 0.0f}; }
+
+// K values with maximum `top` into the sums, S = `factor`.  A -inf logit, and
+// one so large that its product with S overflows, leave a z or t that is not
+// finite (sums_lost): absorb_any then does the thread's part once more.
 template <int K>
-__device__ __forceinline__ float absorb_scaled(Stat& s, const float* x, float factor) {
-    float top = x[0];
-#pragma unroll
-    for (int j = 1; j < K; ++j) top = fmax_nan(top, x[j]);
-    const float c = fmax_nan(s.m, top);
-    const float o_raw = c * factor;
-    const float o = (c == -INFINITY) ? 0.0f : o_raw;
-    const float d = (s.m == -INFINITY) ? kNegBig : fmax_nan(s.m * factor - o_raw, kNegBig);
+__device__ __forceinline__ void absorb_fast(Sums& s, const float* x, float top, float factor) {
+    s.m = fmax_nan(s.m, top);
+    const float o = s.m * factor;
+    const float d = fmaxf(s.o - o, kNegBig);  // NaN where both are infinite: kNegBig
     const float sc = exp2_hw(d);
     float z0 = sc * s.z, z1 = 0.0f;
     float t0 = sc * fmaf(d, s.z, s.t), t1 = 0.0f;
 #pragma unroll
     for (int j = 0; j < K; ++j) {
-        const float u = fmax_nan(fmaf(x[j], factor, -o), kNegBig);
+        const float u = fmaf(x[j], factor, -o);
         const float e = exp2_hw(u);
         if (j & 1) {
             z1 += e;
@@ -84,24 +98,48 @@ __device__ __forceinline__ float absorb_scaled(Stat& s, const float* x, float fa
             t0 = fmaf(u, e, t0);
         }
     }
-    s.m = c;
+    s.o = o;
     s.z = z0 + z1;
     s.t = t0 + t1;
-    return top;
+}
+__device__ __forceinline__ bool sums_lost(const Sums& s) {
+    return !(s.z < INFINITY) || !(s.t > -INFINITY);
 }
 
-__device__ __forceinline__ void rescale_scaled(const Stat& s, float m, float factor, float& z,
-                                               float& t) {
-    const bool live = s.m != -INFINITY;
-    const float d = live ? s.m * factor - m * factor : 0.0f;
-    const float sc = live ? exp2_hw(d) : 0.0f;
-    z = live ? sc * s.z : 0.0f;
-    t = live ? sc * fmaf(d, s.z, s.t) : 0.0f;
+// Offsets that overflow: differences of logits are taken before the product.
+__device__ __forceinline__ bool huge_offset(float o) { return !(fabsf(o) < 1e37f); }
+// (a - b) S of a state's maxima, b the larger; at least kNegBig.
+__device__ __forceinline__ float offset_difference(float a, float b, float factor) {
+    if (huge_offset(b * factor)) return fmaxf((a - b) * factor, kNegBig);
+    return fmaxf(a * factor - b * factor, kNegBig);
 }
+// The same for any values; -inf adds nothing.
+template <int K>
+__device__ __forceinline__ void absorb_any(Sums& s, const float* x, float top, float factor) {
+    const float c = fmax_nan(s.m, top);
+    if (c == -INFINITY) return;
+    const float o = c * factor;
+    const float d = offset_difference(s.m, c, factor);
+    const float sc = exp2_hw(d);
+    float z = sc * s.z, t = sc * fmaf(d, s.z, s.t);
+#pragma unroll
+    for (int j = 0; j < K; ++j) {
+        const float u = fmax_nan(huge_offset(o) ? (x[j] - c) * factor : fmaf(x[j], factor, -o),
+                                 kNegBig);
+        const float e = exp2_hw(u);
+        z += e;
+        t = fmaf(u, e, t);
+    }
+    s = Sums{c, o, z, t};
+}
+
 __device__ __forceinline__ Stat wave_reduce_scaled(const Stat& s, float factor) {
     const float m = xrow_max(row_max16(s.m));
-    float z, t;
-    rescale_scaled(s, m, factor, z, t);
+    const bool live = s.m != -INFINITY;
+    const float d = live ? offset_difference(s.m, m, factor) : 0.0f;
+    const float sc = live ? exp2_hw(d) : 0.0f;
+    const float z = live ? sc * s.z : 0.0f;
+    const float t = live ? sc * fmaf(d, s.z, s.t) : 0.0f;
     return Stat{m, xrow_sum(row_sum16(z)), xrow_sum(row_sum16(t))};
 }
 
@@ -112,12 +150,22 @@ struct RowEnd {
 };
 __device__ __forceinline__ RowEnd row_end(const Stat& s, float factor) {
     const float lnz = logf(s.z);
-    float rho = 0.0f;
-    if (s.m != -INFINITY) rho = -fmaf(s.m, factor, -s.m * factor);
+    const float o = s.m * factor;
+    const float rho = huge_offset(o) ? 0.0f : -fmaf(s.m, factor, -o);
     return RowEnd{s.m, fmaf(rho, kLn2, lnz), fmaf(-kLn2, s.t / s.z, lnz),
                   !(s.m < INFINITY)};
 }
 
+__device__ __forceinline__ uint32_t wave_sum_u32(uint32_t v) {
+    v += __builtin_amdgcn_update_dpp(0, v, 0xB1, 0xF, 0xF, false);   // quad_perm [1, 0, 3, 2]
+    v += __builtin_amdgcn_update_dpp(0, v, 0x4E, 0xF, 0xF, false);   // quad_perm [2, 3, 0, 1]
+    v += __builtin_amdgcn_update_dpp(0, v, 0x141, 0xF, 0xF, false);  // row_half_mirror
+    v += __builtin_amdgcn_update_dpp(0, v, 0x140, 0xF, 0xF, false);  // row_mirror
+    const auto q = __builtin_amdgcn_permlane16_swap(v, v, false, false);
+    v = q[0] + q[1];
+    const auto r = __builtin_amdgcn_permlane32_swap(v, v, false, false);
+    return r[0] + r[1];
+}
 __device__ __forceinline__ unsigned long long shfl_xor_u64(unsigned long long v, int off) {
     return static_cast<unsigned long long>(__shfl_xor(static_cast<long long>(v), off, 64));
 }
@@ -125,8 +173,8 @@ __device__ __forceinline__ unsigned long long shfl_xor_u64(unsigned long long v,
 // A workgroup's part of a row: elements [begin, end), its 16-byte vectors
 // [vb, ve) of those from element `head` on.
 struct Piece {
-    int64_t head, begin, end;
-    int64_t vb, ve;
+    int head, begin, end;
+    int vb, ve;
 };
 
 template <int WAVES, bool kSplit>
@@ -134,22 +182,22 @@ struct TopShared {
     static constexpr int NT = WAVES * 64;
     // Pieces' lists together, of which the merge keeps at most all.
     static constexpr int kList = kSplit ? kTopMergeKeys : kTopList;
-    float record[kRecords][NT];  // histograms of the radix search later
+    uint16_t record[kRecords][NT];  // histograms of the radix search later
     union {
         unsigned long long list[kList];
         float thread_max[NT];
     };
-    uint32_t work[kWork];
+    unsigned long long from;
+    uint16_t found[WAVES][64];  // a wave's records to read again
     Stat wave_stat[WAVES];
     uint32_t wave_count[WAVES];
-    uint32_t n_list, n_work, arrived;
+    uint32_t n_list, before, arrived;
     float tau;
     Stat total;
-    uint32_t count;
 };
 
 template <int DT>
-__device__ __forceinline__ float element(const typename Traits<DT>::elem* rp, int64_t i) {
+__device__ __forceinline__ float element(const typename Traits<DT>::elem* rp, int i) {
     return to_f32<DT>(rp[i]);
 }
 
@@ -168,7 +216,7 @@ __device__ void select_exact(TopShared<WAVES, kSplit>& sh, const typename Traits
     for (int shift = 24; shift >= 0; shift -= 8) {
         for (int b = tid; b < 256; b += NT) hist[b] = 0;
         __syncthreads();
-        for (int64_t i = pc.begin + tid; i < pc.end; i += NT) {
+        for (int i = pc.begin + tid; i < pc.end; i += NT) {
             const uint32_t key = ordered(element<DT>(rp, i));
             if (key <= kOrderedNegInf) continue;
             if (shift == 24 || key >> (shift + 8) == prefix >> (shift + 8))
@@ -219,7 +267,7 @@ __device__ void select_exact(TopShared<WAVES, kSplit>& sh, const typename Traits
     if (tid == 0) sh.n_list = 0;
     __syncthreads();
     const uint32_t bound = all ? kOrderedNegInf : prefix;
-    for (int64_t i = pc.begin + tid; i < pc.end; i += NT) {
+    for (int i = pc.begin + tid; i < pc.end; i += NT) {
         const float x = element<DT>(rp, i);
         if (ordered(x) > bound)
             sh.list[atomicAdd(&sh.n_list, 1u)] = order_key(x, static_cast<uint32_t>(i));
@@ -227,8 +275,8 @@ __device__ void select_exact(TopShared<WAVES, kSplit>& sh, const typename Traits
     __syncthreads();
     if (all) return;
     // The first `left` of the elements equal to it.
-    for (int64_t base = pc.begin; base < pc.end && left > 0; base += NT) {
-        const int64_t i = base + tid;
+    for (int base = pc.begin; base < pc.end && left > 0; base += NT) {
+        const int i = base + tid;
         float x = 0.0f;
         bool tie = false;
         if (i < pc.end) {
@@ -254,19 +302,102 @@ __device__ void select_exact(TopShared<WAVES, kSplit>& sh, const typename Traits
 }
 
 // Places in the order of the list's n keys: f(place, key) for each of the
-// first k.
+// first k.  Four lanes share a key's comparisons.
 template <int NT, typename F>
 __device__ __forceinline__ void ranked(const unsigned long long* list, int n, int k, F f) {
-    for (int i = threadIdx.x; i < n; i += NT) {
-        const unsigned long long mine = list[i];
-        int place = 0;
-        for (int j = 0; j < n; ++j) place += list[j] > mine ? 1 : 0;
-        if (place < k) f(place, mine);
+    const int q = threadIdx.x & 3;
+    for (int base = 0; base < n; base += NT / 4) {  // whole waves
+        const int i = base + (threadIdx.x >> 2);
+        const unsigned long long mine = list[i < n ? i : 0];
+        uint32_t place = 0;
+#pragma unroll 4
+        for (int j = q; j < n; j += 4) place += list[j] > mine ? 1u : 0u;
+        place += __builtin_amdgcn_update_dpp(0, place, 0xB1, 0xF, 0xF, false);
+        place += __builtin_amdgcn_update_dpp(0, place, 0x4E, 0xF, 0xF, false);
+        if (q == 0 && i < n && place < static_cast<uint32_t>(k)) f(static_cast<int>(place), mine);
     }
 }
 
+// A lower bound (finite) that at least k elements of the part
+// reach: one that k or few more of 64 R maxima do, each of the maxima of WAVES /
+// R threads, found bit by bit below the maxima's common ones.  One wave calls
+// it.  64 R is at least 2 k where there are that many threads, so that few more
+// than k elements reach it: where the large ones lie anywhere, 64 R ln(64 R / (64
+// R - k)) of them.
+template <int WAVES, int R>
+__device__ __forceinline__ float bound_of(const float* thread_max, int k) {
+    const int lane = threadIdx.x & 63;
+    float most = -INFINITY, least = INFINITY;
+    uint32_t mine[R];
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+        float m = thread_max[r * 64 + lane];
+#pragma unroll
+        for (int w = r + R; w < WAVES; w += R) m = fmax_nan(m, thread_max[w * 64 + lane]);
+        mine[r] = ordered(m);
+        most = fmax_nan(most, m);
+        least = fmax_nan(-m, -least) * -1.0f;
+    }
+    most = xrow_max(row_max16(most));
+    least = -xrow_max(row_max16(-least));
+    uint32_t bound = __builtin_amdgcn_readfirstlane(ordered(least));
+    const uint32_t differ = bound ^ __builtin_amdgcn_readfirstlane(ordered(most));
+    // All 64 R maxima reach the least of them.
+    if (64 * R > k && differ != 0) {
+        uint32_t bit = 0x80000000u >> __builtin_clz(differ);
+        bound &= ~(2 * bit - 1);
+        for (; bit != 0; bit >>= 1) {
+            const uint32_t b = bound | bit;
+            int n = 0;
+#pragma unroll
+            for (int r = 0; r < R; ++r) n += __popcll(__ballot(mine[r] >= b));
+            if (n >= k) {
+                bound = b;
+                if (n <= k + (k >> 2)) break;
+            }
+        }
+    } else if (64 * R < k) {
+        bound = 0;
+    }
+    return from_ordered(bound > kOrderedNegInf ? bound : kOrderedNegInf + 1);
+}
+
+// count += x[j] >= from for 4 or 8 values, all skipped where no lane's `top`
+// reaches `gate`.  In one block: the compiler's own form holds a mask for each
+// value at a time, and a branch of its own costs the loop its registers.
+__device__ __forceinline__ void count_from(uint32_t& count, float top, float gate, float from,
+                                           const float (&x)[4]) {
+    asm("v_cmp_ge_f32 vcc, %1, %2\n\t"
+        "s_cbranch_vccz .Lnone%=\n\t"
+        "v_cmp_ge_f32 vcc, %4, %3\n\tv_addc_co_u32 %0, vcc, 0, %0, vcc\n\t"
+        "v_cmp_ge_f32 vcc, %5, %3\n\tv_addc_co_u32 %0, vcc, 0, %0, vcc\n\t"
+        "v_cmp_ge_f32 vcc, %6, %3\n\tv_addc_co_u32 %0, vcc, 0, %0, vcc\n\t"
+        "v_cmp_ge_f32 vcc, %7, %3\n\tv_addc_co_u32 %0, vcc, 0, %0, vcc\n"
+        ".Lnone%=:"
+        : "+v"(count)
+        : "v"(top), "v"(gate), "v"(from), "v"(x[0]), "v"(x[1]), "v"(x[2]), "v"(x[3])
+        : "vcc");
+}
+__device__ __forceinline__ void count_from(uint32_t& count, float top, float gate, float from,
+                                           const float (&x)[8]) {
+    asm("v_cmp_ge_f32 vcc, %1, %2\n\t"
+        "s_cbranch_vccz .Lnone%=\n\t"
+        "v_cmp_ge_f32 vcc, %4, %3\n\tv_addc_co_u32 %0, vcc, 0, %0, vcc\n\t"
+        "v_cmp_ge_f32 vcc, %5, %3\n\tv_addc_co_u32 %0, vcc, 0, %0, vcc\n\t"
+        "v_cmp_ge_f32 vcc, %6, %3\n\tv_addc_co_u32 %0, vcc, 0, %0, vcc\n\t"
+        "v_cmp_ge_f32 vcc, %7, %3\n\tv_addc_co_u32 %0, vcc, 0, %0, vcc\n\t"
+        "v_cmp_ge_f32 vcc, %8, %3\n\tv_addc_co_u32 %0, vcc, 0, %0, vcc\n\t"
+        "v_cmp_ge_f32 vcc, %9, %3\n\tv_addc_co_u32 %0, vcc, 0, %0, vcc\n\t"
+        "v_cmp_ge_f32 vcc, %10, %3\n\tv_addc_co_u32 %0, vcc, 0, %0, vcc\n\t"
+        "v_cmp_ge_f32 vcc, %11, %3\n\tv_addc_co_u32 %0, vcc, 0, %0, vcc\n"
+        ".Lnone%=:"
+        : "+v"(count)
+        : "v"(top), "v"(gate), "v"(from), "v"(x[0]), "v"(x[1]), "v"(x[2]), "v"(x[3]), "v"(x[4]),
+          "v"(x[5]), "v"(x[6]), "v"(x[7])
+        : "vcc");
+}
 template <int DT, int WAVES, int U, bool kSplit>
-__global__ __launch_bounds__(WAVES * 64) void klp_top_kernel(TopParams p) {
+__global__ __launch_bounds__(WAVES * 64, kSplit ? 2 : 8) void klp_top_kernel(TopParams p) {
     typedef typename Traits<DT>::elem elem;
     constexpr int NT = WAVES * 64;
     constexpr int EPV = Traits<DT>::kPerVec;
@@ -277,28 +408,29 @@ __global__ __launch_bounds__(WAVES * 64) void klp_top_kernel(TopParams p) {
     const int64_t row = kSplit ? static_cast<int64_t>(blockIdx.x) / p.splits : blockIdx.x;
     const int split = kSplit ? static_cast<int>(blockIdx.x - row * p.splits) : 0;
     const int splits = kSplit ? p.splits : 1;
-    const int64_t vocab = p.vocab;
+    const int vocab = static_cast<int>(p.vocab);  // at most 2^26
     const int k = p.k;
     const elem* rp = static_cast<const elem*>(p.logits) + row_offset(p.rm, row);
 
     Piece pc;
-    pc.head = static_cast<int64_t>(((16u - (reinterpret_cast<uintptr_t>(rp) & 15u)) & 15u) / ESZ);
+    pc.head = static_cast<int>(((16u - (reinterpret_cast<uintptr_t>(rp) & 15u)) & 15u) / ESZ);
     if (pc.head > vocab) pc.head = vocab;
-    const int64_t nvec = (vocab - pc.head) / EPV;
-    const int64_t tail_begin = pc.head + nvec * EPV;
-    const int64_t per = (nvec + splits - 1) / splits;
+    const int nvec = (vocab - pc.head) / EPV;
+    const int tail_begin = pc.head + nvec * EPV;
+    const int per = (nvec + splits - 1) / splits;
     pc.vb = split * per < nvec ? split * per : nvec;
     pc.ve = pc.vb + per < nvec ? pc.vb + per : nvec;
     pc.begin = split == 0 ? 0 : pc.head + pc.vb * EPV;
     pc.end = split == splits - 1 ? vocab : pc.head + pc.ve * EPV;
     const u32x4* vp = reinterpret_cast<const u32x4*>(rp + pc.head) + pc.vb;
-    const int nv = static_cast<int>(pc.ve - pc.vb);
+    const int nv = pc.ve - pc.vb;
 
     constexpr int kStep = NT * U;  // vectors of a chunk
     const int n_full = nv / kStep;
     const int n_chunks = (nv + kStep - 1) / kStep;
     int shift = 0;  // chunks of a record, as a power of two
     while (((n_chunks - 1) >> shift) >= kRecords) ++shift;
+    const int records = n_chunks > 0 ? ((n_chunks - 1) >> shift) + 1 : 0;
 
     // Whole chunks, kFwdRing - 1 in flight; loads past them are out of the
     // buffer's range and are not used.
@@ -315,37 +447,42 @@ __global__ __launch_bounds__(WAVES * 64) void klp_top_kernel(TopParams p) {
     for (int r = 0; r < kFwdRing - 1; ++r) load(set[r], r);
     __builtin_amdgcn_sched_barrier(0);
 
-    // The target, and what counts as before it in the order: from its value up
-    // in vectors before its own, above its value elsewhere.
-    const int64_t target = p.targets[row];
-    const bool has_target = target >= 0 && target < vocab;
+    const int64_t given = p.targets[row];
+    const bool has_target = given >= 0 && given < vocab;
+    const int target = has_target ? static_cast<int>(given) : 0;
+    // A target outside the row counts as a logit of 0.
     const float x_t = has_target ? element<DT>(rp, target) : 0.0f;
+    // What lies before it in the order: from its value up in vectors before its
+    // own (t_vec of the piece's), above its value elsewhere.
     const float above_t = has_target ? from_ordered(ordered(x_t) + 1u) : INFINITY;
-    // (vectors of the piece)
     int t_vec = 0;
     if (has_target && target >= pc.head) {
-        const int64_t v = (target - pc.head) / EPV - pc.vb;
-        t_vec = static_cast<int>(v < 0 ? 0 : v < nv ? v : nv);
+        const int v = (target - pc.head) / EPV - pc.vb;
+        t_vec = v < 0 ? 0 : v < nv ? v : nv;
     }
-    uint32_t count = 0;  // of the wave
+    uint32_t count = 0;
 
-    Stat s = stat_empty();
-    float best = -INFINITY, current = -INFINITY;
-    auto take = [&](const u32x4 (&v)[U], int c) {
-        float x[U * EPV];
+    const float gate = has_target ? x_t : INFINITY;
+
+    Sums s = sums_empty();
+    float current = -INFINITY;
+    const int last = (1 << shift) - 1;
+    auto take = [&](const u32x4 (&v)[U], int c, auto whole) {
+        float x[U][EPV];
 #pragma unroll
-        for (int u = 0; u < U; ++u) unpack<DT>(v[u], x + u * EPV);
-        const float top = absorb_scaled<U * EPV>(s, x, p.factor);
-        current = (c & ((1 << shift) - 1)) == 0 ? top : fmax_nan(current, top);
-        best = fmax_nan(best, top);
-        sh.record[c >> shift][tid] = current;
+        for (int u = 0; u < U; ++u) unpack<DT>(v[u], x[u]);
+        float top = x[0][0];
 #pragma unroll
-        for (int u = 0; u < U; ++u) {
-            const float from = (c * U + u) * NT + tid < t_vec ? x_t : above_t;
+        for (int j = 1; j < U * EPV; ++j) top = fmax_nan(top, x[j / EPV][j % EPV]);
+        __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-            for (int j = 0; j < EPV; ++j)
-                count += static_cast<uint32_t>(__popcll(__ballot(x[u * EPV + j] >= from)));
-        }
+        for (int u = 0; u < U; ++u)
+            count_from(count, top, gate, (c * U + u) * NT + tid < t_vec ? x_t : above_t, x[u]);
+        __builtin_amdgcn_sched_barrier(0);
+        if (decltype(whole)::value) absorb_fast<U * EPV>(s, &x[0][0], top, p.factor);
+        else absorb_any<U * EPV>(s, &x[0][0], top, p.factor);
+        current = (c & last) == 0 ? top : fmax_nan(current, top);
+        sh.record[c >> shift][tid] = record_of<DT>(current);
     };
     int c = 0;
     for (; c + kFwdRing <= n_full; c += kFwdRing) {
@@ -353,12 +490,12 @@ __global__ __launch_bounds__(WAVES * 64) void klp_top_kernel(TopParams p) {
         for (int r = 0; r < kFwdRing; ++r) {
             load(set[(r + kFwdRing - 1) % kFwdRing], c + r + kFwdRing - 1);
             __builtin_amdgcn_sched_barrier(0);
-            take(set[r], c + r);
+            take(set[r], c + r, std::true_type{});
         }
     }
 #pragma unroll
     for (int r = 0; r < kFwdRing - 1; ++r)
-        if (c + r < n_full) take(set[r], c + r);
+        if (c + r < n_full) take(set[r], c + r, std::true_type{});
     if (n_full < n_chunks) {
         u32x4 v[U];
 #pragma unroll
@@ -368,119 +505,134 @@ __global__ __launch_bounds__(WAVES * 64) void klp_top_kernel(TopParams p) {
             v[u] = u32x4{w, w, w, w};
             if (i < nv) v[u] = load16<true>(vp + i);
         }
-        take(v, n_full);
+        take(v, n_full, std::false_type{});
+    }
+    if (sums_lost(s) && s.m < INFINITY) {  // (a NaN or +inf row needs none)
+        s = sums_empty();
+        for (int i = tid; i < nv; i += NT) {
+            float x[EPV];
+            unpack<DT>(vp[i], x);
+            float top = x[0];
+#pragma unroll
+            for (int j = 1; j < EPV; ++j) top = fmax_nan(top, x[j]);
+            absorb_any<EPV>(s, x, top, p.factor);
+        }
     }
     // The elements before the first vector and behind the last.
-    const int n_head = split == 0 ? static_cast<int>(pc.head) : 0;
-    const int n_edge = n_head + (split == splits - 1 ? static_cast<int>(vocab - tail_begin) : 0);
+    const int n_head = split == 0 ? pc.head : 0;
+    const int n_edge = n_head + (split == splits - 1 ? vocab - tail_begin : 0);
     float x_edge = -INFINITY;
-    uint32_t i_edge = 0;
+    int i_edge = 0;
     bool edge_before = false, tie_before = false;
     if (tid < n_edge) {
-        i_edge = static_cast<uint32_t>(tid < n_head ? tid : tail_begin + (tid - n_head));
+        i_edge = tid < n_head ? tid : tail_begin + (tid - n_head);
         x_edge = element<DT>(rp, i_edge);
-        absorb_scaled<1>(s, &x_edge, p.factor);
-        best = fmax_nan(best, x_edge);
+        absorb_any<1>(s, &x_edge, x_edge, p.factor);
         edge_before = x_edge >= (i_edge < target ? x_t : above_t);
     }
     // Ties before the target in its own vector.
     if (has_target && target >= pc.head && target < tail_begin && tid < EPV) {
-        const int64_t v = (target - pc.head) / EPV;
-        const int64_t i = pc.head + v * EPV + tid;
+        const int v = (target - pc.head) / EPV;
+        const int i = pc.head + v * EPV + tid;
         if (v >= pc.vb && v < pc.ve && i < target) tie_before = element<DT>(rp, i) == x_t;
     }
-    count += static_cast<uint32_t>(__popcll(__ballot(edge_before)) +
-                                   __popcll(__ballot(tie_before)));
+    count += (edge_before ? 1u : 0u) + (tie_before ? 1u : 0u);
+    count = wave_sum_u32(count);
 
-    s = wave_reduce_scaled(s, p.factor);
+    const float best = s.m;
+    const Stat of_wave = wave_reduce_scaled(Stat{s.m, s.z, s.t}, p.factor);
     sh.thread_max[tid] = best;
     if (lane == 0) {
-        sh.wave_stat[wave] = s;
+        sh.wave_stat[wave] = of_wave;
         sh.wave_count[wave] = count;
     }
-    if (tid == 0) {
-        sh.n_list = 0;
-        sh.n_work = 0;
-    }
+    if (tid == 0) sh.n_list = 0;
     __syncthreads();
     if (wave == 0) {
+        const float bound = k <= 32 ? bound_of<WAVES, 1>(sh.thread_max, k)
+                               : k <= 64 ? bound_of<WAVES, 2>(sh.thread_max, k)
+                               : k <= 128 || WAVES == 4
+                                   ? bound_of<WAVES, 4>(sh.thread_max, k)
+                                   : bound_of<WAVES, WAVES>(sh.thread_max, k);
+        if (lane == 0) sh.tau = bound;
+    } else if (wave == 1) {
         const Stat total =
             wave_reduce_scaled(lane < WAVES ? sh.wave_stat[lane] : stat_empty(), p.factor);
-        uint32_t mine[WAVES];
-#pragma unroll
-        for (int w = 0; w < WAVES; ++w) mine[w] = ordered(sh.thread_max[w * 64 + lane]);
-        // The largest number that k of the maxima reach, bit by bit; one that
-        // exactly k reach will do.
-        uint32_t bound = 0;
-        for (uint32_t bit = 0x80000000u; bit != 0; bit >>= 1) {
-            const uint32_t b = bound | bit;
-            int n = 0;
-#pragma unroll
-            for (int w = 0; w < WAVES; ++w) n += __popcll(__ballot(mine[w] >= b));
-            if (n >= k) {
-                bound = b;
-                if (n == k) break;
-            }
-        }
         if (lane == 0) {
             sh.total = total;
-            sh.tau = bound <= kOrderedNegInf ? -INFINITY : from_ordered(bound);
             uint32_t n = 0;
 #pragma unroll
             for (int w = 0; w < WAVES; ++w) n += sh.wave_count[w];
-            sh.count = n;
+            sh.before = n;
         }
     }
     __syncthreads();
     const float tau = sh.tau;
     const bool bad_piece = !(sh.total.m < INFINITY);
     if (!bad_piece) {
-        auto keep = [&](float x, uint32_t i) {
-            if (x >= tau && x > -INFINITY) {
-                const uint32_t at = atomicAdd(&sh.n_list, 1u);
-                if (at < static_cast<uint32_t>(TopShared<WAVES, kSplit>::kList))
-                    sh.list[at] = order_key(x, i);
+        // n elements from at[0] on that reach tau go to the list.
+        auto keep = [&](auto& x, int at) {
+            constexpr int kN = sizeof(x) / sizeof(float);
+            uint32_t n = 0;
+#pragma unroll
+            for (int e = 0; e < kN; ++e) n += x[e] >= tau ? 1u : 0u;
+            if (n == 0) return;
+            uint32_t to = atomicAdd(&sh.n_list, n);
+#pragma unroll
+            for (int e = 0; e < kN; ++e) {
+                if (!(x[e] >= tau)) continue;
+                if (to < static_cast<uint32_t>(TopShared<WAVES, kSplit>::kList))
+                    sh.list[to] = order_key(x[e], static_cast<uint32_t>(at + e));
+                ++to;
             }
         };
-        if (tid < n_edge) keep(x_edge, i_edge);
-        if (best >= tau && best > -INFINITY) {
-            const int records = n_chunks > 0 ? ((n_chunks - 1) >> shift) + 1 : 0;
-            for (int r = 0; r < records; ++r) {
-                const float x = sh.record[r][tid];
-                if (x >= tau && x > -INFINITY) {
-                    const uint32_t at = atomicAdd(&sh.n_work, 1u);
-                    if (at < kWork) sh.work[at] = static_cast<uint32_t>(r * NT + tid);
-                }
-            }
+        if (tid < n_edge) {
+            float x[1] = {x_edge};
+            keep(x, i_edge);
         }
-        __syncthreads();
-        const uint32_t n_work = sh.n_work;
-        if (n_work <= kWork) {
-            const uint32_t of_record = static_cast<uint32_t>(U) << shift;
-            for (uint32_t w = tid; w < n_work * of_record; w += NT) {
-                const uint32_t item = sh.work[w / of_record];
-                const int r = static_cast<int>(item / NT), t = static_cast<int>(item % NT);
-                const int i = ((r << shift) * U + static_cast<int>(w % of_record)) * NT + t;
+        // The records that reach tau: a wave's go round by round, one of each
+        // lane that has any, with a lane for each of their vectors.
+        uint32_t reach = 0;
+        if (best >= tau) {
+#pragma unroll
+            for (int r = 0; r < kRecords; ++r)
+                reach |= r < records && record_value(sh.record[r][tid]) >= tau ? 1u << r : 0u;
+        }
+        const int of_record = U << shift;
+        for (;;) {
+            const unsigned long long has = __ballot(reach != 0);
+            if (has == 0) break;
+            const int n = __popcll(has);
+            if (reach != 0) {
+                const int r = __builtin_ctz(reach);
+                reach &= reach - 1;
+                sh.found[wave][__popcll(has & ((1ull << lane) - 1ull))] =
+                    static_cast<uint16_t>(r << 6 | lane);
+            }
+            __builtin_amdgcn_wave_barrier();
+            for (int w = lane; w < n * of_record; w += 64) {
+                const int item = sh.found[wave][w / of_record];
+                const int i = ((item >> 6 << shift) * U + w % of_record) * NT + wave * 64 +
+                              (item & 63);
                 if (i < nv) {
                     float x[EPV];
                     unpack<DT>(vp[i], x);
-                    const uint32_t at =
-                        static_cast<uint32_t>(pc.head + (pc.vb + i) * EPV);
-#pragma unroll
-                    for (int j = 0; j < EPV; ++j) keep(x[j], at + j);
+                    keep(x, pc.head + (pc.vb + i) * EPV);
                 }
             }
+            __builtin_amdgcn_wave_barrier();
         }
         __syncthreads();
-        if (n_work > kWork ||
-            sh.n_list > static_cast<uint32_t>(TopShared<WAVES, kSplit>::kList)) {
+        const bool overflow = sh.n_list > static_cast<uint32_t>(TopShared<WAVES, kSplit>::kList);
+        if (overflow) {
             __syncthreads();
             select_exact<DT, WAVES, kSplit>(sh, rp, pc, k);
         }
+        __syncthreads();
     }
     int n = bad_piece ? 0 : static_cast<int>(sh.n_list);
     Stat total = sh.total;
-    uint32_t before = sh.count;
+    uint32_t before = sh.before;
 
     if constexpr (kSplit) {
         // This piece's state and keys in order, then its arrival: agent-scope
@@ -517,43 +669,51 @@ __global__ __launch_bounds__(WAVES * 64) void klp_top_kernel(TopParams p) {
             __hip_atomic_store(p.counters + row, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
             sh.n_list = 0;
         }
-        // Lane l merges pieces l (at most 64).  Of the pieces' keys, those from
-        // the least of their ceil(k / splits)-th up hold the row's k first, and
-        // so do those from the largest k-th up.
+        // Of the pieces' keys, those from the least of their ceil(k / splits)-th
+        // up hold the row's k first, and so do those from the largest k-th up.
+        // Every load starts before the first wait.
+        constexpr int kKeys = kTopMergeKeys / NT;
+        unsigned long long mine[kKeys];
+#pragma unroll
+        for (int j = 0; j < kKeys; ++j) {
+            mine[j] = kNoKey;
+            if (j * NT + tid < splits * k) mine[j] = keys[j * NT + tid];
+        }
+        // Lane l merges piece l (at most 64).
         if (wave == 0) {
             Stat a = stat_empty();
             uint32_t cnt = 0;
             unsigned long long least = ~0ull, most = 0;
             if (lane < splits) {
                 const float4 q = reinterpret_cast<const float4*>(states)[lane];
-                a = Stat{q.x, q.y, q.z};
-                cnt = __float_as_uint(q.w);
                 least = keys[lane * k + (k + splits - 1) / splits - 1];
                 most = keys[lane * k + k - 1];
+                a = Stat{q.x, q.y, q.z};
+                cnt = __float_as_uint(q.w);
             }
             a = wave_reduce_scaled(a, p.factor);
+            cnt = wave_sum_u32(cnt);
 #pragma unroll
             for (int off = 1; off < 64; off <<= 1) {
-                cnt += __shfl_xor(cnt, off, 64);
                 const unsigned long long l = shfl_xor_u64(least, off), h = shfl_xor_u64(most, off);
                 least = l < least ? l : least;
                 most = h > most ? h : most;
             }
             if (lane == 0) {
                 sh.total = a;
-                sh.count = cnt;
-                *reinterpret_cast<unsigned long long*>(sh.work) = least > most ? least : most;
+                sh.before = cnt;
+                sh.from = least > most ? least : most;
             }
         }
         __syncthreads();
         total = sh.total;
-        before = sh.count;
-        const unsigned long long from = *reinterpret_cast<unsigned long long*>(sh.work);
+        before = sh.before;
+        const unsigned long long from = sh.from;
         if (total.m < INFINITY) {
-            for (int j = tid; j < splits * k; j += NT) {
-                const unsigned long long key = keys[j];
-                if (key != kNoKey && key >= from) sh.list[atomicAdd(&sh.n_list, 1u)] = key;
-            }
+#pragma unroll
+            for (int j = 0; j < kKeys; ++j)
+                if (mine[j] != kNoKey && mine[j] >= from)
+                    sh.list[atomicAdd(&sh.n_list, 1u)] = mine[j];
         }
         __syncthreads();
         n = total.m < INFINITY ? static_cast<int>(sh.n_list) : 0;
@@ -563,7 +723,6 @@ __global__ __launch_bounds__(WAVES * 64) void klp_top_kernel(TopParams p) {
     if (tid == 0) {
         p.lse[row] = fmaf(e.m, p.inv_t, e.l);
         p.entropy[row] = e.ent;
-        // A target outside the row counts as a logit of 0.
         p.logprob[row] = fmaf(x_t - e.m, p.inv_t, -e.l);
         p.rank[row] = has_target && !e.bad ? static_cast<int64_t>(before) : -1;
     }

@@ -147,6 +147,27 @@ def test_masked_logits(rows, vocab):
                     assert (got[5] == -np.inf).all()
 
 
+@pytest.mark.parametrize("rows,vocab", [(2, 700), (1, 140001), (300, 9001)])
+def test_logits_masked_with_the_types_lowest_value(rows, vocab):
+    """Whole rows of it are uniform; in others it is a weight of 0 that is
+    listed behind every other."""
+    ko = _ko()
+    g = torch.Generator().manual_seed(5)
+    k = 20
+    for dtype in DTYPES:
+        low = torch.finfo(dtype).min
+        full = torch.randn(rows, vocab, generator=g).to(dtype)
+        for keep in (0, 1, 19, 300):
+            print(f"lowest {rows} x {vocab} {dtype} {keep} kept", flush=True)
+            x = torch.full_like(full, low)
+            at = torch.randperm(vocab, generator=g)[:keep]
+            x[:, at] = full[:, at]
+            t = torch.randint(0, vocab, (rows,), generator=g)
+            out = [o.cpu().numpy() for o in ko.fused_top_logprobs(x.to(DEV), t.to(DEV), k)]
+            for i in range(min(rows, 3)):
+                _check_row([o[i] for o in out], np64(x[i]), int(t[i]), k, 1.0)
+
+
 def test_rows_without_a_distribution():
     ko = _ko()
     for rows, vocab in ((1, 131072), (300, 9001)):
