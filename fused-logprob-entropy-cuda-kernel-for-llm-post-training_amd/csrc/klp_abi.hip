@@ -447,16 +447,14 @@ TopConfig top_config(int dtype, int64_t n_rows, int64_t vocab, int k) {
     c.splits = s;
     return c;
 }
-// Arrival counters, a fixed region so that no call's states lie where another's
-// counters do; then the pieces' states, then their keys.
-constexpr size_t kTopCounterBytes = kFwdSplitGrid * sizeof(unsigned int);
-size_t top_state_bytes(int64_t n_rows, const TopConfig& c) {
-    return static_cast<size_t>(n_rows) * c.splits * 4 * sizeof(float);
-}
+// Arrival counters, a fixed region so that no call's words lie where another's
+// counters do; then the pieces' words.
+constexpr size_t kTopCounterBytes =
+    kFwdSplitGrid / 2 * klp::kTopCounterStride * sizeof(unsigned int);
 size_t top_workspace(int64_t n_rows, int k, const TopConfig& c) {
     if (c.splits == 1) return 0;
-    return kTopCounterBytes + top_state_bytes(n_rows, c) +
-           static_cast<size_t>(n_rows) * c.splits * k * sizeof(unsigned long long);
+    return kTopCounterBytes + static_cast<size_t>(n_rows) * c.splits * (k + 2) *
+                                  sizeof(unsigned long long);
 }
 
 int check_top(int64_t vocab, int64_t n_rows, int k) {
@@ -1854,9 +1852,7 @@ int klp_fwd_top(const void* logits, int dtype, int64_t n_rows, int64_t vocab, in
     if (c.splits > 1) {
         unsigned char* w = static_cast<unsigned char*>(workspace);
         p.counters = reinterpret_cast<unsigned int*>(w);
-        p.states = reinterpret_cast<float*>(w + kTopCounterBytes);
-        p.keys = reinterpret_cast<unsigned long long*>(w + kTopCounterBytes +
-                                                       top_state_bytes(n_rows, c));
+        p.words = reinterpret_cast<unsigned long long*>(w + kTopCounterBytes);
     }
     p.logprob = logprob;
     p.entropy = entropy;

@@ -390,6 +390,7 @@ hipError_t launch_sample(int dtype, const SampleParams& p, hipStream_t stream);
 constexpr int64_t kTopMaxVocab = int64_t{1} << 26;
 constexpr int kTopMax = 256;            // alternatives of a row at most
 constexpr int kTopMergeKeys = 4096;     // splits * k at most
+constexpr int kTopCounterStride = 16;   // a row's counter has 64 bytes
 struct TopParams {
     const void* logits;
     RowMap rm;
@@ -401,12 +402,11 @@ struct TopParams {
     float inv_t;           // 1 / temperature
     int waves;             // of a workgroup: 4 or 8
     int splits;            // workgroups of a row, at most 64
-    // Pieces (splits > 1): arrival counters [n_rows], zero before the launch
-    // and left zero by it; states [n_rows, splits] float4 and keys [n_rows,
-    // splits, k] of any contents.
+    // Pieces (splits > 1): arrival counters, kTopCounterStride words a row,
+    // zero before the launch and left zero by it, and [n_rows, splits, k + 2]
+    // words of any contents: a piece's state and its keys.
     unsigned int* counters;
-    float* states;
-    unsigned long long* keys;
+    unsigned long long* words;
     float* logprob;
     float* entropy;
     float* lse;

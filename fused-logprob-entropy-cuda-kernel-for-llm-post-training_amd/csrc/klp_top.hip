@@ -166,8 +166,8 @@ __device__ __forceinline__ uint32_t wave_sum_u32(uint32_t v) {
     const auto r = __builtin_amdgcn_permlane32_swap(v, v, false, false);
     return r[0] + r[1];
 }
-__device__ __forceinline__ unsigned long long shfl_xor_u64(unsigned long long v, int off) {
-    return static_cast<unsigned long long>(__shfl_xor(static_cast<long long>(v), off, 64));
+__device__ __forceinline__ unsigned long long two_words(uint32_t low, uint32_t high) {
+    return static_cast<unsigned long long>(high) << 32 | low;
 }
 
 // A workgroup's part of a row: elements [begin, end), its 16-byte vectors
@@ -187,7 +187,7 @@ struct TopShared {
         unsigned long long list[kList];
         float thread_max[NT];
     };
-    unsigned long long from;
+    unsigned long long sorted[kSplit ? kTopMax : 1];  // a piece's
     uint16_t found[WAVES][64];  // a wave's records to read again
     Stat wave_stat[WAVES];
     uint32_t wave_count[WAVES];
@@ -441,7 +441,7 @@ __global__ __launch_bounds__(WAVES * 64, kSplit ? 2 : 8) void klp_top_kernel(Top
 #pragma unroll
         for (int u = 0; u < U; ++u)
             dst[u] = __builtin_amdgcn_raw_buffer_load_b128(rs, ((c * U + u) * NT + tid) * 16, 0,
-                                                           kBufNonTemporal);
+                                                           kSplit ? 0 : kBufNonTemporal);
     };
 #pragma unroll
     for (int r = 0; r < kFwdRing - 1; ++r) load(set[r], r);
@@ -635,85 +635,94 @@ __global__ __launch_bounds__(WAVES * 64, kSplit ? 2 : 8) void klp_top_kernel(Top
     uint32_t before = sh.before;
 
     if constexpr (kSplit) {
-        // This piece's state and keys in order, then its arrival: agent-scope
-        // stores, which write through to the device's coherence point, and a
-        // wait for them before the count.
-        unsigned long long* keys = p.keys + row * splits * k;
-        float* states = p.states + row * splits * 4;
-        ranked<NT>(sh.list, n, k, [&](int place, unsigned long long key) {
-            __hip_atomic_store(keys + split * k + place, key, __ATOMIC_RELAXED,
-                               __HIP_MEMORY_SCOPE_AGENT);
-        });
-        for (int j = n + tid; j < k; j += NT)
-            __hip_atomic_store(keys + split * k + j, kNoKey, __ATOMIC_RELAXED,
-                               __HIP_MEMORY_SCOPE_AGENT);
-        if (tid == 0) {
-            float* slot = states + split * 4;
-            __hip_atomic_store(slot + 0, total.m, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-            __hip_atomic_store(slot + 1, total.z, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-            __hip_atomic_store(slot + 2, total.t, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-            __hip_atomic_store(slot + 3, __uint_as_float(before), __ATOMIC_RELAXED,
-                               __HIP_MEMORY_SCOPE_AGENT);
+        // This piece's state and its k keys in order, side by side, then its
+        // arrival: agent-scope stores, which write through to the device's
+        // coherence point, and a wait for them before the count.
+        const int words = k + 2;
+        unsigned long long* mine = p.words + (row * splits + split) * words;
+        for (int j = tid; j < k; j += NT) sh.sorted[j] = kNoKey;
+        __syncthreads();
+        ranked<NT>(sh.list, n, k,
+                   [&](int place, unsigned long long key) { sh.sorted[place] = key; });
+        __syncthreads();
+        for (int j = tid; j < words; j += NT) {
+            const unsigned long long w =
+                j == 0   ? two_words(__float_as_uint(total.m), __float_as_uint(total.z))
+                : j == 1 ? two_words(__float_as_uint(total.t), before)
+                         : sh.sorted[j - 2];
+            __hip_atomic_store(mine + j, w, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
         }
         __atomic_signal_fence(__ATOMIC_SEQ_CST);
         __builtin_amdgcn_s_waitcnt(kWaitVmcnt0);
         __atomic_signal_fence(__ATOMIC_SEQ_CST);
         __syncthreads();
+        unsigned int* counter = p.counters + row * kTopCounterStride;
         if (tid == 0)
-            sh.arrived = __hip_atomic_fetch_add(p.counters + row, 1u, __ATOMIC_RELAXED,
-                                                __HIP_MEMORY_SCOPE_AGENT);
+            sh.arrived =
+                __hip_atomic_fetch_add(counter, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
         __syncthreads();
         if (sh.arrived != static_cast<uint32_t>(splits - 1)) return;
-        __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "agent");
+        // Agent-scope loads, which no cache answers, see every piece's words: an
+        // acquire fence would drop the XCD's L2 under the other rows' workgroups
+        // (the loads of 64 rows then took 4 us, of one row 1.4).
+        __atomic_signal_fence(__ATOMIC_SEQ_CST);
+        auto word = [](const unsigned long long* w) {
+            return __hip_atomic_load(w, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        };
         if (tid == 0) {
-            __hip_atomic_store(p.counters + row, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+            __hip_atomic_store(counter, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
             sh.n_list = 0;
         }
-        // Of the pieces' keys, those from the least of their ceil(k / splits)-th
-        // up hold the row's k first, and so do those from the largest k-th up.
-        // Every load starts before the first wait.
-        constexpr int kKeys = kTopMergeKeys / NT;
-        unsigned long long mine[kKeys];
+        // Of the pieces' keys, those from the least value of their ceil(k /
+        // splits)-th up hold the row's k first, and so do those from the largest
+        // k-th up.  Every load starts before the first wait.
+        const unsigned long long* all = p.words + row * splits * words;
+        constexpr int kKeys = (kTopMergeKeys + 128 + NT - 1) / NT;
+        unsigned long long held[kKeys];
 #pragma unroll
         for (int j = 0; j < kKeys; ++j) {
-            mine[j] = kNoKey;
-            if (j * NT + tid < splits * k) mine[j] = keys[j * NT + tid];
+            held[j] = kNoKey;
+            if (j * NT + tid < splits * words) held[j] = word(all + j * NT + tid);
         }
         // Lane l merges piece l (at most 64).
         if (wave == 0) {
             Stat a = stat_empty();
             uint32_t cnt = 0;
-            unsigned long long least = ~0ull, most = 0;
+            float least = INFINITY, most = -INFINITY;
             if (lane < splits) {
-                const float4 q = reinterpret_cast<const float4*>(states)[lane];
-                least = keys[lane * k + (k + splits - 1) / splits - 1];
-                most = keys[lane * k + k - 1];
-                a = Stat{q.x, q.y, q.z};
-                cnt = __float_as_uint(q.w);
+                const unsigned long long* of = all + lane * words;
+                const unsigned long long first = word(of), second = word(of + 1),
+                                         l = word(of + 1 + (k + splits - 1) / splits),
+                                         h = word(of + k + 1);
+                a = Stat{__uint_as_float(static_cast<uint32_t>(first)),
+                         __uint_as_float(static_cast<uint32_t>(first >> 32)),
+                         __uint_as_float(static_cast<uint32_t>(second))};
+                cnt = static_cast<uint32_t>(second >> 32);
+                least = l == kNoKey ? -INFINITY : key_value(l);
+                most = h == kNoKey ? -INFINITY : key_value(h);
             }
             a = wave_reduce_scaled(a, p.factor);
             cnt = wave_sum_u32(cnt);
-#pragma unroll
-            for (int off = 1; off < 64; off <<= 1) {
-                const unsigned long long l = shfl_xor_u64(least, off), h = shfl_xor_u64(most, off);
-                least = l < least ? l : least;
-                most = h > most ? h : most;
-            }
+            least = -xrow_max(row_max16(-least));
+            most = xrow_max(row_max16(most));
             if (lane == 0) {
                 sh.total = a;
                 sh.before = cnt;
-                sh.from = least > most ? least : most;
+                sh.tau = fmaxf(least, most);
             }
         }
         __syncthreads();
         total = sh.total;
         before = sh.before;
-        const unsigned long long from = sh.from;
         if (total.m < INFINITY) {
+            const float from = sh.tau;
 #pragma unroll
-            for (int j = 0; j < kKeys; ++j)
-                if (mine[j] != kNoKey && mine[j] >= from)
-                    sh.list[atomicAdd(&sh.n_list, 1u)] = mine[j];
+            for (int j = 0; j < kKeys; ++j) {
+                const int w = j * NT + tid;
+                if (w < splits * words && w % words >= 2 && held[j] != kNoKey &&
+                    key_value(held[j]) >= from)
+                    sh.list[atomicAdd(&sh.n_list, 1u)] = held[j];
+            }
         }
         __syncthreads();
         n = total.m < INFINITY ? static_cast<int>(sh.n_list) : 0;

@@ -656,7 +656,7 @@ int klp_sample(const void* logits, int dtype, int64_t n_rows, int64_t vocab, int
  * k in [1, 256], vocab <= 2^26, n_rows below 2^23 (KLP_EINVAL).
  *
  * The workspace (klp_fwd_top_workspace_bytes; 0 for calls that need none) is
- * for few rows, cut into pieces; NULL leaves them whole.  Its first 1024 bytes
+ * for few rows, cut into pieces; NULL leaves them whole.  Its first 8192 bytes
  * must be zero before its first use and every call leaves them zero (other
  * entry points do not: it is not to be shared with them); calls that share it
  * must be ordered on one stream.

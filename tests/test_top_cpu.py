@@ -74,7 +74,7 @@ def test_output_refusals():
 def test_workspace():
     L = _lib().lib
     need = L.klp_fwd_top_workspace_bytes(0, 2, 152064, 20)
-    assert need > 1024
+    assert need > 8192
     assert L.klp_fwd_top_workspace_bytes(0, 4096, 152064, 20) == 0
     assert L.klp_fwd_top_workspace_bytes(0, 2, 512, 20) == 0
     for bad in ((9, 2, 152064, 20), (0, 0, 152064, 20), (0, 2, 0, 20), (0, 2, 152064, 0),
@@ -87,9 +87,9 @@ def test_workspace():
     for n in (1, 2, 7, 64, 128):
         for k in (1, 20, 64, 256):
             b = L.klp_fwd_top_workspace_bytes(2, n, 262144, k)
-            assert b == 0 or (b - 1024) % (n * (16 + 8 * k)) == 0
+            assert b == 0 or (b - 8192) % (n * (16 + 8 * k)) == 0
             if b:
-                splits = (b - 1024) // (n * (16 + 8 * k))
+                splits = (b - 8192) // (n * (16 + 8 * k))
                 assert splits >= 2 and splits * k <= 4096 and n * splits <= 256
 
 
