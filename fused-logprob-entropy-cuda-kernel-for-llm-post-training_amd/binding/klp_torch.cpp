@@ -1127,6 +1127,168 @@ class FusedTopLogprobs : public torch::autograd::Function<FusedTopLogprobs> {
     }
 };
 
+struct BlockOperands {
+    Matrix x, r;
+    at::Tensor w, post, gate;  // contiguous; undefined where there is none
+    int code, w_code, gate_code;
+    int64_t n, d;
+};
+at::Tensor contiguous_or_none(const at::Tensor& t) {
+    return t.defined() ? t.contiguous() : at::Tensor();
+}
+BlockOperands block_operands(const at::Tensor& x, const at::Tensor& residual,
+                             const at::Tensor& weight, const at::Tensor& post,
+                             const at::Tensor& gate) {
+    BlockOperands o{as_rows(x), as_rows(residual), weight.contiguous(), contiguous_or_none(post),
+                    contiguous_or_none(gate), dtype_code(x.scalar_type()),
+                    dtype_code(weight.scalar_type()),
+                    gate.defined() ? dtype_code(gate.scalar_type()) : KLP_BF16, 0, 0};
+    o.n = o.x.t.size(0);
+    o.d = o.x.t.size(1);
+    return o;
+}
+
+class FusedBlockNorm : public torch::autograd::Function<FusedBlockNorm> {
+   public:
+    static variable_list forward(AutogradContext* ctx, const at::Tensor& x,
+                                 const at::Tensor& residual, const at::Tensor& weight,
+                                 const std::optional<at::Tensor>& post_weight,
+                                 const std::optional<at::Tensor>& gate_, int64_t per_gate,
+                                 double scale, double eps, bool kept) {
+        const int dev = x.get_device();
+        const c10::hip::HIPGuard guard(static_cast<c10::DeviceIndex>(dev));
+        const at::Tensor post = post_weight.value_or(at::Tensor()),
+                         gate = gate_.value_or(at::Tensor());
+        const BlockOperands o = block_operands(x, residual, weight, post, gate);
+        const auto f32 = x.options().dtype(at::kFloat);
+        at::Tensor y = at::empty(x.sizes(), x.options()), h = at::empty(x.sizes(), x.options()),
+                   rstd_x = at::empty({o.n}, f32), rstd_h = at::empty({o.n}, f32), xq, xs, hq, hs;
+        const bool needs_x = post.defined() || gate.defined();
+        const auto codes = x.options().dtype(at::kFloat8_e4m3fn);
+        if (kept && needs_x) {
+            xq = at::empty(x.sizes(), codes);
+            xs = at::empty(scale_shape(x), f32);
+        }
+        if (kept) {
+            hq = at::empty(x.sizes(), codes);
+            hs = at::empty(scale_shape(x), f32);
+        }
+        check_status(klp_block_norm(
+            o.x.t.data_ptr(), o.code, o.x.ld, o.r.t.data_ptr(), o.r.ld, data_or_null(o.post),
+            o.w.data_ptr(), o.w_code, data_or_null(o.gate), o.gate_code, per_gate,
+            static_cast<float>(scale), o.n, o.d, static_cast<float>(eps), y.data_ptr(),
+            h.data_ptr(), out_ptr(rstd_x), out_ptr(rstd_h),
+            static_cast<uint8_t*>(data_or_null(xq)), static_cast<float*>(data_or_null(xs)),
+            static_cast<uint8_t*>(data_or_null(hq)), static_cast<float*>(data_or_null(hs)),
+            current_stream(dev)));
+        ctx->save_for_backward({needs_x && !kept ? x : at::Tensor(), kept ? at::Tensor() : h, xq,
+                                xs, hq, hs, weight, post, gate, rstd_x, rstd_h});
+        ctx->saved_data["per_gate"] = per_gate;
+        ctx->saved_data["scale"] = scale;
+        ctx->saved_data["shape"] = x.sizes().vec();
+        ctx->set_materialize_grads(false);
+        return {y, h};
+    }
+
+    static variable_list backward(AutogradContext* ctx, variable_list grads) {
+        variable_list none(9);
+        at::Tensor g_y = grads[0], g_h = grads[1];
+        const auto saved = ctx->get_saved_variables();
+        const at::Tensor &x = saved[0], &h = saved[1], &xq = saved[2], &xs = saved[3],
+                         &hq = saved[4], &hs = saved[5], &weight = saved[6], &post = saved[7],
+                         &gate = saved[8], &rstd_x = saved[9], &rstd_h = saved[10];
+        // Indices of needs_input_grad count the tensors that were given.
+        const bool need_x = ctx->needs_input_grad(0), need_r = ctx->needs_input_grad(1),
+                   need_w = ctx->needs_input_grad(2),
+                   need_p = post.defined() && ctx->needs_input_grad(3),
+                   need_g = gate.defined() && ctx->needs_input_grad(post.defined() ? 4 : 3);
+        if ((!g_y.defined() && !g_h.defined()) || !(need_x || need_r || need_w || need_p || need_g))
+            return none;
+        if (hq.defined() && at::GradMode::is_enabled())
+            throw std::runtime_error(
+                "kernel_opt: gradients from 8-bit checkpoints cannot be differentiated "
+                "(create_graph)");
+        const at::Tensor& given = g_y.defined() ? g_y : g_h;
+        const int dev = rstd_h.get_device();
+        const c10::hip::HIPGuard guard(static_cast<c10::DeviceIndex>(dev));
+        hipStream_t stream = current_stream(dev);
+        refuse_captured_backward(stream);
+        const std::vector<int64_t> shape = ctx->saved_data["shape"].toIntVector();
+        const int64_t per_gate = ctx->saved_data["per_gate"].toInt();
+        const double scale = ctx->saved_data["scale"].toDouble();
+        const int64_t n = rstd_h.numel(), d = shape.back();
+        const auto options = given.options();
+        // Without a norm, a gate and a scale d_x is d_residual.
+        const bool plain = !post.defined() && !gate.defined() && scale == 1.0;
+        at::Tensor d_x, d_r, d_w, d_p, d_g;
+        if (need_x && !(plain && need_r)) d_x = at::empty(shape, options);
+        if (need_r) d_r = at::empty(shape, options);
+        if (need_w) d_w = at::empty(weight.sizes(), weight.options());
+        if (need_p) d_p = at::empty(post.sizes(), post.options());
+        if (need_g) d_g = at::empty(gate.sizes(), gate.options());
+        if (n == 0) {
+            for (at::Tensor* t : {&d_w, &d_p, &d_g})
+                if (t->defined()) t->zero_();
+        } else {
+            const at::Tensor gy = contiguous_or_none(g_y), gh = contiguous_or_none(g_h);
+            const Matrix xm = x.defined() ? as_rows(x) : Matrix{at::Tensor(), 0};
+            const at::Tensor w = weight.contiguous(), wp = contiguous_or_none(post),
+                             g = contiguous_or_none(gate);
+            size_t bytes = 0;
+            at::Tensor ws;
+            if (need_w || need_p || need_g) {
+                bytes = klp_block_norm_bwd_workspace_bytes(n, d, post.defined(), gate.defined(),
+                                                           per_gate);
+                ws = at::empty({static_cast<int64_t>(bytes)}, rstd_h.options().dtype(at::kByte));
+            }
+            check_status(klp_block_norm_bwd(
+                data_or_null(xm.t), dtype_code(given.scalar_type()), xm.ld,
+                static_cast<const uint8_t*>(data_or_null(xq)), fptr(xs), data_or_null(h),
+                static_cast<const uint8_t*>(data_or_null(hq)), fptr(hs), data_or_null(wp),
+                w.data_ptr(), dtype_code(w.scalar_type()), data_or_null(g),
+                g.defined() ? dtype_code(g.scalar_type()) : KLP_BF16, per_gate,
+                static_cast<float>(scale), fptr(rstd_x), fptr(rstd_h), data_or_null(gy),
+                data_or_null(gh), n, d, data_or_null(d_x), data_or_null(d_r), data_or_null(d_p),
+                data_or_null(d_w), data_or_null(d_g), data_or_null(ws), bytes, stream));
+        }
+        if (plain && need_x && need_r) d_x = d_r;
+        first_order("fused_block_norm", {&d_x, &d_r, &d_w, &d_p, &d_g},
+                    {x, h, weight, post, gate, g_y, g_h});
+        return {d_x, d_r, d_w, d_p, d_g, at::Tensor(), at::Tensor(), at::Tensor(), at::Tensor()};
+    }
+};
+
+std::vector<at::Tensor> block_norm(const at::Tensor& x, const at::Tensor& residual,
+                                   const at::Tensor& weight,
+                                   const std::optional<at::Tensor>& post,
+                                   const std::optional<at::Tensor>& gate, int64_t per_gate,
+                                   double scale, double eps, bool kept) {
+    decline_under_capture(x.get_device());
+    return FusedBlockNorm::apply(x, residual, weight, post, gate, per_gate, scale, eps, kept);
+}
+
+std::vector<at::Tensor> block_norm_fp8(const at::Tensor& x, const at::Tensor& residual,
+                                       const at::Tensor& weight,
+                                       const std::optional<at::Tensor>& post,
+                                       const std::optional<at::Tensor>& gate, int64_t per_gate,
+                                       double scale, double eps) {
+    const int dev = x.get_device();
+    decline_under_capture(dev);
+    const at::AutoDispatchBelowADInplaceOrView below;
+    const c10::hip::HIPGuard guard(static_cast<c10::DeviceIndex>(dev));
+    const BlockOperands o = block_operands(x, residual, weight, post.value_or(at::Tensor()),
+                                           gate.value_or(at::Tensor()));
+    at::Tensor q = at::empty(x.sizes(), x.options().dtype(at::kFloat8_e4m3fn)),
+               scales = at::empty(scale_shape(x), x.options().dtype(at::kFloat)),
+               h = at::empty(x.sizes(), x.options());
+    check_status(klp_block_norm_fp8(
+        o.x.t.data_ptr(), o.code, o.x.ld, o.r.t.data_ptr(), o.r.ld, data_or_null(o.post),
+        o.w.data_ptr(), o.w_code, data_or_null(o.gate), o.gate_code, per_gate,
+        static_cast<float>(scale), o.n, o.d, static_cast<float>(eps),
+        static_cast<uint8_t*>(q.data_ptr()), out_ptr(scales), h.data_ptr(), current_stream(dev)));
+    return {q, scales, h};
+}
+
 std::vector<at::Tensor> top_logprobs(const at::Tensor& logits, const at::Tensor& targets,
                                      int64_t k, double temperature) {
     decline_under_capture(logits.get_device());
@@ -1215,6 +1377,13 @@ PYBIND11_MODULE(klp_torch, m) {
     m.def("quantize_fp8", &quantize_fp8, pybind11::arg("x"), pybind11::arg("block_rows"));
     m.def("fp8_linear", &fp8_linear, pybind11::arg("x"), pybind11::arg("x_scale"),
           pybind11::arg("weight"), pybind11::arg("weight_scale"), pybind11::arg("out_dtype"));
+    m.def("block_norm", &block_norm, pybind11::arg("x"), pybind11::arg("residual"),
+          pybind11::arg("weight"), pybind11::arg("post_weight"), pybind11::arg("gate"),
+          pybind11::arg("per_gate"), pybind11::arg("scale"), pybind11::arg("eps"),
+          pybind11::arg("kept"));
+    m.def("block_norm_fp8", &block_norm_fp8, pybind11::arg("x"), pybind11::arg("residual"),
+          pybind11::arg("weight"), pybind11::arg("post_weight"), pybind11::arg("gate"),
+          pybind11::arg("per_gate"), pybind11::arg("scale"), pybind11::arg("eps"));
     m.def("top_logprobs", &top_logprobs, pybind11::arg("logits"), pybind11::arg("targets"),
           pybind11::arg("k"), pybind11::arg("temperature"));
     m.def("sample", &sample, pybind11::arg("logits"), pybind11::arg("uniform"), pybind11::arg("t"),

@@ -810,6 +810,84 @@ int norm_setup(const void* x, int dtype, int64_t ld_x, const void* residual, int
     return KLP_OK;
 }
 
+// What the norms around a block and their backward take alike.
+int check_block(int dtype, int64_t rows, int64_t dim, const void* post, const void* weight,
+                int weight_dtype, const void* gate, int gate_dtype, int64_t rows_per_gate,
+                float scale) {
+    int rc = check_dtype3(dtype, "x");
+    if (rc != KLP_OK) return rc;
+    if (weight_dtype != dtype && weight_dtype != KLP_FP32)
+        return fail(KLP_EDTYPE, "weights must be float32 or of x's dtype");
+    if (gate != nullptr && gate_dtype != dtype && gate_dtype != KLP_FP32)
+        return fail(KLP_EDTYPE, "gate must be float32 or of x's dtype");
+    if (rows < 0 || rows > INT32_MAX) return fail(KLP_EINVAL, "rows must be in [0, 2^31-1]");
+    if (dim < 1 || dim > klp::kBlockMaxDim)
+        return fail(KLP_EINVAL, "dim must be in [1, %lld], got %lld",
+                    static_cast<long long>(klp::kBlockMaxDim), static_cast<long long>(dim));
+    // A row takes at most 1024 threads.
+    if ((rc = check_threads(rows, 1024, "rows")) != KLP_OK) return rc;
+    if (gate != nullptr && rows_per_gate < 1)
+        return fail(KLP_EINVAL, "rows_per_gate must be >= 1");
+    if (!(scale - scale == 0.0f)) return fail(KLP_EINVAL, "scale must be finite");
+    if (rows == 0) return KLP_OK;
+    if (weight == nullptr || !aligned(weight, elem_bytes(weight_dtype)) ||
+        !aligned(post, elem_bytes(weight_dtype)))
+        return fail(KLP_EINVAL, "weight must be non-null, and weights aligned to their elements");
+    if (!aligned(gate, elem_bytes(gate_dtype)))
+        return fail(KLP_EINVAL, "gate is not aligned to its elements");
+    return KLP_OK;
+}
+
+// The forward's operands into p, but for y.
+int block_setup(const void* x, int dtype, int64_t ld_x, const void* residual, int64_t ld_residual,
+                const void* post, const void* weight, int weight_dtype, const void* gate,
+                int gate_dtype, int64_t rows_per_gate, float scale, int64_t rows, int64_t dim,
+                float eps, void* h, klp::BlockParams* p) {
+    int rc = check_block(dtype, rows, dim, post, weight, weight_dtype, gate, gate_dtype,
+                         rows_per_gate, scale);
+    if (rc != KLP_OK) return rc;
+    if (!(eps >= 0.0f) || isinf(eps)) return fail(KLP_EINVAL, "eps must be finite and >= 0");
+    if (rows == 0) return KLP_OK;
+    const size_t e = elem_bytes(dtype);
+    if ((rc = check_matrix(x, ld_x, dim, e, "x")) != KLP_OK) return rc;
+    if ((rc = check_matrix(residual, ld_residual, dim, e, "residual")) != KLP_OK) return rc;
+    if (h == nullptr || !aligned(h, e))
+        return fail(KLP_EINVAL, "h must be non-null and aligned to its elements");
+    *p = klp::BlockParams{};
+    p->x = x;
+    p->ld_x = ld_x;
+    p->residual = residual;
+    p->ld_r = ld_residual;
+    p->post = post;
+    p->weight = weight;
+    p->weight_f32 = weight_dtype == KLP_FP32;
+    p->gate = gate;
+    p->gate_f32 = gate_dtype == KLP_FP32;
+    p->per_gate = gate != nullptr ? rows_per_gate : 1;
+    p->scale = scale;
+    p->rows = rows;
+    p->dim = dim;
+    p->eps = eps;
+    p->h = h;
+    p->n_blocks = ceil_div(dim, klp::kScaleBlock);
+    return KLP_OK;
+}
+
+// Floats of a backward's shares: the weights', the gate's.
+struct BlockWorkspace {
+    size_t weight, post, gate;
+    size_t bytes() const { return (weight + post + gate) * sizeof(float); }
+};
+BlockWorkspace block_workspace(int64_t rows, int64_t dim, bool post, bool gate,
+                               int64_t rows_per_gate) {
+    const klp::BlockShape s = klp::block_shape(rows, dim);
+    const size_t of_rows = static_cast<size_t>(s.shares) * dim;
+    BlockWorkspace w{of_rows, post ? of_rows : 0, 0};
+    if (gate && rows_per_gate >= rows) w.gate = of_rows;
+    else if (gate && rows_per_gate > 1) w.gate = static_cast<size_t>(2 * s.groups) * dim;
+    return w;
+}
+
 size_t norm_bwd_workspace(int64_t rows, int64_t dim) {
     if (rows <= 0 || dim < 1 || dim > klp::kNormMaxDim) return 0;
     return static_cast<size_t>(klp::norm_bwd_groups(rows, dim) * dim) * sizeof(float);
@@ -1802,6 +1880,144 @@ int klp_fp8_linear(const uint8_t* x, int64_t ld_x, const float* x_scales, const 
     if (injected_failure("fp8 linear")) return KLP_ELAUNCH;
     return after_launch(klp::launch_fp8_linear(out_dtype, p, static_cast<hipStream_t>(stream)),
                         "fp8 linear");
+}
+
+int klp_block_norm(const void* x, int dtype, int64_t ld_x, const void* residual,
+                   int64_t ld_residual, const void* post_weight, const void* weight,
+                   int weight_dtype, const void* gate, int gate_dtype, int64_t rows_per_gate,
+                   float scale, int64_t rows, int64_t dim, float eps, void* y, void* h,
+                   float* rstd_x, float* rstd_h, uint8_t* x_codes, float* x_scales,
+                   uint8_t* h_codes, float* h_scales, void* stream) {
+    klp::BlockParams p;
+    const int rc = block_setup(x, dtype, ld_x, residual, ld_residual, post_weight, weight,
+                               weight_dtype, gate, gate_dtype, rows_per_gate, scale, rows, dim,
+                               eps, h, &p);
+    if (rc != KLP_OK) return rc;
+    if (rows == 0) return ok();
+    if (y == nullptr || !aligned(y, elem_bytes(dtype)))
+        return fail(KLP_EINVAL, "y must be non-null and aligned to its elements");
+    if (!aligned(rstd_x, 4) || !aligned(rstd_h, 4))
+        return fail(KLP_EINVAL, "rstd_x and rstd_h must be 4-byte aligned");
+    if ((x_codes == nullptr) != (x_scales == nullptr) ||
+        (h_codes == nullptr) != (h_scales == nullptr) || !aligned(x_scales, 4) ||
+        !aligned(h_scales, 4))
+        return fail(KLP_EINVAL, "a checkpoint's codes come with their scales, 4-byte aligned");
+    p.y = y;
+    p.rstd_x = rstd_x;
+    p.rstd_h = rstd_h;
+    p.x_codes = x_codes;
+    p.x_scales = x_scales;
+    p.h_codes = h_codes;
+    p.h_scales = h_scales;
+    if (injected_failure("block norm")) return KLP_ELAUNCH;
+    return after_launch(klp::launch_block(dtype, p, static_cast<hipStream_t>(stream)),
+                        "block norm");
+}
+
+int klp_block_norm_fp8(const void* x, int dtype, int64_t ld_x, const void* residual,
+                       int64_t ld_residual, const void* post_weight, const void* weight,
+                       int weight_dtype, const void* gate, int gate_dtype, int64_t rows_per_gate,
+                       float scale, int64_t rows, int64_t dim, float eps, uint8_t* q,
+                       float* scales, void* h, void* stream) {
+    klp::BlockParams p;
+    int rc = block_setup(x, dtype, ld_x, residual, ld_residual, post_weight, weight, weight_dtype,
+                         gate, gate_dtype, rows_per_gate, scale, rows, dim, eps, h, &p);
+    if (rc != KLP_OK) return rc;
+    if (rows == 0) return ok();
+    if (q == nullptr) return fail(KLP_EINVAL, "q must be non-null");
+    if ((rc = check_f32(scales, "scales")) != KLP_OK) return rc;
+    p.q = q;
+    p.scales = scales;
+    if (injected_failure("block norm")) return KLP_ELAUNCH;
+    return after_launch(klp::launch_block(dtype, p, static_cast<hipStream_t>(stream)),
+                        "block norm");
+}
+
+size_t klp_block_norm_bwd_workspace_bytes(int64_t rows, int64_t dim, int has_post, int has_gate,
+                                          int64_t rows_per_gate) {
+    if (rows < 1 || dim < 1 || dim > klp::kBlockMaxDim) return 0;
+    return block_workspace(rows, dim, has_post != 0, has_gate != 0, rows_per_gate).bytes();
+}
+
+int klp_block_norm_bwd(const void* x, int dtype, int64_t ld_x, const uint8_t* x_codes,
+                       const float* x_scales, const void* h, const uint8_t* h_codes,
+                       const float* h_scales, const void* post_weight, const void* weight,
+                       int weight_dtype, const void* gate, int gate_dtype, int64_t rows_per_gate,
+                       float scale, const float* rstd_x, const float* rstd_h, const void* g_y,
+                       const void* g_h, int64_t rows, int64_t dim, void* d_x, void* d_residual,
+                       void* d_post_weight, void* d_weight, void* d_gate, void* workspace,
+                       size_t workspace_bytes, void* stream) {
+    int rc = check_block(dtype, rows, dim, post_weight, weight, weight_dtype, gate, gate_dtype,
+                         rows_per_gate, scale);
+    if (rc != KLP_OK) return rc;
+    if (rows == 0) return fail(KLP_EINVAL, "rows must be >= 1");
+    const size_t e = elem_bytes(dtype);
+    const bool kept = h_codes != nullptr, needs_x = post_weight != nullptr || gate != nullptr;
+    if (kept) {
+        if ((rc = check_f32(h_scales, "h_scales")) != KLP_OK) return rc;
+        if (needs_x && x_codes == nullptr) return fail(KLP_EINVAL, "x_codes must be non-null");
+        if (needs_x && (rc = check_f32(x_scales, "x_scales")) != KLP_OK) return rc;
+    } else {
+        if (h == nullptr || !aligned(h, e))
+            return fail(KLP_EINVAL, "h must be non-null and aligned to its elements");
+        if (needs_x && (rc = check_matrix(x, ld_x, dim, e, "x")) != KLP_OK) return rc;
+    }
+    if ((rc = check_f32(rstd_h, "rstd_h")) != KLP_OK) return rc;
+    if (post_weight != nullptr && (rc = check_f32(rstd_x, "rstd_x")) != KLP_OK) return rc;
+    if ((g_y == nullptr && g_h == nullptr) || !aligned(g_y, e) || !aligned(g_h, e) ||
+        !aligned(d_x, e) || !aligned(d_residual, e))
+        return fail(KLP_EINVAL, "one of g_y and g_h must be non-null, and gradients aligned to "
+                                "their elements");
+    if (!aligned(d_post_weight, elem_bytes(weight_dtype)) ||
+        !aligned(d_weight, elem_bytes(weight_dtype)) || !aligned(d_gate, elem_bytes(gate_dtype)))
+        return fail(KLP_EINVAL, "d_post_weight, d_weight and d_gate must be aligned to their "
+                                "elements");
+    const BlockWorkspace w = block_workspace(rows, dim, post_weight != nullptr, gate != nullptr,
+                                             rows_per_gate);
+    klp::BlockBwdParams p{};
+    if (d_post_weight != nullptr || d_weight != nullptr || d_gate != nullptr) {
+        if (workspace == nullptr || workspace_bytes < w.bytes() || !aligned(workspace, 16))
+            return fail(KLP_EWORKSPACE,
+                        "workspace missing, too small or not 16-byte aligned: have %zu bytes, "
+                        "need %zu",
+                        workspace_bytes, w.bytes());
+        float* f = static_cast<float*>(workspace);
+        p.weight_shares = d_weight != nullptr ? f : nullptr;
+        p.post_shares = post_weight != nullptr && d_post_weight != nullptr ? f + w.weight : nullptr;
+        p.gate_shares = gate != nullptr && d_gate != nullptr ? f + w.weight + w.post : nullptr;
+    }
+    const klp::BlockShape s = klp::block_shape(rows, dim);
+    p.x = x;
+    p.ld_x = ld_x;
+    p.x_codes = x_codes;
+    p.x_scales = x_scales;
+    p.h = h;
+    p.h_codes = h_codes;
+    p.h_scales = h_scales;
+    p.n_blocks = ceil_div(dim, klp::kScaleBlock);
+    p.post = post_weight;
+    p.weight = weight;
+    p.weight_f32 = weight_dtype == KLP_FP32;
+    p.gate = gate;
+    p.gate_f32 = gate_dtype == KLP_FP32;
+    p.per_gate = gate != nullptr ? rows_per_gate : 1;
+    p.scale = scale;
+    p.rstd_x = rstd_x;
+    p.rstd_h = rstd_h;
+    p.g_y = g_y;
+    p.g_h = g_h;
+    p.rows = rows;
+    p.dim = dim;
+    p.groups = s.groups;
+    p.per_group = s.per_group;
+    p.d_x = d_x;
+    p.d_r = d_residual;
+    p.d_post = post_weight != nullptr ? d_post_weight : nullptr;
+    p.d_weight = d_weight;
+    p.d_gate = gate != nullptr ? d_gate : nullptr;
+    if (injected_failure("block norm backward")) return KLP_ELAUNCH;
+    return after_launch(klp::launch_block_bwd(dtype, p, static_cast<hipStream_t>(stream)),
+                        "block norm backward");
 }
 
 size_t klp_fwd_top_workspace_bytes(int dtype, int64_t n_rows, int64_t vocab, int k) {

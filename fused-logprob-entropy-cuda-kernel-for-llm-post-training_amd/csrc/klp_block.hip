@@ -1,0 +1,288 @@
+// klp_block.hip — the norms around a block: its output through a norm, a gate
+// and a residual scale into the residual stream, and the next block's norm;
+// their backward; for gfx950.
+//
+//   s_x = (mean(x^2) + eps)^-1/2,   z = x s_x wp        (z = x without wp)
+//   h = round(r + c g z)
+//   s_h = (mean(h^2) + eps)^-1/2,   y = round(h s_h w), or e4m3 codes of it
+//
+//   dh = gh + s_h (gy w - h s_h^2 mean(gy w h)),        dr = dh
+//   dz = c g dh,   dx = s_x (dz wp - x s_x^2 mean(dz wp x))   (dx = dz without)
+//   dw = sum gy h s_h,   dwp = sum dz x s_x,   dg = sum c z dh
+//
+// the sums over all rows, dg's over the rows that share a gate.  Statistics are
+// those of the stored h; all sums are float32, every output is rounded once.
+//
+// Checkpoints: the forward also leaves e4m3 codes of x and h with a float32
+// scale for each 128 columns, and the backward takes the values that they stand
+// for in place of x and h; s_x and s_h are the exact ones.  An element then
+// keeps 2.06 bytes of the block alive instead of 4.
+//
+// Bound by memory: the forward reads x and r once and writes h and y once, the
+// backward reads x, h and two gradients once and writes two, a row in the
+// registers of a group of 64 to 1024 threads, 8 elements (a chunk) a thread and
+// pass.
+//
+// Sums over rows: a group takes consecutive rows and keeps its sums in
+// registers; the groups of a workgroup are added in LDS, the workgroups' shares
+// by a second kernel in order, so that nothing depends on timing.  A gate of
+// fewer rows ends inside a group or goes on past it: whole ones are written as
+// they end, the parts of others go to the group's two shares.
+#include "klp_block.h"
+
+namespace klp {
+
+namespace {
+
+// Codes and scale of a chunk; 16 lanes hold the 128 columns of a scale.
+__device__ __forceinline__ void put_codes(const float (&v)[kChunk], uint8_t* q, float* scales,
+                                          int64_t row, int64_t dim, int64_t n_blocks, int c) {
+    const E4m3Scale e = e4m3_scale(row_max16(chunk_amax(v)));
+    if (c < dim) {
+        store_codes(q + row * dim + c, dim - c, e4m3_pack8(v, e.inv));
+        if ((threadIdx.x & 15) == 0) scales[row * n_blocks + c / kScaleBlock] = e.scale;
+    }
+}
+
+template <int DT, int T, int N, bool kWF32, bool kPost, bool kFp8>
+__global__ __launch_bounds__(kForwardThreads<T>) void klp_block_kernel(BlockParams p) {
+    typedef typename Traits<DT>::elem elem;
+    constexpr int kGroups = kForwardThreads<T> / T;
+    __shared__ float lds[kGroups][T / 64];
+    const int t = threadIdx.x % T, group = threadIdx.x / T;
+    int64_t row = static_cast<int64_t>(blockIdx.x) * kGroups + group;
+    // Groups past the last row repeat it, with the same results, and meet the
+    // others at every barrier.
+    if (row >= p.rows) row = p.rows - 1;
+    const int dim = static_cast<int>(p.dim);
+    const elem* x = static_cast<const elem*>(p.x) + row * p.ld_x;
+    const elem* r = static_cast<const elem*>(p.residual) + row * p.ld_r;
+
+    // Everything is on its way before the first sum needs it.
+    RawChunk<DT> in[N], res[N];
+    float w[N][kChunk], by[N][kChunk], wp[N][kChunk];
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+        const int c = (i * T + t) * kChunk;
+        in[i] = load_raw<DT>(x + c, dim - c);
+        res[i] = load_raw<DT>(r + c, dim - c);
+    }
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+        const int c = (i * T + t) * kChunk;
+        load_either<DT>(p.weight, kWF32, c, dim - c, w[i]);
+        if constexpr (kPost) load_either<DT>(p.post, kWF32, c, dim - c, wp[i]);
+    }
+    if (p.gate != nullptr) {
+        const int64_t at = row / p.per_gate * p.dim;
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            const int c = (i * T + t) * kChunk;
+            load_either<DT>(p.gate, p.gate_f32, at + c, dim - c, by[i]);
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < N; ++i)
+#pragma unroll
+            for (int j = 0; j < kChunk; ++j) by[i][j] = 1.0f;
+    }
+
+    float h[N][kChunk];
+#pragma unroll
+    for (int i = 0; i < N; ++i) in[i].values(h[i]);
+    if (p.x_codes != nullptr) {
+#pragma unroll
+        for (int i = 0; i < N; ++i)
+            put_codes(h[i], p.x_codes, p.x_scales, row, p.dim, p.n_blocks,
+                      (i * T + t) * kChunk);
+    }
+    if constexpr (kPost) {
+        float sum = 0.0f;
+#pragma unroll
+        for (int i = 0; i < N; ++i)
+#pragma unroll
+            for (int j = 0; j < kChunk; ++j) sum = fmaf(h[i][j], h[i][j], sum);
+        sum = group_sum<T>(sum, lds[group]);
+        const float s = 1.0f / sqrtf(sum / static_cast<float>(dim) + p.eps);
+        if (p.rstd_x != nullptr && t == 0) p.rstd_x[row] = s;
+#pragma unroll
+        for (int i = 0; i < N; ++i)
+#pragma unroll
+            for (int j = 0; j < kChunk; ++j) h[i][j] = h[i][j] * s * wp[i][j];
+    }
+    float sum = 0.0f;
+    elem* out = static_cast<elem*>(p.h) + row * p.dim;
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+        const int c = (i * T + t) * kChunk;
+        float b[kChunk];
+        res[i].values(b);
+#pragma unroll
+        for (int j = 0; j < kChunk; ++j) {
+            h[i][j] = to_f32<DT>(from_f32<DT>(fmaf(h[i][j] * by[i][j], p.scale, b[j])));
+            // Elements past the row stay 0 whatever the loads put there.
+            sum = fmaf(h[i][j], h[i][j], sum);
+        }
+        store_chunk<DT>(out + c, dim - c, h[i]);
+    }
+    if (p.h_codes != nullptr) {
+#pragma unroll
+        for (int i = 0; i < N; ++i)
+            put_codes(h[i], p.h_codes, p.h_scales, row, p.dim, p.n_blocks,
+                      (i * T + t) * kChunk);
+    }
+    sum = group_sum<T>(sum, lds[group]);
+    const float s = 1.0f / sqrtf(sum / static_cast<float>(dim) + p.eps);
+    if (p.rstd_h != nullptr && t == 0) p.rstd_h[row] = s;
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+        const int c = (i * T + t) * kChunk;
+        float y[kChunk];
+#pragma unroll
+        for (int j = 0; j < kChunk; ++j) y[j] = h[i][j] * s * w[i][j];
+        if constexpr (kFp8) put_codes(y, p.q, p.scales, row, p.dim, p.n_blocks, c);
+        else store_chunk<DT>(static_cast<elem*>(p.y) + row * p.dim + c, dim - c, y);
+    }
+}
+
+// out[c] = the shares of column c added in order: 64 columns a workgroup, its
+// 16 waves take every 16th share and are added in order.
+struct BlockSumParams {
+    const float* shares;
+    int64_t n;
+    int64_t dim;
+    void* out;
+    int dtype;
+};
+constexpr int kSumWaves = 16;
+__device__ __forceinline__ void put_either(void* out, int dtype, int64_t at, float v) {
+    switch (dtype) {
+        case kBF16: static_cast<uint16_t*>(out)[at] = from_f32<kBF16>(v); break;
+        case kFP16: static_cast<uint16_t*>(out)[at] = from_f32<kFP16>(v); break;
+        default: static_cast<float*>(out)[at] = v;
+    }
+}
+struct BlockSums {
+    BlockSumParams of[3];
+};
+__global__ __launch_bounds__(kSumWaves * 64) void klp_block_sum_kernel(BlockSums all) {
+    const BlockSumParams& p = all.of[blockIdx.y];
+    __shared__ float part[kSumWaves][64];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int64_t c = static_cast<int64_t>(blockIdx.x) * 64 + lane;
+    float s = 0.0f;
+    if (c < p.dim) {
+#pragma unroll 8
+        for (int64_t g = wave; g < p.n; g += kSumWaves) s += p.shares[g * p.dim + c];
+    }
+    part[wave][lane] = s;
+    __syncthreads();
+    if (wave == 0 && c < p.dim) {
+#pragma unroll
+        for (int i = 1; i < kSumWaves; ++i) s += part[i][lane];
+        put_either(p.out, p.dtype, c, s);
+    }
+}
+
+// Gates whose rows several groups took: the one that begins in group
+// blockIdx.y, if it goes on behind it, from that group's last share and the
+// others' first ones, in order.
+__global__ __launch_bounds__(256) void klp_block_gate_kernel(BlockBwdParams p, int dtype) {
+    const int64_t q = blockIdx.y;
+    const int64_t first = q * p.per_group;
+    const int64_t end = first + p.per_group < p.rows ? first + p.per_group : p.rows;
+    if (first >= end) return;
+    const int64_t gate = (end - 1) / p.per_gate;
+    const int64_t last = (gate + 1) * p.per_gate < p.rows ? (gate + 1) * p.per_gate : p.rows;
+    if (gate * p.per_gate < first || last <= end) return;
+    const int64_t c = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
+    if (c >= p.dim) return;
+    const int64_t to = (last - 1) / p.per_group;
+    float s = p.gate_shares[(2 * q + 1) * p.dim + c];
+    for (int64_t g = q + 1; g <= to; ++g) s += p.gate_shares[2 * g * p.dim + c];
+    put_either(p.d_gate, dtype, gate * p.dim + c, s);
+}
+
+template <int DT, int T, int N, bool kWF32>
+hipError_t launch_block_shape(const BlockParams& p, hipStream_t stream) {
+    constexpr int kThreads = kForwardThreads<T>, kGroups = kThreads / T;
+    const dim3 grid(static_cast<unsigned>((p.rows + kGroups - 1) / kGroups)), block(kThreads);
+    const auto launch = [&](auto kernel) {
+        return launch_kernel(kernel, grid, block, stream, p);
+    };
+    if (p.q != nullptr)
+        return p.post != nullptr ? launch(klp_block_kernel<DT, T, N, kWF32, true, true>)
+                                 : launch(klp_block_kernel<DT, T, N, kWF32, false, true>);
+    return p.post != nullptr ? launch(klp_block_kernel<DT, T, N, kWF32, true, false>)
+                             : launch(klp_block_kernel<DT, T, N, kWF32, false, false>);
+}
+
+template <int DT>
+hipError_t launch_block_dt(const BlockParams& p, hipStream_t stream) {
+    return with_shape(p.dim, [&](auto t, auto n) {
+        constexpr int T = decltype(t)::value, N = decltype(n)::value;
+        return DT == kFP32 || p.weight_f32 ? launch_block_shape<DT, T, N, true>(p, stream)
+                                           : launch_block_shape<DT, T, N, DT == kFP32>(p, stream);
+    });
+}
+}  // namespace
+
+hipError_t launch_block(int dtype, const BlockParams& p, hipStream_t stream) {
+    switch (dtype) {
+        case kBF16: return launch_block_dt<kBF16>(p, stream);
+        case kFP16: return launch_block_dt<kFP16>(p, stream);
+        case kFP32: return launch_block_dt<kFP32>(p, stream);
+        default: return hipErrorInvalidValue;
+    }
+}
+
+// Groups of the backward: 1024 threads a CU, and no more than rows.
+BlockShape block_shape(int64_t rows, int64_t dim) {
+    return with_shape(dim, [&](auto t, auto) {
+        constexpr int T = decltype(t)::value;
+        constexpr int kGroups = kBackwardThreads<T> / T;
+        BlockShape s;
+        s.groups = kNormBwdThreads / T < rows ? kNormBwdThreads / T : rows;
+        s.per_group = (rows + s.groups - 1) / s.groups;
+        s.groups = (rows + s.per_group - 1) / s.per_group;
+        s.shares = (s.groups + kGroups - 1) / kGroups;
+        return s;
+    });
+}
+
+hipError_t launch_block_bwd(int dtype, const BlockBwdParams& p, hipStream_t stream) {
+    hipError_t e = hipErrorInvalidValue;
+    switch (dtype) {
+        case kBF16: e = launch_block_rows<kBF16>(p, stream); break;
+        case kFP16: e = launch_block_rows<kFP16>(p, stream); break;
+        case kFP32: e = launch_block_rows<kFP32>(p, stream); break;
+        default: break;
+    }
+    if (e != hipSuccess) return e;
+    const int weight_dtype = p.weight_f32 ? kFP32 : dtype;
+    const int gate_dtype = p.gate_f32 ? kFP32 : dtype;
+    const int64_t shares = block_shape(p.rows, p.dim).shares;
+    const bool one_gate = p.gate != nullptr && p.per_gate >= p.rows;
+    BlockSums sums{};
+    int n = 0;
+    if (p.d_weight != nullptr)
+        sums.of[n++] = BlockSumParams{p.weight_shares, shares, p.dim, p.d_weight, weight_dtype};
+    if (p.d_post != nullptr)
+        sums.of[n++] = BlockSumParams{p.post_shares, shares, p.dim, p.d_post, weight_dtype};
+    if (one_gate && p.d_gate != nullptr)
+        sums.of[n++] = BlockSumParams{p.gate_shares, shares, p.dim, p.d_gate, gate_dtype};
+    if (n > 0) {
+        const dim3 grid(static_cast<unsigned>((p.dim + 63) / 64), static_cast<unsigned>(n));
+        e = launch_kernel(klp_block_sum_kernel, grid, dim3(kSumWaves * 64), stream, sums);
+        if (e != hipSuccess) return e;
+    }
+    // A gate of one row lies in one group.
+    if (p.gate != nullptr && !one_gate && p.d_gate != nullptr && p.per_gate > 1) {
+        const dim3 grid(static_cast<unsigned>((p.dim + 255) / 256),
+                        static_cast<unsigned>(p.groups));
+        e = launch_kernel(klp_block_gate_kernel, grid, dim3(256), stream, p, gate_dtype);
+    }
+    return e;
+}
+
+}  // namespace klp

@@ -1,0 +1,253 @@
+// klp_block_bwd.h — the rows' pass of the backward of the norms around a block
+// (the formulas: klp_block.hip); each dtype's instances are a file of their own.
+#pragma once
+
+#include "klp_block.h"
+
+namespace klp {
+
+namespace {
+
+// A row's x or h: as stored, or the values of its checkpoint.
+template <int DT, bool kKept>
+struct Stored {
+    RawChunk<DT> raw;
+    __device__ __forceinline__ void load(const void* rows, int64_t ld, const uint8_t*,
+                                         const float*, int64_t row, int64_t, int64_t, int c,
+                                         int left) {
+        raw = load_raw<DT>(static_cast<const typename Traits<DT>::elem*>(rows) + row * ld + c,
+                           left);
+    }
+    __device__ __forceinline__ void values(float (&x)[kChunk]) const { raw.values(x); }
+};
+template <int DT>
+struct Stored<DT, true> {
+    uint2 codes;
+    float scale;
+    __device__ __forceinline__ void load(const void*, int64_t, const uint8_t* q,
+                                         const float* scales, int64_t row, int64_t dim,
+                                         int64_t n_blocks, int c, int left) {
+        codes = load_codes(q + row * dim + c, left);
+        scale = left > 0 ? scales[row * n_blocks + c / kScaleBlock] : 0.0f;
+    }
+    __device__ __forceinline__ void values(float (&x)[kChunk]) const {
+        code_values(codes, scale, x);
+    }
+};
+
+// kGate: 0 none, 1 one for all rows, 2 one for every per_gate rows.
+template <int DT, int T, int N, bool kWF32, bool kPost, int kGate, bool kKept>
+__global__ __launch_bounds__(kBackwardThreads<T>) void klp_block_bwd_kernel(BlockBwdParams p) {
+    typedef typename Traits<DT>::elem elem;
+    constexpr int kGroups = kBackwardThreads<T> / T;
+    constexpr int kCols = T * N * kChunk;
+    constexpr bool kX = kPost || kGate != 0;  // x enters a gradient
+    __shared__ float lds[kGroups][T / 64];
+    // Sums of the other groups of the workgroup, a third of a group's columns at
+    // a time would do; all of one kind at a time here.
+    __shared__ float meet[kGroups > 1 ? (kGroups - 1) * kCols : 1];
+    const int t = threadIdx.x % T, in_block = threadIdx.x / T;
+    const int64_t group = static_cast<int64_t>(blockIdx.x) * kGroups + in_block;
+    const int dim = static_cast<int>(p.dim);
+    const float inv_dim = 1.0f / static_cast<float>(dim);
+    const int64_t first = group * p.per_group;
+    const int64_t end = first + p.per_group < p.rows ? first + p.per_group : p.rows;
+
+    float dw[N][kChunk], dp[kPost ? N : 1][kChunk], dg[kGate != 0 ? N : 1][kChunk];
+#pragma unroll
+    for (int i = 0; i < N; ++i)
+#pragma unroll
+        for (int j = 0; j < kChunk; ++j) {
+            dw[i][j] = 0.0f;
+            if constexpr (kPost) dp[i][j] = 0.0f;
+            if constexpr (kGate != 0) dg[i][j] = 0.0f;
+        }
+
+    Stored<DT, kKept> hs[N], xs[kX ? N : 1];
+    RawChunk<DT> gys[N], ghs[N];
+    auto load_row = [&](int64_t row) {
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            const int c = (i * T + t) * kChunk;
+            const int left = dim - c;
+            hs[i].load(p.h, p.dim, p.h_codes, p.h_scales, row, p.dim, p.n_blocks, c, left);
+            if constexpr (kX)
+                xs[i].load(p.x, p.ld_x, p.x_codes, p.x_scales, row, p.dim, p.n_blocks, c, left);
+            gys[i] = load_raw<DT>(static_cast<const elem*>(p.g_y) + row * p.dim + c,
+                                  p.g_y != nullptr ? left : 0);
+            ghs[i] = load_raw<DT>(static_cast<const elem*>(p.g_h) + row * p.dim + c,
+                                  p.g_h != nullptr ? left : 0);
+        }
+    };
+    // The groups of a workgroup take the same number of steps (p.per_group), for
+    // their barriers; a step past the group's rows does nothing else.
+    for (int64_t step = 0; step < p.per_group; ++step) {
+        const int64_t row = first + step;
+        const bool live = row < end;
+        const int64_t at = live ? row : p.rows - 1;
+        load_row(at);
+        const float s_h = p.rstd_h[at];
+        const float s_x = kPost ? p.rstd_x[at] : 1.0f;
+        const int64_t gate_row = kGate == 2 ? at / p.per_gate : 0;
+
+        float dh[N][kChunk], dot = 0.0f;
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            const int c = (i * T + t) * kChunk;
+            float w[kChunk], h[kChunk], g[kChunk];
+            load_either<DT>(p.weight, kWF32, c, dim - c, w);
+            hs[i].values(h);
+            gys[i].values(g);
+#pragma unroll
+            for (int j = 0; j < kChunk; ++j) {
+                if (live) dw[i][j] = fmaf(g[j] * s_h, h[j], dw[i][j]);
+                dh[i][j] = g[j] * w[j];
+                dot = fmaf(dh[i][j], h[j], dot);
+            }
+        }
+        dot = group_sum<T>(dot, lds[in_block]);
+        const float a_h = s_h * s_h * dot * inv_dim;
+        float dot_x = 0.0f;
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            const int c = (i * T + t) * kChunk;
+            float h[kChunk], gh[kChunk], x[kChunk], by[kChunk], wp[kChunk];
+            hs[i].values(h);
+            ghs[i].values(gh);
+#pragma unroll
+            for (int j = 0; j < kChunk; ++j)
+                dh[i][j] = fmaf(s_h, fmaf(-a_h, h[j], dh[i][j]), gh[j]);
+            if (live && p.d_r != nullptr)
+                store_chunk<DT>(static_cast<elem*>(p.d_r) + row * p.dim + c, dim - c, dh[i]);
+            if constexpr (kX) xs[i].values(x);
+            if constexpr (kPost) load_either<DT>(p.post, kWF32, c, dim - c, wp);
+            if constexpr (kGate != 0)
+                load_either<DT>(p.gate, p.gate_f32, gate_row * p.dim + c, dim - c, by);
+#pragma unroll
+            for (int j = 0; j < kChunk; ++j) {
+                const float d = dh[i][j] * p.scale;  // c dh
+                if constexpr (kGate != 0) {
+                    const float z = kPost ? x[j] * s_x * wp[j] : x[j];
+                    if (live) dg[i][j] = fmaf(d, z, dg[i][j]);
+                }
+                float dz = kGate != 0 ? d * by[j] : d;
+                if constexpr (kPost) {
+                    if (live) dp[i][j] = fmaf(dz * s_x, x[j], dp[i][j]);
+                    dz *= wp[j];
+                    dot_x = fmaf(dz, x[j], dot_x);
+                }
+                dh[i][j] = dz;
+            }
+        }
+        float a_x = 0.0f;
+        if constexpr (kPost) {
+            dot_x = group_sum<T>(dot_x, lds[in_block]);
+            a_x = s_x * s_x * dot_x * inv_dim;
+        }
+        if (live && p.d_x != nullptr) {
+#pragma unroll
+            for (int i = 0; i < N; ++i) {
+                const int c = (i * T + t) * kChunk;
+                if constexpr (kPost) {
+                    float x[kChunk];
+                    xs[i].values(x);
+#pragma unroll
+                    for (int j = 0; j < kChunk; ++j)
+                        dh[i][j] = s_x * fmaf(-a_x, x[j], dh[i][j]);
+                }
+                store_chunk<DT>(static_cast<elem*>(p.d_x) + row * p.dim + c, dim - c, dh[i]);
+            }
+        }
+        if constexpr (kGate == 2) {
+            // The gate's rows end here, or the group's do.
+            const bool gate_ends = row + 1 == p.rows || (row + 1) % p.per_gate == 0;
+            if (live && p.d_gate != nullptr && (gate_ends || row + 1 == end)) {
+                const bool begun_here = gate_row * p.per_gate >= first;
+                const int64_t from = gate_row * p.dim;
+                float* share = p.gate_shares + (2 * group + (begun_here ? 1 : 0)) * p.dim;
+#pragma unroll
+                for (int i = 0; i < N; ++i) {
+                    const int c = (i * T + t) * kChunk;
+                    if (!(gate_ends && begun_here))
+                        store_chunk<kFP32>(reinterpret_cast<uint32_t*>(share) + c, dim - c,
+                                           dg[i]);
+                    else if (DT == kFP32 || p.gate_f32)
+                        store_chunk<kFP32>(static_cast<uint32_t*>(p.d_gate) + from + c, dim - c,
+                                           dg[i]);
+                    else
+                        store_chunk<DT>(static_cast<elem*>(p.d_gate) + from + c, dim - c, dg[i]);
+#pragma unroll
+                    for (int j = 0; j < kChunk; ++j) dg[i][j] = 0.0f;
+                }
+            }
+        }
+    }
+
+    // The workgroup's sums: its groups' in order, into its share.
+    auto share = [&](float (&sum)[N][kChunk], float* shares) {
+        if (shares == nullptr) return;
+        if constexpr (kGroups > 1) {
+            __syncthreads();
+            if (in_block > 0) {
+#pragma unroll
+                for (int i = 0; i < N; ++i)
+#pragma unroll
+                    for (int j = 0; j < kChunk; ++j)
+                        meet[(in_block - 1) * kCols + (i * kChunk + j) * T + t] = sum[i][j];
+            }
+            __syncthreads();
+            if (in_block > 0) return;
+#pragma unroll
+            for (int q = 0; q < kGroups - 1; ++q)
+#pragma unroll
+                for (int i = 0; i < N; ++i)
+#pragma unroll
+                    for (int j = 0; j < kChunk; ++j)
+                        sum[i][j] += meet[q * kCols + (i * kChunk + j) * T + t];
+        }
+        uint32_t* to = reinterpret_cast<uint32_t*>(shares) + blockIdx.x * p.dim;
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            const int c = (i * T + t) * kChunk;
+            store_chunk<kFP32>(to + c, dim - c, sum[i]);
+        }
+    };
+    share(dw, p.weight_shares);
+    if constexpr (kPost) share(dp, p.post_shares);
+    if constexpr (kGate == 1) share(dg, p.gate_shares);
+}
+
+template <int DT, int T, int N, bool kWF32, bool kPost, int kGate>
+hipError_t launch_bwd_kept(const BlockBwdParams& p, hipStream_t stream) {
+    constexpr int kThreads = kBackwardThreads<T>, kGroups = kThreads / T;
+    const dim3 grid(static_cast<unsigned>((p.groups + kGroups - 1) / kGroups)), block(kThreads);
+    return p.h_codes != nullptr
+               ? launch_kernel(klp_block_bwd_kernel<DT, T, N, kWF32, kPost, kGate, true>, grid,
+                               block, stream, p)
+               : launch_kernel(klp_block_bwd_kernel<DT, T, N, kWF32, kPost, kGate, false>, grid,
+                               block, stream, p);
+}
+template <int DT, int T, int N, bool kWF32, bool kPost>
+hipError_t launch_bwd_gate(const BlockBwdParams& p, hipStream_t stream) {
+    if (p.gate == nullptr) return launch_bwd_kept<DT, T, N, kWF32, kPost, 0>(p, stream);
+    return p.per_gate >= p.rows ? launch_bwd_kept<DT, T, N, kWF32, kPost, 1>(p, stream)
+                                : launch_bwd_kept<DT, T, N, kWF32, kPost, 2>(p, stream);
+}
+template <int DT, int T, int N, bool kWF32>
+hipError_t launch_bwd_shape(const BlockBwdParams& p, hipStream_t stream) {
+    return p.post != nullptr ? launch_bwd_gate<DT, T, N, kWF32, true>(p, stream)
+                             : launch_bwd_gate<DT, T, N, kWF32, false>(p, stream);
+}
+
+template <int DT>
+hipError_t launch_rows_dt(const BlockBwdParams& p, hipStream_t stream) {
+    return with_shape(p.dim, [&](auto t, auto n) {
+        constexpr int T = decltype(t)::value, N = decltype(n)::value;
+        return DT == kFP32 || p.weight_f32 ? launch_bwd_shape<DT, T, N, true>(p, stream)
+                                           : launch_bwd_shape<DT, T, N, DT == kFP32>(p, stream);
+    });
+}
+
+}  // namespace
+
+}  // namespace klp

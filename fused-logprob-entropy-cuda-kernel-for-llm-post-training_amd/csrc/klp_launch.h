@@ -335,6 +335,79 @@ hipError_t launch_norm(int dtype, const NormParams& p, hipStream_t stream);
 hipError_t launch_norm_bwd(int dtype, const NormBwdParams& p, hipStream_t stream);
 hipError_t launch_norm_dw(int weight_dtype, const NormBwdParams& p, hipStream_t stream);
 
+// The norms around a block (klp_block.hip).  Rows of x and residual at row
+// strides; every other array dense.
+constexpr int64_t kBlockMaxDim = 16384;
+struct BlockParams {
+    const void* x;         // [rows, ld_x]
+    int64_t ld_x;
+    const void* residual;  // [rows, ld_r]
+    int64_t ld_r;
+    const void* post;      // [dim], nullable: no norm behind the block
+    const void* weight;    // [dim]; both float32 with weight_f32, else of the rows' dtype
+    int weight_f32;
+    const void* gate;      // [ceil(rows / per_gate), dim], nullable
+    int gate_f32;
+    int64_t per_gate;      // consecutive rows that share a gate
+    float scale;
+    int64_t rows;
+    int64_t dim;
+    float eps;
+    void* h;               // [rows, dim]
+    void* y;               // [rows, dim]
+    float* rstd_x;         // [rows], nullable; with `post`
+    float* rstd_h;         // [rows], nullable
+    uint8_t* q;            // [rows, dim] e4m3 codes, instead of y; nullable
+    float* scales;         // [rows, n_blocks]
+    uint8_t* x_codes;      // checkpoints of x and h: codes [rows, dim], nullable,
+    float* x_scales;       // and scales [rows, n_blocks]
+    uint8_t* h_codes;
+    float* h_scales;
+    int64_t n_blocks;      // ceil(dim / kScaleBlock)
+};
+struct BlockBwdParams {
+    const void* x;         // [rows, ld_x], or x_codes and x_scales; null: not needed
+    int64_t ld_x;
+    const uint8_t* x_codes;
+    const float* x_scales;
+    const void* h;         // [rows, dim], or h_codes and h_scales
+    const uint8_t* h_codes;
+    const float* h_scales;
+    int64_t n_blocks;
+    const void* post;
+    const void* weight;
+    int weight_f32;
+    const void* gate;
+    int gate_f32;
+    int64_t per_gate;
+    float scale;
+    const float* rstd_x;
+    const float* rstd_h;
+    const void* g_y;       // [rows, dim], nullable
+    const void* g_h;       // [rows, dim], nullable
+    int64_t rows;
+    int64_t dim;
+    int64_t groups;        // block_groups(rows, dim), of per_group consecutive rows
+    int64_t per_group;
+    void* d_x;             // [rows, dim], nullable
+    void* d_r;             // [rows, dim], nullable
+    void* d_post;          // [dim], nullable
+    void* d_weight;        // [dim], nullable
+    void* d_gate;          // as gate, nullable
+    // Float32 sums of the workgroups (of their groups' rows) for d_post,
+    // d_weight and a gate that all rows share, [block_shares][dim] each; and
+    // of the first and last gate of every group, [2 groups][dim].
+    float* post_shares;
+    float* weight_shares;
+    float* gate_shares;
+};
+struct BlockShape {
+    int64_t groups, per_group, shares;
+};
+BlockShape block_shape(int64_t rows, int64_t dim);
+hipError_t launch_block(int dtype, const BlockParams& p, hipStream_t stream);
+hipError_t launch_block_bwd(int dtype, const BlockBwdParams& p, hipStream_t stream);
+
 // e4m3 codes and scales (klp_fp8.hip): 128 elements of a row share a scale,
 // or 128 x 128 elements do.
 struct QuantizeParams {

@@ -36,22 +36,6 @@ namespace {
 
 constexpr int kBlockThreads = 256;
 
-// Sum over a group of T threads (T = 64: one wave of the workgroup).
-template <int T>
-__device__ __forceinline__ float group_sum(float v, float* lds) {
-    v = xrow_sum(row_sum16(v));
-    if constexpr (T > 64) {
-        const int wave = threadIdx.x >> 6;
-        __syncthreads();  // the last sum's readers
-        if ((threadIdx.x & 63) == 0) lds[wave] = v;
-        __syncthreads();
-        v = lds[0];
-#pragma unroll
-        for (int i = 1; i < T / 64; ++i) v += lds[i];
-    }
-    return v;
-}
-
 template <bool kF32, int DT>
 __device__ __forceinline__ void load_weight(const void* w, int64_t at, int64_t left,
                                             float (&x)[kChunk]) {

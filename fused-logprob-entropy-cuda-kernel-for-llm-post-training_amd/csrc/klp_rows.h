@@ -16,17 +16,29 @@ struct __attribute__((packed, aligned(alignof(E)))) Unaligned16 {
     u32x4 v;
 };
 
-// x[j] = p[j] for j < left, 0 (or with kNegInf -inf) behind; all 8 when left
-// >= 8.  Two branches of one side each, on conditions that the compiler cannot
-// join to an if and else: its registers are then written before either, and on
-// no path hold what another wave left.
+// A chunk as it lies in memory.
+template <int DT>
+struct RawChunk {
+    static constexpr int kVecs = DT == kFP32 ? 2 : 1;
+    u32x4 v[kVecs];
+    __device__ __forceinline__ void values(float (&x)[kChunk]) const {
+        unpack<DT>(v[0], x);
+        if constexpr (DT == kFP32) unpack<DT>(v[1], x + 4);
+    }
+};
+
+// p[j] for j < left, 0 (or with kNegInf -inf) behind; all 8 when left >= 8.
+// Two branches of one side each, on conditions that the compiler cannot join to
+// an if and else: its registers are then written before either, and on no path
+// hold what another wave left.
 template <int DT, bool kNegInf = false>
-__device__ __forceinline__ void load_chunk(const typename Traits<DT>::elem* p, int64_t left,
-                                           float (&x)[kChunk]) {
+__device__ __forceinline__ RawChunk<DT> load_raw(const typename Traits<DT>::elem* p,
+                                                 int64_t left) {
     typedef typename Traits<DT>::elem elem;
-    constexpr int kVecs = DT == kFP32 ? 2 : 1;
+    constexpr int kVecs = RawChunk<DT>::kVecs;
     constexpr uint32_t kFill = kNegInf ? Traits<DT>::kNegInfWord : 0;
-    u32x4 raw[kVecs];
+    RawChunk<DT> chunk;
+    u32x4 (&raw)[kVecs] = chunk.v;
 #pragma unroll
     for (int k = 0; k < kVecs; ++k) raw[k] = u32x4{kFill, kFill, kFill, kFill};
     if (left >= kChunk) {
@@ -49,8 +61,12 @@ __device__ __forceinline__ void load_chunk(const typename Traits<DT>::elem* p, i
             else raw[0][j / 2] = w;
         }
     }
-    unpack<DT>(raw[0], x);
-    if constexpr (DT == kFP32) unpack<DT>(raw[1], x + 4);
+    return chunk;
+}
+template <int DT, bool kNegInf = false>
+__device__ __forceinline__ void load_chunk(const typename Traits<DT>::elem* p, int64_t left,
+                                           float (&x)[kChunk]) {
+    load_raw<DT, kNegInf>(p, left).values(x);
 }
 
 // p[j] = round(x[j]) for j < left.
@@ -115,6 +131,58 @@ __device__ __forceinline__ void store_codes(uint8_t* p, int64_t left, uint2 w) {
         for (int j = 0; j < kChunk; ++j)
             if (j < left) p[j] = static_cast<uint8_t>((j < 4 ? w.x : w.y) >> (8 * (j & 3)));
     }
+}
+
+// 8 codes, 0 behind `left`; the values they stand for are theirs times the
+// block's scale.
+__device__ __forceinline__ uint2 load_codes(const uint8_t* p, int64_t left) {
+    uint2 w = make_uint2(0, 0);
+    if (left >= kChunk) {
+        const Unaligned8 v = *reinterpret_cast<const Unaligned8*>(p);
+        w = make_uint2(v.lo, v.hi);
+    }
+    asm("" : "+v"(w.x), "+v"(w.y));
+    int some = left > 0 && left < kChunk ? static_cast<int>(left) : 0;
+    asm("" : "+v"(some));
+    if (some > 0) {
+#pragma unroll
+        for (int j = 0; j < kChunk; ++j) {
+            const uint32_t e = p[j < some ? j : some - 1];
+            const uint32_t b = j < some ? e << (8 * (j & 3)) : 0;
+            if (j < 4) w.x |= b;
+            else w.y |= b;
+        }
+    }
+    return w;
+}
+__device__ __forceinline__ void code_values(uint2 w, float scale, float (&x)[kChunk]) {
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+        const int v = static_cast<int>(h ? w.y : w.x);
+        const f32x2 lo = __builtin_amdgcn_cvt_pk_f32_fp8(v, false);
+        const f32x2 hi = __builtin_amdgcn_cvt_pk_f32_fp8(v, true);
+        x[4 * h] = lo[0] * scale;
+        x[4 * h + 1] = lo[1] * scale;
+        x[4 * h + 2] = hi[0] * scale;
+        x[4 * h + 3] = hi[1] * scale;
+    }
+}
+
+// Sum over a group of T threads (T = 64: one wave of the workgroup), `lds` of
+// T / 64 floats.
+template <int T>
+__device__ __forceinline__ float group_sum(float v, float* lds) {
+    v = xrow_sum(row_sum16(v));
+    if constexpr (T > 64) {
+        const int wave = (threadIdx.x % T) >> 6;
+        __syncthreads();  // the last sum's readers
+        if ((threadIdx.x & 63) == 0) lds[wave] = v;
+        __syncthreads();
+        v = lds[0];
+#pragma unroll
+        for (int i = 1; i < T / 64; ++i) v += lds[i];
+    }
+    return v;
 }
 
 // Largest magnitude of a chunk; a NaN among them is the result.

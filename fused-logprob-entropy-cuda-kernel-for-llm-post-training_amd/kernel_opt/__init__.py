@@ -25,6 +25,7 @@ from .norm import (  # noqa: F401
     fused_rms_norm,
     fused_rms_norm_fp8,
 )
+from .block import fused_block_norm, fused_block_norm_fp8  # noqa: F401
 from .fp8 import fp8_linear, quantize_fp8  # noqa: F401
 from .sample import fused_sample  # noqa: F401
 from .top import fused_top_logprobs  # noqa: F401

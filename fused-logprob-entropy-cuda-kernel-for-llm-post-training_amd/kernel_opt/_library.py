@@ -103,6 +103,14 @@ SIGNATURES = {
                               _vp]),
     "klp_sample": (_i32, _ROWS + [_vp, ctypes.c_float, _vp, ctypes.c_int32, _vp, ctypes.c_float,
                                   _vp, ctypes.c_float, _vp, _vp, _vp, _vp, _vp]),
+    "klp_block_norm": (_i32, [_vp, _i32, _i64, _vp, _i64, _vp, _vp, _i32, _vp, _i32, _i64,
+                              ctypes.c_float, _i64, _i64, ctypes.c_float] + [_vp] * 9),
+    "klp_block_norm_fp8": (_i32, [_vp, _i32, _i64, _vp, _i64, _vp, _vp, _i32, _vp, _i32, _i64,
+                                  ctypes.c_float, _i64, _i64, ctypes.c_float] + [_vp] * 4),
+    "klp_block_norm_bwd_workspace_bytes": (_sz, [_i64, _i64, _i32, _i32, _i64]),
+    "klp_block_norm_bwd": (_i32, [_vp, _i32, _i64] + [_vp] * 7 + [_i32, _vp, _i32, _i64,
+                                  ctypes.c_float] + [_vp] * 4 + [_i64, _i64] + [_vp] * 6
+                           + [_sz, _vp]),
     "klp_fwd_top_workspace_bytes": (_sz, [_i32, _i64, _i64, _i32]),
     "klp_fwd_top": (_i32, _ROWS + [_vp, ctypes.c_float, _i32] + [_vp] * 7 + [_sz, _vp]),
     "klp_bwd_top": (_i32, _ROWS + [_vp, ctypes.c_float, _i32] + [_vp] * 9),

@@ -639,6 +639,62 @@ int klp_sample(const void* logits, int dtype, int64_t n_rows, int64_t vocab, int
                int64_t* tokens, float* logp, float* sample_logp, void* stream);
 
 /*
+ * The norms around a block, its gate and residual scale.  Per row of x
+ * [rows, ld_x] (the block's output) and residual [rows, ld_residual]:
+ *   z = x rstd_x post_weight,  rstd_x = (mean(x^2) + eps)^-1/2
+ *       (z = x with post_weight NULL)
+ *   h = round(residual + scale gate z)   (gate NULL: 1)
+ *   y = round(h rstd_h weight),  rstd_h = (mean(h^2) + eps)^-1/2
+ * post_weight and weight [dim] are of weight_dtype, gate [ceil(rows /
+ * rows_per_gate), dim] of gate_dtype, each `dtype` or KLP_FP32: row r takes
+ * gate row r / rows_per_gate.  y and h [rows, dim] are dense.  rstd_x, rstd_h
+ * (nullable, float32 [rows]) are what the backward needs.  With x_codes /
+ * x_scales or h_codes / h_scales non-null the call also leaves klp_quantize_fp8's
+ * codes and scales (block_rows 1) of x or of h: checkpoints for the backward.
+ * Sums are float32, h and y are rounded once.  dim is at most 16384, rows
+ * below 2^22 (KLP_EINVAL).
+ */
+int klp_block_norm(const void* x, int dtype, int64_t ld_x, const void* residual,
+                   int64_t ld_residual, const void* post_weight, const void* weight,
+                   int weight_dtype, const void* gate, int gate_dtype, int64_t rows_per_gate,
+                   float scale, int64_t rows, int64_t dim, float eps, void* y, void* h,
+                   float* rstd_x, float* rstd_h, uint8_t* x_codes, float* x_scales,
+                   uint8_t* h_codes, float* h_scales, void* stream);
+
+/* The same with y as klp_rms_norm_fp8's codes q and scales. */
+int klp_block_norm_fp8(const void* x, int dtype, int64_t ld_x, const void* residual,
+                       int64_t ld_residual, const void* post_weight, const void* weight,
+                       int weight_dtype, const void* gate, int gate_dtype, int64_t rows_per_gate,
+                       float scale, int64_t rows, int64_t dim, float eps, uint8_t* q,
+                       float* scales, void* h, void* stream);
+
+/*
+ * Backward of klp_block_norm from the gradients of y and h (one may be NULL: 0),
+ * dense [rows, dim], with x, h and the statistics of the forward:
+ *   dh = g_h + rstd_h (g_y w - h rstd_h^2 mean(g_y w h)),  d_residual = dh
+ *   dz = scale gate dh
+ *   d_x = rstd_x (dz wp - x rstd_x^2 mean(dz wp x))   (dz with post_weight NULL)
+ *   d_weight = sum g_y h rstd_h,  d_post_weight = sum dz x rstd_x  over all rows
+ *   d_gate = sum scale z dh  over the rows that share a gate
+ * each rounded once, NULL where it is not wanted.  With h_codes non-null, h and
+ * x are the values of their checkpoints (h_codes, h_scales and, where there is a
+ * post_weight or a gate, x_codes, x_scales), and `h` and `x` are not read; x is
+ * not read either where there is neither.  d_post_weight, d_weight and d_gate
+ * need the workspace (16-byte aligned, any contents, shared only by calls
+ * ordered on one stream).  Sums have a fixed order for given sizes.
+ */
+size_t klp_block_norm_bwd_workspace_bytes(int64_t rows, int64_t dim, int has_post, int has_gate,
+                                          int64_t rows_per_gate);
+int klp_block_norm_bwd(const void* x, int dtype, int64_t ld_x, const uint8_t* x_codes,
+                       const float* x_scales, const void* h, const uint8_t* h_codes,
+                       const float* h_scales, const void* post_weight, const void* weight,
+                       int weight_dtype, const void* gate, int gate_dtype, int64_t rows_per_gate,
+                       float scale, const float* rstd_x, const float* rstd_h, const void* g_y,
+                       const void* g_h, int64_t rows, int64_t dim, void* d_x, void* d_residual,
+                       void* d_post_weight, void* d_weight, void* d_gate, void* workspace,
+                       size_t workspace_bytes, void* stream);
+
+/*
  * Log-probabilities of given tokens with alternatives, in one read of the
  * logits (row addressing and targets as above).  With y = x / T and the row
  * ordered by falling x (equal ones by index, -0 equal to +0):
