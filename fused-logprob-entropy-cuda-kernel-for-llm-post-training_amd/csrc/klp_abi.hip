@@ -12,6 +12,7 @@
 #include <math.h>
 #include <string.h>
 
+#include <initializer_list>
 #include <mutex>
 #include <string>
 
@@ -838,6 +839,15 @@ int check_block(int dtype, int64_t rows, int64_t dim, const void* post, const vo
     return KLP_OK;
 }
 
+// Whether rows of dim elements at these addresses and row strides are whole
+// 16-byte vectors (codes: of 8 bytes).
+bool whole_rows(int64_t dim, int64_t ld, size_t size, std::initializer_list<const void*> at) {
+    if (dim % 8 != 0 || (ld * static_cast<int64_t>(size)) % 16 != 0) return false;
+    for (const void* p : at)
+        if (!aligned(p, 16)) return false;
+    return true;
+}
+
 // The forward's operands into p, but for y.
 int block_setup(const void* x, int dtype, int64_t ld_x, const void* residual, int64_t ld_residual,
                 const void* post, const void* weight, int weight_dtype, const void* gate,
@@ -870,6 +880,8 @@ int block_setup(const void* x, int dtype, int64_t ld_x, const void* residual, in
     p->eps = eps;
     p->h = h;
     p->n_blocks = ceil_div(dim, klp::kScaleBlock);
+    p->whole = whole_rows(dim, ld_x, e, {x, residual, post, weight, gate}) &&
+               whole_rows(dim, ld_residual, e, {});
     return KLP_OK;
 }
 
@@ -2010,6 +2022,9 @@ int klp_block_norm_bwd(const void* x, int dtype, int64_t ld_x, const uint8_t* x_
     p.dim = dim;
     p.groups = s.groups;
     p.per_group = s.per_group;
+    p.whole = whole_rows(dim, kept || !needs_x ? dim : ld_x, e,
+                         {kept ? nullptr : x, kept ? nullptr : h, x_codes, h_codes, post_weight,
+                          weight, gate, g_y, g_h});
     p.d_x = d_x;
     p.d_r = d_residual;
     p.d_post = post_weight != nullptr ? d_post_weight : nullptr;

@@ -24,14 +24,59 @@ auto with_shape(int64_t dim, F f) {
     return f(Int<1024>{}, Int<2>{});
 }
 
-// 8 elements of a weight or gate, float32 or of the rows' dtype.
+// group_sum of one barrier: calls alternate between two slots of `lds`, so that
+// a slot's readers have met once more before it is written again.
+template <int T>
+__device__ __forceinline__ float group_sum_alternate(float v, float (&lds)[2][T / 64], int& slot) {
+    v = xrow_sum(row_sum16(v));
+    if constexpr (T > 64) {
+        float (&part)[T / 64] = lds[slot];
+        slot ^= 1;
+        if ((threadIdx.x & 63) == 0) part[(threadIdx.x % T) >> 6] = v;
+        __syncthreads();
+        v = part[0];
+#pragma unroll
+        for (int i = 1; i < T / 64; ++i) v += part[i];
+    }
+    return v;
+}
+
+// Columns c .. c + 7 of a row of `dim` elements that starts `at` elements behind
+// `base` (the same for the wave), 0 behind it.  With `whole` (every row at a
+// multiple of 16 bytes, dim of 8) by buffer loads whose range ends with the
+// row: they need no branch and stay on their way until their values are used,
+// where load_raw's tails wait for each.
 template <int DT>
-__device__ __forceinline__ void load_either(const void* w, bool f32, int64_t at, int64_t left,
-                                            float (&x)[kChunk]) {
-    if (DT == kFP32 || f32)
-        load_chunk<kFP32>(static_cast<const uint32_t*>(w) + at, left, x);
-    else
-        load_chunk<DT>(static_cast<const typename Traits<DT>::elem*>(w) + at, left, x);
+__device__ __forceinline__ RawChunk<DT> fetch(const void* base, int64_t at, int c, int dim,
+                                              bool whole) {
+    typedef typename Traits<DT>::elem elem;
+    const elem* row = static_cast<const elem*>(base) + at;
+    if (!whole) return load_raw<DT>(row + c, dim - c);
+    constexpr int kSize = sizeof(elem);
+    const __amdgpu_buffer_rsrc_t rs =
+        __builtin_amdgcn_make_buffer_rsrc(const_cast<elem*>(row), 0, dim * kSize, 0x00020000);
+    RawChunk<DT> r;
+#pragma unroll
+    for (int k = 0; k < RawChunk<DT>::kVecs; ++k)
+        r.v[k] = __builtin_amdgcn_raw_buffer_load_b128(rs, c * kSize + 16 * k, 0, 0);
+    return r;
+}
+// The same of a weight or gate, float32 or of the rows' dtype, as values.
+template <int DT>
+__device__ __forceinline__ void fetch_either(const void* w, bool f32, int64_t at, int c, int dim,
+                                             bool whole, float (&x)[kChunk]) {
+    if (DT == kFP32 || f32) fetch<kFP32>(w, at, c, dim, whole).values(x);
+    else fetch<DT>(w, at, c, dim, whole).values(x);
+}
+// 8 codes of a row of e4m3 codes, as fetch.
+__device__ __forceinline__ uint2 fetch_codes(const uint8_t* base, int64_t at, int c, int dim,
+                                             bool whole) {
+    if (!whole) return load_codes(base + at + c, dim - c);
+    typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
+    const __amdgpu_buffer_rsrc_t rs = __builtin_amdgcn_make_buffer_rsrc(
+        const_cast<uint8_t*>(base + at), 0, dim, 0x00020000);
+    const u32x2 v = __builtin_amdgcn_raw_buffer_load_b64(rs, c, 0, 0);
+    return make_uint2(v[0], v[1]);
 }
 
 // The backward's pass over the rows (klp_block_bwd_*.hip: one dtype each).

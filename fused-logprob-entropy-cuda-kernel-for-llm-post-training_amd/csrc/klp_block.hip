@@ -48,44 +48,33 @@ template <int DT, int T, int N, bool kWF32, bool kPost, bool kFp8>
 __global__ __launch_bounds__(kForwardThreads<T>) void klp_block_kernel(BlockParams p) {
     typedef typename Traits<DT>::elem elem;
     constexpr int kGroups = kForwardThreads<T> / T;
-    __shared__ float lds[kGroups][T / 64];
-    const int t = threadIdx.x % T, group = threadIdx.x / T;
+    __shared__ float lds[kGroups][2][T / 64];
+    int slot = 0;
+    const int t = threadIdx.x % T;
+    const int group = __builtin_amdgcn_readfirstlane(threadIdx.x / T);
     int64_t row = static_cast<int64_t>(blockIdx.x) * kGroups + group;
     // Groups past the last row repeat it, with the same results, and meet the
     // others at every barrier.
     if (row >= p.rows) row = p.rows - 1;
     const int dim = static_cast<int>(p.dim);
-    const elem* x = static_cast<const elem*>(p.x) + row * p.ld_x;
-    const elem* r = static_cast<const elem*>(p.residual) + row * p.ld_r;
 
-    // Everything is on its way before the first sum needs it.
+    // What the first sum does not need is on its way while it is made.
+    constexpr int kW = kWF32 ? kFP32 : DT;
     RawChunk<DT> in[N], res[N];
-    float w[N][kChunk], by[N][kChunk], wp[N][kChunk];
-#pragma unroll
-    for (int i = 0; i < N; ++i) {
-        const int c = (i * T + t) * kChunk;
-        in[i] = load_raw<DT>(x + c, dim - c);
-        res[i] = load_raw<DT>(r + c, dim - c);
-    }
-#pragma unroll
-    for (int i = 0; i < N; ++i) {
-        const int c = (i * T + t) * kChunk;
-        load_either<DT>(p.weight, kWF32, c, dim - c, w[i]);
-        if constexpr (kPost) load_either<DT>(p.post, kWF32, c, dim - c, wp[i]);
-    }
-    if (p.gate != nullptr) {
-        const int64_t at = row / p.per_gate * p.dim;
+    RawChunk<kW> wp[N], w[N];
+    const auto of_row = [&](bool whole) {
 #pragma unroll
         for (int i = 0; i < N; ++i) {
             const int c = (i * T + t) * kChunk;
-            load_either<DT>(p.gate, p.gate_f32, at + c, dim - c, by[i]);
+            in[i] = fetch<DT>(p.x, row * p.ld_x, c, dim, whole);
+            res[i] = fetch<DT>(p.residual, row * p.ld_r, c, dim, whole);
+            if constexpr (kPost) wp[i] = fetch<kW>(p.post, 0, c, dim, whole);
+            w[i] = fetch<kW>(p.weight, 0, c, dim, whole);
         }
-    } else {
-#pragma unroll
-        for (int i = 0; i < N; ++i)
-#pragma unroll
-            for (int j = 0; j < kChunk; ++j) by[i][j] = 1.0f;
-    }
+    };
+    const bool whole = p.whole != 0;
+    if (whole) of_row(true);
+    else of_row(false);
 
     float h[N][kChunk];
 #pragma unroll
@@ -102,13 +91,30 @@ __global__ __launch_bounds__(kForwardThreads<T>) void klp_block_kernel(BlockPara
         for (int i = 0; i < N; ++i)
 #pragma unroll
             for (int j = 0; j < kChunk; ++j) sum = fmaf(h[i][j], h[i][j], sum);
-        sum = group_sum<T>(sum, lds[group]);
+        sum = group_sum_alternate<T>(sum, lds[group], slot);
         const float s = 1.0f / sqrtf(sum / static_cast<float>(dim) + p.eps);
         if (p.rstd_x != nullptr && t == 0) p.rstd_x[row] = s;
 #pragma unroll
-        for (int i = 0; i < N; ++i)
+        for (int i = 0; i < N; ++i) {
+            float v[kChunk];
+            wp[i].values(v);
 #pragma unroll
-            for (int j = 0; j < kChunk; ++j) h[i][j] = h[i][j] * s * wp[i][j];
+            for (int j = 0; j < kChunk; ++j) h[i][j] = h[i][j] * s * v[j];
+        }
+    }
+    if (p.gate != nullptr) {
+        const int64_t at = static_cast<uint32_t>(row) / static_cast<uint32_t>(p.per_gate) * p.dim;
+        const auto by_gate = [&](bool whole) {
+#pragma unroll
+            for (int i = 0; i < N; ++i) {
+                float v[kChunk];
+                fetch_either<DT>(p.gate, p.gate_f32, at, (i * T + t) * kChunk, dim, whole, v);
+#pragma unroll
+                for (int j = 0; j < kChunk; ++j) h[i][j] *= v[j];
+            }
+        };
+        if (whole) by_gate(true);
+        else by_gate(false);
     }
     float sum = 0.0f;
     elem* out = static_cast<elem*>(p.h) + row * p.dim;
@@ -119,8 +125,7 @@ __global__ __launch_bounds__(kForwardThreads<T>) void klp_block_kernel(BlockPara
         res[i].values(b);
 #pragma unroll
         for (int j = 0; j < kChunk; ++j) {
-            h[i][j] = to_f32<DT>(from_f32<DT>(fmaf(h[i][j] * by[i][j], p.scale, b[j])));
-            // Elements past the row stay 0 whatever the loads put there.
+            h[i][j] = to_f32<DT>(from_f32<DT>(fmaf(h[i][j], p.scale, b[j])));
             sum = fmaf(h[i][j], h[i][j], sum);
         }
         store_chunk<DT>(out + c, dim - c, h[i]);
@@ -131,15 +136,16 @@ __global__ __launch_bounds__(kForwardThreads<T>) void klp_block_kernel(BlockPara
             put_codes(h[i], p.h_codes, p.h_scales, row, p.dim, p.n_blocks,
                       (i * T + t) * kChunk);
     }
-    sum = group_sum<T>(sum, lds[group]);
+    sum = group_sum_alternate<T>(sum, lds[group], slot);
     const float s = 1.0f / sqrtf(sum / static_cast<float>(dim) + p.eps);
     if (p.rstd_h != nullptr && t == 0) p.rstd_h[row] = s;
 #pragma unroll
     for (int i = 0; i < N; ++i) {
         const int c = (i * T + t) * kChunk;
-        float y[kChunk];
+        float y[kChunk], v[kChunk];
+        w[i].values(v);
 #pragma unroll
-        for (int j = 0; j < kChunk; ++j) y[j] = h[i][j] * s * w[i][j];
+        for (int j = 0; j < kChunk; ++j) y[j] = h[i][j] * s * v[j];
         if constexpr (kFp8) put_codes(y, p.q, p.scales, row, p.dim, p.n_blocks, c);
         else store_chunk<DT>(static_cast<elem*>(p.y) + row * p.dim + c, dim - c, y);
     }
@@ -184,23 +190,35 @@ __global__ __launch_bounds__(kSumWaves * 64) void klp_block_sum_kernel(BlockSums
     }
 }
 
-// Gates whose rows several groups took: the one that begins in group
-// blockIdx.y, if it goes on behind it, from that group's last share and the
-// others' first ones, in order.
-__global__ __launch_bounds__(256) void klp_block_gate_kernel(BlockBwdParams p, int dtype) {
-    const int64_t q = blockIdx.y;
-    const int64_t first = q * p.per_group;
-    const int64_t end = first + p.per_group < p.rows ? first + p.per_group : p.rows;
-    if (first >= end) return;
-    const int64_t gate = (end - 1) / p.per_gate;
-    const int64_t last = (gate + 1) * p.per_gate < p.rows ? (gate + 1) * p.per_gate : p.rows;
-    if (gate * p.per_gate < first || last <= end) return;
-    const int64_t c = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
-    if (c >= p.dim) return;
-    const int64_t to = (last - 1) / p.per_group;
-    float s = p.gate_shares[(2 * q + 1) * p.dim + c];
-    for (int64_t g = q + 1; g <= to; ++g) s += p.gate_shares[2 * g * p.dim + c];
-    put_either(p.d_gate, dtype, gate * p.dim + c, s);
+// A gate whose rows several groups took: from the last share of the group that
+// it begins in and the first ones of the others, added as above.  blockIdx.y is
+// the gate, or with by_group the group in which one begins that goes on.
+__global__ __launch_bounds__(kSumWaves * 64) void klp_block_gate_kernel(BlockBwdParams p,
+                                                                        int dtype,
+                                                                        bool by_group) {
+    __shared__ float part[kSumWaves][64];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int64_t y = blockIdx.y;
+    const int64_t group_end = (y + 1) * p.per_group < p.rows ? (y + 1) * p.per_group : p.rows;
+    const int64_t gate = by_group ? (group_end - 1) / p.per_gate : y;
+    const int64_t begin = gate * p.per_gate;
+    const int64_t end = begin + p.per_gate < p.rows ? begin + p.per_gate : p.rows;
+    const int64_t from = begin / p.per_group, to = (end - 1) / p.per_group;
+    if (from == to || (by_group && from != y)) return;
+    const int64_t c = static_cast<int64_t>(blockIdx.x) * 64 + lane;
+    float s = 0.0f;
+    if (c < p.dim) {
+#pragma unroll 8
+        for (int64_t g = from + wave; g <= to; g += kSumWaves)
+            s += p.gate_shares[(2 * g + (g == from ? 1 : 0)) * p.dim + c];
+    }
+    part[wave][lane] = s;
+    __syncthreads();
+    if (wave == 0 && c < p.dim) {
+#pragma unroll
+        for (int i = 1; i < kSumWaves; ++i) s += part[i][lane];
+        put_either(p.d_gate, dtype, gate * p.dim + c, s);
+    }
 }
 
 template <int DT, int T, int N, bool kWF32>
@@ -278,9 +296,12 @@ hipError_t launch_block_bwd(int dtype, const BlockBwdParams& p, hipStream_t stre
     }
     // A gate of one row lies in one group.
     if (p.gate != nullptr && !one_gate && p.d_gate != nullptr && p.per_gate > 1) {
-        const dim3 grid(static_cast<unsigned>((p.dim + 255) / 256),
-                        static_cast<unsigned>(p.groups));
-        e = launch_kernel(klp_block_gate_kernel, grid, dim3(256), stream, p, gate_dtype);
+        const int64_t gates = (p.rows + p.per_gate - 1) / p.per_gate;
+        const bool by_group = gates > p.groups;
+        const dim3 grid(static_cast<unsigned>((p.dim + 63) / 64),
+                        static_cast<unsigned>(by_group ? p.groups : gates));
+        e = launch_kernel(klp_block_gate_kernel, grid, dim3(kSumWaves * 64), stream, p, gate_dtype,
+                          by_group);
     }
     return e;
 }

@@ -13,10 +13,9 @@ template <int DT, bool kKept>
 struct Stored {
     RawChunk<DT> raw;
     __device__ __forceinline__ void load(const void* rows, int64_t ld, const uint8_t*,
-                                         const float*, int64_t row, int64_t, int64_t, int c,
-                                         int left) {
-        raw = load_raw<DT>(static_cast<const typename Traits<DT>::elem*>(rows) + row * ld + c,
-                           left);
+                                         const float*, int64_t row, int64_t, int c, int dim,
+                                         bool whole) {
+        raw = fetch<DT>(rows, row * ld, c, dim, whole);
     }
     __device__ __forceinline__ void values(float (&x)[kChunk]) const { raw.values(x); }
 };
@@ -25,10 +24,10 @@ struct Stored<DT, true> {
     uint2 codes;
     float scale;
     __device__ __forceinline__ void load(const void*, int64_t, const uint8_t* q,
-                                         const float* scales, int64_t row, int64_t dim,
-                                         int64_t n_blocks, int c, int left) {
-        codes = load_codes(q + row * dim + c, left);
-        scale = left > 0 ? scales[row * n_blocks + c / kScaleBlock] : 0.0f;
+                                         const float* scales, int64_t row, int64_t n_blocks,
+                                         int c, int dim, bool whole) {
+        codes = fetch_codes(q, row * dim, c, dim, whole);
+        scale = scales[row * n_blocks + (c < dim ? c : 0) / kScaleBlock];
     }
     __device__ __forceinline__ void values(float (&x)[kChunk]) const {
         code_values(codes, scale, x);
@@ -42,11 +41,11 @@ __global__ __launch_bounds__(kBackwardThreads<T>) void klp_block_bwd_kernel(Bloc
     constexpr int kGroups = kBackwardThreads<T> / T;
     constexpr int kCols = T * N * kChunk;
     constexpr bool kX = kPost || kGate != 0;  // x enters a gradient
-    __shared__ float lds[kGroups][T / 64];
-    // Sums of the other groups of the workgroup, a third of a group's columns at
-    // a time would do; all of one kind at a time here.
+    __shared__ float lds[kGroups][2][T / 64];
+    // The sums of the workgroup's other groups, of one kind at a time.
     __shared__ float meet[kGroups > 1 ? (kGroups - 1) * kCols : 1];
-    const int t = threadIdx.x % T, in_block = threadIdx.x / T;
+    const int t = threadIdx.x % T;
+    const int in_block = __builtin_amdgcn_readfirstlane(threadIdx.x / T);
     const int64_t group = static_cast<int64_t>(blockIdx.x) * kGroups + in_block;
     const int dim = static_cast<int>(p.dim);
     const float inv_dim = 1.0f / static_cast<float>(dim);
@@ -63,41 +62,93 @@ __global__ __launch_bounds__(kBackwardThreads<T>) void klp_block_bwd_kernel(Bloc
             if constexpr (kGate != 0) dg[i][j] = 0.0f;
         }
 
-    Stored<DT, kKept> hs[N], xs[kX ? N : 1];
-    RawChunk<DT> gys[N], ghs[N];
-    auto load_row = [&](int64_t row) {
+    // A row's operands; 16-bit rows (and codes) have the next one's on their way
+    // while one is worked on.  Two float32 rows do not fit the registers.
+    constexpr bool kAhead = DT != kFP32 && T < 1024;
+    struct Row {
+        Stored<DT, kKept> hs[N], xs[kX ? N : 1];
+        RawChunk<DT> gys[N], ghs[N];
+        float s_h, s_x;
+    };
+    const bool whole = p.whole != 0;
+    auto load_row = [&](Row& r, int64_t step) {
+        // The groups of a workgroup take the same number of steps, for their
+        // barriers: those past a group's rows repeat the last and store nothing.
+        const int64_t row = first + step < end ? first + step : p.rows - 1;
+        r.s_h = p.rstd_h[row];
+        r.s_x = kPost ? p.rstd_x[row] : 1.0f;
+        const auto all = [&](bool whole) {
+#pragma unroll
+            for (int i = 0; i < N; ++i) {
+                const int c = (i * T + t) * kChunk;
+                r.hs[i].load(p.h, p.dim, p.h_codes, p.h_scales, row, p.n_blocks, c, dim, whole);
+                if constexpr (kX)
+                    r.xs[i].load(p.x, p.ld_x, p.x_codes, p.x_scales, row, p.n_blocks, c, dim,
+                                 whole);
+                r.gys[i] = p.g_y != nullptr ? fetch<DT>(p.g_y, row * p.dim, c, dim, whole)
+                                         : RawChunk<DT>{};
+                r.ghs[i] = p.g_h != nullptr ? fetch<DT>(p.g_h, row * p.dim, c, dim, whole)
+                                         : RawChunk<DT>{};
+            }
+        };
+        if (whole && p.g_y != nullptr && p.g_h != nullptr) all(true);
+        else all(false);
+    };
+    // Weights, and the gate while it lasts, in registers where they fit.
+    constexpr bool kHold = T < 1024;
+    constexpr int kW = kWF32 ? kFP32 : DT;
+    RawChunk<kW> w_held[kHold ? N : 1], wp_held[kHold && kPost ? N : 1];
+    float by_held[kHold && kGate != 0 ? N : 1][kChunk];
+    auto weight = [&](int i, float (&v)[kChunk]) {
+        if constexpr (kHold) w_held[i].values(v);
+        else fetch_either<DT>(p.weight, kWF32, 0, (i * T + t) * kChunk, dim, whole, v);
+    };
+    auto post = [&](int i, float (&v)[kChunk]) {
+        if constexpr (kHold) wp_held[kPost ? i : 0].values(v);
+        else fetch_either<DT>(p.post, kWF32, 0, (i * T + t) * kChunk, dim, whole, v);
+    };
+    auto load_gate = [&](int64_t row) {
+#pragma unroll
+        for (int i = 0; i < N; ++i)
+            fetch_either<DT>(p.gate, p.gate_f32, row * p.dim, (i * T + t) * kChunk, dim, whole,
+                             by_held[kHold && kGate != 0 ? i : 0]);
+    };
+    if constexpr (kHold) {
 #pragma unroll
         for (int i = 0; i < N; ++i) {
             const int c = (i * T + t) * kChunk;
-            const int left = dim - c;
-            hs[i].load(p.h, p.dim, p.h_codes, p.h_scales, row, p.dim, p.n_blocks, c, left);
-            if constexpr (kX)
-                xs[i].load(p.x, p.ld_x, p.x_codes, p.x_scales, row, p.dim, p.n_blocks, c, left);
-            gys[i] = load_raw<DT>(static_cast<const elem*>(p.g_y) + row * p.dim + c,
-                                  p.g_y != nullptr ? left : 0);
-            ghs[i] = load_raw<DT>(static_cast<const elem*>(p.g_h) + row * p.dim + c,
-                                  p.g_h != nullptr ? left : 0);
+            w_held[i] = fetch<kW>(p.weight, 0, c, dim, whole);
+            if constexpr (kPost)
+                wp_held[i] = fetch<kW>(p.post, 0, c, dim, whole);
         }
-    };
-    // The groups of a workgroup take the same number of steps (p.per_group), for
-    // their barriers; a step past the group's rows does nothing else.
+    }
+    // Rows of the gate before `first`, and the gate's.
+    const uint32_t per_gate = static_cast<uint32_t>(p.per_gate);
+    uint32_t gate_row = 0, of_gate = 0;
+    if constexpr (kGate == 2) {
+        gate_row = static_cast<uint32_t>(first < p.rows ? first : p.rows - 1) / per_gate;
+        of_gate = static_cast<uint32_t>(first < p.rows ? first : p.rows - 1) - gate_row * per_gate;
+    }
+    bool begun_here = of_gate == 0;
+    if constexpr (kHold && kGate != 0) load_gate(gate_row);
+    int slot = 0;
+    Row r;
+    if constexpr (kAhead) load_row(r, 0);
     for (int64_t step = 0; step < p.per_group; ++step) {
         const int64_t row = first + step;
         const bool live = row < end;
-        const int64_t at = live ? row : p.rows - 1;
-        load_row(at);
-        const float s_h = p.rstd_h[at];
-        const float s_x = kPost ? p.rstd_x[at] : 1.0f;
-        const int64_t gate_row = kGate == 2 ? at / p.per_gate : 0;
+        Row next;
+        if constexpr (kAhead) load_row(next, step + 1);
+        else load_row(r, step);
+        const float s_h = r.s_h, s_x = r.s_x;
 
         float dh[N][kChunk], dot = 0.0f;
 #pragma unroll
         for (int i = 0; i < N; ++i) {
-            const int c = (i * T + t) * kChunk;
             float w[kChunk], h[kChunk], g[kChunk];
-            load_either<DT>(p.weight, kWF32, c, dim - c, w);
-            hs[i].values(h);
-            gys[i].values(g);
+            weight(i, w);
+            r.hs[i].values(h);
+            r.gys[i].values(g);
 #pragma unroll
             for (int j = 0; j < kChunk; ++j) {
                 if (live) dw[i][j] = fmaf(g[j] * s_h, h[j], dw[i][j]);
@@ -105,24 +156,29 @@ __global__ __launch_bounds__(kBackwardThreads<T>) void klp_block_bwd_kernel(Bloc
                 dot = fmaf(dh[i][j], h[j], dot);
             }
         }
-        dot = group_sum<T>(dot, lds[in_block]);
+        dot = group_sum_alternate<T>(dot, lds[in_block], slot);
         const float a_h = s_h * s_h * dot * inv_dim;
         float dot_x = 0.0f;
 #pragma unroll
         for (int i = 0; i < N; ++i) {
             const int c = (i * T + t) * kChunk;
             float h[kChunk], gh[kChunk], x[kChunk], by[kChunk], wp[kChunk];
-            hs[i].values(h);
-            ghs[i].values(gh);
+            r.hs[i].values(h);
+            r.ghs[i].values(gh);
 #pragma unroll
             for (int j = 0; j < kChunk; ++j)
                 dh[i][j] = fmaf(s_h, fmaf(-a_h, h[j], dh[i][j]), gh[j]);
             if (live && p.d_r != nullptr)
                 store_chunk<DT>(static_cast<elem*>(p.d_r) + row * p.dim + c, dim - c, dh[i]);
-            if constexpr (kX) xs[i].values(x);
-            if constexpr (kPost) load_either<DT>(p.post, kWF32, c, dim - c, wp);
-            if constexpr (kGate != 0)
-                load_either<DT>(p.gate, p.gate_f32, gate_row * p.dim + c, dim - c, by);
+            if constexpr (kX) r.xs[i].values(x);
+            if constexpr (kPost) post(i, wp);
+            if constexpr (kGate != 0 && kHold) {
+#pragma unroll
+                for (int j = 0; j < kChunk; ++j) by[j] = by_held[i][j];
+            } else if constexpr (kGate != 0) {
+                fetch_either<DT>(p.gate, p.gate_f32, static_cast<int64_t>(gate_row) * p.dim, c, dim,
+                                 whole, by);
+            }
 #pragma unroll
             for (int j = 0; j < kChunk; ++j) {
                 const float d = dh[i][j] * p.scale;  // c dh
@@ -141,7 +197,7 @@ __global__ __launch_bounds__(kBackwardThreads<T>) void klp_block_bwd_kernel(Bloc
         }
         float a_x = 0.0f;
         if constexpr (kPost) {
-            dot_x = group_sum<T>(dot_x, lds[in_block]);
+            dot_x = group_sum_alternate<T>(dot_x, lds[in_block], slot);
             a_x = s_x * s_x * dot_x * inv_dim;
         }
         if (live && p.d_x != nullptr) {
@@ -150,7 +206,7 @@ __global__ __launch_bounds__(kBackwardThreads<T>) void klp_block_bwd_kernel(Bloc
                 const int c = (i * T + t) * kChunk;
                 if constexpr (kPost) {
                     float x[kChunk];
-                    xs[i].values(x);
+                    r.xs[i].values(x);
 #pragma unroll
                     for (int j = 0; j < kChunk; ++j)
                         dh[i][j] = s_x * fmaf(-a_x, x[j], dh[i][j]);
@@ -160,10 +216,9 @@ __global__ __launch_bounds__(kBackwardThreads<T>) void klp_block_bwd_kernel(Bloc
         }
         if constexpr (kGate == 2) {
             // The gate's rows end here, or the group's do.
-            const bool gate_ends = row + 1 == p.rows || (row + 1) % p.per_gate == 0;
+            const bool gate_ends = row + 1 == p.rows || of_gate + 1 == per_gate;
             if (live && p.d_gate != nullptr && (gate_ends || row + 1 == end)) {
-                const bool begun_here = gate_row * p.per_gate >= first;
-                const int64_t from = gate_row * p.dim;
+                const int64_t from = static_cast<int64_t>(gate_row) * p.dim;
                 float* share = p.gate_shares + (2 * group + (begun_here ? 1 : 0)) * p.dim;
 #pragma unroll
                 for (int i = 0; i < N; ++i) {
@@ -180,7 +235,16 @@ __global__ __launch_bounds__(kBackwardThreads<T>) void klp_block_bwd_kernel(Bloc
                     for (int j = 0; j < kChunk; ++j) dg[i][j] = 0.0f;
                 }
             }
+            if (live) {
+                if (gate_ends && row + 1 < p.rows) {
+                    ++gate_row;
+                    if constexpr (kHold) load_gate(gate_row);
+                }
+                of_gate = gate_ends ? 0 : of_gate + 1;
+                begun_here |= gate_ends;
+            }
         }
+        if constexpr (kAhead) r = next;
     }
 
     // The workgroup's sums: its groups' in order, into its share.

@@ -364,6 +364,7 @@ struct BlockParams {
     uint8_t* h_codes;
     float* h_scales;
     int64_t n_blocks;      // ceil(dim / kScaleBlock)
+    int whole;             // dim a multiple of 8, every row at one of 16 bytes
 };
 struct BlockBwdParams {
     const void* x;         // [rows, ld_x], or x_codes and x_scales; null: not needed
@@ -389,6 +390,7 @@ struct BlockBwdParams {
     int64_t dim;
     int64_t groups;        // block_groups(rows, dim), of per_group consecutive rows
     int64_t per_group;
+    int whole;             // as BlockParams'
     void* d_x;             // [rows, dim], nullable
     void* d_r;             // [rows, dim], nullable
     void* d_post;          // [dim], nullable
