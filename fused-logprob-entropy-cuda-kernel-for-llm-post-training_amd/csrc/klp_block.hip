@@ -193,10 +193,12 @@ __global__ __launch_bounds__(kSumWaves * 64) void klp_block_sum_kernel(BlockSums
 // A gate whose rows several groups took: from the last share of the group that
 // it begins in and the first ones of the others, added as above.  blockIdx.y is
 // the gate, or with by_group the group in which one begins that goes on.
-__global__ __launch_bounds__(kSumWaves * 64) void klp_block_gate_kernel(BlockBwdParams p,
+// A lane takes 4 columns, the workgroup's 4 waves every 4th share.
+constexpr int kGateWaves = 4;
+__global__ __launch_bounds__(kGateWaves * 64) void klp_block_gate_kernel(BlockBwdParams p,
                                                                         int dtype,
                                                                         bool by_group) {
-    __shared__ float part[kSumWaves][64];
+    __shared__ float part[kGateWaves][4][64];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const int64_t y = blockIdx.y;
     const int64_t group_end = (y + 1) * p.per_group < p.rows ? (y + 1) * p.per_group : p.rows;
@@ -205,19 +207,23 @@ __global__ __launch_bounds__(kSumWaves * 64) void klp_block_gate_kernel(BlockBwd
     const int64_t end = begin + p.per_gate < p.rows ? begin + p.per_gate : p.rows;
     const int64_t from = begin / p.per_group, to = (end - 1) / p.per_group;
     if (from == to || (by_group && from != y)) return;
-    const int64_t c = static_cast<int64_t>(blockIdx.x) * 64 + lane;
-    float s = 0.0f;
-    if (c < p.dim) {
-#pragma unroll 8
-        for (int64_t g = from + wave; g <= to; g += kSumWaves)
-            s += p.gate_shares[(2 * g + (g == from ? 1 : 0)) * p.dim + c];
-    }
-    part[wave][lane] = s;
-    __syncthreads();
-    if (wave == 0 && c < p.dim) {
+    const int64_t c = (static_cast<int64_t>(blockIdx.x) * 64 + lane) * 4;
+    float s[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll 4
+    for (int64_t g = from + wave; g <= to; g += kGateWaves) {
+        const float* share = p.gate_shares + (2 * g + (g == from ? 1 : 0)) * p.dim;
 #pragma unroll
-        for (int i = 1; i < kSumWaves; ++i) s += part[i][lane];
-        put_either(p.d_gate, dtype, gate * p.dim + c, s);
+        for (int j = 0; j < 4; ++j) s[j] += share[c + j < p.dim ? c + j : 0];
+    }
+#pragma unroll
+    for (int j = 0; j < 4; ++j) part[wave][j][lane] = s[j];
+    __syncthreads();
+    if (wave != 0) return;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+#pragma unroll
+        for (int i = 1; i < kGateWaves; ++i) s[j] += part[i][j][lane];
+        if (c + j < p.dim) put_either(p.d_gate, dtype, gate * p.dim + c + j, s[j]);
     }
 }
 
@@ -298,9 +304,9 @@ hipError_t launch_block_bwd(int dtype, const BlockBwdParams& p, hipStream_t stre
     if (p.gate != nullptr && !one_gate && p.d_gate != nullptr && p.per_gate > 1) {
         const int64_t gates = (p.rows + p.per_gate - 1) / p.per_gate;
         const bool by_group = gates > p.groups;
-        const dim3 grid(static_cast<unsigned>((p.dim + 63) / 64),
+        const dim3 grid(static_cast<unsigned>((p.dim + 255) / 256),
                         static_cast<unsigned>(by_group ? p.groups : gates));
-        e = launch_kernel(klp_block_gate_kernel, grid, dim3(kSumWaves * 64), stream, p, gate_dtype,
+        e = launch_kernel(klp_block_gate_kernel, grid, dim3(kGateWaves * 64), stream, p, gate_dtype,
                           by_group);
     }
     return e;

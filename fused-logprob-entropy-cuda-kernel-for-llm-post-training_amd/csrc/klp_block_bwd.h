@@ -52,14 +52,32 @@ __global__ __launch_bounds__(kBackwardThreads<T>) void klp_block_bwd_kernel(Bloc
     const int64_t first = group * p.per_group;
     const int64_t end = first + p.per_group < p.rows ? first + p.per_group : p.rows;
 
-    float dw[N][kChunk], dp[kPost ? N : 1][kChunk], dg[kGate != 0 ? N : 1][kChunk];
+    // A thread's sums.  A thread of 1024 has 128 registers: there the gate's and
+    // the post weight's are kept in LDS, each by its own thread.
+    constexpr bool kInLds = T == 1024;
+    constexpr int kLdsSums = kInLds ? (kPost ? 1 : 0) + (kGate != 0 ? 1 : 0) : 0;
+    __shared__ float held[kLdsSums > 0 ? kLdsSums * kCols : 1];
+    float dw[N][kChunk], dp[kPost && !kInLds ? N : 1][kChunk],
+        dg[kGate != 0 && !kInLds ? N : 1][kChunk];
+    auto in_lds = [&](int which, int i, int j) -> float& {
+        return held[(which * N * kChunk + i * kChunk + j) * T + t];
+    };
+    constexpr int kGateAt = kPost ? 1 : 0;
+    auto sum_p = [&](int i, int j) -> float& {
+        if constexpr (kInLds) return in_lds(0, i, j);
+        else return dp[i][j];
+    };
+    auto sum_g = [&](int i, int j) -> float& {
+        if constexpr (kInLds) return in_lds(kGateAt, i, j);
+        else return dg[i][j];
+    };
 #pragma unroll
     for (int i = 0; i < N; ++i)
 #pragma unroll
         for (int j = 0; j < kChunk; ++j) {
             dw[i][j] = 0.0f;
-            if constexpr (kPost) dp[i][j] = 0.0f;
-            if constexpr (kGate != 0) dg[i][j] = 0.0f;
+            if constexpr (kPost) sum_p(i, j) = 0.0f;
+            if constexpr (kGate != 0) sum_g(i, j) = 0.0f;
         }
 
     // A row's operands; 16-bit rows (and codes) have the next one's on their way
@@ -184,11 +202,11 @@ __global__ __launch_bounds__(kBackwardThreads<T>) void klp_block_bwd_kernel(Bloc
                 const float d = dh[i][j] * p.scale;  // c dh
                 if constexpr (kGate != 0) {
                     const float z = kPost ? x[j] * s_x * wp[j] : x[j];
-                    if (live) dg[i][j] = fmaf(d, z, dg[i][j]);
+                    if (live) sum_g(i, j) = fmaf(d, z, sum_g(i, j));
                 }
                 float dz = kGate != 0 ? d * by[j] : d;
                 if constexpr (kPost) {
-                    if (live) dp[i][j] = fmaf(dz * s_x, x[j], dp[i][j]);
+                    if (live) sum_p(i, j) = fmaf(dz * s_x, x[j], sum_p(i, j));
                     dz *= wp[j];
                     dot_x = fmaf(dz, x[j], dot_x);
                 }
@@ -223,16 +241,19 @@ __global__ __launch_bounds__(kBackwardThreads<T>) void klp_block_bwd_kernel(Bloc
 #pragma unroll
                 for (int i = 0; i < N; ++i) {
                     const int c = (i * T + t) * kChunk;
+                    float v[kChunk];
+#pragma unroll
+                    for (int j = 0; j < kChunk; ++j) {
+                        v[j] = sum_g(i, j);
+                        sum_g(i, j) = 0.0f;
+                    }
                     if (!(gate_ends && begun_here))
-                        store_chunk<kFP32>(reinterpret_cast<uint32_t*>(share) + c, dim - c,
-                                           dg[i]);
+                        store_chunk<kFP32>(reinterpret_cast<uint32_t*>(share) + c, dim - c, v);
                     else if (DT == kFP32 || p.gate_f32)
                         store_chunk<kFP32>(static_cast<uint32_t*>(p.d_gate) + from + c, dim - c,
-                                           dg[i]);
+                                           v);
                     else
-                        store_chunk<DT>(static_cast<elem*>(p.d_gate) + from + c, dim - c, dg[i]);
-#pragma unroll
-                    for (int j = 0; j < kChunk; ++j) dg[i][j] = 0.0f;
+                        store_chunk<DT>(static_cast<elem*>(p.d_gate) + from + c, dim - c, v);
                 }
             }
             if (live) {
@@ -248,8 +269,13 @@ __global__ __launch_bounds__(kBackwardThreads<T>) void klp_block_bwd_kernel(Bloc
     }
 
     // The workgroup's sums: its groups' in order, into its share.
-    auto share = [&](float (&sum)[N][kChunk], float* shares) {
+    auto share = [&](auto of, float* shares) {
         if (shares == nullptr) return;
+        float sum[N][kChunk];
+#pragma unroll
+        for (int i = 0; i < N; ++i)
+#pragma unroll
+            for (int j = 0; j < kChunk; ++j) sum[i][j] = of(i, j);
         if constexpr (kGroups > 1) {
             __syncthreads();
             if (in_block > 0) {
@@ -276,9 +302,9 @@ __global__ __launch_bounds__(kBackwardThreads<T>) void klp_block_bwd_kernel(Bloc
             store_chunk<kFP32>(to + c, dim - c, sum[i]);
         }
     };
-    share(dw, p.weight_shares);
-    if constexpr (kPost) share(dp, p.post_shares);
-    if constexpr (kGate == 1) share(dg, p.gate_shares);
+    share([&](int i, int j) { return dw[i][j]; }, p.weight_shares);
+    if constexpr (kPost) share(sum_p, p.post_shares);
+    if constexpr (kGate == 1) share(sum_g, p.gate_shares);
 }
 
 template <int DT, int T, int N, bool kWF32, bool kPost, int kGate>
