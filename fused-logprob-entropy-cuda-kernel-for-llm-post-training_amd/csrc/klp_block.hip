@@ -39,12 +39,12 @@ __device__ __forceinline__ void put_codes(const float (&v)[kChunk], uint8_t* q, 
                                           int64_t row, int64_t dim, int64_t n_blocks, int c) {
     const E4m3Scale e = e4m3_scale(row_max16(chunk_amax(v)));
     if (c < dim) {
-        store_codes(q + row * dim + c, dim - c, e4m3_pack8(v, e.inv));
+        store_codes(column<uint8_t>(q, row * dim, c), dim - c, e4m3_pack8(v, e.inv));
         if ((threadIdx.x & 15) == 0) scales[row * n_blocks + c / kScaleBlock] = e.scale;
     }
 }
 
-template <int DT, int T, int N, bool kWF32, bool kPost, bool kFp8>
+template <int DT, int T, int N, int kMode, bool kPost, bool kFp8>
 __global__ __launch_bounds__(kForwardThreads<T>) void klp_block_kernel(BlockParams p) {
     typedef typename Traits<DT>::elem elem;
     constexpr int kGroups = kForwardThreads<T> / T;
@@ -59,22 +59,17 @@ __global__ __launch_bounds__(kForwardThreads<T>) void klp_block_kernel(BlockPara
     const int dim = static_cast<int>(p.dim);
 
     // What the first sum does not need is on its way while it is made.
-    constexpr int kW = kWF32 ? kFP32 : DT;
+    constexpr bool kWholeRow = kMode != kAny;
     RawChunk<DT> in[N], res[N];
-    RawChunk<kW> wp[N], w[N];
-    const auto of_row = [&](bool whole) {
+    RawChunk<kWeight<DT, kMode>> wp[N], w[N];
 #pragma unroll
-        for (int i = 0; i < N; ++i) {
-            const int c = (i * T + t) * kChunk;
-            in[i] = fetch<DT>(p.x, row * p.ld_x, c, dim, whole);
-            res[i] = fetch<DT>(p.residual, row * p.ld_r, c, dim, whole);
-            if constexpr (kPost) wp[i] = fetch<kW>(p.post, 0, c, dim, whole);
-            w[i] = fetch<kW>(p.weight, 0, c, dim, whole);
-        }
-    };
-    const bool whole = p.whole != 0;
-    if (whole) of_row(true);
-    else of_row(false);
+    for (int i = 0; i < N; ++i) {
+        const int c = (i * T + t) * kChunk;
+        in[i] = fetch<DT, kWholeRow>(p.x, row * p.ld_x, c, dim);
+        res[i] = fetch<DT, kWholeRow>(p.residual, row * p.ld_r, c, dim);
+        if constexpr (kPost) wp[i] = fetch_weight<DT, kMode>(p.post, p.weight_f32, c, dim);
+        w[i] = fetch_weight<DT, kMode>(p.weight, p.weight_f32, c, dim);
+    }
 
     float h[N][kChunk];
 #pragma unroll
@@ -104,20 +99,15 @@ __global__ __launch_bounds__(kForwardThreads<T>) void klp_block_kernel(BlockPara
     }
     if (p.gate != nullptr) {
         const int64_t at = static_cast<uint32_t>(row) / static_cast<uint32_t>(p.per_gate) * p.dim;
-        const auto by_gate = [&](bool whole) {
 #pragma unroll
-            for (int i = 0; i < N; ++i) {
-                float v[kChunk];
-                fetch_either<DT>(p.gate, p.gate_f32, at, (i * T + t) * kChunk, dim, whole, v);
+        for (int i = 0; i < N; ++i) {
+            float v[kChunk];
+            fetch_either<DT, kWholeRow>(p.gate, p.gate_f32, at, (i * T + t) * kChunk, dim, v);
 #pragma unroll
-                for (int j = 0; j < kChunk; ++j) h[i][j] *= v[j];
-            }
-        };
-        if (whole) by_gate(true);
-        else by_gate(false);
+            for (int j = 0; j < kChunk; ++j) h[i][j] *= v[j];
+        }
     }
     float sum = 0.0f;
-    elem* out = static_cast<elem*>(p.h) + row * p.dim;
 #pragma unroll
     for (int i = 0; i < N; ++i) {
         const int c = (i * T + t) * kChunk;
@@ -128,7 +118,7 @@ __global__ __launch_bounds__(kForwardThreads<T>) void klp_block_kernel(BlockPara
             h[i][j] = to_f32<DT>(from_f32<DT>(fmaf(h[i][j], p.scale, b[j])));
             sum = fmaf(h[i][j], h[i][j], sum);
         }
-        store_chunk<DT>(out + c, dim - c, h[i]);
+        store_chunk<DT>(column<elem>(p.h, row * p.dim, c), dim - c, h[i]);
     }
     if (p.h_codes != nullptr) {
 #pragma unroll
@@ -147,7 +137,7 @@ __global__ __launch_bounds__(kForwardThreads<T>) void klp_block_kernel(BlockPara
 #pragma unroll
         for (int j = 0; j < kChunk; ++j) y[j] = h[i][j] * s * v[j];
         if constexpr (kFp8) put_codes(y, p.q, p.scales, row, p.dim, p.n_blocks, c);
-        else store_chunk<DT>(static_cast<elem*>(p.y) + row * p.dim + c, dim - c, y);
+        else store_chunk<DT>(column<elem>(p.y, row * p.dim, c), dim - c, y);
     }
 }
 
@@ -227,7 +217,7 @@ __global__ __launch_bounds__(kGateWaves * 64) void klp_block_gate_kernel(BlockBw
     }
 }
 
-template <int DT, int T, int N, bool kWF32>
+template <int DT, int T, int N, int kMode>
 hipError_t launch_block_shape(const BlockParams& p, hipStream_t stream) {
     constexpr int kThreads = kForwardThreads<T>, kGroups = kThreads / T;
     const dim3 grid(static_cast<unsigned>((p.rows + kGroups - 1) / kGroups)), block(kThreads);
@@ -235,18 +225,19 @@ hipError_t launch_block_shape(const BlockParams& p, hipStream_t stream) {
         return launch_kernel(kernel, grid, block, stream, p);
     };
     if (p.q != nullptr)
-        return p.post != nullptr ? launch(klp_block_kernel<DT, T, N, kWF32, true, true>)
-                                 : launch(klp_block_kernel<DT, T, N, kWF32, false, true>);
-    return p.post != nullptr ? launch(klp_block_kernel<DT, T, N, kWF32, true, false>)
-                             : launch(klp_block_kernel<DT, T, N, kWF32, false, false>);
+        return p.post != nullptr ? launch(klp_block_kernel<DT, T, N, kMode, true, true>)
+                                 : launch(klp_block_kernel<DT, T, N, kMode, false, true>);
+    return p.post != nullptr ? launch(klp_block_kernel<DT, T, N, kMode, true, false>)
+                             : launch(klp_block_kernel<DT, T, N, kMode, false, false>);
 }
 
 template <int DT>
 hipError_t launch_block_dt(const BlockParams& p, hipStream_t stream) {
     return with_shape(p.dim, [&](auto t, auto n) {
         constexpr int T = decltype(t)::value, N = decltype(n)::value;
-        return DT == kFP32 || p.weight_f32 ? launch_block_shape<DT, T, N, true>(p, stream)
-                                           : launch_block_shape<DT, T, N, DT == kFP32>(p, stream);
+        return with_mode<DT>(p, [&](auto mode) {
+            return launch_block_shape<DT, T, N, decltype(mode)::value>(p, stream);
+        });
     });
 }
 }  // namespace

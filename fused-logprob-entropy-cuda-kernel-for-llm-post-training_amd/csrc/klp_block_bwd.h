@@ -9,25 +9,25 @@ namespace klp {
 namespace {
 
 // A row's x or h: as stored, or the values of its checkpoint.
-template <int DT, bool kKept>
+template <int DT, bool kKept, bool kWholeRow>
 struct Stored {
     RawChunk<DT> raw;
     __device__ __forceinline__ void load(const void* rows, int64_t ld, const uint8_t*,
-                                         const float*, int64_t row, int64_t, int c, int dim,
-                                         bool whole) {
-        raw = fetch<DT>(rows, row * ld, c, dim, whole);
+                                         const float*, int64_t row, int64_t, int c, int dim) {
+        raw = fetch<DT, kWholeRow>(rows, row * ld, c, dim);
     }
     __device__ __forceinline__ void values(float (&x)[kChunk]) const { raw.values(x); }
 };
-template <int DT>
-struct Stored<DT, true> {
+template <int DT, bool kWholeRow>
+struct Stored<DT, true, kWholeRow> {
     uint2 codes;
     float scale;
     __device__ __forceinline__ void load(const void*, int64_t, const uint8_t* q,
                                          const float* scales, int64_t row, int64_t n_blocks,
-                                         int c, int dim, bool whole) {
-        codes = fetch_codes(q, row * dim, c, dim, whole);
-        scale = scales[row * n_blocks + (c < dim ? c : 0) / kScaleBlock];
+                                         int c, int dim) {
+        codes = fetch_codes<kWholeRow>(q, row * dim, c, dim);
+        const float* of_row = scales + row * n_blocks;
+        scale = of_row[static_cast<uint32_t>(c < dim ? c : 0) / kScaleBlock];
     }
     __device__ __forceinline__ void values(float (&x)[kChunk]) const {
         code_values(codes, scale, x);
@@ -35,7 +35,7 @@ struct Stored<DT, true> {
 };
 
 // kGate: 0 none, 1 one for all rows, 2 one for every per_gate rows.
-template <int DT, int T, int N, bool kWF32, bool kPost, int kGate, bool kKept>
+template <int DT, int T, int N, int kMode, bool kPost, int kGate, bool kKept>
 __global__ __launch_bounds__(kBackwardThreads<T>) void klp_block_bwd_kernel(BlockBwdParams p) {
     typedef typename Traits<DT>::elem elem;
     constexpr int kGroups = kBackwardThreads<T> / T;
@@ -82,62 +82,65 @@ __global__ __launch_bounds__(kBackwardThreads<T>) void klp_block_bwd_kernel(Bloc
 
     // A row's operands; 16-bit rows (and codes) have the next one's on their way
     // while one is worked on.  Two float32 rows do not fit the registers.
-    constexpr bool kAhead = DT != kFP32 && T < 1024;
+    constexpr bool kAhead = DT != kFP32 && T < 1024 && kMode != kAny;
+    constexpr bool kWholeRow = kMode != kAny;
     struct Row {
-        Stored<DT, kKept> hs[N], xs[kX ? N : 1];
+        Stored<DT, kKept, kWholeRow> hs[N], xs[kX ? N : 1];
         RawChunk<DT> gys[N], ghs[N];
         float s_h, s_x;
     };
-    const bool whole = p.whole != 0;
+    // Keeps the chunks' work apart where registers are few.
+    auto apart = [] {
+        if constexpr (T == 1024 || kMode == kAny) __builtin_amdgcn_sched_barrier(0);
+    };
+    // A lane's column; hidden there, so that no address made of it is kept.
+    auto column_of = [&](int i) {
+        int c = (i * T + t) * kChunk;
+        if constexpr (T == 1024) asm volatile("" : "+v"(c));
+        return c;
+    };
     auto load_row = [&](Row& r, int64_t step) {
         // The groups of a workgroup take the same number of steps, for their
         // barriers: those past a group's rows repeat the last and store nothing.
         const int64_t row = first + step < end ? first + step : p.rows - 1;
         r.s_h = p.rstd_h[row];
         r.s_x = kPost ? p.rstd_x[row] : 1.0f;
-        const auto all = [&](bool whole) {
 #pragma unroll
-            for (int i = 0; i < N; ++i) {
-                const int c = (i * T + t) * kChunk;
-                r.hs[i].load(p.h, p.dim, p.h_codes, p.h_scales, row, p.n_blocks, c, dim, whole);
-                if constexpr (kX)
-                    r.xs[i].load(p.x, p.ld_x, p.x_codes, p.x_scales, row, p.n_blocks, c, dim,
-                                 whole);
-                r.gys[i] = p.g_y != nullptr ? fetch<DT>(p.g_y, row * p.dim, c, dim, whole)
-                                         : RawChunk<DT>{};
-                r.ghs[i] = p.g_h != nullptr ? fetch<DT>(p.g_h, row * p.dim, c, dim, whole)
-                                         : RawChunk<DT>{};
-            }
-        };
-        if (whole && p.g_y != nullptr && p.g_h != nullptr) all(true);
-        else all(false);
+        for (int i = 0; i < N; ++i) {
+            apart();
+            const int c = column_of(i);
+            r.hs[i].load(p.h, p.dim, p.h_codes, p.h_scales, row, p.n_blocks, c, dim);
+            if constexpr (kX)
+                r.xs[i].load(p.x, p.ld_x, p.x_codes, p.x_scales, row, p.n_blocks, c, dim);
+            r.gys[i] = fetch<DT, kWholeRow>(p.g_y, row * p.dim, c, dim);
+            r.ghs[i] = fetch<DT, kWholeRow>(p.g_h, row * p.dim, c, dim);
+        }
     };
     // Weights, and the gate while it lasts, in registers where they fit.
-    constexpr bool kHold = T < 1024;
-    constexpr int kW = kWF32 ? kFP32 : DT;
-    RawChunk<kW> w_held[kHold ? N : 1], wp_held[kHold && kPost ? N : 1];
+    constexpr bool kHold = T < 1024 && kMode != kAny;
+    RawChunk<kWeight<DT, kMode>> w_held[kHold ? N : 1], wp_held[kHold && kPost ? N : 1];
     float by_held[kHold && kGate != 0 ? N : 1][kChunk];
     auto weight = [&](int i, float (&v)[kChunk]) {
         if constexpr (kHold) w_held[i].values(v);
-        else fetch_either<DT>(p.weight, kWF32, 0, (i * T + t) * kChunk, dim, whole, v);
+        else fetch_weight<DT, kMode>(p.weight, p.weight_f32, column_of(i), dim).values(v);
     };
     auto post = [&](int i, float (&v)[kChunk]) {
         if constexpr (kHold) wp_held[kPost ? i : 0].values(v);
-        else fetch_either<DT>(p.post, kWF32, 0, (i * T + t) * kChunk, dim, whole, v);
+        else fetch_weight<DT, kMode>(p.post, p.weight_f32, column_of(i), dim).values(v);
     };
     auto load_gate = [&](int64_t row) {
 #pragma unroll
         for (int i = 0; i < N; ++i)
-            fetch_either<DT>(p.gate, p.gate_f32, row * p.dim, (i * T + t) * kChunk, dim, whole,
-                             by_held[kHold && kGate != 0 ? i : 0]);
+            fetch_either<DT, kWholeRow>(p.gate, p.gate_f32, row * p.dim, column_of(i), dim,
+                                        by_held[kHold && kGate != 0 ? i : 0]);
     };
     if constexpr (kHold) {
 #pragma unroll
         for (int i = 0; i < N; ++i) {
-            const int c = (i * T + t) * kChunk;
-            w_held[i] = fetch<kW>(p.weight, 0, c, dim, whole);
+            const int c = column_of(i);
+            w_held[i] = fetch_weight<DT, kMode>(p.weight, p.weight_f32, c, dim);
             if constexpr (kPost)
-                wp_held[i] = fetch<kW>(p.post, 0, c, dim, whole);
+                wp_held[i] = fetch_weight<DT, kMode>(p.post, p.weight_f32, c, dim);
         }
     }
     // Rows of the gate before `first`, and the gate's.
@@ -163,6 +166,7 @@ __global__ __launch_bounds__(kBackwardThreads<T>) void klp_block_bwd_kernel(Bloc
         float dh[N][kChunk], dot = 0.0f;
 #pragma unroll
         for (int i = 0; i < N; ++i) {
+            apart();
             float w[kChunk], h[kChunk], g[kChunk];
             weight(i, w);
             r.hs[i].values(h);
@@ -179,7 +183,8 @@ __global__ __launch_bounds__(kBackwardThreads<T>) void klp_block_bwd_kernel(Bloc
         float dot_x = 0.0f;
 #pragma unroll
         for (int i = 0; i < N; ++i) {
-            const int c = (i * T + t) * kChunk;
+            apart();
+            const int c = column_of(i);
             float h[kChunk], gh[kChunk], x[kChunk], by[kChunk], wp[kChunk];
             r.hs[i].values(h);
             r.ghs[i].values(gh);
@@ -187,15 +192,15 @@ __global__ __launch_bounds__(kBackwardThreads<T>) void klp_block_bwd_kernel(Bloc
             for (int j = 0; j < kChunk; ++j)
                 dh[i][j] = fmaf(s_h, fmaf(-a_h, h[j], dh[i][j]), gh[j]);
             if (live && p.d_r != nullptr)
-                store_chunk<DT>(static_cast<elem*>(p.d_r) + row * p.dim + c, dim - c, dh[i]);
+                store_chunk<DT>(column<elem>(p.d_r, row * p.dim, c), dim - c, dh[i]);
             if constexpr (kX) r.xs[i].values(x);
             if constexpr (kPost) post(i, wp);
             if constexpr (kGate != 0 && kHold) {
 #pragma unroll
                 for (int j = 0; j < kChunk; ++j) by[j] = by_held[i][j];
             } else if constexpr (kGate != 0) {
-                fetch_either<DT>(p.gate, p.gate_f32, static_cast<int64_t>(gate_row) * p.dim, c, dim,
-                                 whole, by);
+                fetch_either<DT, kWholeRow>(p.gate, p.gate_f32,
+                                            static_cast<int64_t>(gate_row) * p.dim, c, dim, by);
             }
 #pragma unroll
             for (int j = 0; j < kChunk; ++j) {
@@ -221,7 +226,8 @@ __global__ __launch_bounds__(kBackwardThreads<T>) void klp_block_bwd_kernel(Bloc
         if (live && p.d_x != nullptr) {
 #pragma unroll
             for (int i = 0; i < N; ++i) {
-                const int c = (i * T + t) * kChunk;
+                apart();
+                const int c = column_of(i);
                 if constexpr (kPost) {
                     float x[kChunk];
                     r.xs[i].values(x);
@@ -229,7 +235,7 @@ __global__ __launch_bounds__(kBackwardThreads<T>) void klp_block_bwd_kernel(Bloc
                     for (int j = 0; j < kChunk; ++j)
                         dh[i][j] = s_x * fmaf(-a_x, x[j], dh[i][j]);
                 }
-                store_chunk<DT>(static_cast<elem*>(p.d_x) + row * p.dim + c, dim - c, dh[i]);
+                store_chunk<DT>(column<elem>(p.d_x, row * p.dim, c), dim - c, dh[i]);
             }
         }
         if constexpr (kGate == 2) {
@@ -240,7 +246,7 @@ __global__ __launch_bounds__(kBackwardThreads<T>) void klp_block_bwd_kernel(Bloc
                 float* share = p.gate_shares + (2 * group + (begun_here ? 1 : 0)) * p.dim;
 #pragma unroll
                 for (int i = 0; i < N; ++i) {
-                    const int c = (i * T + t) * kChunk;
+                    const int c = column_of(i);
                     float v[kChunk];
 #pragma unroll
                     for (int j = 0; j < kChunk; ++j) {
@@ -248,12 +254,11 @@ __global__ __launch_bounds__(kBackwardThreads<T>) void klp_block_bwd_kernel(Bloc
                         sum_g(i, j) = 0.0f;
                     }
                     if (!(gate_ends && begun_here))
-                        store_chunk<kFP32>(reinterpret_cast<uint32_t*>(share) + c, dim - c, v);
+                        store_chunk<kFP32>(column<uint32_t>(share, 0, c), dim - c, v);
                     else if (DT == kFP32 || p.gate_f32)
-                        store_chunk<kFP32>(static_cast<uint32_t*>(p.d_gate) + from + c, dim - c,
-                                           v);
+                        store_chunk<kFP32>(column<uint32_t>(p.d_gate, from, c), dim - c, v);
                     else
-                        store_chunk<DT>(static_cast<elem*>(p.d_gate) + from + c, dim - c, v);
+                        store_chunk<DT>(column<elem>(p.d_gate, from, c), dim - c, v);
                 }
             }
             if (live) {
@@ -295,11 +300,10 @@ __global__ __launch_bounds__(kBackwardThreads<T>) void klp_block_bwd_kernel(Bloc
                     for (int j = 0; j < kChunk; ++j)
                         sum[i][j] += meet[q * kCols + (i * kChunk + j) * T + t];
         }
-        uint32_t* to = reinterpret_cast<uint32_t*>(shares) + blockIdx.x * p.dim;
 #pragma unroll
         for (int i = 0; i < N; ++i) {
             const int c = (i * T + t) * kChunk;
-            store_chunk<kFP32>(to + c, dim - c, sum[i]);
+            store_chunk<kFP32>(column<uint32_t>(shares, blockIdx.x * p.dim, c), dim - c, sum[i]);
         }
     };
     share([&](int i, int j) { return dw[i][j]; }, p.weight_shares);
@@ -307,34 +311,35 @@ __global__ __launch_bounds__(kBackwardThreads<T>) void klp_block_bwd_kernel(Bloc
     if constexpr (kGate == 1) share(sum_g, p.gate_shares);
 }
 
-template <int DT, int T, int N, bool kWF32, bool kPost, int kGate>
+template <int DT, int T, int N, int kMode, bool kPost, int kGate>
 hipError_t launch_bwd_kept(const BlockBwdParams& p, hipStream_t stream) {
     constexpr int kThreads = kBackwardThreads<T>, kGroups = kThreads / T;
     const dim3 grid(static_cast<unsigned>((p.groups + kGroups - 1) / kGroups)), block(kThreads);
     return p.h_codes != nullptr
-               ? launch_kernel(klp_block_bwd_kernel<DT, T, N, kWF32, kPost, kGate, true>, grid,
+               ? launch_kernel(klp_block_bwd_kernel<DT, T, N, kMode, kPost, kGate, true>, grid,
                                block, stream, p)
-               : launch_kernel(klp_block_bwd_kernel<DT, T, N, kWF32, kPost, kGate, false>, grid,
+               : launch_kernel(klp_block_bwd_kernel<DT, T, N, kMode, kPost, kGate, false>, grid,
                                block, stream, p);
 }
-template <int DT, int T, int N, bool kWF32, bool kPost>
+template <int DT, int T, int N, int kMode, bool kPost>
 hipError_t launch_bwd_gate(const BlockBwdParams& p, hipStream_t stream) {
-    if (p.gate == nullptr) return launch_bwd_kept<DT, T, N, kWF32, kPost, 0>(p, stream);
-    return p.per_gate >= p.rows ? launch_bwd_kept<DT, T, N, kWF32, kPost, 1>(p, stream)
-                                : launch_bwd_kept<DT, T, N, kWF32, kPost, 2>(p, stream);
+    if (p.gate == nullptr) return launch_bwd_kept<DT, T, N, kMode, kPost, 0>(p, stream);
+    return p.per_gate >= p.rows ? launch_bwd_kept<DT, T, N, kMode, kPost, 1>(p, stream)
+                                : launch_bwd_kept<DT, T, N, kMode, kPost, 2>(p, stream);
 }
-template <int DT, int T, int N, bool kWF32>
+template <int DT, int T, int N, int kMode>
 hipError_t launch_bwd_shape(const BlockBwdParams& p, hipStream_t stream) {
-    return p.post != nullptr ? launch_bwd_gate<DT, T, N, kWF32, true>(p, stream)
-                             : launch_bwd_gate<DT, T, N, kWF32, false>(p, stream);
+    return p.post != nullptr ? launch_bwd_gate<DT, T, N, kMode, true>(p, stream)
+                             : launch_bwd_gate<DT, T, N, kMode, false>(p, stream);
 }
 
 template <int DT>
 hipError_t launch_rows_dt(const BlockBwdParams& p, hipStream_t stream) {
     return with_shape(p.dim, [&](auto t, auto n) {
         constexpr int T = decltype(t)::value, N = decltype(n)::value;
-        return DT == kFP32 || p.weight_f32 ? launch_bwd_shape<DT, T, N, true>(p, stream)
-                                           : launch_bwd_shape<DT, T, N, DT == kFP32>(p, stream);
+        return with_mode<DT>(p, [&](auto mode) {
+            return launch_bwd_shape<DT, T, N, decltype(mode)::value>(p, stream);
+        });
     });
 }
 

@@ -1,4 +1,4 @@
-// klp_block_bwd_bf16.hip — klp_block_bwd.h's kernels for bf16 rows.
+// klp_block_bwd_bf16.hip — klp_block_bwd.h's __global__ functions for bf16 rows.
 #include "klp_block_bwd.h"
 
 namespace klp {

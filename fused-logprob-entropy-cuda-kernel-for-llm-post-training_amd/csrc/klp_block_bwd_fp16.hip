@@ -1,4 +1,4 @@
-// klp_block_bwd_fp16.hip — klp_block_bwd.h's kernels for fp16 rows.
+// klp_block_bwd_fp16.hip — klp_block_bwd.h's __global__ functions for fp16 rows.
 #include "klp_block_bwd.h"
 
 namespace klp {

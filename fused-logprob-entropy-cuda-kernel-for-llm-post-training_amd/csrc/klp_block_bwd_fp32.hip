@@ -1,4 +1,4 @@
-// klp_block_bwd_fp32.hip — klp_block_bwd.h's kernels for fp32 rows.
+// klp_block_bwd_fp32.hip — klp_block_bwd.h's __global__ functions for fp32 rows.
 #include "klp_block_bwd.h"
 
 namespace klp {

@@ -368,12 +368,12 @@ __device__ __forceinline__ float bound_of(const float* thread_max, int k) {
 __device__ __forceinline__ void count_from(uint32_t& count, float top, float gate, float from,
                                            const float (&x)[4]) {
     asm("v_cmp_ge_f32 vcc, %1, %2\n\t"
-        "s_cbranch_vccz .Lnone%=\n\t"
+        "s_cbranch_vccz .LBBnone%=\n\t"
         "v_cmp_ge_f32 vcc, %4, %3\n\tv_addc_co_u32 %0, vcc, 0, %0, vcc\n\t"
         "v_cmp_ge_f32 vcc, %5, %3\n\tv_addc_co_u32 %0, vcc, 0, %0, vcc\n\t"
         "v_cmp_ge_f32 vcc, %6, %3\n\tv_addc_co_u32 %0, vcc, 0, %0, vcc\n\t"
         "v_cmp_ge_f32 vcc, %7, %3\n\tv_addc_co_u32 %0, vcc, 0, %0, vcc\n"
-        ".Lnone%=:"
+        ".LBBnone%=:"
         : "+v"(count)
         : "v"(top), "v"(gate), "v"(from), "v"(x[0]), "v"(x[1]), "v"(x[2]), "v"(x[3])
         : "vcc");
@@ -381,7 +381,7 @@ __device__ __forceinline__ void count_from(uint32_t& count, float top, float gat
 __device__ __forceinline__ void count_from(uint32_t& count, float top, float gate, float from,
                                            const float (&x)[8]) {
     asm("v_cmp_ge_f32 vcc, %1, %2\n\t"
-        "s_cbranch_vccz .Lnone%=\n\t"
+        "s_cbranch_vccz .LBBnone%=\n\t"
         "v_cmp_ge_f32 vcc, %4, %3\n\tv_addc_co_u32 %0, vcc, 0, %0, vcc\n\t"
         "v_cmp_ge_f32 vcc, %5, %3\n\tv_addc_co_u32 %0, vcc, 0, %0, vcc\n\t"
         "v_cmp_ge_f32 vcc, %6, %3\n\tv_addc_co_u32 %0, vcc, 0, %0, vcc\n\t"
@@ -390,7 +390,7 @@ __device__ __forceinline__ void count_from(uint32_t& count, float top, float gat
         "v_cmp_ge_f32 vcc, %9, %3\n\tv_addc_co_u32 %0, vcc, 0, %0, vcc\n\t"
         "v_cmp_ge_f32 vcc, %10, %3\n\tv_addc_co_u32 %0, vcc, 0, %0, vcc\n\t"
         "v_cmp_ge_f32 vcc, %11, %3\n\tv_addc_co_u32 %0, vcc, 0, %0, vcc\n"
-        ".Lnone%=:"
+        ".LBBnone%=:"
         : "+v"(count)
         : "v"(top), "v"(gate), "v"(from), "v"(x[0]), "v"(x[1]), "v"(x[2]), "v"(x[3]), "v"(x[4]),
           "v"(x[5]), "v"(x[6]), "v"(x[7])
