@@ -973,7 +973,9 @@ std::vector<at::Tensor> quantize_fp8(const at::Tensor& x, int64_t block_rows) {
 }
 
 at::Tensor fp8_linear(const at::Tensor& x, const at::Tensor& x_scale, const at::Tensor& weight,
-                      const at::Tensor& weight_scale, at::ScalarType out_dtype) {
+                      const at::Tensor& weight_scale, at::ScalarType out_dtype,
+                      const std::optional<at::Tensor>& bias, int64_t act, double cap,
+                      const std::optional<at::Tensor>& residual) {
     const int dev = x.get_device();
     decline_under_capture(dev);
     const at::AutoDispatchBelowADInplaceOrView below;
@@ -983,10 +985,15 @@ at::Tensor fp8_linear(const at::Tensor& x, const at::Tensor& x_scale, const at::
     std::vector<int64_t> shape = x.sizes().vec();
     shape.back() = wm.t.size(0);
     at::Tensor out = at::empty(shape, x.options().dtype(out_dtype));
-    check_status(klp_fp8_linear(static_cast<const uint8_t*>(xm.t.data_ptr()), xm.ld, fptr(xs),
-                                static_cast<const uint8_t*>(wm.t.data_ptr()), wm.ld, fptr(ws),
-                                xm.t.size(0), wm.t.size(0), wm.t.size(1), dtype_code(out_dtype),
-                                out.data_ptr(), wm.t.size(0), current_stream(dev)));
+    const at::Tensor b = bias.has_value() ? bias->contiguous() : at::Tensor();
+    const Matrix rm = residual.has_value() ? as_rows(*residual) : Matrix{at::Tensor(), 0};
+    check_status(klp_fp8_linear_act(
+        static_cast<const uint8_t*>(xm.t.data_ptr()), xm.ld, fptr(xs),
+        static_cast<const uint8_t*>(wm.t.data_ptr()), wm.ld, fptr(ws), xm.t.size(0),
+        wm.t.size(0), wm.t.size(1), data_or_null(b),
+        b.defined() ? dtype_code(b.scalar_type()) : KLP_BF16, static_cast<int>(act),
+        static_cast<float>(cap), data_or_null(rm.t), rm.ld, dtype_code(out_dtype),
+        out.data_ptr(), wm.t.size(0), current_stream(dev)));
     return out;
 }
 
@@ -1376,7 +1383,9 @@ PYBIND11_MODULE(klp_torch, m) {
           pybind11::arg("weight"), pybind11::arg("eps"));
     m.def("quantize_fp8", &quantize_fp8, pybind11::arg("x"), pybind11::arg("block_rows"));
     m.def("fp8_linear", &fp8_linear, pybind11::arg("x"), pybind11::arg("x_scale"),
-          pybind11::arg("weight"), pybind11::arg("weight_scale"), pybind11::arg("out_dtype"));
+          pybind11::arg("weight"), pybind11::arg("weight_scale"), pybind11::arg("out_dtype"),
+          pybind11::arg("bias") = pybind11::none(), pybind11::arg("act") = 0,
+          pybind11::arg("cap") = 1.0, pybind11::arg("residual") = pybind11::none());
     m.def("block_norm", &block_norm, pybind11::arg("x"), pybind11::arg("residual"),
           pybind11::arg("weight"), pybind11::arg("post_weight"), pybind11::arg("gate"),
           pybind11::arg("per_gate"), pybind11::arg("scale"), pybind11::arg("eps"),

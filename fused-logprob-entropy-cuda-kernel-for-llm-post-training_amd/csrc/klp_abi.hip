@@ -905,6 +905,52 @@ size_t norm_bwd_workspace(int64_t rows, int64_t dim) {
     return static_cast<size_t>(klp::norm_bwd_groups(rows, dim) * dim) * sizeof(float);
 }
 
+int fp8_linear(const uint8_t* x, int64_t ld_x, const float* x_scales, const uint8_t* w,
+               int64_t ld_w, const float* w_scales, int64_t m, int64_t n, int64_t k,
+               int out_dtype, void* out, int64_t ld_out, const klp::Fp8LinearParams& epilogue,
+               void* stream) {
+    int rc = check_dtype3(out_dtype, "out");
+    if (rc != KLP_OK) return rc;
+    if (m < 0 || n < 1) return fail(KLP_EINVAL, "m must be >= 0 and n >= 1");
+    if (k < 16 || k % 16 != 0)
+        return fail(KLP_EINVAL, "k must be a positive multiple of 16, got %lld",
+                    static_cast<long long>(k));
+    if (m == 0) return ok();
+    if ((rc = check_matrix(x, ld_x, k, 16, "x")) != KLP_OK) return rc;
+    if ((rc = check_matrix(w, ld_w, k, 16, "w")) != KLP_OK) return rc;
+    if (ld_x % 16 != 0 || ld_w % 16 != 0)
+        return fail(KLP_EINVAL, "row strides of x and w must be multiples of 16");
+    if ((rc = check_f32(x_scales, "x_scales")) != KLP_OK) return rc;
+    if ((rc = check_f32(w_scales, "w_scales")) != KLP_OK) return rc;
+    if (out == nullptr || !aligned(out, elem_bytes(out_dtype)) || ld_out < n)
+        return fail(KLP_EINVAL,
+                    "out must be non-null and aligned to its elements, with a row stride >= n");
+    if (m > (1 << 20) || n > (int64_t{1} << 31) || k > (1 << 24))
+        return fail(KLP_EINVAL, "m, n and k must not exceed 2^20, 2^31 and 2^24");
+    // The narrowest tiles, 128 x 64 outputs, and their grid's multiple of 8;
+    // or 16 weight rows and 64 tokens a workgroup, where row strides are long.
+    if ((rc = check_threads(ceil_div(m, 64) * ceil_div(n, 128) + 8, 512, "output tiles")) !=
+            KLP_OK ||
+        (rc = check_threads(ceil_div(n, 16), 256, "weight rows")) != KLP_OK)
+        return rc;
+    klp::Fp8LinearParams p = epilogue;
+    p.x = x;
+    p.ld_x = ld_x;
+    p.xs = x_scales;
+    p.w = w;
+    p.ld_w = ld_w;
+    p.ws = w_scales;
+    p.m = m;
+    p.n = n;
+    p.k = k;
+    p.n_blocks = ceil_div(k, klp::kScaleBlock);
+    p.out = out;
+    p.ld_out = ld_out;
+    if (injected_failure("fp8 linear")) return KLP_ELAUNCH;
+    return after_launch(klp::launch_fp8_linear(out_dtype, p, static_cast<hipStream_t>(stream)),
+                        "fp8 linear");
+}
+
 }  // namespace
 
 extern "C" {
@@ -1852,46 +1898,43 @@ int klp_quantize_fp8(const void* x, int dtype, int64_t ld_x, int64_t rows, int64
 int klp_fp8_linear(const uint8_t* x, int64_t ld_x, const float* x_scales, const uint8_t* w,
                    int64_t ld_w, const float* w_scales, int64_t m, int64_t n, int64_t k,
                    int out_dtype, void* out, int64_t ld_out, void* stream) {
+    return fp8_linear(x, ld_x, x_scales, w, ld_w, w_scales, m, n, k, out_dtype, out, ld_out,
+                      klp::Fp8LinearParams{}, stream);
+}
+
+int klp_fp8_linear_act(const uint8_t* x, int64_t ld_x, const float* x_scales, const uint8_t* w,
+                       int64_t ld_w, const float* w_scales, int64_t m, int64_t n, int64_t k,
+                       const void* bias, int bias_dtype, int act, float cap,
+                       const void* residual, int64_t ld_residual, int out_dtype, void* out,
+                       int64_t ld_out, void* stream) {
     int rc = check_dtype3(out_dtype, "out");
     if (rc != KLP_OK) return rc;
-    if (m < 0 || n < 1) return fail(KLP_EINVAL, "m must be >= 0 and n >= 1");
-    if (k < 16 || k % 16 != 0)
-        return fail(KLP_EINVAL, "k must be a positive multiple of 16, got %lld",
-                    static_cast<long long>(k));
-    if (m == 0) return ok();
-    if ((rc = check_matrix(x, ld_x, k, 16, "x")) != KLP_OK) return rc;
-    if ((rc = check_matrix(w, ld_w, k, 16, "w")) != KLP_OK) return rc;
-    if (ld_x % 16 != 0 || ld_w % 16 != 0)
-        return fail(KLP_EINVAL, "row strides of x and w must be multiples of 16");
-    if ((rc = check_f32(x_scales, "x_scales")) != KLP_OK) return rc;
-    if ((rc = check_f32(w_scales, "w_scales")) != KLP_OK) return rc;
-    if (out == nullptr || !aligned(out, elem_bytes(out_dtype)) || ld_out < n)
-        return fail(KLP_EINVAL,
-                    "out must be non-null and aligned to its elements, with a row stride >= n");
-    if (m > (1 << 20) || n > (int64_t{1} << 31) || k > (1 << 24))
-        return fail(KLP_EINVAL, "m, n and k must not exceed 2^20, 2^31 and 2^24");
-    // The narrowest tiles, 128 x 64 outputs, and their grid's multiple of 8;
-    // or 16 weight rows and 64 tokens a workgroup, where row strides are long.
-    if ((rc = check_threads(ceil_div(m, 64) * ceil_div(n, 128) + 8, 512, "output tiles")) !=
-            KLP_OK ||
-        (rc = check_threads(ceil_div(n, 16), 256, "weight rows")) != KLP_OK)
-        return rc;
     klp::Fp8LinearParams p{};
-    p.x = x;
-    p.ld_x = ld_x;
-    p.xs = x_scales;
-    p.w = w;
-    p.ld_w = ld_w;
-    p.ws = w_scales;
-    p.m = m;
-    p.n = n;
-    p.k = k;
-    p.n_blocks = ceil_div(k, klp::kScaleBlock);
-    p.out = out;
-    p.ld_out = ld_out;
-    if (injected_failure("fp8 linear")) return KLP_ELAUNCH;
-    return after_launch(klp::launch_fp8_linear(out_dtype, p, static_cast<hipStream_t>(stream)),
-                        "fp8 linear");
+    if (bias != nullptr) {
+        if (bias_dtype != out_dtype && bias_dtype != KLP_FP32)
+            return fail(KLP_EDTYPE, "bias must be float32 or of out's dtype");
+        if (!aligned(bias, elem_bytes(bias_dtype)))
+            return fail(KLP_EINVAL, "bias is not aligned to its elements");
+    }
+    if (act < KLP_ACT_NONE || act > KLP_ACT_SOFTCAP)
+        return fail(KLP_EINVAL, "unknown activation %d", act);
+    if (act == KLP_ACT_SOFTCAP && !(cap >= 0x1p-100f && cap <= 0x1p100f))
+        return fail(KLP_EINVAL, "cap must be within 2^-100 and 2^100, got %g",
+                    static_cast<double>(cap));
+    if (residual != nullptr) {
+        const size_t size = elem_bytes(out_dtype);
+        if ((rc = check_matrix(residual, ld_residual, n, size, "residual")) != KLP_OK) return rc;
+        p.res_aligned = aligned(residual, 4 * size) && ld_residual % 4 == 0;
+    }
+    p.epilogue = bias != nullptr || act != KLP_ACT_NONE || residual != nullptr;
+    p.bias = bias;
+    p.bias_f32 = bias_dtype == KLP_FP32;
+    p.act = act;
+    p.cap = act == KLP_ACT_SOFTCAP ? cap : 1.0f;
+    p.residual = residual;
+    p.ld_res = ld_residual;
+    return fp8_linear(x, ld_x, x_scales, w, ld_w, w_scales, m, n, k, out_dtype, out, ld_out, p,
+                      stream);
 }
 
 int klp_block_norm(const void* x, int dtype, int64_t ld_x, const void* residual,

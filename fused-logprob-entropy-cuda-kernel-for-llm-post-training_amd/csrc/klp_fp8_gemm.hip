@@ -11,6 +11,11 @@
 // holds row l % 16 of an operand block and 32 of its 128 k; which 32 is free,
 // as long as both operands agree: two 16-byte pieces, at 16 (l / 16) and 64 +
 // 16 (l / 16), so that 4 lanes read 64 consecutive bytes.
+//
+// With an epilogue (kEpilogue) the float32 sums take a bias, an activation or a
+// soft cap and a residual before their only rounding: what a separate pass would
+// read and write once more, at the price of ALU work that the tiles' stores do
+// not overlap.
 #include "klp_launch.h"
 #include "klp_mfma.h"
 #include "klp_rows.h"
@@ -110,11 +115,106 @@ __device__ __forceinline__ void store4(typename Traits<DT>::elem* p, int64_t lef
     }
 }
 
+// ---------------------------------------------------------------------------
+// The epilogue.  exp(-v) in the sigmoids and exp(-2 |t|) in the soft cap are the
+// hardware's exponential and reciprocal for 16-bit outputs, whose rounding is
+// 1000 times theirs, and the library's functions and a division for float32.
+// ---------------------------------------------------------------------------
+template <int DT>
+__device__ __forceinline__ float exp_of(float x) {
+    if constexpr (DT == kFP32) return expf(x);
+    else return exp2_hw(x * kLog2e);
+}
+// v / (1 + e)
+template <int DT>
+__device__ __forceinline__ float over_one_plus(float v, float e) {
+    if constexpr (DT == kFP32) return v / (1.0f + e);
+    else return v * __builtin_amdgcn_rcpf(1.0f + e);
+}
+// cap tanh(t), t = v / cap.  Near 0 it is v (1 - t^2 / 3), off by 2 t^4 / 15 of
+// itself: 2^-27 below 1/64, where the 1 - e of (1 - e) / (1 + e), e = exp(-2 |t|),
+// loses its digits, and v itself below 2^-12 for float32.
+template <int DT>
+__device__ __forceinline__ float capped(float v, float cap, float inv_cap) {
+    if constexpr (DT == kFP32) {
+        const float t = v / cap;
+        return fabsf(t) < 0x1p-12f ? v : cap * tanhf(t);
+    } else {
+        const float t = v * inv_cap;
+        const float a = fabsf(t);
+        const float e = exp_of<DT>(-2.0f * a);
+        const float far = copysignf(cap * over_one_plus<DT>(1.0f - e, e), t);
+        return a < 0x1p-6f ? fmaf(v * t * t, -1.0f / 3.0f, v) : far;
+    }
+}
+template <int DT>
+__device__ __forceinline__ float activated(float v, int act, float cap, float inv_cap) {
+    switch (act) {
+        case KLP_ACT_RELU: return v < 0.0f ? 0.0f : v;
+        case KLP_ACT_SILU: return over_one_plus<DT>(v, exp_of<DT>(-v));
+        case KLP_ACT_GELU_TANH: {
+            // v (1 + tanh u) / 2 = v / (1 + exp(-2 u)), u = sqrt(2 / pi) (v + 0.044715 v^3)
+            const float u = 0.79788456080286535588f * fmaf(0.044715f * v * v, v, v);
+            return over_one_plus<DT>(v, exp_of<DT>(-2.0f * u));
+        }
+        case KLP_ACT_SOFTCAP:
+            return capped<DT>(v, cap, inv_cap);
+        default: return v;
+    }
+}
+
+// 4 biases from n on (n + 3 may lie past the last).
+template <int DT>
+__device__ __forceinline__ f32x4 bias4(const Fp8LinearParams& p, int64_t n) {
+    f32x4 b = {0.0f, 0.0f, 0.0f, 0.0f};
+    if (p.bias == nullptr) return b;
+    typedef typename Traits<DT>::elem elem;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+        const int64_t at = n + j < p.n ? n + j : p.n - 1;
+        b[j] = DT == kFP32 || p.bias_f32 ? static_cast<const float*>(p.bias)[at]
+                                         : to_f32<DT>(static_cast<const elem*>(p.bias)[at]);
+    }
+    return b;
+}
+// 4 residuals of token m < p.m.
+template <int DT>
+__device__ __forceinline__ f32x4 residual4(const Fp8LinearParams& p, int64_t m, int64_t n) {
+    f32x4 r = {0.0f, 0.0f, 0.0f, 0.0f};
+    if (p.residual == nullptr) return r;
+    typedef typename Traits<DT>::elem elem;
+    const elem* row = static_cast<const elem*>(p.residual) + m * p.ld_res;
+    elem e[4];
+    if (p.res_aligned && n + 3 < p.n) {
+        __builtin_memcpy(e, __builtin_assume_aligned(row + n, sizeof e), sizeof e);
+    } else {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) e[j] = row[n + j < p.n ? n + j : p.n - 1];
+    }
+#pragma unroll
+    for (int j = 0; j < 4; ++j) r[j] = to_f32<DT>(e[j]);
+    return r;
+}
+// The outputs n .. n + 3 of token m < p.m, from its sums.
+template <int DT, bool kEpilogue>
+__device__ __forceinline__ void finish4(const Fp8LinearParams& p, int64_t m, int64_t n, f32x4 v,
+                                        f32x4 bias, float inv_cap) {
+    if constexpr (kEpilogue) {
+        if (n >= p.n) return;
+        const f32x4 r = residual4<DT>(p, m, n);
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+            v[j] = activated<DT>(v[j] + bias[j], p.act, p.cap, inv_cap) + r[j];
+    }
+    typedef typename Traits<DT>::elem elem;
+    store4<DT>(static_cast<elem*>(p.out) + m * p.ld_out + n, p.n - n, v);
+}
+
 // Small products: a workgroup's waves share the K of 16 weight rows and 16 MB
 // tokens, both straight from memory to registers (the tokens' rows stay in the
 // caches); their sums meet in LDS and are added in order.
 constexpr int kSplit = 4;
-template <int DT, int MB, bool kExact>
+template <int DT, int MB, bool kExact, bool kEpilogue>
 __global__ __launch_bounds__(64 * kSplit) void klp_fp8_stream_kernel(Fp8LinearParams p) {
     __shared__ f32x4 part[(kSplit - 1) * MB * 64];
     const int lane = threadIdx.x & 63;
@@ -210,12 +310,17 @@ __global__ __launch_bounds__(64 * kSplit) void klp_fp8_stream_kernel(Fp8LinearPa
 #pragma unroll
         for (int j = 0; j < MB; ++j) acc[j] += part[(z * MB + j) * 64 + lane];
 
-    typedef typename Traits<DT>::elem elem;
+    const int64_t n = v0 + 4 * lq;
+    f32x4 bias = {0.0f, 0.0f, 0.0f, 0.0f};
+    float inv_cap = 1.0f;
+    if constexpr (kEpilogue) {
+        bias = bias4<DT>(p, n);
+        inv_cap = 1.0f / p.cap;
+    }
 #pragma unroll
     for (int j = 0; j < MB; ++j) {
         const int64_t m = t0 + 16 * j + lrow;
-        const int64_t n = v0 + 4 * lq;
-        if (m < p.m) store4<DT>(static_cast<elem*>(p.out) + m * p.ld_out + n, p.n - n, acc[j]);
+        if (m < p.m) finish4<DT, kEpilogue>(p, m, n, acc[j], bias, inv_cap);
     }
 }
 
@@ -271,7 +376,7 @@ __device__ __forceinline__ void copy_dwords_to_lds(u32x4 rsrc, uint32_t lds, uin
                  : "memory");
 }
 
-template <int DT, typename Shape>
+template <int DT, typename Shape, bool kEpilogue>
 __global__
 __launch_bounds__(kTileThreads, Shape::kSmall && DT != kFP32 ? 4 : 2) void klp_fp8_tile_kernel(
     Fp8LinearParams p) {
@@ -468,8 +573,22 @@ __launch_bounds__(kTileThreads, Shape::kSmall && DT != kFP32 ? 4 : 2) void klp_f
     // The last copies write zeros to LDS: before the workgroup gives it up.
     __builtin_amdgcn_s_waitcnt(waitcnt(0, 15));
 
-    typedef typename Traits<DT>::elem elem;
     const int64_t n0 = v0 + wv * (16 * VB);
+    if constexpr (kEpilogue) {
+        const float inv_cap = 1.0f / p.cap;
+#pragma unroll
+        for (int i = 0; i < VB; ++i) {
+            const int64_t n = n0 + 16 * i + 4 * lq;
+            const f32x4 bias = bias4<DT>(p, n);
+#pragma unroll
+            for (int j = 0; j < MB; ++j) {
+                const int64_t m = t0 + wm * (16 * MB) + 16 * j + lrow;
+                if (m < p.m) finish4<DT, true>(p, m, n, acc[i][j], bias, inv_cap);
+            }
+        }
+        return;
+    }
+    typedef typename Traits<DT>::elem elem;
 #pragma unroll
     for (int j = 0; j < MB; ++j) {
         const int64_t m = t0 + wm * (16 * MB) + 16 * j + lrow;
@@ -487,14 +606,22 @@ hipError_t launch_tile(const Fp8LinearParams& p, hipStream_t stream) {
     const int64_t tiles = ((p.n + Shape::kRowsV - 1) / Shape::kRowsV) *
                           ((p.m + Shape::kRowsM - 1) / Shape::kRowsM);
     const dim3 grid(static_cast<unsigned>((tiles + 7) / 8 * 8));
-    return launch_kernel(klp_fp8_tile_kernel<DT, Shape>, grid, dim3(kTileThreads), stream, p);
+    return p.epilogue
+               ? launch_kernel(klp_fp8_tile_kernel<DT, Shape, true>, grid, dim3(kTileThreads),
+                               stream, p)
+               : launch_kernel(klp_fp8_tile_kernel<DT, Shape, false>, grid, dim3(kTileThreads),
+                               stream, p);
 }
 
 template <int DT, int MB>
 hipError_t launch_stream(const Fp8LinearParams& p, hipStream_t stream) {
     const dim3 grid(static_cast<unsigned>((p.n + 15) / 16),
                     static_cast<unsigned>((p.m + 16 * MB - 1) / (16 * MB)));
-    return launch_kernel(klp_fp8_stream_kernel<DT, MB, DT == kFP32>, grid, dim3(256), stream, p);
+    return p.epilogue
+               ? launch_kernel(klp_fp8_stream_kernel<DT, MB, DT == kFP32, true>, grid, dim3(256),
+                               stream, p)
+               : launch_kernel(klp_fp8_stream_kernel<DT, MB, DT == kFP32, false>, grid, dim3(256),
+                               stream, p);
 }
 
 template <typename Shape>

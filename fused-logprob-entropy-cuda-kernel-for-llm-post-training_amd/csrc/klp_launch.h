@@ -437,6 +437,15 @@ struct Fp8LinearParams {
     int64_t n_blocks;   // ceil(k / 128)
     void* out;          // [m, ld_out]
     int64_t ld_out;
+    // Epilogue: out = act(product + bias) + residual.
+    int epilogue;          // any of the following
+    const void* bias;      // [n], nullable; float32 with bias_f32, else of out's dtype
+    int bias_f32;
+    int act;               // klp_activation
+    float cap;             // KLP_ACT_SOFTCAP
+    const void* residual;  // [m, ld_res] of out's dtype, nullable
+    int64_t ld_res;
+    int res_aligned;       // 4 consecutive elements at a multiple of their size
 };
 hipError_t launch_fp8_linear(int out_dtype, const Fp8LinearParams& p, hipStream_t stream);
 

@@ -37,6 +37,8 @@ KLP_OK, KLP_EINVAL, KLP_EDTYPE, KLP_ELAUNCH, KLP_EWORKSPACE = 0, 1, 2, 3, 4
 # klp_grpo_loss_type / klp_grpo_level values
 KLP_GRPO_LOSS_GRPO, KLP_GRPO_LOSS_BNPO, KLP_GRPO_LOSS_FIXED = 0, 1, 2
 KLP_GRPO_TOKEN, KLP_GRPO_SEQUENCE = 0, 1
+# klp_activation values
+KLP_ACT_NONE, KLP_ACT_RELU, KLP_ACT_SILU, KLP_ACT_GELU_TANH, KLP_ACT_SOFTCAP = 0, 1, 2, 3, 4
 # klp_fwd_noalloc's split-row scratch per GPU (KLP_FWD_NOALLOC_SCRATCH_BYTES).
 KLP_FWD_NOALLOC_SCRATCH_BYTES = 65536
 # klp_grpo_step's row counter (KLP_GRPO_STEP_SCHED_BYTES).
@@ -101,6 +103,8 @@ SIGNATURES = {
     "klp_quantize_fp8": (_i32, [_vp, _i32, _i64, _i64, _i64, _i32, _vp, _vp, _vp]),
     "klp_fp8_linear": (_i32, [_vp, _i64, _vp, _vp, _i64, _vp, _i64, _i64, _i64, _i32, _vp, _i64,
                               _vp]),
+    "klp_fp8_linear_act": (_i32, [_vp, _i64, _vp, _vp, _i64, _vp, _i64, _i64, _i64, _vp, _i32,
+                                  _i32, ctypes.c_float, _vp, _i64, _i32, _vp, _i64, _vp]),
     "klp_sample": (_i32, _ROWS + [_vp, ctypes.c_float, _vp, ctypes.c_int32, _vp, ctypes.c_float,
                                   _vp, ctypes.c_float, _vp, _vp, _vp, _vp, _vp]),
     "klp_block_norm": (_i32, [_vp, _i32, _i64, _vp, _i64, _vp, _vp, _i32, _vp, _i32, _i64,

@@ -13,19 +13,23 @@ on the codes, whose float32 sums are scaled and added in float32.  For a 16-bit
 bits below the largest of 8 neighbours (5 10^-5 of a result on normal data, a
 hundredth of the output's rounding); for float32 the bf16 one, with exact
 products, at about half the rate.  There is no gradient: codes are data, not
-leaves.
+leaves.  ``bias``, ``activation`` (or ``softcap``) and ``residual`` go into the
+product's epilogue, between its float32 sums and their only rounding.
 """
 from __future__ import annotations
 
 import torch
 
-from ._library import (DTYPE_CODES, binding, check_status, device_guard, lib, ptr,
+from ._library import (DTYPE_CODES, KLP_ACT_GELU_TANH, KLP_ACT_NONE, KLP_ACT_RELU, KLP_ACT_SILU,
+                       KLP_ACT_SOFTCAP, binding, check_status, device_guard, lib, ptr,
                        stream_handle)
 from .norm import SCALE_BLOCK, _rows
 
 __all__ = ["quantize_fp8", "fp8_linear"]
 
 MAX_ROWS = 2 ** 20  # of one product's x
+ACTIVATIONS = {None: KLP_ACT_NONE, "relu": KLP_ACT_RELU, "silu": KLP_ACT_SILU,
+               "gelu_tanh": KLP_ACT_GELU_TANH}
 
 
 def quantize_fp8(x: torch.Tensor, block_rows: int = 1):
@@ -92,17 +96,55 @@ def _check_linear(x, x_scale, weight, weight_scale, out_dtype):
         raise RuntimeError("fp8_linear has no gradient: pass detached codes and scales")
 
 
+def _check_epilogue(x, weight, out_dtype, bias, activation, softcap, residual):
+    """(activation's code, cap)."""
+    if activation not in ACTIVATIONS:
+        raise ValueError(f"activation must be one of {[a for a in ACTIVATIONS if a]} or None, got "
+                         f"{activation!r}")
+    act, cap = ACTIVATIONS[activation], 1.0
+    if softcap is not None:
+        if activation is not None:
+            raise ValueError("activation and softcap exclude each other")
+        act, cap = KLP_ACT_SOFTCAP, float(softcap)
+        if not 2.0 ** -100 <= cap <= 2.0 ** 100:
+            raise ValueError(f"softcap must be within 2**-100 and 2**100, got {softcap}")
+    N = weight.size(0)
+    if bias is not None:
+        if bias.device != x.device or tuple(bias.shape) != (N,):
+            raise RuntimeError(f"bias must be [{N}] on {x.device}, got {tuple(bias.shape)} on "
+                               f"{bias.device}")
+        if bias.dtype not in (out_dtype, torch.float32):
+            raise RuntimeError("bias must be float32 or of out_dtype")
+    if residual is not None:
+        if residual.device != x.device or residual.dtype != out_dtype \
+                or tuple(residual.shape) != (*x.shape[:-1], N):
+            raise RuntimeError(f"residual must be {out_dtype} {(*x.shape[:-1], N)} on {x.device}, "
+                               f"got {residual.dtype} {tuple(residual.shape)} on "
+                               f"{residual.device}")
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad
+                                       for t in (bias, residual)):
+        raise RuntimeError("fp8_linear has no gradient: pass a detached bias and residual")
+    return act, cap
+
+
 def fp8_linear(x: torch.Tensor, x_scale: torch.Tensor, weight: torch.Tensor,
-               weight_scale: torch.Tensor, out_dtype: torch.dtype = torch.bfloat16):
-    """``out[..., n] = sum_k x[..., k] x_scale[..., k / 128] * weight[n, k]
-    weight_scale[n / 128, k / 128]``, float32 sums rounded once to
-    ``out_dtype``.
+               weight_scale: torch.Tensor, out_dtype: torch.dtype = torch.bfloat16, *,
+               bias: torch.Tensor | None = None, activation: str | None = None,
+               softcap: float | None = None, residual: torch.Tensor | None = None):
+    """``out = round(act(product + bias) + residual)`` with ``product[..., n] =
+    sum_k x[..., k] x_scale[..., k / 128] * weight[n, k] weight_scale[n / 128,
+    k / 128]``, float32 until the rounding to ``out_dtype``.
 
     Args:
         x: ``[..., K]`` float8_e4m3fn, K a multiple of 16, at most 2**20 rows.
         x_scale: ``[..., ceil(K / 128)]`` float32.
         weight: ``[N, K]`` float8_e4m3fn.
         weight_scale: ``[ceil(N / 128), ceil(K / 128)]`` float32.
+        bias: ``[N]``, float32 or of ``out_dtype``.
+        activation: "relu", "silu" or "gelu_tanh" (the tanh form).
+        softcap: c, 2**-100 to 2**100, in place of an activation:
+            ``c * tanh(v / c)``, the cap some heads put on their logits.
+        residual: ``[..., N]`` of ``out_dtype``, added last.
 
     Rows of ``x`` and ``weight`` start at multiples of 16 bytes (RuntimeError
     otherwise).  A NaN code or scale gives NaN in the outputs it enters.  The
@@ -110,18 +152,23 @@ def fp8_linear(x: torch.Tensor, x_scale: torch.Tensor, weight: torch.Tensor,
     to stay in its range.
     """
     _check_linear(x, x_scale, weight, weight_scale, out_dtype)
+    act, cap = _check_epilogue(x, weight, out_dtype, bias, activation, softcap, residual)
     try:
-        return binding.fp8_linear(x, x_scale, weight, weight_scale, out_dtype)
+        return binding.fp8_linear(x, x_scale, weight, weight_scale, out_dtype, bias, act, cap,
+                                  residual)
     except binding.CaptureDeclined:
         pass
     dev = x.device
     x2, ld_x = _rows(x)
     w2, ld_w = _rows(weight)
+    r2, ld_r = (None, 0) if residual is None else _rows(residual.detach())
+    b = None if bias is None else bias.detach().contiguous()
     xs, ws = x_scale.contiguous(), weight_scale.contiguous()
     M, N, K = x2.size(0), w2.size(0), w2.size(1)
     out = torch.empty(*x.shape[:-1], N, dtype=out_dtype, device=dev)
     with device_guard(dev.index):
-        check_status(lib.klp_fp8_linear(ptr(x2), ld_x, ptr(xs), ptr(w2), ld_w, ptr(ws), M, N, K,
-                                        DTYPE_CODES[out_dtype], ptr(out), N,
-                                        stream_handle(dev.index)))
+        check_status(lib.klp_fp8_linear_act(
+            ptr(x2), ld_x, ptr(xs), ptr(w2), ld_w, ptr(ws), M, N, K, ptr(b),
+            0 if b is None else DTYPE_CODES[b.dtype], act, cap, ptr(r2), ld_r,
+            DTYPE_CODES[out_dtype], ptr(out), N, stream_handle(dev.index)))
     return out

@@ -611,6 +611,31 @@ int klp_fp8_linear(const uint8_t* x, int64_t ld_x, const float* x_scales, const 
                    int out_dtype, void* out, int64_t ld_out, void* stream);
 
 /*
+ * The product with an epilogue, before its only rounding:
+ *   out = round(act(product + bias) + residual)
+ * bias [n] (nullable) of bias_dtype, out_dtype or KLP_FP32; residual [m,
+ * ld_residual] (nullable) of out_dtype; act a klp_activation:
+ *   RELU max(v, 0), SILU v / (1 + e^-v), GELU_TANH v / (1 + e^-2u) with
+ *   u = sqrt(2 / pi) (v + 0.044715 v^3), SOFTCAP cap tanh(v / cap)
+ * (cap from 2^-100 to 2^100, read with SOFTCAP only).  For 16-bit outputs
+ * exponentials and reciprocals are the hardware's: e^x is off by less than
+ * (2 + |x|) 2^-22 of itself.  residual may be out's own memory, with out's row
+ * stride.
+ */
+typedef enum klp_activation {
+    KLP_ACT_NONE = 0,
+    KLP_ACT_RELU = 1,
+    KLP_ACT_SILU = 2,
+    KLP_ACT_GELU_TANH = 3,
+    KLP_ACT_SOFTCAP = 4
+} klp_activation;
+int klp_fp8_linear_act(const uint8_t* x, int64_t ld_x, const float* x_scales, const uint8_t* w,
+                       int64_t ld_w, const float* w_scales, int64_t m, int64_t n, int64_t k,
+                       const void* bias, int bias_dtype, int act, float cap,
+                       const void* residual, int64_t ld_residual, int out_dtype, void* out,
+                       int64_t ld_out, void* stream);
+
+/*
  * One token a row, drawn from logits (row addressing as above) by inverse
  * transform of uniform[row] in [0, 1).  With y = (x - max x) / T, w = exp(y)
  * and the row ordered by falling x (equal ones by index): K are its first
