@@ -13,9 +13,16 @@
 // 16 (l / 16), so that 4 lanes read 64 consecutive bytes.
 //
 // With an epilogue (kEpilogue) the float32 sums take a bias, an activation or a
-// soft cap and a residual before their only rounding: what a separate pass would
-// read and write once more, at the price of ALU work that the tiles' stores do
-// not overlap.
+// soft cap and a residual before their only rounding: what passes of their own
+// would read and write once more each.  A product bound by its weight's bytes
+// hides it, one bound by its instructions pays for the arithmetic and for the
+// residual's bytes, which nothing overlaps (us, eager calls back to back):
+//   m     n       k      out   plain  bias  relu  bias+silu  gelu  cap  bias+residual
+//   16    152064  3584   bf16  102    102   101   102        100   101  102
+//   2048  16384   4096   bf16  132    135   133   137        137   142  146
+//   2048  4096    16384  fp16  134    133   131   132        132   133  135
+//   1024  152064  3584   bf16  611    633   621   635        636   656  716
+//   2048  16384   4096   fp32  269    261   260   269        275   274  318
 #include "klp_launch.h"
 #include "klp_mfma.h"
 #include "klp_rows.h"
@@ -147,27 +154,44 @@ __device__ __forceinline__ float capped(float v, float cap, float inv_cap) {
         return a < 0x1p-6f ? fmaf(v * t * t, -1.0f / 3.0f, v) : far;
     }
 }
-template <int DT>
-__device__ __forceinline__ float activated(float v, int act, float cap, float inv_cap) {
-    switch (act) {
-        case KLP_ACT_RELU: return v < 0.0f ? 0.0f : v;
-        case KLP_ACT_SILU: return over_one_plus<DT>(v, exp_of<DT>(-v));
-        case KLP_ACT_GELU_TANH: {
-            // v (1 + tanh u) / 2 = v / (1 + exp(-2 u)), u = sqrt(2 / pi) (v + 0.044715 v^3)
-            const float u = 0.79788456080286535588f * fmaf(0.044715f * v * v, v, v);
-            return over_one_plus<DT>(v, exp_of<DT>(-2.0f * u));
+// Act of N x 4 sums.  The choice is made once around them, not at each: a 256 x
+// 256 tile's 128 sums a lane with every activation's code beside each are 50 KB
+// of instructions, fetched for one pass.
+template <int DT, int N>
+__device__ __forceinline__ void activate(f32x4 (&v)[N], int act, float cap) {
+    auto each = [&](auto f) {
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+#pragma unroll
+            for (int j = 0; j < 4; ++j) v[i][j] = f(v[i][j]);
+            mfma::pin();  // else they are all started, and spilled
         }
-        case KLP_ACT_SOFTCAP:
-            return capped<DT>(v, cap, inv_cap);
-        default: return v;
+    };
+    switch (act) {
+        case KLP_ACT_RELU: each([](float x) { return x < 0.0f ? 0.0f : x; }); break;
+        case KLP_ACT_SILU:
+            each([](float x) { return over_one_plus<DT>(x, exp_of<DT>(-x)); });
+            break;
+        case KLP_ACT_GELU_TANH:
+            // x (1 + tanh u) / 2 = x / (1 + exp(-2 u)), u = sqrt(2 / pi) (x + 0.044715 x^3)
+            each([](float x) {
+                const float u = 0.79788456080286535588f * fmaf(0.044715f * x * x, x, x);
+                return over_one_plus<DT>(x, exp_of<DT>(-2.0f * u));
+            });
+            break;
+        case KLP_ACT_SOFTCAP: {
+            const float inv_cap = 1.0f / cap;
+            each([&](float x) { return capped<DT>(x, cap, inv_cap); });
+            break;
+        }
+        default: break;
     }
 }
 
 // 4 biases from n on (n + 3 may lie past the last).
 template <int DT>
 __device__ __forceinline__ f32x4 bias4(const Fp8LinearParams& p, int64_t n) {
-    f32x4 b = {0.0f, 0.0f, 0.0f, 0.0f};
-    if (p.bias == nullptr) return b;
+    f32x4 b;
     typedef typename Traits<DT>::elem elem;
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
@@ -177,11 +201,9 @@ __device__ __forceinline__ f32x4 bias4(const Fp8LinearParams& p, int64_t n) {
     }
     return b;
 }
-// 4 residuals of token m < p.m.
+// 4 residuals of token m < p.m, from n < p.n on.
 template <int DT>
 __device__ __forceinline__ f32x4 residual4(const Fp8LinearParams& p, int64_t m, int64_t n) {
-    f32x4 r = {0.0f, 0.0f, 0.0f, 0.0f};
-    if (p.residual == nullptr) return r;
     typedef typename Traits<DT>::elem elem;
     const elem* row = static_cast<const elem*>(p.residual) + m * p.ld_res;
     elem e[4];
@@ -191,23 +213,53 @@ __device__ __forceinline__ f32x4 residual4(const Fp8LinearParams& p, int64_t m, 
 #pragma unroll
         for (int j = 0; j < 4; ++j) e[j] = row[n + j < p.n ? n + j : p.n - 1];
     }
+    f32x4 r;
 #pragma unroll
     for (int j = 0; j < 4; ++j) r[j] = to_f32<DT>(e[j]);
     return r;
 }
-// The outputs n .. n + 3 of token m < p.m, from its sums.
-template <int DT, bool kEpilogue>
-__device__ __forceinline__ void finish4(const Fp8LinearParams& p, int64_t m, int64_t n, f32x4 v,
-                                        f32x4 bias, float inv_cap) {
-    if constexpr (kEpilogue) {
-        if (n >= p.n) return;
-        const f32x4 r = residual4<DT>(p, m, n);
-#pragma unroll
-        for (int j = 0; j < 4; ++j)
-            v[j] = activated<DT>(v[j] + bias[j], p.act, p.cap, inv_cap) + r[j];
-    }
+// A lane's outputs: sums v[i * MB + j] of the weight rows n0 + 16 i .. + 3 and the
+// token m0 + 16 j.  A token's VB stores follow one another, and its residuals, in
+// flight together, come before them.
+template <int DT, int VB, int MB, bool kEpilogue>
+__device__ __forceinline__ void finish(const Fp8LinearParams& p, int64_t m0, int64_t n0,
+                                       f32x4 (&v)[VB * MB]) {
     typedef typename Traits<DT>::elem elem;
-    store4<DT>(static_cast<elem*>(p.out) + m * p.ld_out + n, p.n - n, v);
+    f32x4 bias[VB];
+    if constexpr (kEpilogue) {
+        if (p.bias != nullptr)
+#pragma unroll
+            for (int i = 0; i < VB; ++i) bias[i] = bias4<DT>(p, n0 + 16 * i);
+        else
+#pragma unroll
+            for (int i = 0; i < VB; ++i) bias[i] = f32x4{-0.0f, -0.0f, -0.0f, -0.0f};
+    }
+#pragma unroll
+    for (int j = 0; j < MB; ++j) {
+        const int64_t m = m0 + 16 * j;
+        f32x4 u[VB];
+#pragma unroll
+        for (int i = 0; i < VB; ++i) u[i] = v[i * MB + j];
+        if constexpr (kEpilogue) {
+#pragma unroll
+            for (int i = 0; i < VB; ++i) u[i] += bias[i];
+            mfma::pin();
+            activate<DT>(u, p.act, p.cap);
+            if (p.residual != nullptr && m < p.m) {
+                f32x4 r[VB];
+#pragma unroll
+                for (int i = 0; i < VB; ++i)
+                    r[i] = residual4<DT>(p, m, n0 + 16 * i < p.n ? n0 + 16 * i : p.n - 1);
+#pragma unroll
+                for (int i = 0; i < VB; ++i) u[i] += r[i];
+            }
+        }
+        elem* out = static_cast<elem*>(p.out) + m * p.ld_out;
+#pragma unroll
+        for (int i = 0; i < VB; ++i)
+            if (m < p.m) store4<DT>(out + n0 + 16 * i, p.n - n0 - 16 * i, u[i]);
+        if constexpr (kEpilogue) mfma::pin();
+    }
 }
 
 // Small products: a workgroup's waves share the K of 16 weight rows and 16 MB
@@ -310,18 +362,7 @@ __global__ __launch_bounds__(64 * kSplit) void klp_fp8_stream_kernel(Fp8LinearPa
 #pragma unroll
         for (int j = 0; j < MB; ++j) acc[j] += part[(z * MB + j) * 64 + lane];
 
-    const int64_t n = v0 + 4 * lq;
-    f32x4 bias = {0.0f, 0.0f, 0.0f, 0.0f};
-    float inv_cap = 1.0f;
-    if constexpr (kEpilogue) {
-        bias = bias4<DT>(p, n);
-        inv_cap = 1.0f / p.cap;
-    }
-#pragma unroll
-    for (int j = 0; j < MB; ++j) {
-        const int64_t m = t0 + 16 * j + lrow;
-        if (m < p.m) finish4<DT, kEpilogue>(p, m, n, acc[j], bias, inv_cap);
-    }
+    finish<DT, 1, MB, kEpilogue>(p, t0 + lrow, v0 + 4 * lq, acc);
 }
 
 // Many tokens: a workgroup of 8 waves computes 256 outputs of a token for
@@ -493,11 +534,9 @@ __launch_bounds__(kTileThreads, Shape::kSmall && DT != kFP32 ? 4 : 2) void klp_f
     const const_float* ws =
         (const const_float*)(uintptr_t)(p.ws + first_row / kScaleBlock * p.n_blocks);
 
-    f32x4 acc[VB][MB];
+    f32x4 acc[VB * MB];
 #pragma unroll
-    for (int i = 0; i < VB; ++i)
-#pragma unroll
-        for (int j = 0; j < MB; ++j) acc[i][j] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+    for (int q = 0; q < VB * MB; ++q) acc[q] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
 
 #pragma unroll
     for (int b = 0; b < 2; ++b) {
@@ -541,10 +580,9 @@ __launch_bounds__(kTileThreads, Shape::kSmall && DT != kFP32 ? 4 : 2) void klp_f
         g = g_next;
         float f_next[MB];
         auto fold = [&](int q) {
-            const int i = q / MB, j = q % MB;
 #pragma unroll
             for (int r = 0; r < 4; ++r)
-                acc[i][j][r] = fmaf(c[q % (kLag + 1)][r], f[j], acc[i][j][r]);
+                acc[q][r] = fmaf(c[q % (kLag + 1)][r], f[q % MB], acc[q][r]);
         };
 #pragma unroll
         for (int q = 0; q < kSteps; ++q) {
@@ -573,32 +611,8 @@ __launch_bounds__(kTileThreads, Shape::kSmall && DT != kFP32 ? 4 : 2) void klp_f
     // The last copies write zeros to LDS: before the workgroup gives it up.
     __builtin_amdgcn_s_waitcnt(waitcnt(0, 15));
 
-    const int64_t n0 = v0 + wv * (16 * VB);
-    if constexpr (kEpilogue) {
-        const float inv_cap = 1.0f / p.cap;
-#pragma unroll
-        for (int i = 0; i < VB; ++i) {
-            const int64_t n = n0 + 16 * i + 4 * lq;
-            const f32x4 bias = bias4<DT>(p, n);
-#pragma unroll
-            for (int j = 0; j < MB; ++j) {
-                const int64_t m = t0 + wm * (16 * MB) + 16 * j + lrow;
-                if (m < p.m) finish4<DT, true>(p, m, n, acc[i][j], bias, inv_cap);
-            }
-        }
-        return;
-    }
-    typedef typename Traits<DT>::elem elem;
-#pragma unroll
-    for (int j = 0; j < MB; ++j) {
-        const int64_t m = t0 + wm * (16 * MB) + 16 * j + lrow;
-        elem* out = static_cast<elem*>(p.out) + m * p.ld_out;
-#pragma unroll
-        for (int i = 0; i < VB; ++i) {
-            const int64_t n = n0 + 16 * i + 4 * lq;
-            if (m < p.m) store4<DT>(out + n, p.n - n, acc[i][j]);
-        }
-    }
+    finish<DT, VB, MB, kEpilogue>(p, t0 + wm * (16 * MB) + lrow,
+                                  v0 + wv * (16 * VB) + 4 * lq, acc);
 }
 
 template <int DT, typename Shape>
