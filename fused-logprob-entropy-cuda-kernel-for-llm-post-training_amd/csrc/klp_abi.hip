@@ -439,8 +439,11 @@ struct TopConfig {
 };
 TopConfig top_config(int dtype, int64_t n_rows, int64_t vocab, int k) {
     TopConfig c{4, 1};
+    if (vocab <= klp::kTopShort) return c;
     const int64_t nvec = body_vectors(dtype, vocab);
-    if (nvec >= int64_t{8} * 64 * 8) c.waves = 8;
+    // More alternatives take more maxima than 4 waves' to bound them (4096 rows
+    // of 20000 bf16, k = 256: 483 us with 4 waves, most rows searched by radix).
+    if (nvec >= int64_t{8} * 64 * 8 || k > 128) c.waves = 8;
     int s = 1;
     while (s < kMaxSplits && n_rows * 2 * s <= kFwdSplitGrid &&
            nvec >= int64_t{3} * c.waves * 64 * 2 * s && 2 * s * k <= klp::kTopMergeKeys)

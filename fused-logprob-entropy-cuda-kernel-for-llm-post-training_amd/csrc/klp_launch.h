@@ -475,6 +475,8 @@ constexpr int64_t kTopMaxVocab = int64_t{1} << 26;
 constexpr int kTopMax = 256;            // alternatives of a row at most
 constexpr int kTopMergeKeys = 4096;     // splits * k at most
 constexpr int kTopCounterStride = 16;   // a row's counter has 64 bytes
+// Rows of up to this many logits stay in a workgroup's registers.
+constexpr int64_t kTopShort = 4096;
 struct TopParams {
     const void* logits;
     RowMap rm;

@@ -26,6 +26,15 @@
 //
 // Few rows are cut into pieces of a workgroup each; a piece leaves its state
 // and its own k largest in the workspace, and the last to arrive merges them.
+//
+// One pass over the bytes bounds many long rows: 4096 rows of 128256 fp16 take
+// 179 us, 5.9 TB/s (155 for klp_fwd_kernel's three numbers), 1024 of 152064 bf16
+// 57 (k = 20; 62 with k = 64; 47).  Few long rows are bound by their steps: 64 of
+// 152064 take 14 us, of which the bytes are 4.
+//
+// Short rows (klp_top_short_kernel) stay in the registers of as many waves as
+// they need, and the bound comes from maxima of a few elements or from the
+// elements themselves.
 #include "klp_launch.h"
 
 namespace klp {
@@ -33,7 +42,8 @@ namespace klp {
 namespace {
 
 constexpr int kRecords = 16;           // a thread's records at most
-constexpr int kTopList = 1024;         // elements ranked at most (unsplit)
+// Elements ranked at most (unsplit; fewer where more workgroups then fit a CU).
+constexpr int kTopList = 1024, kTopListSmall = 512;
 constexpr unsigned long long kNoKey = 0;
 
 // A rising whole number of a float; -0 counts as +0.
@@ -181,7 +191,7 @@ template <int WAVES, bool kSplit>
 struct TopShared {
     static constexpr int NT = WAVES * 64;
     // Pieces' lists together, of which the merge keeps at most all.
-    static constexpr int kList = kSplit ? kTopMergeKeys : kTopList;
+    static constexpr int kList = kSplit ? kTopMergeKeys : WAVES <= 2 ? kTopListSmall : kTopList;
     uint16_t record[kRecords][NT];  // histograms of the radix search later
     union {
         unsigned long long list[kList];
@@ -194,6 +204,9 @@ struct TopShared {
     uint32_t n_list, before, arrived;
     float tau;
     Stat total;
+    __device__ __forceinline__ int listed() const {
+        return static_cast<int>(n_list < static_cast<uint32_t>(kList) ? n_list : kList);
+    }
 };
 
 template <int DT>
@@ -203,7 +216,9 @@ __device__ __forceinline__ float element(const typename Traits<DT>::elem* rp, in
 
 // The piece's k first elements in the order into sh.list (sh.n_list of them,
 // not in order): digits of the k-th value from the top by histograms, then its
-// ties in index order.  All threads call it; elements are read as they come.
+// ties in index order.  All threads call it; elements are read as they come,
+// and again in each step: logits that another stream writes meanwhile may leave
+// any list, but none beyond its end.
 template <int DT, int WAVES, bool kSplit>
 __device__ void select_exact(TopShared<WAVES, kSplit>& sh, const typename Traits<DT>::elem* rp,
                              const Piece& pc, int k) {
@@ -267,10 +282,14 @@ __device__ void select_exact(TopShared<WAVES, kSplit>& sh, const typename Traits
     if (tid == 0) sh.n_list = 0;
     __syncthreads();
     const uint32_t bound = all ? kOrderedNegInf : prefix;
+    auto list = [&](float x, int i) {
+        const uint32_t at = atomicAdd(&sh.n_list, 1u);
+        if (at < static_cast<uint32_t>(TopShared<WAVES, kSplit>::kList))
+            sh.list[at] = order_key(x, static_cast<uint32_t>(i));
+    };
     for (int i = pc.begin + tid; i < pc.end; i += NT) {
         const float x = element<DT>(rp, i);
-        if (ordered(x) > bound)
-            sh.list[atomicAdd(&sh.n_list, 1u)] = order_key(x, static_cast<uint32_t>(i));
+        if (ordered(x) > bound) list(x, i);
     }
     __syncthreads();
     if (all) return;
@@ -294,27 +313,75 @@ __device__ void select_exact(TopShared<WAVES, kSplit>& sh, const typename Traits
             if (w < wave) before += found[3 + w];
             here += found[3 + w];
         }
-        if (tie && before < left)
-            sh.list[atomicAdd(&sh.n_list, 1u)] = order_key(x, static_cast<uint32_t>(i));
+        if (tie && before < left) list(x, i);
         left -= here < left ? here : left;
         __syncthreads();
     }
 }
 
 // Places in the order of the list's n keys: f(place, key) for each of the
-// first k.  Four lanes share a key's comparisons.
+// first k.  Four lanes share a key's comparisons, and a key that is read is
+// compared with as many of a lane's own as there are, up to 4: LDS reads bound
+// it (4096 rows of 1000 bf16, k = 128: 28 us with one key at a time, 23 so; 64
+// rows of 152064: 22.6 and 20.5).
+template <int NT, int G, typename F>
+__device__ __forceinline__ void rank_keys(const unsigned long long* list, int n, int k, int base,
+                                          F f) {
+    const int q = threadIdx.x & 3;
+    unsigned long long mine[G];
+    uint32_t place[G];
+#pragma unroll
+    for (int g = 0; g < G; ++g) {
+        const int i = base + g * (NT / 4) + (threadIdx.x >> 2);
+        mine[g] = list[i < n ? i : 0];
+        place[g] = 0;
+    }
+#pragma unroll 4
+    for (int j = q; j < n; j += 4) {
+        const unsigned long long other = list[j];
+#pragma unroll
+        for (int g = 0; g < G; ++g) place[g] += other > mine[g] ? 1u : 0u;
+    }
+#pragma unroll
+    for (int g = 0; g < G; ++g) {
+        uint32_t at = place[g];
+        at += __builtin_amdgcn_update_dpp(0, at, 0xB1, 0xF, 0xF, false);
+        at += __builtin_amdgcn_update_dpp(0, at, 0x4E, 0xF, 0xF, false);
+        if (q == 0 && base + g * (NT / 4) + static_cast<int>(threadIdx.x >> 2) < n &&
+            at < static_cast<uint32_t>(k))
+            f(static_cast<int>(at), mine[g]);
+    }
+}
 template <int NT, typename F>
 __device__ __forceinline__ void ranked(const unsigned long long* list, int n, int k, F f) {
-    const int q = threadIdx.x & 3;
-    for (int base = 0; base < n; base += NT / 4) {  // whole waves
-        const int i = base + (threadIdx.x >> 2);
-        const unsigned long long mine = list[i < n ? i : 0];
-        uint32_t place = 0;
-#pragma unroll 4
-        for (int j = q; j < n; j += 4) place += list[j] > mine ? 1u : 0u;
-        place += __builtin_amdgcn_update_dpp(0, place, 0xB1, 0xF, 0xF, false);
-        place += __builtin_amdgcn_update_dpp(0, place, 0x4E, 0xF, 0xF, false);
-        if (q == 0 && i < n && place < static_cast<uint32_t>(k)) f(static_cast<int>(place), mine);
+    int base = 0;  // whole waves all the way
+    for (; n - base > NT / 2; base += NT) rank_keys<NT, 4>(list, n, k, base, f);
+    if (n - base > NT / 4) rank_keys<NT, 2>(list, n, k, base, f);
+    else if (n > base) rank_keys<NT, 1>(list, n, k, base, f);
+}
+
+// A row's outputs, from its sums and the list that holds its first k.
+template <int NT>
+__device__ __forceinline__ void put_row(const TopParams& p, int64_t row,
+                                        const unsigned long long* list, int n, const Stat& total,
+                                        bool has_target, float x_t, uint32_t before) {
+    const int tid = threadIdx.x, k = p.k;
+    const RowEnd e = row_end(total, p.factor);
+    if (tid == 0) {
+        p.lse[row] = fmaf(e.m, p.inv_t, e.l);
+        p.entropy[row] = e.ent;
+        p.logprob[row] = fmaf(x_t - e.m, p.inv_t, -e.l);
+        p.rank[row] = has_target && !e.bad ? static_cast<int64_t>(before) : -1;
+    }
+    int64_t* ids = p.top_ids + row * k;
+    float* logps = p.top_logprob + row * k;
+    ranked<NT>(list, n, k, [&](int place, unsigned long long key) {
+        ids[place] = key_index(key);
+        logps[place] = fmaf(key_value(key) - e.m, p.inv_t, -e.l);
+    });
+    for (int j = n + tid; j < k; j += NT) {
+        ids[j] = -1;
+        logps[j] = e.bad ? NAN : -INFINITY;
     }
 }
 
@@ -356,8 +423,6 @@ __device__ __forceinline__ float bound_of(const float* thread_max, int k) {
                 if (n <= k + (k >> 2)) break;
             }
         }
-    } else if (64 * R < k) {
-        bound = 0;
     }
     return from_ordered(bound > kOrderedNegInf ? bound : kOrderedNegInf + 1);
 }
@@ -630,7 +695,7 @@ __global__ __launch_bounds__(WAVES * 64, kSplit ? 2 : 8) void klp_top_kernel(Top
         }
         __syncthreads();
     }
-    int n = bad_piece ? 0 : static_cast<int>(sh.n_list);
+    int n = bad_piece ? 0 : sh.listed();
     Stat total = sh.total;
     uint32_t before = sh.before;
 
@@ -728,23 +793,151 @@ __global__ __launch_bounds__(WAVES * 64, kSplit ? 2 : 8) void klp_top_kernel(Top
         n = total.m < INFINITY ? static_cast<int>(sh.n_list) : 0;
     }
 
-    const RowEnd e = row_end(total, p.factor);
-    if (tid == 0) {
-        p.lse[row] = fmaf(e.m, p.inv_t, e.l);
-        p.entropy[row] = e.ent;
-        p.logprob[row] = fmaf(x_t - e.m, p.inv_t, -e.l);
-        p.rank[row] = has_target && !e.bad ? static_cast<int64_t>(before) : -1;
+    put_row<NT>(p, row, sh.list, n, total, has_target, x_t, before);
+}
+
+// Rows of at most 1024 WAVES elements, 16 of them and one of the row's edges in
+// a lane's registers: one load, nothing read again.  Bound by its own steps, not
+// by bytes: the target's two dependent loads, the bound's search bit by bit and
+// the ranking.  Next to klp_top_kernel on the same rows (us, bf16; k = 5 / 64 / 128):
+//   rows x vocab   here                other
+//   4096 x 500     10.3  16.0  23.1    16.1  127   128
+//   4096 x 1000    10.7  15.5  22.7    17.1  28.3  470
+//   4096 x 2000    12.9  19.2  29.8    19.2  28.1  45.2
+//   4096 x 4000    19.2  25.0  37.9    18.9  30.2  49.2
+//   4096 x 5000    35 (k = 20)         24
+//   16 x 1000      5.6   11.1  18.3    5.8   9.3   87.4
+template <int DT, int WAVES>
+__global__ __launch_bounds__(WAVES * 64, 4) void klp_top_short_kernel(TopParams p) {
+    typedef typename Traits<DT>::elem elem;
+    constexpr int NT = WAVES * 64;
+    constexpr int EPV = Traits<DT>::kPerVec;
+    constexpr int ESZ = 16 / EPV;
+    constexpr int kHeld = 16, U = kHeld / EPV;
+    typedef TopShared<WAVES, false> Shared;
+    __shared__ Shared sh;
+
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    const int64_t row = blockIdx.x;
+    const int vocab = static_cast<int>(p.vocab);
+    const int k = p.k;
+    const elem* rp = static_cast<const elem*>(p.logits) + row_offset(p.rm, row);
+    int head = static_cast<int>(((16u - (reinterpret_cast<uintptr_t>(rp) & 15u)) & 15u) / ESZ);
+    if (head > vocab) head = vocab;
+    const int nv = (vocab - head) / EPV;
+    const int tail_begin = head + nv * EPV;
+    const u32x4* vp = reinterpret_cast<const u32x4*>(rp + head);
+    const int n_edge = head + (vocab - tail_begin);
+    const int i_edge = tid < head ? tid : tail_begin + (tid - head);
+
+    u32x4 v[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+        const uint32_t w = Traits<DT>::kNegInfWord;
+        v[u] = u32x4{w, w, w, w};
+        if (u * NT + tid < nv) v[u] = vp[u * NT + tid];
     }
-    int64_t* ids = p.top_ids + row * k;
-    float* logps = p.top_logprob + row * k;
-    ranked<NT>(sh.list, n, k, [&](int place, unsigned long long key) {
-        ids[place] = key_index(key);
-        logps[place] = fmaf(key_value(key) - e.m, p.inv_t, -e.l);
-    });
-    for (int j = n + tid; j < k; j += NT) {
-        ids[j] = -1;
-        logps[j] = e.bad ? NAN : -INFINITY;
+    float x_edge[1] = {-INFINITY};
+    if (tid < n_edge) x_edge[0] = element<DT>(rp, i_edge);
+    const int64_t given = p.targets[row];
+    const bool has_target = given >= 0 && given < vocab;
+    const int target = has_target ? static_cast<int>(given) : 0;
+    const float x_t = has_target ? element<DT>(rp, target) : 0.0f;
+    const float above_t = has_target ? from_ordered(ordered(x_t) + 1u) : INFINITY;
+
+    float x[kHeld];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+        float part[EPV];
+        unpack<DT>(v[u], part);
+#pragma unroll
+        for (int j = 0; j < EPV; ++j) x[u * EPV + j] = part[j];
     }
+    // The row's element x[e] is index(e).
+    auto index = [&](int e) { return head + (e / EPV * NT + tid) * EPV + e % EPV; };
+    float top = x_edge[0];
+#pragma unroll
+    for (int e = 0; e < kHeld; ++e) top = fmax_nan(top, x[e]);
+    Sums s = sums_empty();
+    absorb_any<kHeld>(s, x, top, p.factor);
+    absorb_any<1>(s, x_edge, x_edge[0], p.factor);
+    uint32_t count = has_target && x_edge[0] >= (i_edge < target ? x_t : above_t) ? 1u : 0u;
+    // (Lanes without a vector stand behind tail_begin with -inf.)
+    const int ties_to = target < tail_begin ? target : tail_begin;
+#pragma unroll
+    for (int e = 0; e < kHeld; ++e)
+        count += has_target && x[e] >= (index(e) < ties_to ? x_t : above_t) ? 1u : 0u;
+    count = wave_sum_u32(count);
+    const Stat of_wave = wave_reduce_scaled(Stat{s.m, s.z, s.t}, p.factor);
+
+    // 64 R maxima of 16 WAVES / R elements.  With fewer than k of them above -inf
+    // the whole row, of less than 64 k / R elements, is listed; all the elements
+    // themselves, or 512 maxima and more, where that would be many.
+    float* maxima = reinterpret_cast<float*>(sh.list);
+    auto leave = [&](auto of_thread) {
+        constexpr int kOf = decltype(of_thread)::value, kEach = kHeld / kOf;
+#pragma unroll
+        for (int q = 0; q < kOf; ++q) {
+            float m = q == 0 ? fmax_nan(x[0], x_edge[0]) : x[q * kEach];
+#pragma unroll
+            for (int e = 1; e < kEach; ++e) m = fmax_nan(m, x[q * kEach + e]);
+            maxima[q * NT + tid] = m;
+        }
+    };
+    constexpr int kFew = WAVES < 4 ? 4 : WAVES, kMany = 16;
+    const bool few = k <= 64;
+    if (few) leave(std::integral_constant<int, kFew / WAVES>{});
+    else leave(std::integral_constant<int, kMany / WAVES>{});
+    if (lane == 0) {
+        sh.wave_stat[wave] = of_wave;
+        sh.wave_count[wave] = count;
+    }
+    if (tid == 0) sh.n_list = 0;
+    __syncthreads();
+    if (wave == 0) {
+        const float bound = few ? bound_of<kFew, kFew>(maxima, k) : bound_of<kMany, kMany>(maxima, k);
+        if (lane == 0) sh.tau = bound;
+    }
+    if (wave == WAVES - 1) {
+        const Stat total =
+            wave_reduce_scaled(lane < WAVES ? sh.wave_stat[lane] : stat_empty(), p.factor);
+        if (lane == 0) {
+            sh.total = total;
+            uint32_t n = 0;
+#pragma unroll
+            for (int w = 0; w < WAVES; ++w) n += sh.wave_count[w];
+            sh.before = n;
+        }
+    }
+    __syncthreads();
+    const Stat total = sh.total;
+    const float tau = sh.tau;
+    int n = 0;
+    if (total.m < INFINITY) {
+        uint32_t mine = x_edge[0] >= tau ? 1u : 0u;
+#pragma unroll
+        for (int e = 0; e < kHeld; ++e) mine += x[e] >= tau ? 1u : 0u;
+        if (mine != 0) {
+            uint32_t to = atomicAdd(&sh.n_list, mine);
+            auto keep = [&](float value, int at) {
+                if (!(value >= tau)) return;
+                if (to < static_cast<uint32_t>(Shared::kList))
+                    sh.list[to] = order_key(value, static_cast<uint32_t>(at));
+                ++to;
+            };
+            keep(x_edge[0], i_edge);
+#pragma unroll
+            for (int e = 0; e < kHeld; ++e) keep(x[e], index(e));
+        }
+        __syncthreads();
+        if (sh.n_list > static_cast<uint32_t>(Shared::kList)) {
+            __syncthreads();
+            select_exact<DT, WAVES, false>(sh, rp, Piece{head, 0, vocab, 0, nv}, k);
+        }
+        __syncthreads();
+        n = sh.listed();
+    }
+    put_row<NT>(p, row, sh.list, n, total, has_target, x_t, sh.before);
 }
 
 template <int DT, int WAVES, int U>
@@ -755,8 +948,19 @@ hipError_t launch_top_t(const TopParams& p, hipStream_t stream) {
                                         p);
 }
 
+template <int DT, int WAVES>
+hipError_t launch_top_short(const TopParams& p, hipStream_t stream) {
+    return launch_kernel(klp_top_short_kernel<DT, WAVES>, dim3(static_cast<unsigned>(p.n_rows)),
+                         dim3(WAVES * 64), stream, p);
+}
+
 template <int DT>
 hipError_t launch_top_dt(const TopParams& p, hipStream_t stream) {
+    if (p.vocab <= kTopShort) {
+        if (p.vocab <= 1024) return launch_top_short<DT, 1>(p, stream);
+        if (p.vocab <= 2048) return launch_top_short<DT, 2>(p, stream);
+        return launch_top_short<DT, 4>(p, stream);
+    }
     return p.waves == 8 ? launch_top_t<DT, 8, 2>(p, stream) : launch_top_t<DT, 4, 2>(p, stream);
 }
 
