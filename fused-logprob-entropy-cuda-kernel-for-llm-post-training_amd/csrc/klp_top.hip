@@ -220,8 +220,9 @@ __device__ __forceinline__ float element(const typename Traits<DT>::elem* rp, in
 // and again in each step: logits that another stream writes meanwhile may leave
 // any list, but none beyond its end.
 template <int DT, int WAVES, bool kSplit>
-__device__ void select_exact(TopShared<WAVES, kSplit>& sh, const typename Traits<DT>::elem* rp,
-                             const Piece& pc, int k) {
+__device__ __forceinline__ void select_exact(TopShared<WAVES, kSplit>& sh,
+                                             const typename Traits<DT>::elem* rp, const Piece& pc,
+                                             int k) {
     constexpr int NT = WAVES * 64;
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     uint32_t* hist = reinterpret_cast<uint32_t*>(&sh.record[0][0]);  // 256 bins
