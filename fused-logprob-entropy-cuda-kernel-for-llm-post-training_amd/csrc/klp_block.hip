@@ -21,7 +21,23 @@
 // Bound by memory: the forward reads x and r once and writes h and y once, the
 // backward reads x, h and two gradients once and writes two, a row in the
 // registers of a group of 64 to 1024 threads, 8 elements (a chunk) a thread and
-// pass.
+// pass.  bf16, us (TB/s), post norm and a gate of all rows:
+//   rows x dim     forward     backward                its sums
+//   32768 x 1024   49 (5.5)    84 (4.8)                4
+//   8192 x 4096    51 (5.3)    87 (4.6)                6
+//     no gate      51          82
+//     bare         42 (6.4)    50 (6.7: 5 arrays)
+//     gate of 128 rows         87                      5 + 7 (the gate's)
+//     of a row     60 (5.6)    111 (4.8: 8 arrays)     5
+//     checkpoints  65 (5.2)    78 (4.3)                5
+//   4096 x 8192    54          90                      11
+//   2048 x 16384   55          118                     9
+//   4096 x 4096    61          84 (float32)            5
+//   64 x 3584, e4m3 output     4.4: the launch
+// The forward prefetches nothing beyond its row: many workgroups a CU do that.
+// The backward's groups are few and long, and with each load waiting for the one
+// before (143 us at 8192 x 4096) it was bound by latency, so 16-bit rows have the
+// next row's under this row's sums.
 //
 // Sums over rows: a group takes consecutive rows and keeps its sums in
 // registers; the groups of a workgroup are added in LDS, the workgroups' shares
