@@ -842,6 +842,11 @@ int check_block(int dtype, int64_t rows, int64_t dim, const void* post, const vo
     return KLP_OK;
 }
 
+// Rows that share a gate, of the rows there are: the kernels divide in 32 bits.
+int64_t gate_rows(const void* gate, int64_t rows_per_gate, int64_t rows) {
+    return gate == nullptr ? 1 : rows_per_gate < rows ? rows_per_gate : rows;
+}
+
 // Whether rows of dim elements at these addresses and row strides are whole
 // 16-byte vectors (codes: of 8 bytes).
 bool whole_rows(int64_t dim, int64_t ld, size_t size, std::initializer_list<const void*> at) {
@@ -876,7 +881,7 @@ int block_setup(const void* x, int dtype, int64_t ld_x, const void* residual, in
     p->weight_f32 = weight_dtype == KLP_FP32;
     p->gate = gate;
     p->gate_f32 = gate_dtype == KLP_FP32;
-    p->per_gate = gate != nullptr ? rows_per_gate : 1;
+    p->per_gate = gate_rows(gate, rows_per_gate, rows);
     p->scale = scale;
     p->rows = rows;
     p->dim = dim;
@@ -2058,7 +2063,7 @@ int klp_block_norm_bwd(const void* x, int dtype, int64_t ld_x, const uint8_t* x_
     p.weight_f32 = weight_dtype == KLP_FP32;
     p.gate = gate;
     p.gate_f32 = gate_dtype == KLP_FP32;
-    p.per_gate = gate != nullptr ? rows_per_gate : 1;
+    p.per_gate = gate_rows(gate, rows_per_gate, rows);
     p.scale = scale;
     p.rstd_x = rstd_x;
     p.rstd_h = rstd_h;
