@@ -75,21 +75,23 @@ __global__ __launch_bounds__(kForwardThreads<T>) void klp_block_kernel(BlockPara
     const int dim = static_cast<int>(p.dim);
 
     // What the first sum does not need is on its way while it is made.
-    constexpr bool kWholeRow = kMode != kAny;
     RawChunk<DT> in[N], res[N];
     RawChunk<kWeight<DT, kMode>> wp[N], w[N];
 #pragma unroll
     for (int i = 0; i < N; ++i) {
         const int c = (i * T + t) * kChunk;
-        in[i] = fetch<DT, kWholeRow>(p.x, row * p.ld_x, c, dim);
-        res[i] = fetch<DT, kWholeRow>(p.residual, row * p.ld_r, c, dim);
+        in[i] = fetch<DT, kMode>(p.x, row * p.ld_x, c, dim);
+        res[i] = fetch<DT, kMode>(p.residual, row * p.ld_r, c, dim);
         if constexpr (kPost) wp[i] = fetch_weight<DT, kMode>(p.post, p.weight_f32, c, dim);
         w[i] = fetch_weight<DT, kMode>(p.weight, p.weight_f32, c, dim);
     }
 
     float h[N][kChunk];
 #pragma unroll
-    for (int i = 0; i < N; ++i) in[i].values(h[i]);
+    for (int i = 0; i < N; ++i) {
+        settle<DT, kMode>(in[i], (i * T + t) * kChunk, dim);
+        in[i].values(h[i]);
+    }
     if (p.x_codes != nullptr) {
 #pragma unroll
         for (int i = 0; i < N; ++i)
@@ -108,6 +110,7 @@ __global__ __launch_bounds__(kForwardThreads<T>) void klp_block_kernel(BlockPara
 #pragma unroll
         for (int i = 0; i < N; ++i) {
             float v[kChunk];
+            settle_weight<DT, kMode>(wp[i], p.weight_f32, (i * T + t) * kChunk, dim);
             wp[i].values(v);
 #pragma unroll
             for (int j = 0; j < kChunk; ++j) h[i][j] = h[i][j] * s * v[j];
@@ -118,7 +121,7 @@ __global__ __launch_bounds__(kForwardThreads<T>) void klp_block_kernel(BlockPara
 #pragma unroll
         for (int i = 0; i < N; ++i) {
             float v[kChunk];
-            fetch_either<DT, kWholeRow>(p.gate, p.gate_f32, at, (i * T + t) * kChunk, dim, v);
+            fetch_either<DT, kMode>(p.gate, p.gate_f32, at, (i * T + t) * kChunk, dim, v);
 #pragma unroll
             for (int j = 0; j < kChunk; ++j) h[i][j] *= v[j];
         }
@@ -128,6 +131,7 @@ __global__ __launch_bounds__(kForwardThreads<T>) void klp_block_kernel(BlockPara
     for (int i = 0; i < N; ++i) {
         const int c = (i * T + t) * kChunk;
         float b[kChunk];
+        settle<DT, kMode>(res[i], c, dim);
         res[i].values(b);
 #pragma unroll
         for (int j = 0; j < kChunk; ++j) {
@@ -149,6 +153,7 @@ __global__ __launch_bounds__(kForwardThreads<T>) void klp_block_kernel(BlockPara
     for (int i = 0; i < N; ++i) {
         const int c = (i * T + t) * kChunk;
         float y[kChunk], v[kChunk];
+        settle_weight<DT, kMode>(w[i], p.weight_f32, c, dim);
         w[i].values(v);
 #pragma unroll
         for (int j = 0; j < kChunk; ++j) y[j] = h[i][j] * s * v[j];
@@ -251,7 +256,7 @@ template <int DT>
 hipError_t launch_block_dt(const BlockParams& p, hipStream_t stream) {
     return with_shape(p.dim, [&](auto t, auto n) {
         constexpr int T = decltype(t)::value, N = decltype(n)::value;
-        return with_mode<DT>(p, [&](auto mode) {
+        return with_mode<DT, T, N>(p, [&](auto mode) {
             return launch_block_shape<DT, T, N, decltype(mode)::value>(p, stream);
         });
     });

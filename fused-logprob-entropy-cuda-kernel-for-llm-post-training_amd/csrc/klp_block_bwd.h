@@ -9,26 +9,28 @@ namespace klp {
 namespace {
 
 // A row's x or h: as stored, or the values of its checkpoint.
-template <int DT, bool kKept, bool kWholeRow>
+template <int DT, bool kKept, int kMode>
 struct Stored {
     RawChunk<DT> raw;
     __device__ __forceinline__ void load(const void* rows, int64_t ld, const uint8_t*,
                                          const float*, int64_t row, int64_t, int c, int dim) {
-        raw = fetch<DT, kWholeRow>(rows, row * ld, c, dim);
+        raw = fetch<DT, kMode>(rows, row * ld, c, dim);
     }
+    __device__ __forceinline__ void in_place(int c, int dim) { settle<DT, kMode>(raw, c, dim); }
     __device__ __forceinline__ void values(float (&x)[kChunk]) const { raw.values(x); }
 };
-template <int DT, bool kWholeRow>
-struct Stored<DT, true, kWholeRow> {
+template <int DT, int kMode>
+struct Stored<DT, true, kMode> {
     uint2 codes;
     float scale;
     __device__ __forceinline__ void load(const void*, int64_t, const uint8_t* q,
                                          const float* scales, int64_t row, int64_t n_blocks,
                                          int c, int dim) {
-        codes = fetch_codes<kWholeRow>(q, row * dim, c, dim);
+        codes = fetch_codes<kMode>(q, row * dim, c, dim);
         const float* of_row = scales + row * n_blocks;
         scale = of_row[static_cast<uint32_t>(c < dim ? c : 0) / kScaleBlock];
     }
+    __device__ __forceinline__ void in_place(int c, int dim) { settle_codes<kMode>(codes, c, dim); }
     __device__ __forceinline__ void values(float (&x)[kChunk]) const {
         code_values(codes, scale, x);
     }
@@ -83,9 +85,8 @@ __global__ __launch_bounds__(kBackwardThreads<T>) void klp_block_bwd_kernel(Bloc
     // A row's operands; 16-bit rows (and codes) have the next one's on their way
     // while one is worked on.  Two float32 rows do not fit the registers.
     constexpr bool kAhead = DT != kFP32 && T < 1024 && kMode != kAny;
-    constexpr bool kWholeRow = kMode != kAny;
     struct Row {
-        Stored<DT, kKept, kWholeRow> hs[N], xs[kX ? N : 1];
+        Stored<DT, kKept, kMode> hs[N], xs[kX ? N : 1];
         RawChunk<DT> gys[N], ghs[N];
         float s_h, s_x;
     };
@@ -99,6 +100,9 @@ __global__ __launch_bounds__(kBackwardThreads<T>) void klp_block_bwd_kernel(Bloc
         if constexpr (T == 1024) asm volatile("" : "+v"(c));
         return c;
     };
+    // (kOdd reads the other gradient in the place of one that is not there.)
+    const void* g_y = kMode == kOdd && p.g_y == nullptr ? p.g_h : p.g_y;
+    const void* g_h = kMode == kOdd && p.g_h == nullptr ? p.g_y : p.g_h;
     auto load_row = [&](Row& r, int64_t step) {
         // The groups of a workgroup take the same number of steps, for their
         // barriers: those past a group's rows repeat the last and store nothing.
@@ -112,35 +116,58 @@ __global__ __launch_bounds__(kBackwardThreads<T>) void klp_block_bwd_kernel(Bloc
             r.hs[i].load(p.h, p.dim, p.h_codes, p.h_scales, row, p.n_blocks, c, dim);
             if constexpr (kX)
                 r.xs[i].load(p.x, p.ld_x, p.x_codes, p.x_scales, row, p.n_blocks, c, dim);
-            r.gys[i] = fetch<DT, kWholeRow>(p.g_y, row * p.dim, c, dim);
-            r.ghs[i] = fetch<DT, kWholeRow>(p.g_h, row * p.dim, c, dim);
+            r.gys[i] = fetch<DT, kMode>(g_y, row * p.dim, c, dim);
+            r.ghs[i] = fetch<DT, kMode>(g_h, row * p.dim, c, dim);
+        }
+    };
+    // Before a row's first use.
+    auto in_place = [&](Row& r) {
+        if constexpr (kMode == kOdd) {
+#pragma unroll
+            for (int i = 0; i < N; ++i) {
+                apart();
+                const int c = column_of(i);
+                r.hs[i].in_place(c, dim);
+                if constexpr (kX) r.xs[i].in_place(c, dim);
+                settle<DT, kMode>(r.gys[i], c, dim);
+                settle<DT, kMode>(r.ghs[i], c, dim);
+#pragma unroll
+                for (int k = 0; k < RawChunk<DT>::kVecs; ++k) {
+                    r.gys[i].v[k] &= p.g_y != nullptr ? ~0u : 0u;
+                    r.ghs[i].v[k] &= p.g_h != nullptr ? ~0u : 0u;
+                }
+            }
         }
     };
     // Weights, and the gate while it lasts, in registers where they fit.
     constexpr bool kHold = T < 1024 && kMode != kAny;
     RawChunk<kWeight<DT, kMode>> w_held[kHold ? N : 1], wp_held[kHold && kPost ? N : 1];
     float by_held[kHold && kGate != 0 ? N : 1][kChunk];
+    auto loaded_weight = [&](const void* of, int i) {
+        const int c = column_of(i);
+        auto w = fetch_weight<DT, kMode>(of, p.weight_f32, c, dim);
+        settle_weight<DT, kMode>(w, p.weight_f32, c, dim);
+        return w;
+    };
     auto weight = [&](int i, float (&v)[kChunk]) {
         if constexpr (kHold) w_held[i].values(v);
-        else fetch_weight<DT, kMode>(p.weight, p.weight_f32, column_of(i), dim).values(v);
+        else loaded_weight(p.weight, i).values(v);
     };
     auto post = [&](int i, float (&v)[kChunk]) {
         if constexpr (kHold) wp_held[kPost ? i : 0].values(v);
-        else fetch_weight<DT, kMode>(p.post, p.weight_f32, column_of(i), dim).values(v);
+        else loaded_weight(p.post, i).values(v);
     };
     auto load_gate = [&](int64_t row) {
 #pragma unroll
         for (int i = 0; i < N; ++i)
-            fetch_either<DT, kWholeRow>(p.gate, p.gate_f32, row * p.dim, column_of(i), dim,
+            fetch_either<DT, kMode>(p.gate, p.gate_f32, row * p.dim, column_of(i), dim,
                                         by_held[kHold && kGate != 0 ? i : 0]);
     };
     if constexpr (kHold) {
 #pragma unroll
         for (int i = 0; i < N; ++i) {
-            const int c = column_of(i);
-            w_held[i] = fetch_weight<DT, kMode>(p.weight, p.weight_f32, c, dim);
-            if constexpr (kPost)
-                wp_held[i] = fetch_weight<DT, kMode>(p.post, p.weight_f32, c, dim);
+            w_held[i] = loaded_weight(p.weight, i);
+            if constexpr (kPost) wp_held[i] = loaded_weight(p.post, i);
         }
     }
     // Rows of the gate before `first`, and the gate's.
@@ -161,6 +188,7 @@ __global__ __launch_bounds__(kBackwardThreads<T>) void klp_block_bwd_kernel(Bloc
         Row next;
         if constexpr (kAhead) load_row(next, step + 1);
         else load_row(r, step);
+        in_place(r);
         const float s_h = r.s_h, s_x = r.s_x;
 
         float dh[N][kChunk], dot = 0.0f;
@@ -199,7 +227,7 @@ __global__ __launch_bounds__(kBackwardThreads<T>) void klp_block_bwd_kernel(Bloc
 #pragma unroll
                 for (int j = 0; j < kChunk; ++j) by[j] = by_held[i][j];
             } else if constexpr (kGate != 0) {
-                fetch_either<DT, kWholeRow>(p.gate, p.gate_f32,
+                fetch_either<DT, kMode>(p.gate, p.gate_f32,
                                             static_cast<int64_t>(gate_row) * p.dim, c, dim, by);
             }
 #pragma unroll
@@ -337,7 +365,7 @@ template <int DT>
 hipError_t launch_rows_dt(const BlockBwdParams& p, hipStream_t stream) {
     return with_shape(p.dim, [&](auto t, auto n) {
         constexpr int T = decltype(t)::value, N = decltype(n)::value;
-        return with_mode<DT>(p, [&](auto mode) {
+        return with_mode<DT, T, N>(p, [&](auto mode) {
             return launch_bwd_shape<DT, T, N, decltype(mode)::value>(p, stream);
         });
     });
