@@ -47,9 +47,9 @@ __device__ __forceinline__ float group_sum_alternate(float v, float (&lds)[2][T 
 // the loads of other rows (kOdd): a chunk that the row ends in is read 8 elements
 // from its end and moved into place when it is used (settle).  Short rows of that
 // kind (kAny, up to 512 elements, fewer than 8 among them) wait for their tails.
-// bf16, forward + backward, us, as kAny and so: 8192 x 4090 94 + 199, 56 + 91; 16384 x
-// 1601 85 + 185, 57 + 81; 2048 x 13001 82 + 152, 78 + 126; float32 8192 x 1601 53 +
-// 104, 49 + 66, 4096 x 4097 69 + 123, 76 + 93.
+// bf16, forward + backward, us, as kAny and so: 8192 x 4090 94 + 199, 58 + 91; 16384 x
+// 1601 85 + 185, 64 + 82; 2048 x 13001 82 + 152, 84 + 125; float32 8192 x 1601 53 +
+// 104, 48 + 66, 4096 x 4097 69 + 123, 76 + 94.
 enum : int {
     kWhole = 0,     // weights of the rows' dtype
     kWholeF32 = 1,  // float32 weights
@@ -150,15 +150,18 @@ __device__ __forceinline__ RawChunk<kFP32> fetch_two(const void* w, bool f32, in
 }
 template <int DT>
 __device__ __forceinline__ void settle_two(RawChunk<kFP32>& r, bool f32, int c, int dim) {
+    // Both, one of them chosen: the two sides of a branch would leave registers
+    // that neither is sure to write.
     const int s = shift_of(c, dim);
-    if (f32) {
-        settle32(r.v, s);
-    } else {
-        float x[kChunk];
-        settle16(r.v[0], s);
-        unpack<DT>(r.v[0], x);
-        r.v[0] = pack<kFP32>(x);
-        r.v[1] = pack<kFP32>(x + 4);
+    u32x4 narrow = r.v[0];
+    float x[kChunk];
+    settle16(narrow, s);
+    unpack<DT>(narrow, x);
+    settle32(r.v, s);
+#pragma unroll
+    for (int j = 0; j < kChunk; ++j) {
+        const uint32_t wide = r.v[j / 4][j % 4];
+        r.v[j / 4][j % 4] = f32 ? wide : __float_as_uint(x[j]);
     }
 }
 // A weight or gate, float32 or of the rows' dtype, as values.
@@ -174,8 +177,7 @@ __device__ __forceinline__ void fetch_either(const void* w, bool f32, int64_t at
         settle_two<DT>(r, f32, c, dim);
         r.values(x);
     } else {
-        // Both, one of them empty: the two sides of a branch would leave registers
-        // that neither is sure to write.
+        // Both, one of them empty, as there.
         float wide[kChunk];
         fetch<kFP32, kMode>(f32 ? w : nullptr, at, c, dim).values(wide);
         fetch<DT, kMode>(f32 ? nullptr : w, at, c, dim).values(x);
