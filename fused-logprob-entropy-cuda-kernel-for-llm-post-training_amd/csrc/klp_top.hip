@@ -430,34 +430,51 @@ __device__ __forceinline__ float bound_of(const float* thread_max, int k) {
 
 // count += x[j] >= from for 4 or 8 values, all skipped where no lane's `top`
 // reaches `gate`.  In one block: the compiler's own form holds a mask for each
-// value at a time, and a branch of its own costs the loop its registers.
+// value at a time, and a branch of its own costs the loop its registers.  A vector
+// read of an SGPR that a vector instruction wrote takes two wait states, which the
+// compiler does not add in here: four comparisons come before their four additions,
+// so that three other instructions lie between each and its own.
 __device__ __forceinline__ void count_from(uint32_t& count, float top, float gate, float from,
                                            const float (&x)[4]) {
-    asm("v_cmp_ge_f32 vcc, %1, %2\n\t"
+    unsigned long long m0, m1, m2, m3;
+    asm("v_cmp_ge_f32 vcc, %5, %6\n\t"
         "s_cbranch_vccz .LBBnone%=\n\t"
-        "v_cmp_ge_f32 vcc, %4, %3\n\tv_addc_co_u32 %0, vcc, 0, %0, vcc\n\t"
-        "v_cmp_ge_f32 vcc, %5, %3\n\tv_addc_co_u32 %0, vcc, 0, %0, vcc\n\t"
-        "v_cmp_ge_f32 vcc, %6, %3\n\tv_addc_co_u32 %0, vcc, 0, %0, vcc\n\t"
-        "v_cmp_ge_f32 vcc, %7, %3\n\tv_addc_co_u32 %0, vcc, 0, %0, vcc\n"
+        "v_cmp_ge_f32 %1, %8, %7\n\t"
+        "v_cmp_ge_f32 %2, %9, %7\n\t"
+        "v_cmp_ge_f32 %3, %10, %7\n\t"
+        "v_cmp_ge_f32 %4, %11, %7\n\t"
+        "v_addc_co_u32 %0, vcc, 0, %0, %1\n\t"
+        "v_addc_co_u32 %0, vcc, 0, %0, %2\n\t"
+        "v_addc_co_u32 %0, vcc, 0, %0, %3\n\t"
+        "v_addc_co_u32 %0, vcc, 0, %0, %4\n"
         ".LBBnone%=:"
-        : "+v"(count)
+        : "+v"(count), "=&s"(m0), "=&s"(m1), "=&s"(m2), "=&s"(m3)
         : "v"(top), "v"(gate), "v"(from), "v"(x[0]), "v"(x[1]), "v"(x[2]), "v"(x[3])
         : "vcc");
 }
 __device__ __forceinline__ void count_from(uint32_t& count, float top, float gate, float from,
                                            const float (&x)[8]) {
-    asm("v_cmp_ge_f32 vcc, %1, %2\n\t"
+    unsigned long long m0, m1, m2, m3;
+    asm("v_cmp_ge_f32 vcc, %5, %6\n\t"
         "s_cbranch_vccz .LBBnone%=\n\t"
-        "v_cmp_ge_f32 vcc, %4, %3\n\tv_addc_co_u32 %0, vcc, 0, %0, vcc\n\t"
-        "v_cmp_ge_f32 vcc, %5, %3\n\tv_addc_co_u32 %0, vcc, 0, %0, vcc\n\t"
-        "v_cmp_ge_f32 vcc, %6, %3\n\tv_addc_co_u32 %0, vcc, 0, %0, vcc\n\t"
-        "v_cmp_ge_f32 vcc, %7, %3\n\tv_addc_co_u32 %0, vcc, 0, %0, vcc\n\t"
-        "v_cmp_ge_f32 vcc, %8, %3\n\tv_addc_co_u32 %0, vcc, 0, %0, vcc\n\t"
-        "v_cmp_ge_f32 vcc, %9, %3\n\tv_addc_co_u32 %0, vcc, 0, %0, vcc\n\t"
-        "v_cmp_ge_f32 vcc, %10, %3\n\tv_addc_co_u32 %0, vcc, 0, %0, vcc\n\t"
-        "v_cmp_ge_f32 vcc, %11, %3\n\tv_addc_co_u32 %0, vcc, 0, %0, vcc\n"
+        "v_cmp_ge_f32 %1, %8, %7\n\t"
+        "v_cmp_ge_f32 %2, %9, %7\n\t"
+        "v_cmp_ge_f32 %3, %10, %7\n\t"
+        "v_cmp_ge_f32 %4, %11, %7\n\t"
+        "v_addc_co_u32 %0, vcc, 0, %0, %1\n\t"
+        "v_addc_co_u32 %0, vcc, 0, %0, %2\n\t"
+        "v_addc_co_u32 %0, vcc, 0, %0, %3\n\t"
+        "v_addc_co_u32 %0, vcc, 0, %0, %4\n\t"
+        "v_cmp_ge_f32 %1, %12, %7\n\t"
+        "v_cmp_ge_f32 %2, %13, %7\n\t"
+        "v_cmp_ge_f32 %3, %14, %7\n\t"
+        "v_cmp_ge_f32 %4, %15, %7\n\t"
+        "v_addc_co_u32 %0, vcc, 0, %0, %1\n\t"
+        "v_addc_co_u32 %0, vcc, 0, %0, %2\n\t"
+        "v_addc_co_u32 %0, vcc, 0, %0, %3\n\t"
+        "v_addc_co_u32 %0, vcc, 0, %0, %4\n"
         ".LBBnone%=:"
-        : "+v"(count)
+        : "+v"(count), "=&s"(m0), "=&s"(m1), "=&s"(m2), "=&s"(m3)
         : "v"(top), "v"(gate), "v"(from), "v"(x[0]), "v"(x[1]), "v"(x[2]), "v"(x[3]), "v"(x[4]),
           "v"(x[5]), "v"(x[6]), "v"(x[7])
         : "vcc");

@@ -9,6 +9,8 @@ comes too early (instructions count one wait state, ``s_nop n`` n + 1):
   * an MFMA's A, B or C operand after a VALU write of it: 2;
   * a vector-memory instruction's SGPR after a VALU write of it
     (v_readlane of a spilled one, v_readfirstlane, a compare): 5;
+  * a VALU instruction's SGPR or VCC (a mask, a carry, a constant) after a VALU
+    write of it: 2;
   * a copy to LDS after a write of m0: 1;
   * anything but an MFMA reading or writing an MFMA's result, or an MFMA
     reading it as A or B: 11 (an MFMA of 8 passes); an MFMA adding to it: 2.
@@ -21,6 +23,7 @@ from isa_dataflow import _blocks, _operands, kernels
 
 VALU_TO_MFMA = 2
 VALU_TO_VMEM_SGPR = 5
+VALU_TO_VALU_SGPR = 2
 M0_TO_COPY = 1
 MFMA_RESULT = 11
 MFMA_CHAIN = 2
@@ -76,8 +79,11 @@ def _step(ins: str, age: dict, found: list | None) -> dict:
                 need("m0", {("s", "m0")}, M0_TO_COPY)
         elif op.startswith("v_"):
             dst = set(first)
+            reads = others
             if _TWO_RESULTS.match(op) or _SECOND_SGPR.match(op):
                 dst |= _registers(ops[1])
+                reads = set().union(*(_registers(o) for o in ops[2:]))
+            need("valu", {r for r in reads if r[0] == "s"} - {("s", "m0")}, VALU_TO_VALU_SGPR)
             wrote = [("valu", r) for r in dst]
         if ("s", "m0") in first and not op.startswith(_VMEM):
             wrote.append(("m0", ("s", "m0")))
