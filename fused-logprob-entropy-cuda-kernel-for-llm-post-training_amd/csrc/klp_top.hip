@@ -85,9 +85,9 @@ struct Sums {
 };
 __device__ __forceinline__ Sums sums_empty() { return Sums{-INFINITY, -INFINITY, 0.0f, 0.0f}; }
 
-// K values with maximum `top` into the sums, S = `factor`.  A -inf logit, and
-// one so large that its product with S overflows, leave a z or t that is not
-// finite (sums_lost): absorb_any then does the thread's part once more.
+// K values with maximum `top` into the sums, S = `factor`.  A -inf logit leaves a
+// t that is not finite, and a maximum so large that o's rounding reaches float32's
+// exponents any z: absorb_any then does the thread's part once more (sums_lost).
 template <int K>
 __device__ __forceinline__ void absorb_fast(Sums& s, const float* x, float top, float factor) {
     s.m = fmax_nan(s.m, top);
@@ -112,12 +112,13 @@ __device__ __forceinline__ void absorb_fast(Sums& s, const float* x, float top, 
     s.z = z0 + z1;
     s.t = t0 + t1;
 }
-__device__ __forceinline__ bool sums_lost(const Sums& s) {
-    return !(s.z < INFINITY) || !(s.t > -INFINITY);
-}
-
 // Offsets that overflow: differences of logits are taken before the product.
 __device__ __forceinline__ bool huge_offset(float o) { return !(fabsf(o) < 1e37f); }
+// (A maximum that was huge on the way left a z of 0, or one that is not finite.)
+__device__ __forceinline__ bool sums_lost(const Sums& s) {
+    return !(s.z < INFINITY) || !(s.t > -INFINITY) ||
+           (huge_offset(s.o) && s.m != -INFINITY);
+}
 // (a - b) S of a state's maxima, b the larger; at least kNegBig.
 __device__ __forceinline__ float offset_difference(float a, float b, float factor) {
     if (huge_offset(b * factor)) return fmaxf((a - b) * factor, kNegBig);
