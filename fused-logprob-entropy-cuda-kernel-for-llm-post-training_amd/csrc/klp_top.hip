@@ -11,7 +11,9 @@
 // far, S = log2(e) / T and o = RN(m S), z = sum 2^(x S - o) and t = sum (x S -
 // o) 2^(x S - o).  x S - o is one fma, so that a temperature costs no rounding
 // of its own and the differences that log-probabilities are, (x - m) / T - ln
-// z, keep their precision next to 0.
+// z, keep their precision next to 0.  o's rounding stays in z as an exponent and
+// is taken out at the end; where it could be more than 64, from |o| = 2^31 on,
+// sums are relative to m S itself, with (x - m) S for x S - o.
 //
 // The k largest come from maxima, without a sort and without a second pass:
 // while a thread streams, it leaves the maximum of every few vectors (a
@@ -112,17 +114,23 @@ __device__ __forceinline__ void absorb_fast(Sums& s, const float* x, float top, 
     s.z = z0 + z1;
     s.t = t0 + t1;
 }
-// Offsets that overflow: differences of logits are taken before the product.
-__device__ __forceinline__ bool huge_offset(float o) { return !(fabsf(o) < 1e37f); }
-// (A maximum that was huge on the way left a z of 0, or one that is not finite.)
+// Offsets whose rounding could reach float32's exponents, and those that
+// overflow: the sums are relative to m S itself.
+__device__ __forceinline__ bool huge_offset(float o) { return !(fabsf(o) < 0x1p31f); }
+// (A maximum that was huge on the way left nothing beside one that is not, or a z
+// or t that is not finite.)
 __device__ __forceinline__ bool sums_lost(const Sums& s) {
     return !(s.z < INFINITY) || !(s.t > -INFINITY) ||
            (huge_offset(s.o) && s.m != -INFINITY);
 }
-// (a - b) S of a state's maxima, b the larger; at least kNegBig.
+// What sums relative to a state's maximum a are moved by to another's, b >= a.
+// Unequal floats whose product with S lies there are at least 64 apart in it: next
+// to the larger one's weight the other's is nothing.  (2^-2^20 is 0, and -2^20
+// times any z finite.)
 __device__ __forceinline__ float offset_difference(float a, float b, float factor) {
-    if (huge_offset(b * factor)) return fmaxf((a - b) * factor, kNegBig);
-    return fmaxf(a * factor - b * factor, kNegBig);
+    const float oa = a * factor, ob = b * factor;
+    if (!huge_offset(oa) && !huge_offset(ob)) return oa - ob;
+    return a == b ? 0.0f : -0x1p20f;
 }
 // The same for any values; -inf adds nothing.
 template <int K>
