@@ -175,17 +175,32 @@ struct Stat {
 
 __device__ __forceinline__ Stat stat_empty() { return Stat{-INFINITY, 0.0f, 0.0f}; }
 
+// z and t are relative to 2^o, o = RN(m log2e).  The rounding of o stands in them
+// as an exponent of the maximum itself and is taken out in finalize(): up to 64
+// below |m| = 2^30.  From there on (masks with a finite fill lie there) it would
+// reach float32's exponents, and the product overflow: sums of a far maximum are
+// relative to 2^(m log2e) itself.
+constexpr float kFarMax = 0x1p30f;
+__device__ __forceinline__ bool far_max(float m) { return !(fabsf(m) < kFarMax); }
+
+// Sums relative to the maximum a count 2^d of themselves relative to m >= a;
+// returns whether they count at all.  Unequal floats are 64 apart next to a far
+// one, and beside the larger one's weight the other's is nothing.
+__device__ __forceinline__ bool rebase(float a, float m, float& d) {
+    const bool near = fmaxf(fabsf(a), fabsf(m)) < kFarMax;
+    d = near ? a * kLog2e - m * kLog2e : 0.0f;
+    return near || a == m;
+}
+
 // Associative merge; restates combine() of csrc/fused_logprob.cu:141-154
 // (including its empty-side early returns) in base-2 units.
 __device__ __forceinline__ Stat combine(const Stat a, const Stat b) {
     if (b.m == -INFINITY) return a;
     if (a.m == -INFINITY) return b;
     const float m = fmax_nan(a.m, b.m);
-    const float o = m * kLog2e;
-    const float da = a.m * kLog2e - o;  // <= 0
-    const float db = b.m * kLog2e - o;  // <= 0
-    const float sa = exp2_hw(da);
-    const float sb = exp2_hw(db);
+    float da, db;  // <= 0
+    const float sa = rebase(a.m, m, da) ? exp2_hw(da) : 0.0f;
+    const float sb = rebase(b.m, m, db) ? exp2_hw(db) : 0.0f;
     Stat r;
     r.m = m;
     r.z = sa * a.z + sb * b.z;
@@ -194,25 +209,35 @@ __device__ __forceinline__ Stat combine(const Stat a, const Stat b) {
 }
 
 // Absorb K values into the state: one rescale of (z, t) to the new maximum,
-// then one exp2 per value.  With kClamp == false a -inf value makes t NaN
-// (-inf * 0) while z stays finite; the caller detects that and redoes the
-// values with kClamp == true, which maps -inf exponents to kNegBig.
-template <int K, bool kClamp>
+// then one exp2 per value.  kPlain: a -inf value makes t NaN (-inf * 0), a far
+// maximum z and t of any kind; the caller detects both (needs_rescan) and redoes
+// the values with kEvery.  kPadded: -inf values add nothing (their exponents are
+// mapped to kNegBig), far ones as kPlain.
+enum : int { kPlain = 0, kPadded = 1, kEvery = 2 };
+template <int K, int kValues>
 __device__ __forceinline__ void absorb(Stat& s, const float* x) {
     float c = s.m;
 #pragma unroll
     for (int j = 0; j < K; ++j) c = fmax_nan(c, x[j]);
+    if (kValues == kEvery && c == -INFINITY) return;
+    const bool far = kValues == kEvery && far_max(c);
+    const float first = far ? c : 0.0f;  // taken from the values, or o from their product
     const float o_raw = c * kLog2e;
-    const float o = (c == -INFINITY) ? 0.0f : o_raw;
-    const float d = (s.m == -INFINITY) ? kNegBig : fmax_nan(s.m * kLog2e - o_raw, kNegBig);
-    const float sc = exp2_hw(d);
+    const float o = (far || c == -INFINITY) ? 0.0f : o_raw;
+    float d, sc;
+    if constexpr (kValues == kEvery) {
+        sc = rebase(s.m, c, d) ? exp2_hw(d) : 0.0f;
+    } else {
+        d = (s.m == -INFINITY) ? kNegBig : fmax_nan(s.m * kLog2e - o_raw, kNegBig);
+        sc = exp2_hw(d);
+    }
     float z0 = sc * s.z;
     float t0 = sc * fmaf(d, s.z, s.t);
     float z1 = 0.0f, t1 = 0.0f;
 #pragma unroll
     for (int j = 0; j < K; ++j) {
-        float u = fmaf(x[j], kLog2e, -o);
-        if (kClamp) u = fmax_nan(u, kNegBig);
+        float u = fmaf(kValues == kEvery ? x[j] - first : x[j], kLog2e, -o);
+        if (kValues != kPlain) u = fmax_nan(u, kNegBig);
         const float e = exp2_hw(u);
         if (j & 1) {
             z1 += e;
@@ -227,9 +252,12 @@ __device__ __forceinline__ void absorb(Stat& s, const float* x) {
     s.t = t0 + t1;
 }
 
-// True when the unclamped scan met a -inf value (t is NaN, z is not).
-__device__ __forceinline__ bool needs_clamped_rescan(const Stat& s) {
-    return __builtin_isnan(s.t) && !__builtin_isnan(s.z);
+// True when a plain scan met a -inf value or a far maximum, in a row that has a
+// distribution (no NaN, no +inf).  (A far maximum on the way to one that is not
+// left nothing, or a t that is not finite.)
+__device__ __forceinline__ bool needs_rescan(const Stat& s) {
+    return s.m < INFINITY &&
+           (!(fabsf(s.t) < INFINITY) || (far_max(s.m) && s.m != -INFINITY));
 }
 
 // The state of the partner lane under DPP control `Ctrl` (a lane move
@@ -321,11 +349,11 @@ __device__ __forceinline__ float xrow_sum(float v) {
     return __uint_as_float(r[0]) + __uint_as_float(r[1]);
 }
 
-// (z, t) of state s rescaled to the offset RN(m * log2e), m >= s.m (or m
-// NaN); an empty state contributes zeros.
+// (z, t) of state s relative to the maximum m >= s.m (or m NaN); an empty state
+// contributes zeros.
 __device__ __forceinline__ void rescale_to(const Stat& s, float m, float& z, float& t) {
-    const bool live = s.m != -INFINITY;
-    const float d = live ? s.m * kLog2e - m * kLog2e : 0.0f;
+    float d;
+    const bool live = rebase(s.m, m, d);
     const float sc = live ? exp2_hw(d) : 0.0f;
     z = live ? sc * s.z : 0.0f;
     t = live ? sc * fmaf(d, s.z, s.t) : 0.0f;
@@ -352,7 +380,7 @@ __device__ __forceinline__ Stat row_reduce_flat(const Stat s) {
 //   entropy = ln z - ln2 * t / z
 //   logprob = x_target - lse
 // The middle term of lse undoes the rounding of o = RN(m*log2e); it is the
-// exact product remainder, obtained with one fma.
+// exact product remainder, obtained with one fma (0 for a far maximum).
 struct RowOut {
     float logp;
     float ent;
@@ -362,7 +390,7 @@ struct RowOut {
 __device__ __forceinline__ RowOut finalize(const Stat s, float x_target) {
     const float lnz = logf(s.z);
     float rho = 0.0f;
-    if (s.m != -INFINITY) {
+    if (!far_max(s.m)) {
         const float o = s.m * kLog2e;
         rho = -fmaf(s.m, kLog2e, -o);
     }

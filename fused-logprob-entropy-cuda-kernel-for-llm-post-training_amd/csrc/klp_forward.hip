@@ -40,7 +40,7 @@ namespace klp {
 // wave that loaded and then computed had nothing in flight while it
 // computed), and prefetches past the last whole chunk are out of the
 // buffer's range, so they read nothing and are never used.
-template <int DT, bool kClamp, int U, bool kScaled>
+template <int DT, int kValues, int U, bool kScaled>
 __device__ __forceinline__ void absorb_chunk(Stat& s, const u32x4* v, float scale) {
     constexpr int EPV = Traits<DT>::kPerVec;
     float x[U * EPV];
@@ -50,7 +50,7 @@ __device__ __forceinline__ void absorb_chunk(Stat& s, const u32x4* v, float scal
 #pragma unroll
         for (int j = 0; j < U * EPV; ++j) x[j] *= scale;
     }
-    absorb<U * EPV, kClamp>(s, x);
+    absorb<U * EPV, kValues>(s, x);
 }
 
 template <int U, int NTHREADS>
@@ -62,11 +62,12 @@ __device__ __forceinline__ void load_chunk(u32x4* dst, const __amdgpu_buffer_rsr
             rs, ((c * U + u) * NTHREADS + tid) * 16, 0, kBufNonTemporal);
 }
 
-template <int DT, bool kClamp, int U, int NTHREADS, bool kScaled>
+template <int DT, bool kRescan, int U, int NTHREADS, bool kScaled>
 __device__ __forceinline__ void scan_row_piece(Stat& s, const typename Traits<DT>::elem* rp,
                                                const u32x4* vp, int64_t head, int64_t tail_begin,
                                                int64_t vocab, bool with_edges, int64_t vb,
                                                int64_t ve, int tid, float scale) {
+    constexpr int kBody = kRescan ? kEvery : kPlain, kEdges = kRescan ? kEvery : kPadded;
     // Scalar head / tail elements (fewer than 2 * EPV of them).
     if (with_edges) {
         const int64_t n_edge = head + (vocab - tail_begin);
@@ -74,7 +75,7 @@ __device__ __forceinline__ void scan_row_piece(Stat& s, const typename Traits<DT
             const int64_t idx = (tid < head) ? tid : tail_begin + (tid - head);
             float x = to_f32<DT>(rp[idx]);
             if (kScaled) x *= scale;
-            absorb<1, true>(s, &x);
+            absorb<1, kEdges>(s, &x);
         }
     }
     constexpr int step = NTHREADS * U;  // vectors per chunk
@@ -96,17 +97,16 @@ __device__ __forceinline__ void scan_row_piece(Stat& s, const typename Traits<DT
             // Keeps the prefetch ahead of the arithmetic: the scheduler would
             // otherwise sink it below to save registers.
             __builtin_amdgcn_sched_barrier(0);
-            absorb_chunk<DT, kClamp, U, kScaled>(s, set[r], scale);
+            absorb_chunk<DT, kBody, U, kScaled>(s, set[r], scale);
         }
     }
 #pragma unroll
     for (int r = 0; r < kFwdRing - 1; ++r)
-        if (k + r < n_full) absorb_chunk<DT, kClamp, U, kScaled>(s, set[r], scale);
+        if (k + r < n_full) absorb_chunk<DT, kBody, U, kScaled>(s, set[r], scale);
 
     const int64_t i = vb + static_cast<int64_t>(n_full) * step + tid;
     if (i - tid < ve) {
-        // Remainder: vectors past the end read as -inf, which the clamped
-        // absorb ignores.
+        // Remainder: vectors past the end read as -inf, which adds nothing.
         u32x4 v[U];
 #pragma unroll
         for (int u = 0; u < U; ++u) {
@@ -118,7 +118,7 @@ __device__ __forceinline__ void scan_row_piece(Stat& s, const typename Traits<DT
                 v[u] = u32x4{w, w, w, w};
             }
         }
-        absorb_chunk<DT, true, U, kScaled>(s, v, scale);
+        absorb_chunk<DT, kEdges, U, kScaled>(s, v, scale);
     }
 }
 
@@ -220,9 +220,10 @@ __device__ __forceinline__ void fwd_row(const FwdParams& p) {
     Stat s = stat_empty();
     scan_row_piece<DT, false, U, NTHREADS, kScaled>(s, rp, vp, head, tail_begin, vocab,
                                                     split == 0, vb, ve, tid, p.scale);
-    if (needs_clamped_rescan(s)) {
-        // This lane met a -inf logit: redo its values with -inf excluded, as
-        // the reference's sentinel rule does (csrc/fused_logprob.cu:142-143).
+    if (needs_rescan(s)) {
+        // This lane met a -inf logit, which the reference's sentinel rule
+        // excludes (csrc/fused_logprob.cu:142-143), or a far maximum: redo its
+        // values.
         s = stat_empty();
         scan_row_piece<DT, true, U, NTHREADS, kScaled>(s, rp, vp, head, tail_begin, vocab,
                                                        split == 0, vb, ve, tid, p.scale);

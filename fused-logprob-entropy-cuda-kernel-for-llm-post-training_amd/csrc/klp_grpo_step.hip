@@ -99,8 +99,8 @@ __device__ __forceinline__ Stat scan_regs(const u32x4 (&r)[NV], int n_full, bool
                                           float scale) {
     constexpr int EPV = Traits<DT>::kPerVec;
     constexpr uint32_t pad = Traits<DT>::kNegInfWord;
-    auto scan = [&](auto clamp_tag) {
-        constexpr bool kClamp = decltype(clamp_tag)::value;
+    auto scan = [&](auto rescan) {
+        constexpr bool kRescan = decltype(rescan)::value;
         Stat s = stat_empty();
 #pragma unroll
         for (int k = 0; k < NV; ++k) {
@@ -116,13 +116,14 @@ __device__ __forceinline__ Stat scan_regs(const u32x4 (&r)[NV], int n_full, bool
 #pragma unroll
                 for (int j = 0; j < EPV; ++j) x[j] *= scale;
             }
-            if (k < n_full) absorb<EPV, kClamp>(s, x);
-            else absorb<EPV, true>(s, x);  // padding of the last vector is -inf
+            // The padding of the last vector is -inf.
+            if (k < n_full) absorb<EPV, kRescan ? kEvery : kPlain>(s, x);
+            else absorb<EPV, kRescan ? kEvery : kPadded>(s, x);
         }
         return s;
     };
     Stat s = scan(std::false_type{});
-    if (needs_clamped_rescan(s)) s = scan(std::true_type{});
+    if (needs_rescan(s)) s = scan(std::true_type{});
     return s;
 }
 

@@ -407,7 +407,7 @@ __global__ __launch_bounds__(kThreads) void klp_lmh_kernel(LmhParams p) {
 #pragma unroll
                     for (int j = 0; j < 8; ++j)
                         if (16 * (2 * g + j / 4) + j % 4 >= last) x[j] = -INFINITY;
-                    absorb<8, true>(st[b], x);
+                    absorb<8, kEvery>(st[b], x);
                     pin();
                 }
             }
@@ -418,14 +418,16 @@ __global__ __launch_bounds__(kThreads) void klp_lmh_kernel(LmhParams p) {
                 float x[32];
 #pragma unroll
                 for (int g = 0; g < 4; ++g) values(b, g, x + 8 * g);
-                absorb<32, false>(st[b], x);
+                absorb<32, kPlain>(st[b], x);
                 pin();
-                if (needs_clamped_rescan(st[b])) {  // a -inf logit
+                // A -inf logit, or a far one (needs_rescan, of a state that has
+                // values).
+                if (!(fabsf(st[b].t) < INFINITY) || far_max(st[b].m)) {
                     st[b] = before;
 #pragma unroll
                     for (int g = 0; g < 4; ++g) {
                         values(b, g, x);
-                        absorb<8, true>(st[b], x);
+                        absorb<8, kEvery>(st[b], x);
                     }
                 }
             }
