@@ -169,11 +169,84 @@ __device__ __forceinline__ float top_at(const TopHits& h, int64_t v) {
     return g;
 }
 
+// A workgroup's part of a row.
+struct BwdPart {
+    int64_t head, tail_begin;  // elements before the first vector, and from here on
+    int64_t vb, ve;            // its vectors
+};
+template <int EPV>
+__device__ __forceinline__ BwdPart bwd_part(uintptr_t out_addr, int64_t vocab, int splits,
+                                            int split) {
+    constexpr int ESZ = 16 / EPV;
+    int64_t head = static_cast<int64_t>(((16u - (out_addr & 15u)) & 15u) / ESZ);
+    if (head > vocab) head = vocab;
+    const int64_t nvec = (vocab - head) / EPV;
+    // Pieces are whole multiples of 8 vectors (128 bytes, one cache line
+    // when the row is line-aligned), so that no line is written, or read,
+    // by two workgroups (C4's 18992-vector rows in 8 pieces would otherwise
+    // split a line at every boundary: +1.2% HBM writes).
+    int64_t per = (nvec + splits - 1) / splits;
+    per = (per + 7) & ~int64_t{7};
+    int64_t vb = static_cast<int64_t>(split) * per;
+    int64_t ve = vb + per;
+    if (vb > nvec) vb = nvec;
+    if (ve > nvec) ve = nvec;
+    return BwdPart{head, head + nvec * EPV, vb, ve};
+}
+
+// A far row's part (far_row) once more, over what was put there, element by
+// element.  It reads the kernel's arguments again: kept for it, they would take the
+// usual way's SGPRs beyond what lets 8 waves of it run (4096 x 151936 bf16 386 to
+// 417 us), and a branch before that would keep its loads waiting for lse (397).
+template <int DT, int WAVES, bool kScaled, bool kTop>
+__device__ __forceinline__ void redo_far(TopOf<kTop>& top) {
+    typedef typename Traits<DT>::elem elem;
+    constexpr int EPV = Traits<DT>::kPerVec;
+    uintptr_t args = reinterpret_cast<uintptr_t>(__builtin_amdgcn_kernarg_segment_ptr());
+    asm volatile("" : "+v"(args));
+    BwdParams p;
+    __builtin_memcpy(&p, reinterpret_cast<const void*>(args), sizeof p);
+    const int64_t row = blockIdx.x / p.splits;
+    const int split = static_cast<int>(blockIdx.x - row * p.splits);
+    const elem* rp = static_cast<const elem*>(p.logits) + row_offset(p.rm, row);
+    elem* dp = static_cast<elem*>(p.d_logits) + row * p.vocab;
+    const float ent = p.entropy[row];
+    const float maximum = far_maximum(p.lse[row], ent);
+    const int64_t tgt = p.targets[row];
+    const BwdPart part =
+        bwd_part<EPV>(reinterpret_cast<uintptr_t>(dp), p.vocab, p.splits, split);
+    RowGrad g = row_grad(ent, ent, p.g_logp ? p.g_logp[row] : 0.0f, p.g_ent ? p.g_ent[row] : 0.0f,
+                         p.g_lse ? p.g_lse[row] : 0.0f);
+    // Its vectors' elements [b, e), with split 0 those before and behind all vectors.
+    const int64_t b = part.head + part.vb * EPV, e = part.head + part.ve * EPV;
+    const int64_t e0 = split == 0 ? part.head : 0, b1 = split == 0 ? part.tail_begin : p.vocab;
+    __builtin_amdgcn_s_waitcnt(kWaitVmcnt0);
+    __syncthreads();
+    if constexpr (kTop)
+        g.c0 -= list_top<WAVES>(p, row, top.h, [&](int64_t id, int* vec, int* elem) {
+            *vec = -1;
+            *elem = static_cast<int>(id);
+            return (id >= b && id < e) || id < e0 || id >= b1;
+        });
+    const int64_t n = e - b + e0 + (p.vocab - b1);
+    for (int64_t i = threadIdx.x; i < n; i += WAVES * 64) {
+        const int64_t edge = i - (e - b);
+        const int64_t v = edge < 0 ? b + i : edge < e0 ? edge : b1 + (edge - e0);
+        float x = to_f32<DT>(rp[v]);
+        if (kScaled) x *= p.scale;
+        x = near_logit(x, maximum);
+        float d = grad_elem<DT, true>(x, g);
+        if (v == tgt) d += g.g_logp;
+        if constexpr (kTop) d += top_at(top.h, v);
+        if (kScaled) d *= p.scale;
+        dp[v] = from_f32<DT>(d);
+    }
+}
+
 template <int DT, int WAVES, int U, bool kNtStore, bool kScaled, bool kTop>
 __global__ __launch_bounds__(WAVES * 64) void klp_bwd_kernel(BwdParams p) {
     typedef typename Traits<DT>::elem elem;
     constexpr int EPV = Traits<DT>::kPerVec;
-    constexpr int ESZ = 16 / EPV;
 
     const int tid = threadIdx.x;
     const int64_t row = static_cast<int64_t>(blockIdx.x) / p.splits;
@@ -190,7 +263,7 @@ __global__ __launch_bounds__(WAVES * 64) void klp_bwd_kernel(BwdParams p) {
 
     const uintptr_t in_addr = reinterpret_cast<uintptr_t>(rp);
     const uintptr_t out_addr = reinterpret_cast<uintptr_t>(dp);
-    if (((in_addr ^ out_addr) & 15u) != 0 && vocab <= kBwdElementRow) {
+    if (((in_addr ^ out_addr) & 15u) != 0 && vocab <= kBwdElementRow && !far_row(g.lse)) {
         const int64_t per = (vocab + p.splits - 1) / p.splits;
         const int64_t b = static_cast<int64_t>(split) * per;
         const int64_t e = b + per < vocab ? b + per : vocab;
@@ -212,23 +285,10 @@ __global__ __launch_bounds__(WAVES * 64) void klp_bwd_kernel(BwdParams p) {
         return;
     }
 
-    int64_t head = static_cast<int64_t>(((16u - (out_addr & 15u)) & 15u) / ESZ);
-    if (head > vocab) head = vocab;
-    const int64_t nvec = (vocab - head) / EPV;
-    const int64_t tail_begin = head + nvec * EPV;
-
+    const BwdPart part = bwd_part<EPV>(out_addr, vocab, p.splits, split);
+    const int64_t head = part.head, tail_begin = part.tail_begin, vb = part.vb, ve = part.ve;
     const u32x4* vin = reinterpret_cast<const u32x4*>(rp + head);
     u32x4* vout = reinterpret_cast<u32x4*>(dp + head);
-    // Pieces are whole multiples of 8 vectors (128 bytes, one cache line
-    // when the row is line-aligned), so that no line is written, or read,
-    // by two workgroups (C4's 18992-vector rows in 8 pieces would otherwise
-    // split a line at every boundary: +1.2% HBM writes).
-    int64_t per = (nvec + p.splits - 1) / p.splits;
-    per = (per + 7) & ~int64_t{7};
-    int64_t vb = static_cast<int64_t>(split) * per;
-    int64_t ve = vb + per;
-    if (vb > nvec) vb = nvec;
-    if (ve > nvec) ve = nvec;
 
     if constexpr (kTop)
         g.c0 -= list_top<WAVES>(p, row, top.h, [&](int64_t id, int* vec, int* elem) {
@@ -275,6 +335,7 @@ __global__ __launch_bounds__(WAVES * 64) void klp_bwd_kernel(BwdParams p) {
     else
         bwd_piece<DT, WAVES, U, kNtStore, kScaled, true>(p, vin, vout, vb, ve, t_vec,
                                                          t_lane_elem, g, top);
+    if (far_row(g.lse)) redo_far<DT, WAVES, kScaled, kTop>(top);
 }
 
 template <int DT, int WAVES, int U, bool kNtStore, bool kTop>

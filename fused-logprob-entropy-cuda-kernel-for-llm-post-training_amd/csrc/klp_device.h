@@ -420,6 +420,33 @@ __device__ __forceinline__ RowGrad row_grad(float lse, float ent, float g_logp, 
     return g;
 }
 
+// A far row (masked as a whole with a finite fill, say): beyond 2^28 floats are 32
+// or more apart, so that the logits that have a probability are equal to the row's
+// maximum (e^-32 of a vocabulary is nothing), the entropy is the ln of their number,
+// and the maximum is what of lse is left without it.  (The products of logits and
+// maximum with 1/T may overflow alike.)  The row's gradient is that of a row whose
+// lse is this entropy, with such logits at 0 and all others masked.  In rows that
+// are not, p = exp(x - lse) has a relative error of |lse| 2^-24 from lse's rounding.
+__device__ __forceinline__ bool far_row(float lse) { return fabsf(lse) > 0x1p28f; }
+__device__ __forceinline__ float far_maximum(float lse, float ent) { return lse - ent; }
+__device__ __forceinline__ float near_logit(float x, float maximum) {
+    return x == maximum ? 0.0f : -INFINITY;
+}
+// The same by grad_one's constants alone: with the maximum for lse its p is 1 there
+// and nothing elsewhere, and e^-entropy goes into c0.  lse_hi stays finite where
+// the product overflows, and lse_lo is what it lacks.
+__device__ __forceinline__ RowGrad far_grad(float lse, float ent, float g_logp, float g_lse) {
+    constexpr float kMost = 3.4028234664e38f;
+    RowGrad g;
+    g.lse = far_maximum(lse, ent);
+    g.lse_hi = fminf(fmaxf(g.lse * kLog2e, -kMost), kMost);
+    g.lse_lo = fmaf(g.lse, kLog2e, -g.lse_hi);
+    g.g_logp = g_logp;
+    g.g_ent = 0.0f;
+    g.c0 = (g_lse - g_logp) * expf(-ent);
+    return g;
+}
+
 // Gradient with respect to the (temperature-scaled) logit x, without the
 // one-hot term; the chain-rule factor 1/T for the unscaled logit is applied
 // by the caller.  p = 2^(x*log2e - lse*log2e) with one rounding in the

@@ -156,7 +156,8 @@ __device__ __forceinline__ void publish_target(const u32x4 (&r)[NV], int64_t tgt
 struct StepShared {
     Stat wave_stat[kStepWaves];
     float target_logit;
-    float row_vals[3];  // lse, entropy, g_logp
+    RowGrad grad;       // the row's constants of the backward
+    float far_top;      // float32: a far row's maximum, else NaN
     int64_t next_row;   // persistent kernel: the workgroup's next row
 };
 
@@ -169,11 +170,11 @@ struct StepShared {
 // here; `s` is this thread's state.  With kPublishNext, thread 0 also
 // publishes `next_row` (its claim of the workgroup's next row) between the
 // barriers: every wave read the previous one before the first.
-template <bool kPublishNext, int kWaves>
-__device__ __forceinline__ RowGrad row_results(const GrpoStepParams& p, int64_t row, Stat s,
-                                               bool has_t, const RowInputs& in, bool has_ref,
-                                               float eps_low, float eps_high, float beta,
-                                               int64_t next_row, StepShared& sh) {
+template <int DT, bool kPublishNext, int kWaves>
+__device__ __forceinline__ void row_results(const GrpoStepParams& p, int64_t row, Stat s,
+                                            bool has_t, const RowInputs& in, bool has_ref,
+                                            float eps_low, float eps_high, float beta,
+                                            int64_t next_row, StepShared& sh) {
     const int lane = threadIdx.x & 63;
     // Uniform in the wave: an SGPR (as a VGPR it is one more register live
     // across the persistent kernel's loop).
@@ -192,9 +193,14 @@ __device__ __forceinline__ RowGrad row_results(const GrpoStepParams& p, int64_t 
         const float g_logp = in.wt * (tl.dw + tl.dlp) * p.grad_scale;
         if (lane == 0) {
             if (kPublishNext) sh.next_row = next_row;
-            sh.row_vals[0] = o.lse;
-            sh.row_vals[1] = o.ent;
-            sh.row_vals[2] = g_logp;
+            const bool far = far_row(o.lse);
+            if constexpr (DT == kFP32) {
+                sh.grad = row_grad(far ? o.ent : o.lse, o.ent, g_logp, 0.0f, 0.0f);
+                sh.far_top = far ? far_maximum(o.lse, o.ent) : NAN;
+            } else {
+                sh.grad = far ? far_grad(o.lse, o.ent, g_logp, 0.0f)
+                              : row_grad(o.lse, o.ent, g_logp, 0.0f, 0.0f);
+            }
             p.logprob[row] = o.logp;
             p.entropy[row] = o.ent;
             if (p.lse) p.lse[row] = o.lse;
@@ -202,7 +208,25 @@ __device__ __forceinline__ RowGrad row_results(const GrpoStepParams& p, int64_t 
         }
     }
     __syncthreads();
-    return row_grad(sh.row_vals[0], sh.row_vals[1], sh.row_vals[2], 0.0f, 0.0f);
+}
+
+// A far row's logits (far_row) as float32's gradient takes them: its differences,
+// unlike the constants of the 16-bit one (far_grad), do not reach that far.
+template <int DT, int NV, bool kScaled>
+__device__ __forceinline__ void near_regs(u32x4 (&r)[NV], const StepShared& sh, float scale) {
+    if constexpr (DT == kFP32) {
+        const float top = sh.far_top;
+        if (__builtin_isnan(top)) return;
+#pragma unroll
+        for (int k = 0; k < NV; ++k) {
+            float x[Traits<DT>::kPerVec];
+            unpack<DT>(r[k], x);
+#pragma unroll
+            for (float& v : x) v = near_logit(kScaled ? v * scale : v, top);
+            r[k] = pack<DT>(x);
+            __builtin_amdgcn_sched_barrier(0);
+        }
+    }
 }
 
 // Pass 2 for one vector (the row's vector i): klp_bwd's gradient with
@@ -276,8 +300,10 @@ __global__ __launch_bounds__(kThreads) void klp_grpo_step_kernel(GrpoStepParams 
     const Stat s = scan_regs<DT, NV, kScaled>(r, n_full, has_tail, p.scale);
     __shared__ StepShared sh;
     if (has_t) publish_target<DT, NV, kScaled, kThreads>(r, in.tgt, tid, p.scale, &sh.target_logit);
-    const RowGrad g = row_results<false, kThreads / 64>(p, row, s, has_t, in, has_ref, p.eps_low, p.eps_high,
-                                         p.beta, 0, sh);
+    row_results<DT, false, kThreads / 64>(p, row, s, has_t, in, has_ref, p.eps_low, p.eps_high,
+                                          p.beta, 0, sh);
+    const RowGrad g = sh.grad;
+    near_regs<DT, NV, kScaled>(r, sh, p.scale);
 
     // Pass 2: d_logits from the registers.  Stores past the row's end are
     // dropped by the descriptor.
@@ -387,9 +413,11 @@ __global__ __launch_bounds__(kStepThreads) void klp_grpo_step_rows_kernel(GrpoSt
         // spilled) across the loop.
         float eps_low = p.eps_low, eps_high = p.eps_high, beta = p.beta;
         asm volatile("" : "+s"(eps_low), "+s"(eps_high), "+s"(beta));
-        const RowGrad g = row_results<true, kStepWaves>(
+        row_results<DT, true, kStepWaves>(
             p, row, s, has_t, in, has_ref, eps_low, eps_high, beta,
             static_cast<int64_t>(gridDim.x) + static_cast<int64_t>(claimed), sh);
+        const RowGrad g = sh.grad;
+        near_regs<DT, NV, kScaled>(r, sh, p.scale);
 
         // The next row, and its inputs, read before pass 2's stores and
         // loads.  Past the last row the descriptor has length 0 (no memory

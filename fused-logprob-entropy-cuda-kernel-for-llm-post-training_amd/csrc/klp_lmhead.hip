@@ -320,6 +320,9 @@ __global__ __launch_bounds__(kThreads) void klp_lmh_kernel(LmhParams p) {
                                           p.g_ent ? p.g_ent[tok] : 0.0f,
                                           p.g_lse ? p.g_lse[tok] : 0.0f)
                                : row_grad(0.0f, 0.0f, 0.0f, 0.0f, 0.0f);
+                    if (far_row(rg[b].lse))
+                        rg[b] = far_grad(rg[b].lse, p.saved_entropy[tok], rg[b].g_logp,
+                                         p.g_lse ? p.g_lse[tok] : 0.0f);
                 }
             }
             const bool whole = vlim == kBV && p.out_align >= 16;

@@ -378,7 +378,9 @@ __device__ __forceinline__ void put_row(const TopParams& p, int64_t row,
     const int tid = threadIdx.x, k = p.k;
     const RowEnd e = row_end(total, p.factor);
     if (tid == 0) {
-        p.lse[row] = fmaf(e.m, p.inv_t, e.l);
+        // (A far row's m / T as the backward rounds the logits': far_row.)
+        const float y = e.m * p.inv_t;
+        p.lse[row] = far_row(y) ? y + e.l : fmaf(e.m, p.inv_t, e.l);
         p.entropy[row] = e.ent;
         p.logprob[row] = fmaf(x_t - e.m, p.inv_t, -e.l);
         p.rank[row] = has_target && !e.bad ? static_cast<int64_t>(before) : -1;
