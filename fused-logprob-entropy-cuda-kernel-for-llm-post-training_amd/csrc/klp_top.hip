@@ -17,9 +17,12 @@
 //
 // The k largest come from maxima, without a sort and without a second pass:
 // while a thread streams, it leaves the maximum of every few vectors (a
-// record) in LDS.  The k-th largest of the threads' own maxima is a lower
-// bound tau of the row's k-th largest element, and only records that reach it
-// are read again, some k of them, 32 to 64 bytes each.  Their elements from tau
+// record) in LDS: 32 bytes of a thread's logits, or as many times that, in powers
+// of two, as leave it 16 records of its part (32 bytes up to 256 KB of a row, 64
+// for 152064 bf16, 128 for 152064 float32, 32 KB for 2^26).  The k-th largest of
+// the threads' own maxima is a lower bound tau of the row's k-th largest element,
+// and only records that reach it are read again, some k of them.  Their elements
+// from tau
 // up, about k (1 + k / (2 threads)) of them where large ones lie anywhere, are
 // ranked against each other as whole numbers: the value's bits above, the
 // index below.  Rows whose list overflows (many equal logits, or large ones
@@ -30,9 +33,16 @@
 // and its own k largest in the workspace, and the last to arrive merges them.
 //
 // One pass over the bytes bounds many long rows: 4096 rows of 128256 fp16 take
-// 179 us, 5.9 TB/s (155 for klp_fwd_kernel's three numbers), 1024 of 152064 bf16
-// 57 (k = 20; 62 with k = 64; 47).  Few long rows are bound by their steps: 64 of
+// 180 us, 5.8 TB/s (154 for klp_fwd_kernel's three numbers), 1024 of 152064 bf16
+// 56 (k = 20; 61 with k = 64; 47).  Few long rows are bound by their steps: 64 of
 // 152064 take 14 us, of which the bytes are 4.
+//
+// Masks cost (152064 bf16, k = 20, us for 64 / 1024 rows; the last 128, half, all
+// but 100 logits of a row masked):
+//   none           14 / 56
+//   -inf           14 / 56, 14 / 114, 19 / 111   (a thread's part read again)
+//   -1e9           14 / 57, 183 / 56, 149 / 56   (a piece of equal logits: its
+//   lowest value   14 / 55, 187 / 114, 154 / 114  list overflows)
 //
 // Short rows (klp_top_short_kernel) stay in the registers of as many waves as
 // they need, and the bound comes from maxima of a few elements or from the
@@ -442,50 +452,36 @@ __device__ __forceinline__ float bound_of(const float* thread_max, int k) {
 // count += x[j] >= from for 4 or 8 values, all skipped where no lane's `top`
 // reaches `gate`.  In one block: the compiler's own form holds a mask for each
 // value at a time, and a branch of its own costs the loop its registers.  A vector
-// read of an SGPR that a vector instruction wrote takes two wait states, which the
-// compiler does not add in here: four comparisons come before their four additions,
-// so that three other instructions lie between each and its own.
+// read of VCC behind a vector write of it takes two wait states, which the compiler
+// does not add in here.  (Four masks in SGPR pairs and their additions behind them
+// need none, and take 1 to 4% longer: 1024 rows of 152064 bf16 53.9 us, so 52.6.)
 __device__ __forceinline__ void count_from(uint32_t& count, float top, float gate, float from,
                                            const float (&x)[4]) {
-    unsigned long long m0, m1, m2, m3;
-    asm("v_cmp_ge_f32 vcc, %5, %6\n\t"
+    asm("v_cmp_ge_f32 vcc, %1, %2\n\t"
         "s_cbranch_vccz .LBBnone%=\n\t"
-        "v_cmp_ge_f32 %1, %8, %7\n\t"
-        "v_cmp_ge_f32 %2, %9, %7\n\t"
-        "v_cmp_ge_f32 %3, %10, %7\n\t"
-        "v_cmp_ge_f32 %4, %11, %7\n\t"
-        "v_addc_co_u32 %0, vcc, 0, %0, %1\n\t"
-        "v_addc_co_u32 %0, vcc, 0, %0, %2\n\t"
-        "v_addc_co_u32 %0, vcc, 0, %0, %3\n\t"
-        "v_addc_co_u32 %0, vcc, 0, %0, %4\n"
+        "v_cmp_ge_f32 vcc, %4, %3\n\ts_nop 1\n\tv_addc_co_u32 %0, vcc, 0, %0, vcc\n\t"
+        "v_cmp_ge_f32 vcc, %5, %3\n\ts_nop 1\n\tv_addc_co_u32 %0, vcc, 0, %0, vcc\n\t"
+        "v_cmp_ge_f32 vcc, %6, %3\n\ts_nop 1\n\tv_addc_co_u32 %0, vcc, 0, %0, vcc\n\t"
+        "v_cmp_ge_f32 vcc, %7, %3\n\ts_nop 1\n\tv_addc_co_u32 %0, vcc, 0, %0, vcc\n"
         ".LBBnone%=:"
-        : "+v"(count), "=&s"(m0), "=&s"(m1), "=&s"(m2), "=&s"(m3)
+        : "+v"(count)
         : "v"(top), "v"(gate), "v"(from), "v"(x[0]), "v"(x[1]), "v"(x[2]), "v"(x[3])
         : "vcc");
 }
 __device__ __forceinline__ void count_from(uint32_t& count, float top, float gate, float from,
                                            const float (&x)[8]) {
-    unsigned long long m0, m1, m2, m3;
-    asm("v_cmp_ge_f32 vcc, %5, %6\n\t"
+    asm("v_cmp_ge_f32 vcc, %1, %2\n\t"
         "s_cbranch_vccz .LBBnone%=\n\t"
-        "v_cmp_ge_f32 %1, %8, %7\n\t"
-        "v_cmp_ge_f32 %2, %9, %7\n\t"
-        "v_cmp_ge_f32 %3, %10, %7\n\t"
-        "v_cmp_ge_f32 %4, %11, %7\n\t"
-        "v_addc_co_u32 %0, vcc, 0, %0, %1\n\t"
-        "v_addc_co_u32 %0, vcc, 0, %0, %2\n\t"
-        "v_addc_co_u32 %0, vcc, 0, %0, %3\n\t"
-        "v_addc_co_u32 %0, vcc, 0, %0, %4\n\t"
-        "v_cmp_ge_f32 %1, %12, %7\n\t"
-        "v_cmp_ge_f32 %2, %13, %7\n\t"
-        "v_cmp_ge_f32 %3, %14, %7\n\t"
-        "v_cmp_ge_f32 %4, %15, %7\n\t"
-        "v_addc_co_u32 %0, vcc, 0, %0, %1\n\t"
-        "v_addc_co_u32 %0, vcc, 0, %0, %2\n\t"
-        "v_addc_co_u32 %0, vcc, 0, %0, %3\n\t"
-        "v_addc_co_u32 %0, vcc, 0, %0, %4\n"
+        "v_cmp_ge_f32 vcc, %4, %3\n\ts_nop 1\n\tv_addc_co_u32 %0, vcc, 0, %0, vcc\n\t"
+        "v_cmp_ge_f32 vcc, %5, %3\n\ts_nop 1\n\tv_addc_co_u32 %0, vcc, 0, %0, vcc\n\t"
+        "v_cmp_ge_f32 vcc, %6, %3\n\ts_nop 1\n\tv_addc_co_u32 %0, vcc, 0, %0, vcc\n\t"
+        "v_cmp_ge_f32 vcc, %7, %3\n\ts_nop 1\n\tv_addc_co_u32 %0, vcc, 0, %0, vcc\n\t"
+        "v_cmp_ge_f32 vcc, %8, %3\n\ts_nop 1\n\tv_addc_co_u32 %0, vcc, 0, %0, vcc\n\t"
+        "v_cmp_ge_f32 vcc, %9, %3\n\ts_nop 1\n\tv_addc_co_u32 %0, vcc, 0, %0, vcc\n\t"
+        "v_cmp_ge_f32 vcc, %10, %3\n\ts_nop 1\n\tv_addc_co_u32 %0, vcc, 0, %0, vcc\n\t"
+        "v_cmp_ge_f32 vcc, %11, %3\n\ts_nop 1\n\tv_addc_co_u32 %0, vcc, 0, %0, vcc\n"
         ".LBBnone%=:"
-        : "+v"(count), "=&s"(m0), "=&s"(m1), "=&s"(m2), "=&s"(m3)
+        : "+v"(count)
         : "v"(top), "v"(gate), "v"(from), "v"(x[0]), "v"(x[1]), "v"(x[2]), "v"(x[3]), "v"(x[4]),
           "v"(x[5]), "v"(x[6]), "v"(x[7])
         : "vcc");
