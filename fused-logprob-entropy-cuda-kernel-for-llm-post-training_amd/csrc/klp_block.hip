@@ -33,7 +33,18 @@
 //   4096 x 8192    54          90                      11
 //   2048 x 16384   55          118                     9
 //   4096 x 4096    61          84 (float32)            5
-//   64 x 3584, e4m3 output     4.4: the launch
+// Widths between a shape's, 8192 rows, us (TB/s); lanes behind the row hold nothing:
+//   2304           35 (4.3)    58 (3.9)                4
+//   3584           46 (5.2)    72 (4.9)                6
+//   4097 (odd)     123 (2.2)   136 (3.0)               7
+//   4608           71 (4.3)    101 (4.5)               7
+//   5120           74 (4.5)    110 (4.6)               7
+//   6144           82 (4.9)    140 (4.3)               11
+//   7168           92 (5.1)    158 (4.5)               12
+//   2048 x 12288   48 (4.2)    93 (3.3)                7
+//   2048 x 13001   86 (2.5)    128 (2.5)               10
+// e4m3 output, no gate: 64 x 3584 4.4 (the launch); 8192 x 3584 36 (5.7), x 4096 39
+// (6.0), x 5120 59 (5.0); 2048 x 16384 46 (5.1).
 // The forward prefetches nothing beyond its row: many workgroups a CU do that.
 // The backward's groups are few and long, and with each load waiting for the one
 // before (143 us at 8192 x 4096) it was bound by latency, so 16-bit rows have the

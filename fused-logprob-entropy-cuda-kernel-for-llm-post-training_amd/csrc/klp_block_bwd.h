@@ -55,7 +55,9 @@ __global__ __launch_bounds__(kBackwardThreads<T>) void klp_block_bwd_kernel(Bloc
     const int64_t end = first + p.per_group < p.rows ? first + p.per_group : p.rows;
 
     // A thread's sums.  A thread of 1024 has 128 registers: there the gate's and
-    // the post weight's are kept in LDS, each by its own thread.
+    // the post weight's are kept in LDS, each by its own thread.  Even so, with a
+    // post norm and a gate of all rows, 5 to 24 registers are spilled there, and 11
+    // to 20 of 256 in 16-bit rows off 16-byte boundaries with a gate of some rows.
     constexpr bool kInLds = T == 1024;
     constexpr int kLdsSums = kInLds ? (kPost ? 1 : 0) + (kGate != 0 ? 1 : 0) : 0;
     __shared__ float held[kLdsSums > 0 ? kLdsSums * kCols : 1];

@@ -16,13 +16,15 @@
 // soft cap and a residual before their only rounding: what passes of their own
 // would read and write once more each.  A product bound by its weight's bytes
 // hides it, one bound by its instructions pays for the arithmetic and for the
-// residual's bytes, which nothing overlaps (us, eager calls back to back):
-//   m     n       k      out   plain  bias  relu  bias+silu  gelu  cap  bias+residual
-//   16    152064  3584   bf16  102    102   101   102        100   101  102
-//   2048  16384   4096   bf16  132    135   133   137        137   142  146
-//   2048  4096    16384  fp16  134    133   131   132        132   133  135
-//   1024  152064  3584   bf16  611    633   621   635        636   656  716
-//   2048  16384   4096   fp32  269    261   260   269        275   274  318
+// residual's bytes, which nothing overlaps (us, eager calls back to back; first on
+// the same operands, which the caches then hold where they fit, then on 8 sets of
+// operands in turn, as the layers of a model have them):
+//   m     n       k      out   plain    bias     bias+silu  cap      bias+residual
+//   16    152064  3584   bf16  102 103  101 105  101 105    101 104  102 103
+//   2048  16384   4096   bf16  130 138  132 140  133 140    138 145  142 157
+//   2048  4096    16384  fp16  127 156  128 156  128 157    130 159  132 163
+//   1024  152064  3584   bf16  602 606  613 621  617 624    637 648  692 696
+//   2048  16384   4096   fp32  257 262  259 261  264 269    263 272  314 316
 #include "klp_launch.h"
 #include "klp_mfma.h"
 #include "klp_rows.h"

@@ -388,7 +388,7 @@ struct BlockBwdParams {
     const void* g_h;       // [rows, dim], nullable
     int64_t rows;
     int64_t dim;
-    int64_t groups;        // block_groups(rows, dim), of per_group consecutive rows
+    int64_t groups;        // block_shape(rows, dim): of per_group consecutive rows
     int64_t per_group;
     int whole;             // as BlockParams'
     void* d_x;             // [rows, dim], nullable
@@ -397,8 +397,8 @@ struct BlockBwdParams {
     void* d_weight;        // [dim], nullable
     void* d_gate;          // as gate, nullable
     // Float32 sums of the workgroups (of their groups' rows) for d_post,
-    // d_weight and a gate that all rows share, [block_shares][dim] each; and
-    // of the first and last gate of every group, [2 groups][dim].
+    // d_weight and a gate that all rows share, [BlockShape::shares][dim] each;
+    // and of the first and last gate of every group, [2 groups][dim].
     float* post_shares;
     float* weight_shares;
     float* gate_shares;

@@ -24,7 +24,8 @@ that the codes stand for; the outputs and the statistics are the exact ones
 
 Calls run in the compiled binding (binding/klp_torch.cpp), the autograd function
 included; under graph capture, which it declines, the Python statement of them
-below runs.
+below runs.  ``torch.compile`` breaks the graph at a call and runs it as it is
+(:func:`fused_add_rms_norm` is traced).
 """
 from __future__ import annotations
 
@@ -191,7 +192,7 @@ def fused_block_norm(x: torch.Tensor, residual: torch.Tensor, weight: torch.Tens
 
     Args:
         x, residual: ``[..., dim]`` bf16 / fp16 / fp32 on the GPU, dim at most
-            16384.
+            16384, fewer than 2**22 rows (RuntimeError otherwise).
         weight, post_weight: ``[dim]``, both of ``x``'s dtype or both float32.
         gate: ``[dim]``, or ``x``'s shape with 1 in place of the last leading
             dims (``[batch, 1, dim]`` gates each sequence), of ``x``'s dtype or

@@ -17,7 +17,8 @@ gradient is of first order: a second derivative raises RuntimeError.
 
 Calls run in the compiled binding (binding/klp_torch.cpp), the autograd
 function included; under graph capture, which it declines, the Python statement
-of them below runs.
+of them below runs.  ``torch.compile`` breaks the graph at a call and runs it as it
+is.
 """
 from __future__ import annotations
 
@@ -122,7 +123,8 @@ def fused_top_logprobs(logits: torch.Tensor, targets: torch.Tensor, k: int,
 
     Args:
         logits: ``[..., V]`` bf16 / fp16 / fp32 on the GPU, any layout
-            :func:`kernel_opt.fused_logprob_entropy` takes; V at most 2**26.
+            :func:`kernel_opt.fused_logprob_entropy` takes; V at most 2**26, fewer
+            than 2**23 rows (RuntimeError otherwise).
         targets: ``[...]`` int64.  One outside [0, V), an ignore index, has
             logprob -lse (as :func:`fused_logprob_entropy` gives it) and rank -1.
         k: alternatives of a row, 1 to 256.
@@ -134,7 +136,9 @@ def fused_top_logprobs(logits: torch.Tensor, targets: torch.Tensor, k: int,
         first, equal logits by index.  Logits of -inf are not listed: places left
         over hold -1 and -inf.  A row with a NaN or +inf logit has rank and
         top_ids -1 and NaN otherwise; one of -inf logits only has lse -inf, and
-        logprob and entropy NaN.
+        logprob and entropy NaN.  Finite logits are right at any size, as far as
+        float32 holds the result: a row masked as a whole with a finite fill is
+        uniform.
     """
     k, t = _check(logits, targets, k, temperature)
     try:

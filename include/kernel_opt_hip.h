@@ -121,6 +121,10 @@ int klp_fwd_naive(const void* logits, int dtype, int64_t n_rows, int64_t vocab,
  * read + one write pass.  `g_logp`, `g_ent` and `g_lse` may each be NULL,
  * meaning an all-zero upstream gradient (autograd's None).  `d_logits` is a
  * dense row-major [N, V] array of `dtype`, written with round-to-nearest-even.
+ * The rounding of the saved lse is a relative error of |lse| 2^-24 of p; in rows
+ * with |lse| above 2^28 (masked as a whole with a finite fill, say) lse is the
+ * row's maximum itself, and the logits equal to it share the probability:
+ * exp(-H) each, from the saved entropy.
  *
  * Replaces kernel_opt::fused_logprob_entropy_v1_backward
  * (reference csrc/fused_logprob.cu:284-346, bound at csrc/bindings.cpp:24-26).
@@ -619,7 +623,8 @@ int klp_fp8_linear(const uint8_t* x, int64_t ld_x, const float* x_scales, const 
  *   u = sqrt(2 / pi) (v + 0.044715 v^3), SOFTCAP cap tanh(v / cap)
  * (cap from 2^-100 to 2^100, read with SOFTCAP only).  For 16-bit outputs
  * exponentials and reciprocals are the hardware's: e^x is off by less than
- * (2 + |x|) 2^-22 of itself.  residual may be out's own memory, with out's row
+ * (2 + |x|) 2^-22 of itself.  Results of SILU and GELU_TANH below 2^-118, where
+ * the exponential or its reciprocal leaves float32's range, may be 0.  residual may be out's own memory, with out's row
  * stride.
  */
 typedef enum klp_activation {
