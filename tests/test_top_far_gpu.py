@@ -118,3 +118,22 @@ def test_maxima_around_the_border():
             else:
                 assert a == b
         assert abs(got[2] - want[2]) <= 4 * U * abs(want[2])
+
+
+def test_extreme_rows():
+    """Logits around 10^30, rows of one large value of either sign, one logit far
+    above the others."""
+    g = torch.Generator().manual_seed(5)
+    for vocab in (1000, 9001, 140001):
+        x = torch.randn(4, vocab, generator=g) * 2.0
+        x[0] *= 1e30
+        x[1] = 3e38
+        x[2] = -3e38
+        x[2, 17] = -1e38
+        x[3] = 10.0 ** (torch.rand(vocab, generator=g) * 43 - 5)
+        x[3] *= torch.where(torch.rand(vocab, generator=g) < 0.5, -1.0, 1.0)
+        t = torch.tensor([5, 6, 17, vocab - 1])
+        for k in (4, 64):
+            out = _run(x, t, k, 1.0)
+            for i in range(4):
+                _check_row([o[i] for o in out], np64(x[i]), int(t[i]), k, 1.0)
